@@ -110,6 +110,19 @@ _SIGS = {
     "gncx_attention_prefill": (c_int32, [P, P, P, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, P]),
     "gncx_mqa_attention_step_noalloc": (c_int32, [P, P, P, P, P, c_int32, c_int32, c_int32, c_int32, c_float,
                                                   c_int32, c_int32, P, P]),
+    # several candidates, bounded caches
+    "gncx_attention_tree": (c_int32, [P, P, P, P, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, P, P,
+                                      c_size_t]),
+    "gncx_attention_tree_workspace": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "gncx_mqa_attention_step_weights": (c_int32, [P, P, P, P, P, c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
+                                                  c_int32, P, P, P, c_int32, P, c_size_t]),
+    "gncx_mqa_attention_step_weights_workspace": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
+    "gncx_kv_evict": (c_int32, [P, P, P, P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, P, P, c_int32, P,
+                                c_size_t]),
+    "gncx_kv_evict_workspace": (c_size_t, [c_int32, c_int32, c_int32]),
+    "gncx_beam_select": (c_int32, [P, P, P, c_int32, c_int32, c_int32, c_int32, P, P, P, P, P, c_size_t]),
+    "gncx_beam_select_workspace": (c_size_t, [c_int32, c_int32, c_int32]),
+    "gncx_state_reorder": (c_int32, [P, c_int32, c_size_t, c_int32, c_size_t, c_size_t, P]),
     # model engine
     "gncx_engine_create": (c_void_p, [c_char_p, c_int32]),
     "gncx_engine_create_tp": (c_void_p, [c_char_p, c_int32, c_int32, c_int32]),

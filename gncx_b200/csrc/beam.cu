@@ -1,0 +1,429 @@
+// beam.cu -- beam search's selection over beams and vocabulary, and the
+// in-place reordering of per-slot state that follows it (and that follows the
+// verification of a drafted tree).  No reference counterpart: the reference
+// samples one sequence greedily (lua/gncx_streamer.lua:1229-1273).
+//
+// Selection.  Beam b's candidates are its tokens t with the score
+//   c(b, t) = scores[b] + (x[b][t] - L_b),  L_b = log sum_t exp(x[b][t]),
+// in double precision; an ended beam has the one candidate (eos, scores[b]).
+// The order is total: score descending, then beam, then logit descending,
+// then token, so that the chosen parents and tokens do not depend on how the
+// work was split.
+//   * beam_part_kernel: one CTA per (part of the vocabulary, beam) reads its
+//     logits once.  It keeps sum exp(x - m) per thread (terms and sums in
+//     double: an error of 1e-7 in L_b, as fp32 terms give, could swap two
+//     beams' candidates) and a list of the part's best n_out logits: a
+//     threshold T that at least n_out seen elements reach, first the n_out-th
+//     largest of the threads' maxima, filters what is appended.
+//   * beam_merge_kernel: one CTA forms the L_b, scores the parts' lists rank
+//     by rank (they are sorted, so it stops at a rank at which no list beats
+//     the n_out-th best) and writes the best n_out.
+#include <cuda_runtime.h>
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+#include "tma.cuh"
+
+namespace gncx {
+
+constexpr int kBsThreads = 256;
+constexpr int kBsPer = 16;
+constexpr int kBsTile = kBsThreads * kBsPer;
+constexpr int kBsSort = 1024;             // largest list that is sorted
+constexpr int kBsList = kBsSort + kBsTile;
+constexpr int kBmThreads = 1024;
+constexpr int kBmList = 2 * kBmThreads;
+
+using u64 = unsigned long long;
+
+// fp32 as an unsigned integer in the same order (-0 as +0; a NaN anywhere)
+__device__ __forceinline__ uint32_t ord32(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ float unord32(uint32_t o) {
+    return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ u64 ord64(double x) {
+    const u64 u = (u64)__double_as_longlong(x + 0.0);
+    return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ double unord64(u64 o) {
+    return __longlong_as_double((long long)(o ^ ((o >> 63) ? 1ull << 63 : ~0ull)));
+}
+
+// Descending bitonic sort of list[0, P), P a power of two; whole CTA.
+template <class Key>
+__device__ __forceinline__ void bitonic_desc(Key* list, int P) {
+    for (int k = 2; k <= P; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < P / 2; i += blockDim.x) {
+                const int a = 2 * i - (i & (j - 1)), b = a + j;
+                const Key x = list[a], y = list[b];
+                const bool down = (a & k) == 0;
+                if ((x < y) == down) {
+                    list[a] = y;
+                    list[b] = x;
+                }
+            }
+        }
+    __syncthreads();
+}
+
+struct BeamPart {
+    double sum;  // sum of exp(x - max) over the part
+    float max;
+    int pad;
+};
+
+// Keep the n largest of list[0, cnt) (distinct keys, kBsSort < cnt <=
+// kBsList), in any order: the n-th largest is found bit by bit.  Returns it.
+__device__ u64 beam_keep_n(u64* list, int* s_cnt, int cnt, int n) {
+    constexpr int kPer = (kBsList + kBsThreads - 1) / kBsThreads;
+    __shared__ int s_count;
+    u64 k[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int p = threadIdx.x + i * kBsThreads;
+        k[i] = p < cnt ? list[p] : 0;
+    }
+    u64 t = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+        const u64 cand = t | (1ull << bit);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) c += k[i] >= cand;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (threadIdx.x == 0) s_count = 0;
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) atomicAdd(&s_count, c);
+        __syncthreads();
+        const int total = s_count;
+        __syncthreads();
+        if (total >= n) t = cand;
+        if (total == n) break;
+    }
+    if (threadIdx.x == 0) *s_cnt = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (k[i] >= t && k[i] != 0) list[atomicAdd(s_cnt, 1)] = k[i];
+    __syncthreads();
+    return t;
+}
+
+__global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __restrict__ logits,
+                                                               const int32_t* __restrict__ finished, int vocab,
+                                                               int parts, int per, int n, u64* __restrict__ keys,
+                                                               BeamPart* __restrict__ stats) {
+    __shared__ __align__(16) u64 list[kBsList];
+    __shared__ int s_cnt;
+    __shared__ float s_m[kBsThreads / 32];
+    __shared__ double s_l[kBsThreads / 32];
+    pdl_launch_dependents();
+    const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    if (finished && finished[b]) return;  // the merge does not look at an ended beam's lists
+    const float* x = logits + (size_t)b * vocab;
+    const int i0 = part * per, i1 = min(vocab, i0 + per);
+    float m = -INFINITY;
+    double l = 0.0;
+    u64 T = 0;
+    if (tid == 0) s_cnt = 0;
+    for (int base = i0; base < i1; base += kBsTile) {
+        float v[kBsPer];
+        float tm = -INFINITY;
+        u64 best = 0;
+#pragma unroll
+        for (int j = 0; j < kBsPer; ++j) {
+            const int i = base + j * kBsThreads + tid;
+            v[j] = i < i1 ? __ldg(x + i) : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < kBsPer; ++j) tm = fmaxf(tm, v[j]);
+        if (tm > m) {
+            l *= exp((double)m - (double)tm);  // m = -inf: l is 0
+            m = tm;
+        }
+#pragma unroll
+        for (int j = 0; j < kBsPer; ++j)
+            l += v[j] == -INFINITY ? 0.0 : exp((double)v[j] - (double)m);
+        auto key = [&](int j) {
+            const int i = base + j * kBsThreads + tid;
+            return i < i1 ? (u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)i) : 0ull;
+        };
+        if (base == i0) {
+#pragma unroll
+            for (int j = 0; j < kBsPer; ++j) {
+                const u64 k = key(j);
+                best = k > best ? k : best;
+            }
+            list[tid] = best;
+            bitonic_desc(list, kBsThreads);
+            T = list[n - 1];  // n <= kBsThreads
+            __syncthreads();
+        }
+#pragma unroll
+        for (int j = 0; j < kBsPer; ++j) {
+            const u64 k = key(j);
+            if (k >= T && k != 0) list[atomicAdd(&s_cnt, 1)] = k;
+        }
+        __syncthreads();
+        const int cnt = s_cnt;
+        __syncthreads();
+        if (cnt > kBsSort) T = beam_keep_n(list, &s_cnt, cnt, n);
+    }
+    __syncthreads();
+    const int cnt = s_cnt;
+    int P = kBsThreads;
+    while (P < cnt) P <<= 1;
+    for (int i = cnt + tid; i < P; i += kBsThreads) list[i] = 0;
+    bitonic_desc(list, P);
+    u64* out = keys + ((size_t)b * parts + part) * n;
+    for (int i = tid; i < n; i += kBsThreads) out[i] = list[i];
+    // the threads' (m, l) as one
+    float M = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (m != -INFINITY) l *= exp((double)m - (double)M);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if ((tid & 31) == 0) {
+        s_m[tid >> 5] = M;
+        s_l[tid >> 5] = l;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        float mm = -INFINITY;
+        for (int w = 0; w < kBsThreads / 32; ++w) mm = fmaxf(mm, s_m[w]);
+        double ll = 0.0;
+        for (int w = 0; w < kBsThreads / 32; ++w)
+            ll += s_m[w] == -INFINITY ? s_l[w] : s_l[w] * exp((double)s_m[w] - (double)mm);
+        stats[(size_t)b * parts + part] = BeamPart{ll, mm, 0};
+    }
+}
+
+// (score, then lo = ~(beam | inverted logit | token)): greater is better; hi = 0 is no candidate
+struct BeamKey {
+    u64 hi, lo;
+    __device__ bool operator<(const BeamKey& o) const { return hi < o.hi || (hi == o.hi && lo < o.lo); }
+};
+
+__global__ void __launch_bounds__(kBmThreads) beam_merge_kernel(
+    const u64* __restrict__ keys, const BeamPart* __restrict__ stats, const float* scores, const int32_t* finished,
+    int n_beam, int parts, int n, int eos, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+    int32_t* out_finished) {
+    __shared__ __align__(16) BeamKey list[kBmList];
+    __shared__ double s_lse[kBeamMax];
+    __shared__ int s_cnt;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
+    for (int b = warp; b < n_beam; b += kBmThreads / 32) {
+        if (finished && finished[b]) continue;
+        float M = -INFINITY;
+        for (int p = lane; p < parts; p += 32) M = fmaxf(M, stats[(size_t)b * parts + p].max);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        double l = 0.0;
+        for (int p = lane; p < parts; p += 32) {
+            const BeamPart s = stats[(size_t)b * parts + p];
+            l += s.max == -INFINITY ? s.sum : s.sum * exp((double)s.max - (double)M);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) s_lse[b] = (double)M + log(l);
+    }
+    if (tid == 0) s_cnt = 0;
+    __syncthreads();
+    const int lists = n_beam * parts;
+    BeamKey T{0, 0};
+    for (int base = 0; base < lists * n; base += kBmThreads) {
+        const int c = base + tid;
+        BeamKey k{0, 0};
+        if (c < lists * n) {
+            const int r = c / lists, li = c - r * lists, b = li / parts;
+            if (finished && finished[b]) {
+                if (r == 0 && li == b * parts) {
+                    const double s = (double)scores[b];
+                    k.hi = s > -INFINITY ? ord64(s) : 0;  // false for NaN
+                    k.lo = ~((u64)b << 56 | (u64)eos);
+                }
+            } else {
+                const u64 e = keys[(size_t)li * n + r];
+                if (e) {
+                    const uint32_t o = (uint32_t)(e >> 32);
+                    const uint32_t token = 0xFFFFFFFFu - (uint32_t)e;
+                    const double s = (double)scores[b] + ((double)unord32(o) - s_lse[b]);
+                    k.hi = s > -INFINITY ? ord64(s) : 0;
+                    k.lo = ~((u64)b << 56 | (u64)~o << 24 | token);
+                }
+            }
+        }
+        const bool better = k.hi != 0 && T < k;
+        if (better) list[atomicAdd(&s_cnt, 1)] = k;
+        const bool any = __syncthreads_or(better);
+        const int cnt = s_cnt;
+        __syncthreads();
+        if (!any && lists <= kBmThreads) break;  // every list's next entry lost, so all later ones do
+        if ((T.hi == 0 && cnt >= n) || cnt > kBmList - kBmThreads) {
+            int P = kBmThreads / 4;
+            while (P < cnt) P <<= 1;
+            for (int i = cnt + tid; i < P; i += kBmThreads) list[i] = BeamKey{0, 0};
+            bitonic_desc(list, P);
+            T = list[n - 1];
+            if (tid == 0) s_cnt = n;  // cnt >= n: n <= kBmList - kBmThreads
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+    const int cnt = s_cnt;
+    int P = kBmThreads / 4;
+    while (P < cnt) P <<= 1;
+    for (int i = cnt + tid; i < P; i += kBmThreads) list[i] = BeamKey{0, 0};
+    bitonic_desc(list, P);
+    const BeamKey k = list[tid < n ? tid : 0];
+    const u64 id = ~k.lo;
+    const bool some = tid < n && k.hi != 0;
+    const int b = some ? (int)(id >> 56) : -1;
+    const int token = some ? (int)(id & 0xFFFFFFu) : -1;
+    const bool ended = some && ((finished && finished[b]) || token == eos);
+    __syncthreads();  // the inputs are read: the outputs may be the same arrays
+    if (tid < n) {
+        out_scores[tid] = some ? (float)unord64(k.hi) : -INFINITY;
+        out_parents[tid] = b;
+        out_tokens[tid] = token;
+        if (out_finished) out_finished[tid] = ended;
+    }
+}
+
+// Parts of a beam's vocabulary: about two CTAs per SM over all beams, no part
+// shorter than one tile.
+static int beam_parts(int n_beam, int vocab, int sm_count) {
+    const int tiles = (vocab + kBsTile - 1) / kBsTile;
+    const int want = (2 * sm_count + n_beam - 1) / n_beam;
+    return tiles < want ? tiles : want;
+}
+
+size_t beam_workspace_bytes(int n_beam, int vocab, int n_out, int sm_count) {
+    const size_t lists = (size_t)n_beam * beam_parts(n_beam, vocab, sm_count);
+    return (lists * n_out * sizeof(u64) + 255) / 256 * 256 + lists * sizeof(BeamPart);
+}
+
+int beam_select_launch(const float* logits, const float* scores, const int32_t* finished, int n_beam, int vocab,
+                       int eos, int n_out, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                       int32_t* out_finished, void* ws, cudaStream_t st) {
+    static_assert(kBeamMaxOut <= kBsThreads && kBeamMaxOut <= kBmThreads / 4, "the lists' capacities");
+    const int parts = beam_parts(n_beam, vocab, device_info().sm_count);
+    const int per = (vocab + parts - 1) / parts;
+    u64* keys = static_cast<u64*>(ws);
+    const size_t lists = (size_t)n_beam * parts;
+    BeamPart* stats = reinterpret_cast<BeamPart*>(static_cast<uint8_t*>(ws) + (lists * n_out * sizeof(u64) + 255) / 256 * 256);
+    beam_part_kernel<<<dim3(parts, n_beam), kBsThreads, 0, st>>>(logits, finished, vocab, parts, per, n_out, keys, stats);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    return launch_after(beam_merge_kernel, dim3(1), dim3(kBmThreads), 0, st, (const u64*)keys, (const BeamPart*)stats,
+                        scores, finished, n_beam, parts, n_out, eos, out_scores, out_parents, out_tokens,
+                        out_finished) == cudaSuccess
+               ? kOk
+               : kErrCuda;
+}
+
+// ---------------------------------------------------------------- reordering
+// new[s][i] = old[s][index[i]] for every state s, in place.  A thread owns one
+// column (16 or 4 bytes at one offset of every slot), reads the sources of
+// all slots that change before it writes any, so no second buffer and no
+// barrier is needed; slots that stay (-1, or their own index) are not touched.
+// An index outside [-1, n_slots) leaves its slot and records an error.
+struct ReorderArgs {
+    uint8_t* state;
+    size_t state_stride, slot_stride;
+    size_t cols;  // columns per slot
+    int n_states, n_slots;
+    const int32_t* index;
+    int32_t* err;
+};
+
+// The (destination, source) pairs of the slots that change; whole CTA.
+__device__ __forceinline__ int reorder_moves(const ReorderArgs& a, int2* s_move, int* s_n) {
+    if (threadIdx.x == 0) *s_n = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.n_slots; i += blockDim.x) {
+        const int j = a.index[i];
+        if (j < -1 || j >= a.n_slots) record_error(a.err, kErrInvalidArg);
+        else if (j >= 0 && j != i) s_move[atomicAdd(s_n, 1)] = make_int2(i, j);
+    }
+    __syncthreads();
+    return *s_n;
+}
+
+constexpr int kReorderRegs = 16;  // slots whose columns a thread holds in registers
+
+template <class V, int N>
+__global__ void __launch_bounds__(256) reorder_regs_kernel(const ReorderArgs a) {
+    __shared__ int2 s_move[N];
+    __shared__ int s_n;
+    const int m = reorder_moves(a, s_move, &s_n);
+    if (m == 0) return;
+    const size_t c = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (c >= a.cols) return;
+    for (int s = blockIdx.y; s < a.n_states; s += gridDim.y) {
+        uint8_t* p = a.state + (size_t)s * a.state_stride + c * sizeof(V);
+        V v[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < m) v[j] = *reinterpret_cast<const V*>(p + (size_t)s_move[j].y * a.slot_stride);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < m) *reinterpret_cast<V*>(p + (size_t)s_move[j].x * a.slot_stride) = v[j];
+    }
+}
+
+template <class V>
+__global__ void reorder_smem_kernel(const ReorderArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int2 s_move[kReorderMaxSlots];
+    __shared__ int s_n;
+    const int m = reorder_moves(a, s_move, &s_n);
+    if (m == 0) return;
+    const size_t c = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (c >= a.cols) return;
+    V* hold = reinterpret_cast<V*>(smem) + threadIdx.x;
+    for (int s = blockIdx.y; s < a.n_states; s += gridDim.y) {
+        uint8_t* p = a.state + (size_t)s * a.state_stride + c * sizeof(V);
+#pragma unroll 8
+        for (int j = 0; j < m; ++j) hold[j * blockDim.x] = *reinterpret_cast<const V*>(p + (size_t)s_move[j].y * a.slot_stride);
+#pragma unroll 8
+        for (int j = 0; j < m; ++j) *reinterpret_cast<V*>(p + (size_t)s_move[j].x * a.slot_stride) = hold[j * blockDim.x];
+    }
+}
+
+template <class V>
+static cudaError_t reorder_launch_v(ReorderArgs a, size_t n_bytes, cudaStream_t st) {
+    a.cols = n_bytes / sizeof(V);
+    int threads = 256;
+    while (threads > 32 && (size_t)threads / 2 >= a.cols) threads >>= 1;
+    const int gy = a.n_states < 65535 ? a.n_states : 65535;
+    if (a.n_slots <= kReorderRegs) {
+        const dim3 grid((unsigned)((a.cols + threads - 1) / threads), gy);
+        if (a.n_slots <= 4) reorder_regs_kernel<V, 4><<<grid, threads, 0, st>>>(a);
+        else if (a.n_slots <= 8) reorder_regs_kernel<V, 8><<<grid, threads, 0, st>>>(a);
+        else reorder_regs_kernel<V, kReorderRegs><<<grid, threads, 0, st>>>(a);
+        return cudaGetLastError();
+    }
+    while (threads > 32 && (size_t)threads * a.n_slots * sizeof(V) > 64 * 1024) threads >>= 1;
+    const size_t smem = (size_t)threads * a.n_slots * sizeof(V);
+    const cudaError_t e = set_smem_limit(reorder_smem_kernel<V>, smem);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)((a.cols + threads - 1) / threads), gy);
+    reorder_smem_kernel<V><<<grid, threads, smem, st>>>(a);
+    return cudaGetLastError();
+}
+
+int reorder_launch(void* state, int n_states, size_t state_stride, int n_slots, size_t slot_stride, size_t n_bytes,
+                   const int32_t* index, int32_t* err, cudaStream_t st) {
+    ReorderArgs a{static_cast<uint8_t*>(state), state_stride, slot_stride, 0, n_states, n_slots, index, err};
+    const bool wide = (((uintptr_t)state | state_stride | slot_stride | n_bytes) & 15) == 0;
+    const cudaError_t e = wide ? reorder_launch_v<uint4>(a, n_bytes, st) : reorder_launch_v<uint32_t>(a, n_bytes, st);
+    return e == cudaSuccess ? kOk : kErrCuda;
+}
+
+}  // namespace gncx

@@ -829,4 +829,246 @@ int32_t gncx_sample_greedy(const float* logits, int32_t vocab, const int32_t* re
     return idx;
 }
 
+// ---------------------------------------------------------------- several candidates, bounded caches
+static int32_t refuse(int32_t code, const char* fn, const char* why) {
+    const std::string m = std::string(fn) + ": " + why;
+    set_error(code, m.c_str());
+    return code;
+}
+
+// Start of a call: the library is up, and a capture of its stream can hold
+// the call (synchronous mode would wait inside the capture).
+static int32_t begin_call(const char* fn, bool* capturing) {
+    const int32_t st = ensure_init();
+    if (st != kOk) return st;
+    cudaStreamCaptureStatus c = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream(), &c) != cudaSuccess) {
+        cudaGetLastError();
+        return refuse(kErrCuda, fn, "the stream's capture status cannot be read");
+    }
+    *capturing = c != cudaStreamCaptureStatusNone;
+    if (*capturing && g_rt.synchronous)
+        return refuse(kErrInvalidArg, fn, "a stream is captured in stream-ordered mode only (gncx_set_synchronous(0))");
+    return kOk;
+}
+
+// p must be memory of the current device (or host memory it can reach),
+// aligned to `align` bytes.
+static int32_t check_buf(const char* fn, const void* p, const char* name, size_t align) {
+    if (!p) return refuse(kErrInvalidArg, fn, (std::string("null pointer: ") + name).c_str());
+    if ((uintptr_t)p & (align - 1))
+        return refuse(kErrUnaligned, fn, (std::string(name) + " must be aligned to " + std::to_string(align) + " bytes").c_str());
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+        cudaGetLastError();
+        a.type = cudaMemoryTypeUnregistered;
+    }
+    if (a.type == cudaMemoryTypeDevice && a.device != g_rt.device)
+        return refuse(kErrInvalidArg, fn, (std::string(name) + " is memory of another device than the current one").c_str());
+    if (a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged ||
+        (a.type == cudaMemoryTypeHost && a.devicePointer == p))
+        return kOk;
+    return refuse(kErrNotHostAccessible, fn, (std::string("pointer is not device-accessible: ") + name).c_str());
+}
+
+// The caller's workspace, or the library's own where the caller gives none.
+static int32_t pick_workspace(const char* fn, void* given, size_t given_bytes, size_t need, bool capturing, void** ws) {
+    *ws = given;
+    if (need == 0) return kOk;
+    if (given) {
+        const int32_t st = check_buf(fn, given, "workspace", 16);
+        if (st != kOk) return st;
+        if (given_bytes >= need) return kOk;
+        return refuse(kErrCapacity, fn, ("the workspace needs " + std::to_string(need) + " bytes").c_str());
+    }
+    if (capturing)  // the library's own may be freed when a later call needs a larger one
+        return refuse(kErrInvalidArg, fn, "a captured call needs a workspace of the caller's");
+    *ws = workspace(need);
+    return *ws ? kOk : kErrOutOfMemory;
+}
+
+#define GNCX_TRY(x)                              \
+    do {                                         \
+        const int32_t try_st = (x);              \
+        if (try_st != kOk) return try_st;        \
+    } while (0)
+
+static bool tree_shape_ok(int32_t pos0, int32_t n_tok, int32_t n_heads, int32_t n_kv, int32_t hd) {
+    return pos0 >= 0 && n_tok > 0 && n_tok <= kTreeMaxTok && pos0 <= INT32_MAX - n_tok && n_kv <= 65535 &&
+           attention_shape_ok(n_heads, n_kv, hd);
+}
+static const char* const kTreeShape =
+    "pos0 >= 0, n_tok in 1..1024, n_heads a multiple of n_kv_heads, head_dim a multiple of 4 up to 256 are needed";
+
+size_t gncx_attention_tree_workspace(int32_t pos0, int32_t n_tok, int32_t n_heads, int32_t n_kv, int32_t hd,
+                                     int32_t window) {
+    if (!tree_shape_ok(pos0, n_tok, n_heads, n_kv, hd)) {
+        refuse(kErrInvalidArg, "gncx_attention_tree_workspace", kTreeShape);
+        return 0;
+    }
+    if (ensure_init() != kOk) return 0;
+    return tree_workspace_bytes(pos0, n_tok, n_heads, n_kv, hd, window);
+}
+
+int32_t gncx_attention_tree(const float* q, const float* k_cache, const float* v_cache, const int32_t* parents,
+                            int32_t pos0, int32_t n_tok, int32_t n_heads, int32_t n_kv, int32_t hd, float attn_scale,
+                            int32_t window, float* out, void* given, size_t given_bytes) {
+    static const char* fn = "gncx_attention_tree";
+    if (!tree_shape_ok(pos0, n_tok, n_heads, n_kv, hd)) return refuse(kErrInvalidArg, fn, kTreeShape);
+    bool capturing;
+    GNCX_TRY(begin_call(fn, &capturing));
+    GNCX_TRY(check_buf(fn, q, "q", 16));
+    GNCX_TRY(check_buf(fn, k_cache, "k_cache", 16));
+    GNCX_TRY(check_buf(fn, v_cache, "v_cache", 16));
+    GNCX_TRY(check_buf(fn, parents, "parents", 4));
+    GNCX_TRY(check_buf(fn, out, "out", 16));
+    void* ws;
+    GNCX_TRY(pick_workspace(fn, given, given_bytes, tree_workspace_bytes(pos0, n_tok, n_heads, n_kv, hd, window), capturing, &ws));
+    return finish(tree_launch(q, k_cache, v_cache, parents, pos0, n_tok, n_heads, n_kv, hd, attn_scale, window, out, ws,
+                              g_rt.d_err, stream()));
+}
+
+static bool step_shape_ok(int32_t pos, int32_t n_heads, int32_t n_kv, int32_t hd) {
+    return pos >= 0 && pos < INT32_MAX - 1024 && n_kv <= 65535 && attention_shape_ok(n_heads, n_kv, hd);
+}
+static const char* const kStepShape =
+    "pos >= 0, n_heads a multiple of n_kv_heads, head_dim a multiple of 4 up to 256 are needed";
+
+size_t gncx_mqa_attention_step_weights_workspace(int32_t pos, int32_t n_heads, int32_t n_kv, int32_t hd) {
+    if (!step_shape_ok(pos, n_heads, n_kv, hd)) {
+        refuse(kErrInvalidArg, "gncx_mqa_attention_step_weights_workspace", kStepShape);
+        return 0;
+    }
+    if (ensure_init() != kOk) return 0;
+    return weights_workspace_bytes(pos, n_heads, n_kv, hd, device_info().sm_count);
+}
+
+int32_t gncx_mqa_attention_step_weights(const float* q_vec, const float* k_vec, const float* v_vec, float* k_cache,
+                                        float* v_cache, int32_t pos, int32_t token_pos, int32_t n_heads, int32_t n_kv,
+                                        int32_t hd, float attn_scale, int32_t write_kv, float* out, float* weight_sum,
+                                        int32_t* positions, int32_t row_stride, void* given, size_t given_bytes) {
+    static const char* fn = "gncx_mqa_attention_step_weights";
+    if (!step_shape_ok(pos, n_heads, n_kv, hd)) return refuse(kErrInvalidArg, fn, kStepShape);
+    if (row_stride <= pos) return refuse(kErrInvalidArg, fn, "row_stride must hold rows 0 .. pos");
+    bool capturing;
+    GNCX_TRY(begin_call(fn, &capturing));
+    GNCX_TRY(check_buf(fn, q_vec, "q_vec", 16));
+    GNCX_TRY(check_buf(fn, k_cache, "k_cache_layer", 16));
+    GNCX_TRY(check_buf(fn, v_cache, "v_cache_layer", 16));
+    GNCX_TRY(check_buf(fn, out, "out_attn_vec", 16));
+    GNCX_TRY(check_buf(fn, weight_sum, "weight_sum", 4));
+    if (positions) GNCX_TRY(check_buf(fn, positions, "positions", 4));
+    if (write_kv) {
+        GNCX_TRY(check_buf(fn, k_vec, "k_vec", 16));
+        GNCX_TRY(check_buf(fn, v_vec, "v_vec", 16));
+    }
+    void* ws;
+    GNCX_TRY(pick_workspace(fn, given, given_bytes, weights_workspace_bytes(pos, n_heads, n_kv, hd, device_info().sm_count),
+                            capturing, &ws));
+    return finish(weights_step_launch(q_vec, write_kv ? k_vec : nullptr, write_kv ? v_vec : nullptr, k_cache, v_cache, pos,
+                                      token_pos, n_heads, n_kv, hd, attn_scale, out, weight_sum, positions, row_stride, ws,
+                                      stream()));
+}
+
+static bool evict_shape_ok(int32_t n_rows, int32_t n_keep, int32_t n_kv, int32_t hd) {
+    return n_rows >= 0 && n_rows < INT32_MAX - 1024 && n_keep >= 0 && n_keep <= n_rows && n_kv > 0 && n_kv <= 65535 && hd > 0 &&
+           hd % 4 == 0;
+}
+static const char* const kEvictShape = "0 <= n_keep <= n_rows, n_kv_heads > 0, head_dim a positive multiple of 4 are needed";
+
+size_t gncx_kv_evict_workspace(int32_t n_rows, int32_t n_keep, int32_t n_kv) {
+    if (!evict_shape_ok(n_rows, n_keep, n_kv, 4)) {
+        refuse(kErrInvalidArg, "gncx_kv_evict_workspace", kEvictShape);
+        return 0;
+    }
+    return evict_workspace_bytes(n_rows, n_keep, n_kv);
+}
+
+int32_t gncx_kv_evict(float* k_cache, float* v_cache, const float* weight_sum, const int32_t* positions,
+                      int32_t row_stride, int32_t n_rows, int32_t n_keep, int32_t recent_pos, int32_t n_kv, int32_t hd,
+                      float* weight_out, int32_t* positions_out, int32_t out_stride, void* given, size_t given_bytes) {
+    static const char* fn = "gncx_kv_evict";
+    if (!evict_shape_ok(n_rows, n_keep, n_kv, hd)) return refuse(kErrInvalidArg, fn, kEvictShape);
+    if (row_stride < n_rows || out_stride < n_keep)
+        return refuse(kErrInvalidArg, fn, "row_stride must hold n_rows rows and out_stride n_keep");
+    if ((positions == nullptr) != (positions_out == nullptr))
+        return refuse(kErrInvalidArg, fn, "positions and positions_out go together");
+    if ((weight_out == weight_sum || (positions && positions_out == positions)) && out_stride != row_stride)
+        return refuse(kErrInvalidArg, fn, "in place, out_stride is row_stride");
+    bool capturing;
+    GNCX_TRY(begin_call(fn, &capturing));
+    if (n_keep == 0) return finish(kOk);
+    GNCX_TRY(check_buf(fn, k_cache, "k_cache_layer", 16));
+    GNCX_TRY(check_buf(fn, v_cache, "v_cache_layer", 16));
+    GNCX_TRY(check_buf(fn, weight_sum, "weight_sum", 4));
+    GNCX_TRY(check_buf(fn, weight_out, "weight_out", 4));
+    if (positions) {
+        GNCX_TRY(check_buf(fn, positions, "positions", 4));
+        GNCX_TRY(check_buf(fn, positions_out, "positions_out", 4));
+    }
+    void* ws;
+    GNCX_TRY(pick_workspace(fn, given, given_bytes, evict_workspace_bytes(n_rows, n_keep, n_kv), capturing, &ws));
+    return finish(evict_launch(k_cache, v_cache, weight_sum, positions, row_stride, n_rows, n_keep, recent_pos, n_kv, hd,
+                               weight_out, positions_out, out_stride, ws, stream()));
+}
+
+static bool beam_shape_ok(int32_t n_beam, int32_t vocab, int32_t n_out) {
+    return n_beam > 0 && n_beam <= kBeamMax && vocab > 0 && vocab <= kBeamMaxVocab && n_out > 0 && n_out <= kBeamMaxOut;
+}
+static const char* const kBeamShape = "n_beam and n_out in 1..256 and vocab in 1..16777216 are needed";
+
+size_t gncx_beam_select_workspace(int32_t n_beam, int32_t vocab, int32_t n_out) {
+    if (!beam_shape_ok(n_beam, vocab, n_out)) {
+        refuse(kErrInvalidArg, "gncx_beam_select_workspace", kBeamShape);
+        return 0;
+    }
+    if (ensure_init() != kOk) return 0;
+    return beam_workspace_bytes(n_beam, vocab, n_out, device_info().sm_count);
+}
+
+int32_t gncx_beam_select(const float* logits, const float* scores, const int32_t* finished, int32_t n_beam,
+                         int32_t vocab, int32_t eos, int32_t n_out, float* out_scores, int32_t* out_parents,
+                         int32_t* out_tokens, int32_t* out_finished, void* given, size_t given_bytes) {
+    static const char* fn = "gncx_beam_select";
+    if (!beam_shape_ok(n_beam, vocab, n_out)) return refuse(kErrInvalidArg, fn, kBeamShape);
+    if (finished && (eos < 0 || eos >= vocab))
+        return refuse(kErrInvalidArg, fn, "ended beams need an end token of the vocabulary");
+    bool capturing;
+    GNCX_TRY(begin_call(fn, &capturing));
+    GNCX_TRY(check_buf(fn, logits, "logits", 4));
+    GNCX_TRY(check_buf(fn, scores, "scores", 4));
+    if (finished) GNCX_TRY(check_buf(fn, finished, "finished", 4));
+    GNCX_TRY(check_buf(fn, out_scores, "out_scores", 4));
+    GNCX_TRY(check_buf(fn, out_parents, "out_parents", 4));
+    GNCX_TRY(check_buf(fn, out_tokens, "out_tokens", 4));
+    if (out_finished) GNCX_TRY(check_buf(fn, out_finished, "out_finished", 4));
+    void* ws;
+    GNCX_TRY(pick_workspace(fn, given, given_bytes, beam_workspace_bytes(n_beam, vocab, n_out, device_info().sm_count),
+                            capturing, &ws));
+    return finish(beam_select_launch(logits, scores, finished, n_beam, vocab, eos, n_out, out_scores, out_parents,
+                                     out_tokens, out_finished, ws, stream()));
+}
+
+int32_t gncx_state_reorder(void* state, int32_t n_states, size_t state_stride, int32_t n_slots, size_t slot_stride,
+                           size_t n_bytes, const int32_t* index) {
+    static const char* fn = "gncx_state_reorder";
+    if (n_states < 0 || n_slots < 0 || n_slots > kReorderMaxSlots)
+        return refuse(kErrInvalidArg, fn, "n_states >= 0 and n_slots in 0..256 are needed");
+    if ((state_stride | slot_stride | n_bytes) & 3)
+        return refuse(kErrUnaligned, fn, "strides and sizes must be multiples of 4 bytes");
+    if (n_bytes > (size_t)1 << 36) return refuse(kErrInvalidArg, fn, "a slot holds at most 64 GiB");
+    // the slots of all states must be apart: state by state, or slot by slot
+    if (slot_stride > (size_t)1 << 48 || state_stride > ((size_t)1 << 60) / (size_t)(n_states > 1 ? n_states : 1))
+        return refuse(kErrInvalidArg, fn, "a stride is out of range");
+    const bool by_state = slot_stride >= n_bytes && (n_states <= 1 || state_stride >= (size_t)(n_slots - 1) * slot_stride + n_bytes);
+    const bool by_slot = (n_states <= 1 || state_stride >= n_bytes) && slot_stride >= (size_t)(n_states - 1) * state_stride + n_bytes;
+    bool capturing;
+    GNCX_TRY(begin_call(fn, &capturing));
+    if (n_states == 0 || n_slots < 2 || n_bytes == 0) return finish(kOk);
+    if (!by_state && !by_slot) return refuse(kErrInvalidArg, fn, "the slots overlap");
+    GNCX_TRY(check_buf(fn, state, "state", 4));
+    GNCX_TRY(check_buf(fn, index, "index", 4));
+    return finish(reorder_launch(state, n_states, state_stride, n_slots, slot_stride, n_bytes, index, g_rt.d_err, stream()));
+}
+
 }  // extern "C"

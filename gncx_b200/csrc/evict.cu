@@ -1,0 +1,633 @@
+// evict.cu -- a KV cache held to a budget by accumulated attention weight:
+// the decode attention step that sums the weight each cache row receives, and
+// the eviction of the rows with the least.  No reference counterpart (the
+// reference's cache only grows; its decode step is
+// csrc/gncx_llm_kernels.cpp:1887-1994).
+//
+// Step: for each query head p = softmax(scale q.K), out = p V, and
+// weight[kv][t] += sum of p[t] over the KV head's group.  p[t] is known only
+// when the whole row of scores is, so
+//   * weights_part_kernel streams K and V once (each warp walks batches of
+//     rows through registers, with an online softmax), and leaves the scores
+//     (4 bytes per (head, row) against the 8 hd per (KV head, row) read) and a
+//     {max, sum, o} record per range of rows;
+//   * weights_merge_kernel merges the records and turns the scores into
+//     weights, one CTA per 1024 rows of a KV head, more CTAs for the outputs.
+//
+// Eviction: per KV head the rows are ranked (protected ones first, then by
+// weight, a NaN weight last, equal weights by row), the first n_keep stay.
+// The i-th free row below n_keep takes the i-th row that stays from behind
+// it: rows that are read and rows that are written are disjoint, so the cache
+// is compacted in place, in parallel, and no row moves that need not.
+//   * evict_select_kernel, one CTA per KV head: radix selection of the
+//     n_keep-th key, then the lists of free and of moving rows by prefix sums;
+//   * evict_move_kernel copies the rows.
+#include <cuda_runtime.h>
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+#include "tma.cuh"
+
+namespace gncx {
+
+// ---------------------------------------------------------------- decode step with weight sums
+constexpr int kWsThreads = 256;
+constexpr int kWsWarps = kWsThreads / 32;
+constexpr int kWsRows = 1024;      // rows per CTA of the merge kernel's weight part
+constexpr int kWsMaxParts = 256;
+
+struct WeightsArgs {
+    const float* q;
+    const float* new_k;  // null: the row is in the cache
+    const float* new_v;
+    float* kc;
+    float* vc;
+    int pos, token_pos;
+    int n_heads, n_kv, hd, G;
+    float scale;
+    float* out;
+    float* weight;
+    int32_t* positions;
+    int row_stride;
+    int parts, ppc;      // ranges per KV head, rows per range
+    float* part;         // records [head][parts][hd + 4]
+    float* scores;       // [head][score_ld]
+    size_t score_ld;
+};
+
+// Sum each v[i] over the LPR lanes of a row, NV sums at once (NV, LPR powers
+// of two, NV <= LPR): lane l ends with the total of v[(l % LPR) >> SH].
+template <int NV, int LPR>
+__device__ __forceinline__ float lanes_reduce(float (&v)[NV], int lane) {
+    int off = LPR / 2;
+#pragma unroll
+    for (int n = NV; n > 1; n >>= 1) {
+        const bool up = (lane & off) != 0;
+#pragma unroll
+        for (int i = 0; i < n / 2; ++i) {
+            const float send = up ? v[i] : v[i + n / 2];
+            const float keep = up ? v[i + n / 2] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+        }
+        off >>= 1;
+    }
+    float s = v[0];
+#pragma unroll
+    for (; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    return s;
+}
+
+__host__ __device__ constexpr int ilog2(int n) { return n <= 1 ? 0 : 1 + ilog2(n / 2); }
+
+__device__ __forceinline__ float4 ld_row(const float* p, bool ok) {
+    return ok ? __ldcs(reinterpret_cast<const float4*>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
+    return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c))));
+}
+
+// LPR lanes hold a row (NJ float4 each; columns past hd are zero), 32 / LPR
+// rows side by side in a warp, B rows per lane and batch, GT query heads.
+template <int LPR, int NJ, int GT, int B>
+__global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const WeightsArgs a) {
+    constexpr int SUB = 32 / LPR;
+    constexpr int NV = B * GT;
+    constexpr int SH = ilog2(LPR) - ilog2(NV);
+    constexpr int LG = ilog2(GT);
+    constexpr int RB = B * SUB;  // rows per warp and batch
+    static_assert(NV <= LPR, "one total per lane");
+    extern __shared__ __align__(16) float ost[];  // [warp][GT][hd]
+    __shared__ float wsh[kWsWarps][SUB * NV + GT];
+    __shared__ float mst[kWsWarps][GT], lst[kWsWarps][GT];
+    pdl_launch_dependents();
+    const int part = blockIdx.x, kvh = blockIdx.y, h0 = kvh * a.G + blockIdx.z * GT;
+    const int heads = min(GT, a.G - (int)blockIdx.z * GT);
+    const int len = a.pos + 1;
+    const int p0 = part * a.ppc, p1 = min(len, p0 + a.ppc);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = lane / LPR, lr = lane % LPR;
+    const size_t ps = (size_t)a.n_kv * a.hd;
+    float* kbase = a.kc + (size_t)kvh * a.hd;
+    float* vbase = a.vc + (size_t)kvh * a.hd;
+    bool on[NJ];
+    int col[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        col[j] = 4 * (lr + j * LPR);
+        on[j] = col[j] < a.hd;
+    }
+    float4 q[GT][NJ], o[GT][NJ];
+#pragma unroll
+    for (int g = 0; g < GT; ++g)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            q[g][j] = ld_row(a.q + (size_t)(h0 + min(g, heads - 1)) * a.hd + col[j], on[j]);
+            o[g][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    // the new row: stored by the lanes that read it below (each reads back what it stored itself)
+    if (a.new_k && a.pos >= p0 && a.pos < p1) {
+        const int r = a.pos - p0;
+        if (warp == (r / RB) % kWsWarps && sub == (r % RB) / B) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                if (on[j]) {
+                    const size_t at = (size_t)a.pos * ps + col[j];
+                    *reinterpret_cast<float4*>(kbase + at) = ld_row(a.new_k + (size_t)kvh * a.hd + col[j], true);
+                    *reinterpret_cast<float4*>(vbase + at) = ld_row(a.new_v + (size_t)kvh * a.hd + col[j], true);
+                }
+        }
+    }
+    float m = -INFINITY, l = 0.0f;  // of head ((lane % LPR) >> SH) % GT
+    const int my = lr >> SH;
+    for (int b0 = p0 + warp * RB; b0 < p1; b0 += kWsWarps * RB) {
+        const int r0 = b0 + sub * B;
+        float4 kr[B][NJ], vr[B][NJ];
+#pragma unroll
+        for (int p = 0; p < B; ++p)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const size_t at = (size_t)min(r0 + p, p1 - 1) * ps + col[j];
+                kr[p][j] = ld_row(kbase + at, on[j] && r0 + p < p1);
+                vr[p][j] = ld_row(vbase + at, on[j] && r0 + p < p1);
+            }
+        float v[NV];
+#pragma unroll
+        for (int p = 0; p < B; ++p)
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                float c = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) c = dot4(q[g][j], kr[p][j], c);
+                v[p * GT + g] = c;
+            }
+        float sc = lanes_reduce<NV, LPR>(v, lane) * a.scale;
+        const int mp = my / GT, mg = my % GT;
+        const bool live = r0 + mp < p1;
+        const bool lead = (lr & ((1 << SH) - 1)) == 0;
+        if (live && lead && mg < heads) a.scores[(size_t)(h0 + mg) * a.score_ld + r0 + mp] = sc;
+        if (!live) sc = -INFINITY;
+        float bm = sc;
+#pragma unroll
+        for (int off = 16; off >= (1 << (SH + LG)); off >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, off));
+        const float m_new = fmaxf(m, bm);
+        // a batch holds at least one live row, so m_new > -inf unless its scores are
+        const float e = sc == -INFINITY ? 0.0f : __expf(sc - m_new);
+        const float corr = m == -INFINITY ? 0.0f : __expf(m - m_new);
+        float bs = e;
+#pragma unroll
+        for (int off = 16; off >= (1 << (SH + LG)); off >>= 1) bs += __shfl_xor_sync(0xffffffffu, bs, off);
+        l = fmaf(l, corr, bs);
+        m = m_new;
+        float* wr = wsh[warp];
+        if (lead) wr[sub * NV + my] = e;
+        if (sub == 0 && lead && my < GT) wr[SUB * NV + my] = corr;
+        __syncwarp();
+        float w[NV], cg[GT];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) w[i] = wr[sub * NV + i];
+#pragma unroll
+        for (int g = 0; g < GT; ++g) cg[g] = wr[SUB * NV + g];
+        __syncwarp();
+#pragma unroll
+        for (int g = 0; g < GT; ++g)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                float4 c = o[g][j];
+                c.x *= cg[g]; c.y *= cg[g]; c.z *= cg[g]; c.w *= cg[g];
+#pragma unroll
+                for (int p = 0; p < B; ++p) {
+                    const float ww = w[p * GT + g];
+                    c.x = fmaf(ww, vr[p][j].x, c.x);
+                    c.y = fmaf(ww, vr[p][j].y, c.y);
+                    c.z = fmaf(ww, vr[p][j].z, c.z);
+                    c.w = fmaf(ww, vr[p][j].w, c.w);
+                }
+                o[g][j] = c;
+            }
+    }
+    // the warps' states as one record per head
+    if (sub == 0 && (lr & ((1 << SH) - 1)) == 0 && my < GT) {
+        mst[warp][my] = m;
+        lst[warp][my] = l;
+    }
+#pragma unroll
+    for (int g = 0; g < GT; ++g)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            float4 c = o[g][j];
+#pragma unroll
+            for (int off = 16; off >= LPR; off >>= 1) {
+                c.x += __shfl_xor_sync(0xffffffffu, c.x, off);
+                c.y += __shfl_xor_sync(0xffffffffu, c.y, off);
+                c.z += __shfl_xor_sync(0xffffffffu, c.z, off);
+                c.w += __shfl_xor_sync(0xffffffffu, c.w, off);
+            }
+            if (sub == 0 && on[j]) *reinterpret_cast<float4*>(ost + (size_t)(warp * GT + g) * a.hd + col[j]) = c;
+        }
+    __syncthreads();
+    for (int t = threadIdx.x; t < heads * a.hd; t += kWsThreads) {
+        const int g = t / a.hd, d = t - g * a.hd;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWsWarps; ++w) M = fmaxf(M, mst[w][g]);
+        float L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWsWarps; ++w) {
+            const float f = mst[w][g] == -INFINITY ? 0.0f : __expf(mst[w][g] - M);
+            L = fmaf(lst[w][g], f, L);
+            O = fmaf(ost[(size_t)(w * GT + g) * a.hd + d], f, O);
+        }
+        float* rec = a.part + ((size_t)(h0 + g) * a.parts + part) * (a.hd + 4);
+        rec[4 + d] = O;
+        if (d == 0) {
+            rec[0] = M;
+            rec[1] = L;
+        }
+    }
+}
+
+// Maximum and sum of one head's records; one warp.
+__device__ __forceinline__ void head_max_sum(const WeightsArgs& a, int h, int lane, float& M, float& L) {
+    const float* rec = a.part + (size_t)h * a.parts * (a.hd + 4);
+    M = -INFINITY;
+    L = 0.0f;
+    for (int p = lane; p < a.parts; p += 32) M = fmaxf(M, rec[(size_t)p * (a.hd + 4)]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int p = lane; p < a.parts; p += 32) {
+        const float m = rec[(size_t)p * (a.hd + 4)];
+        if (m != -INFINITY) L = fmaf(rec[(size_t)p * (a.hd + 4) + 1], __expf(m - M), L);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+}
+
+// blockIdx.x < row_ctas: the weights of rows [1024 x, ..) of KV head y;
+// else the output of the group's head x - row_ctas.
+__global__ void __launch_bounds__(kWsThreads) weights_merge_kernel(const WeightsArgs a, int row_ctas) {
+    __shared__ float s_M[kWsWarps], s_inv[kWsWarps];
+    __shared__ float s_f[kWsMaxParts];
+    const int kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
+    if ((int)blockIdx.x >= row_ctas) {
+        const int h = kvh * a.G + (int)blockIdx.x - row_ctas;
+        float M, L;
+        if (warp == 0) {
+            head_max_sum(a, h, lane, M, L);
+            if (lane == 0) {
+                s_M[0] = M;
+                s_inv[0] = 1.0f / L;
+            }
+        }
+        __syncthreads();
+        M = s_M[0];
+        const float* rec = a.part + (size_t)h * a.parts * (a.hd + 4);
+        for (int p = tid; p < a.parts; p += kWsThreads) {
+            const float m = rec[(size_t)p * (a.hd + 4)];
+            s_f[p] = m == -INFINITY ? 0.0f : __expf(m - M);
+        }
+        __syncthreads();
+        for (int d = tid; d < a.hd; d += kWsThreads) {
+            float o = 0.0f;
+#pragma unroll 8
+            for (int p = 0; p < a.parts; ++p) o = fmaf(rec[(size_t)p * (a.hd + 4) + 4 + d], s_f[p], o);
+            a.out[(size_t)h * a.hd + d] = o * s_inv[0];
+        }
+        return;
+    }
+    constexpr int kPer = kWsRows / kWsThreads;
+    const int t0 = blockIdx.x * kWsRows + tid;
+    float w[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) w[i] = 0.0f;
+    for (int g0 = 0; g0 < a.G; g0 += kWsWarps) {
+        __syncthreads();
+        if (g0 + warp < a.G) {
+            float M, L;
+            head_max_sum(a, kvh * a.G + g0 + warp, lane, M, L);
+            if (lane == 0) {
+                s_M[warp] = M;
+                s_inv[warp] = 1.0f / L;
+            }
+        }
+        __syncthreads();
+        for (int g = 0; g < min(kWsWarps, a.G - g0); ++g) {
+            const float* s = a.scores + (size_t)(kvh * a.G + g0 + g) * a.score_ld;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int t = t0 + i * kWsThreads;
+                if (t <= a.pos) w[i] = fmaf(__expf(s[t] - s_M[g]), s_inv[g], w[i]);
+            }
+        }
+    }
+    float* wt = a.weight + (size_t)kvh * a.row_stride;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int t = t0 + i * kWsThreads;
+        if (t > a.pos) continue;
+        const bool fresh = a.new_k && t == a.pos;  // the new row's sum starts here
+        wt[t] = fresh ? w[i] : wt[t] + w[i];
+        if (fresh && a.positions) a.positions[(size_t)kvh * a.row_stride + t] = a.token_pos;
+    }
+}
+
+// Ranges per KV head: about two CTAs per SM, at least 32 rows each.
+static int weights_parts(int len, int n_kv, int zgroups, int sm_count) {
+    int parts = (2 * sm_count + n_kv * zgroups - 1) / (n_kv * zgroups);
+    const int most = (len + 31) / 32;
+    if (parts > most) parts = most;
+    if (parts > kWsMaxParts) parts = kWsMaxParts;
+    return parts < 1 ? 1 : parts;
+}
+static int weights_group(int G) { return G >= 3 ? 4 : G; }  // query heads a CTA serves
+
+size_t weights_workspace_bytes(int pos, int n_heads, int n_kv, int hd, int sm_count) {
+    const int G = n_heads / n_kv, GT = weights_group(G);
+    const int parts = weights_parts(pos + 1, n_kv, (G + GT - 1) / GT, sm_count);
+    const size_t rec = ((size_t)n_heads * parts * (hd + 4) * 4 + 255) / 256 * 256;
+    return rec + (size_t)n_heads * (((size_t)pos + 1 + 31) / 32 * 32) * 4;
+}
+
+template <int LPR, int NJ>
+static cudaError_t launch_weights_part(const WeightsArgs& a, dim3 grid, int GT, cudaStream_t st) {
+    const size_t smem = (size_t)kWsWarps * GT * a.hd * 4;
+    auto go = [&](auto k) {
+        const cudaError_t e = set_smem_limit(k, smem);
+        if (e != cudaSuccess) return e;
+        k<<<grid, kWsThreads, smem, st>>>(a);
+        return cudaGetLastError();
+    };
+    constexpr int B = NJ == 1 ? 4 : 2;
+    switch (GT) {
+        case 1: return go(weights_part_kernel<LPR, NJ, 1, B>);
+        case 2: return go(weights_part_kernel<LPR, NJ, 2, B>);
+        default: return go(weights_part_kernel<LPR, NJ, 4, B>);
+    }
+}
+
+int weights_step_launch(const float* q, const float* new_k, const float* new_v, float* kc, float* vc, int pos,
+                        int token_pos, int n_heads, int n_kv, int hd, float scale, float* out, float* weight,
+                        int32_t* positions, int row_stride, void* ws, cudaStream_t st) {
+    const int G = n_heads / n_kv, GT = weights_group(G), z = (G + GT - 1) / GT, len = pos + 1;
+    WeightsArgs a{};
+    a.q = q;
+    a.new_k = new_k;
+    a.new_v = new_v;
+    a.kc = kc;
+    a.vc = vc;
+    a.pos = pos;
+    a.token_pos = token_pos;
+    a.n_heads = n_heads;
+    a.n_kv = n_kv;
+    a.hd = hd;
+    a.G = G;
+    a.scale = scale;
+    a.out = out;
+    a.weight = weight;
+    a.positions = positions;
+    a.row_stride = row_stride;
+    a.parts = weights_parts(len, n_kv, z, device_info().sm_count);
+    a.ppc = (len + a.parts - 1) / a.parts;
+    a.parts = (len + a.ppc - 1) / a.ppc;
+    a.part = static_cast<float*>(ws);
+    a.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + ((size_t)n_heads * a.parts * (hd + 4) * 4 + 255) / 256 * 256);
+    a.score_ld = ((size_t)len + 31) / 32 * 32;
+    const dim3 grid(a.parts, n_kv, z);
+    const cudaError_t e = hd <= 64    ? launch_weights_part<16, 1>(a, grid, GT, st)
+                          : hd <= 128 ? launch_weights_part<32, 1>(a, grid, GT, st)
+                                      : launch_weights_part<32, 2>(a, grid, GT, st);
+    if (e != cudaSuccess) return kErrCuda;
+    const int row_ctas = (len + kWsRows - 1) / kWsRows;
+    return launch_after(weights_merge_kernel, dim3(row_ctas + G, n_kv), dim3(kWsThreads), 0, st, a, row_ctas) == cudaSuccess
+               ? kOk
+               : kErrCuda;
+}
+
+// ---------------------------------------------------------------- eviction
+constexpr int kEvThreads = 1024;
+constexpr int kEvBins = 2048;
+
+struct EvictArgs {
+    float* kc;
+    float* vc;
+    const float* weight;
+    const int32_t* positions;  // null: nothing is protected
+    int row_stride, n_rows, n_keep, recent_pos, n_kv, hd;
+    float* weight_out;
+    int32_t* positions_out;
+    int out_stride;
+    int32_t* moves;  // per KV head: count, then max_moves free rows, then max_moves moving rows
+    int max_moves;
+    uint32_t* masks;  // per KV head: words of "above the threshold", then of "at the threshold"
+    int words;
+};
+
+// Greater keys stay: protected rows, then the weights in order, NaN last.
+__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, int h, int i) {
+    if (a.positions && a.positions[(size_t)h * a.row_stride + i] >= a.recent_pos) return 0xFFFFFFFFu;
+    const float w = a.weight[(size_t)h * a.row_stride + i];
+    if (w != w) return 0u;
+    const uint32_t u = __float_as_uint(w + 0.0f);  // -0 as +0
+    return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+
+// Exclusive prefix sum of one value per thread over the CTA, and the total.
+__device__ __forceinline__ u_int64_t cta_scan(u_int64_t v, u_int64_t* s_warp, u_int64_t& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    u_int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u_int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        u_int64_t w = lane < nw ? s_warp[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u_int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        s_warp[lane] = w;
+    }
+    __syncthreads();
+    total = s_warp[nw - 1];
+    return x - v + (warp ? s_warp[warp - 1] : 0);
+}
+
+__global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs a) {
+    __shared__ int hist[kEvBins];
+    __shared__ u_int64_t s_warp[32];
+    __shared__ uint32_t s_prefix;
+    __shared__ int s_need;
+    pdl_launch_dependents();
+    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // The n_keep-th largest key by digits of 11, 11 and 10 bits from the top:
+    // each pass counts the keys that share the digits found so far.
+    uint32_t prefix = 0;
+    int need = a.n_keep;  // how many of the keys that share the prefix stay
+    int shift = 32;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int bits = pass < 2 ? 11 : 10;
+        const uint32_t high = shift == 32 ? 0u : ~0u << shift;  // the digits found so far
+        shift -= bits;
+        for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = 0;
+        __syncthreads();
+        for (int base = 0; base < a.n_rows; base += kEvThreads) {
+            const int i = base + tid;
+            const uint32_t k = i < a.n_rows ? evict_key(a, h, i) : 0u;
+            const bool in = i < a.n_rows && (k & high) == prefix;
+            const uint32_t d = (k >> shift) & ((1u << bits) - 1);
+            int same;
+            const unsigned act = __ballot_sync(0xffffffffu, in);
+            if (!in) continue;
+            __match_all_sync(act, d, &same);
+            if (same) {  // rows of equal weight: one addition for the warp
+                if (lane == __ffs(act) - 1) atomicAdd(&hist[d], __popc(act));
+            } else {
+                atomicAdd(&hist[d], 1);
+            }
+        }
+        __syncthreads();
+        // bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t
+        const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
+        const int c1 = hist[b1], c0 = hist[b0];
+        u_int64_t total;
+        const int before = (int)cta_scan((u_int64_t)(c1 + c0), s_warp, total);
+        if (before < need && need <= before + c1) {
+            s_prefix = prefix | (uint32_t)b1 << shift;
+            s_need = need - before;
+        } else if (before + c1 < need && need <= before + c1 + c0) {
+            s_prefix = prefix | (uint32_t)b0 << shift;
+            s_need = need - before - c1;
+        }
+        __syncthreads();
+        prefix = s_prefix;
+        need = s_need;
+        __syncthreads();
+    }
+    // prefix is the n_keep-th largest key; the first `need` rows that have it stay
+    uint32_t* above = a.masks + (size_t)h * 2 * a.words;
+    uint32_t* at = above + a.words;
+    for (int w = warp; w < a.words; w += kEvThreads / 32) {
+        const int i = w * 32 + lane;
+        const uint32_t k = i < a.n_rows ? evict_key(a, h, i) : 0u;
+        const unsigned gt = __ballot_sync(0xffffffffu, i < a.n_rows && k > prefix);
+        const unsigned eq = __ballot_sync(0xffffffffu, i < a.n_rows && k == prefix);
+        if (lane == 0) {
+            above[w] = gt;
+            at[w] = eq;
+        }
+    }
+    if (a.weight_out != a.weight)
+        for (int i = tid; i < a.n_keep; i += kEvThreads)
+            a.weight_out[(size_t)h * a.out_stride + i] = a.weight[(size_t)h * a.row_stride + i];
+    if (a.positions && a.positions_out != a.positions)
+        for (int i = tid; i < a.n_keep; i += kEvThreads)
+            a.positions_out[(size_t)h * a.out_stride + i] = a.positions[(size_t)h * a.row_stride + i];
+    __syncthreads();
+    int32_t* count = a.moves + (size_t)h * (1 + 2 * (size_t)a.max_moves);
+    int32_t* to = count + 1;
+    int32_t* from = to + a.max_moves;
+    int ties = 0, n_to = 0, n_from = 0;  // before this tile of words
+    for (int base = 0; base < a.words; base += kEvThreads) {
+        const int w = base + tid;
+        uint32_t keep = w < a.words ? above[w] : 0u;
+        const uint32_t eq = w < a.words ? at[w] : 0u;
+        u_int64_t total;
+        const int before = ties + (int)cta_scan((u_int64_t)__popc(eq), s_warp, total);
+        ties += (int)total;
+        uint32_t left = eq;
+        for (int r = min(__popc(eq), max(0, need - before)); r > 0; --r) {
+            keep |= left & (0u - left);
+            left &= left - 1;
+        }
+        // rows of this word below n_keep, and rows that exist
+        const int i0 = w * 32;
+        const uint32_t low = i0 >= a.n_keep ? 0u : a.n_keep - i0 >= 32 ? ~0u : (1u << (a.n_keep - i0)) - 1;
+        uint32_t free_bits = w < a.words ? low & ~keep : 0u;
+        uint32_t move_bits = keep & ~low;
+        const u_int64_t mine = (u_int64_t)__popc(free_bits) << 32 | __popc(move_bits);
+        const u_int64_t pre = cta_scan(mine, s_warp, total);
+        int pt = n_to + (int)(pre >> 32), pf = n_from + (int)(uint32_t)pre;
+        n_to += (int)(total >> 32);
+        n_from += (int)(uint32_t)total;
+        for (; free_bits; free_bits &= free_bits - 1) to[pt++] = i0 + __ffs(free_bits) - 1;
+        for (; move_bits; move_bits &= move_bits - 1) from[pf++] = i0 + __ffs(move_bits) - 1;
+    }
+    if (tid == 0) *count = n_to;  // = n_from
+}
+
+constexpr int kEvMoveThreads = 256;
+constexpr int kEvMoveRows = 4;  // rows in flight per warp
+
+__global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const EvictArgs a) {
+    const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    const int32_t* count = a.moves + (size_t)h * (1 + 2 * (size_t)a.max_moves);
+    const int32_t* to = count + 1;
+    const int32_t* from = to + a.max_moves;
+    const int n = *count;
+    const int hd4 = a.hd / 4;
+    const size_t ps = (size_t)a.n_kv * a.hd;
+    for (int i0 = (blockIdx.x * (kEvMoveThreads / 32) + warp) * kEvMoveRows; i0 < n;
+         i0 += gridDim.x * (kEvMoveThreads / 32) * kEvMoveRows) {
+        int f[kEvMoveRows], t[kEvMoveRows];
+#pragma unroll
+        for (int r = 0; r < kEvMoveRows; ++r) {
+            const int i = min(i0 + r, n - 1);
+            f[r] = from[i];
+            t[r] = to[i];
+        }
+        for (int c = lane; c < hd4; c += 32) {
+            float4 k[kEvMoveRows], v[kEvMoveRows];
+#pragma unroll
+            for (int r = 0; r < kEvMoveRows; ++r) {
+                const size_t at = (size_t)f[r] * ps + (size_t)h * a.hd + 4 * c;
+                k[r] = __ldcs(reinterpret_cast<const float4*>(a.kc + at));
+                v[r] = __ldcs(reinterpret_cast<const float4*>(a.vc + at));
+            }
+#pragma unroll
+            for (int r = 0; r < kEvMoveRows; ++r)
+                if (i0 + r < n) {
+                    const size_t at = (size_t)t[r] * ps + (size_t)h * a.hd + 4 * c;
+                    *reinterpret_cast<float4*>(a.kc + at) = k[r];
+                    *reinterpret_cast<float4*>(a.vc + at) = v[r];
+                }
+        }
+        if (lane < kEvMoveRows && i0 + lane < n) {
+            const int ff = from[i0 + lane], tt = to[i0 + lane];
+            a.weight_out[(size_t)h * a.out_stride + tt] = a.weight[(size_t)h * a.row_stride + ff];
+            if (a.positions)
+                a.positions_out[(size_t)h * a.out_stride + tt] = a.positions[(size_t)h * a.row_stride + ff];
+        }
+    }
+}
+
+static int evict_max_moves(int n_rows, int n_keep) { return n_keep < n_rows - n_keep ? n_keep : n_rows - n_keep; }
+
+size_t evict_workspace_bytes(int n_rows, int n_keep, int n_kv) {
+    const size_t moves = ((size_t)n_kv * (1 + 2 * (size_t)evict_max_moves(n_rows, n_keep)) * 4 + 255) / 256 * 256;
+    return moves + (size_t)n_kv * 2 * ((size_t)(n_rows + 31) / 32) * 4;
+}
+
+int evict_launch(float* kc, float* vc, const float* weight, const int32_t* positions, int row_stride, int n_rows,
+                 int n_keep, int recent_pos, int n_kv, int hd, float* weight_out, int32_t* positions_out,
+                 int out_stride, void* ws, cudaStream_t st) {
+    EvictArgs a{kc, vc, weight, positions, row_stride, n_rows, n_keep, recent_pos, n_kv, hd, weight_out, positions_out,
+                out_stride, static_cast<int32_t*>(ws), evict_max_moves(n_rows, n_keep), nullptr, (n_rows + 31) / 32};
+    a.masks = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(ws) +
+                                          ((size_t)n_kv * (1 + 2 * (size_t)a.max_moves) * 4 + 255) / 256 * 256);
+    evict_select_kernel<<<n_kv, kEvThreads, 0, st>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    if (a.max_moves == 0) return kOk;
+    const int per_cta = kEvMoveThreads / 32 * kEvMoveRows;
+    int gx = (a.max_moves + per_cta - 1) / per_cta;
+    const int most = (8 * device_info().sm_count + n_kv - 1) / n_kv;
+    if (gx > most) gx = most;
+    return launch_after(evict_move_kernel, dim3(gx, n_kv), dim3(kEvMoveThreads), 0, st, a) == cudaSuccess ? kOk : kErrCuda;
+}
+
+}  // namespace gncx

@@ -146,6 +146,33 @@ int attention_launch(const float* q, float* kc, float* vc, int32_t pos, int32_t 
                      const float* new_v = nullptr);
 int32_t attention_scratch_records(int32_t pos, int32_t n_heads, int32_t window);
 
+// ---- several candidates, bounded caches (tree.cu, evict.cu, beam.cu) ----
+// Workspaces are 16-byte aligned; their content need not survive or be set.
+constexpr int kTreeMaxTok = 1024;       // drafted nodes per call
+constexpr int kBeamMax = 256;           // beams
+constexpr int kBeamMaxOut = 256;        // candidates kept
+constexpr int kBeamMaxVocab = 1 << 24;  // tokens
+constexpr int kReorderMaxSlots = 256;
+size_t tree_workspace_bytes(int pos0, int n_tok, int n_heads, int n_kv, int hd, int window);
+int tree_launch(const float* q, const float* kc, const float* vc, const int32_t* parents, int pos0, int n_tok,
+                int n_heads, int n_kv, int hd, float scale, int window, float* out, void* ws, int32_t* err,
+                cudaStream_t st);
+size_t weights_workspace_bytes(int pos, int n_heads, int n_kv, int hd, int sm_count);
+// new_k / new_v (both or neither): the row to store at pos, whose weight sum then starts at zero.
+int weights_step_launch(const float* q, const float* new_k, const float* new_v, float* kc, float* vc, int pos,
+                        int token_pos, int n_heads, int n_kv, int hd, float scale, float* out, float* weight,
+                        int32_t* positions, int row_stride, void* ws, cudaStream_t st);
+size_t evict_workspace_bytes(int n_rows, int n_keep, int n_kv);
+int evict_launch(float* kc, float* vc, const float* weight, const int32_t* positions, int row_stride, int n_rows,
+                 int n_keep, int recent_pos, int n_kv, int hd, float* weight_out, int32_t* positions_out,
+                 int out_stride, void* ws, cudaStream_t st);
+size_t beam_workspace_bytes(int n_beam, int vocab, int n_out, int sm_count);
+int beam_select_launch(const float* logits, const float* scores, const int32_t* finished, int n_beam, int vocab,
+                       int eos, int n_out, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                       int32_t* out_finished, void* ws, cudaStream_t st);
+int reorder_launch(void* state, int n_states, size_t state_stride, int n_slots, size_t slot_stride, size_t n_bytes,
+                   const int32_t* index, int32_t* err, cudaStream_t st);
+
 // ---- sampling ----
 // Penalized greedy argmax (lua/gncx_streamer.lua:1229-1273) -> *out_idx.
 int argmax_penalized_launch(const float* logits, int32_t vocab, const int32_t* recent, int32_t n_recent,

@@ -28,4 +28,24 @@ inline cudaError_t launch_k(void (*k)(KArgs...), dim3 grid, dim3 block, size_t s
     return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...);
 }
 
+// Launch `k` as the second kernel of one call: it may begin while its
+// predecessor (launched by the same call, which runs
+// pdl_launch_dependents()) still runs, and calls pdl_wait() before it touches
+// what that predecessor reads or writes.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_after(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...);
+}
+
 }  // namespace gncx

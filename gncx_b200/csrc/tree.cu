@@ -1,0 +1,372 @@
+// tree.cu -- attention of a tree of drafted tokens over the KV cache
+// (verification step of speculative decoding; no reference counterpart: the
+// reference attends with one query per call, csrc/gncx_llm_kernels.cpp:1887-1994).
+//
+// Drafted node i has its K/V row at cache row pos0 + i, its parent at
+// parents[i] < i (-1: the last cached token) and the position
+// pos0 + depth(i).  Its query sees the cached rows 0 .. pos0 - 1 and its
+// ancestors and itself, with a sliding window W only rows whose position is
+// above its own minus W:
+//   o = sum_j softmax_j(scale q.k_j) v_j over those rows.
+//
+// The rows that every node sees are one dense range [lo, pos0) (lo = 0, or with
+// a window the first row that even the deepest possible node, at position
+// pos0 + n_tok - 1, sees).  tree_dense_kernel computes that range split over
+// CTAs, with no mask, and leaves a record {max, sum, o} per (query row,
+// split).  tree_merge_kernel, one CTA per (node, KV head), walks the node's
+// remaining rows one by one -- window rows below lo, then its ancestors, whose
+// list it builds from the parents -- and merges the records.  Rows that a node
+// does not see are never read for it, so what they hold (NaN, infinities,
+// another branch) cannot reach its output.
+#include <cuda_runtime.h>
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+#include "tma.cuh"
+
+namespace gncx {
+
+struct TreeArgs {
+    const float* q;
+    const float* kc;
+    const float* vc;
+    const int32_t* parents;
+    int pos0, n_tok, n_heads, n_kv, hd, G;
+    float scale;
+    int window;
+    int lo;            // the dense range is [lo, pos0)
+    int splits, per;   // its splits, and rows per split
+    int max_splits;    // at least splits; does not shrink when the range grows
+    float* part;       // records [kv head][query row][split] of hd + 4 floats
+    float* out;
+    int32_t* err;
+};
+
+// ---------------------------------------------------------------- dense range, CUDA cores
+constexpr int kTdRows = 32;     // query rows (node, head of the group) per CTA
+constexpr int kTdKeys = 32;     // cache rows per tile
+constexpr int kTdThreads = 256; // 8 threads per query row
+
+static size_t tree_dense_smem(int hd) {
+    return ((size_t)(kTdRows + 2 * kTdKeys) * (hd + 4) + kTdRows * (kTdKeys + 1)) * 4;
+}
+
+__global__ void __launch_bounds__(kTdThreads) tree_dense_kernel(const TreeArgs a) {
+    extern __shared__ __align__(16) float sm[];
+    const int ld = a.hd + 4, hd4 = a.hd / 4;
+    float* qs = sm;
+    float* ks = qs + kTdRows * ld;
+    float* vs = ks + kTdKeys * ld;
+    float* ps = vs + kTdKeys * ld;
+    pdl_launch_dependents();
+    const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTdRows;
+    const int rows = a.n_tok * a.G;
+    const int tid = threadIdx.x, r = tid >> 3, c = tid & 7;
+    const size_t pstride = (size_t)a.n_kv * a.hd;
+    for (int i = tid; i < kTdRows * hd4; i += kTdThreads) {
+        const int rr = i / hd4, x = i - rr * hd4, row = r0 + rr;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row < rows)
+            v = *reinterpret_cast<const float4*>(a.q + ((size_t)(row / a.G) * a.n_heads + kvh * a.G + row % a.G) * a.hd + 4 * x);
+        *reinterpret_cast<float4*>(qs + rr * ld + 4 * x) = v;
+    }
+    const int j0 = a.lo + split * a.per, j1 = min(a.pos0, j0 + a.per);
+    float m = -INFINITY, l = 0.0f;
+    float4 o[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int base = j0; base < j1; base += kTdKeys) {
+        __syncthreads();
+        for (int i = tid; i < kTdKeys * hd4; i += kTdThreads) {
+            const int jj = i / hd4, x = i - jj * hd4;
+            float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+            if (base + jj < j1) {
+                const size_t at = (size_t)(base + jj) * pstride + (size_t)kvh * a.hd + 4 * x;
+                k = *reinterpret_cast<const float4*>(a.kc + at);
+                v = *reinterpret_cast<const float4*>(a.vc + at);
+            }
+            *reinterpret_cast<float4*>(ks + jj * ld + 4 * x) = k;
+            *reinterpret_cast<float4*>(vs + jj * ld + 4 * x) = v;
+        }
+        __syncthreads();
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < hd4; ++x) {
+            const float4 q4 = *reinterpret_cast<const float4*>(qs + r * ld + 4 * x);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 k4 = *reinterpret_cast<const float4*>(ks + (c + 8 * k) * ld + 4 * x);
+                s[k] = fmaf(q4.w, k4.w, fmaf(q4.z, k4.z, fmaf(q4.y, k4.y, fmaf(q4.x, k4.x, s[k]))));
+            }
+        }
+        float bm = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            s[k] = base + c + 8 * k < j1 ? s[k] * a.scale : -INFINITY;
+            bm = fmaxf(bm, s[k]);
+        }
+#pragma unroll
+        for (int x = 4; x > 0; x >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, x));
+        const float m_new = fmaxf(m, bm);
+        const float corr = m == -INFINITY ? 0.0f : __expf(m - m_new);
+        float bs = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float e = s[k] == -INFINITY ? 0.0f : __expf(s[k] - m_new);
+            bs += e;
+            ps[r * (kTdKeys + 1) + c + 8 * k] = e;
+        }
+#pragma unroll
+        for (int x = 4; x > 0; x >>= 1) bs += __shfl_xor_sync(0xffffffffu, bs, x);
+        l = fmaf(l, corr, bs);
+        m = m_new;
+        __syncwarp();  // a row's eight threads are in one warp
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const int col = c + 8 * x;
+            if (col >= hd4) break;
+            float4 acc = o[x];
+            acc.x *= corr; acc.y *= corr; acc.z *= corr; acc.w *= corr;
+            for (int k = 0; k < min(kTdKeys, j1 - base); ++k) {
+                const float p = ps[r * (kTdKeys + 1) + k];
+                const float4 v4 = *reinterpret_cast<const float4*>(vs + k * ld + 4 * col);
+                acc.x = fmaf(p, v4.x, acc.x);
+                acc.y = fmaf(p, v4.y, acc.y);
+                acc.z = fmaf(p, v4.z, acc.z);
+                acc.w = fmaf(p, v4.w, acc.w);
+            }
+            o[x] = acc;
+        }
+        __syncwarp();
+    }
+    if (r0 + r >= rows) return;
+    float* rec = a.part + (((size_t)kvh * rows + r0 + r) * a.splits + split) * (a.hd + 4);
+    if (c == 0) {
+        rec[0] = m;
+        rec[1] = l;
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        const int col = c + 8 * x;
+        if (col < hd4) *reinterpret_cast<float4*>(rec + 4 + 4 * col) = o[x];
+    }
+}
+
+// ---------------------------------------------------------------- ancestors and merge
+constexpr int kTmThreads = 128;
+constexpr int kTmWarps = kTmThreads / 32;
+constexpr int kTmHeads = 4;  // query heads of the group at a time
+
+// NJ float4 columns per lane: head_dim <= 128 * NJ
+template <int NJ>
+__global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a) {
+    extern __shared__ __align__(16) float sm[];
+    float* os = sm;                                             // [warp][kTmHeads][hd]
+    float* fs = os + kTmWarps * kTmHeads * a.hd;                // [kTmHeads][splits]
+    int* up = reinterpret_cast<int*>(fs + kTmHeads * a.splits); // parents, then
+    int* chain = up + a.n_tok;                                  // the path from the node up
+    __shared__ float s_m[kTmWarps][kTmHeads], s_l[kTmWarps][kTmHeads], s_inv[kTmHeads];
+    __shared__ int s_len;
+    const int node = blockIdx.x, kvh = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rows = a.n_tok * a.G, rl = a.hd + 4;
+    for (int i = tid; i <= node; i += kTmThreads) up[i] = a.parents[i];
+    __syncthreads();
+    if (tid == 0) {  // parents are below their children, so the walk ends
+        int n = 0, i = node;
+        while (true) {
+            chain[n++] = i;
+            const int p = up[i];
+            if (p < -1 || p >= i) record_error(a.err, kErrInvalidArg);
+            if (p < 0 || p >= i) break;
+            i = p;
+        }
+        s_len = n;
+    }
+    __syncthreads();
+    const int depth = s_len - 1;                // of this node
+    const int first = a.window > 0 ? max(0, a.pos0 + depth - a.window + 1) : 0;  // lowest position seen
+    const int n_win = max(0, min(a.lo, a.pos0) - first);                     // cached rows below the dense range
+    const int n_anc = min(depth + 1, a.pos0 + depth - first + 1);            // of the path, from the node up
+    const int n_keys = n_win + n_anc;
+    const size_t pstride = (size_t)a.n_kv * a.hd;
+    const float* kb = a.kc + (size_t)kvh * a.hd;
+    const float* vb = a.vc + (size_t)kvh * a.hd;
+    bool waited = false;
+    for (int g0 = 0; g0 < a.G; g0 += kTmHeads) {
+        const int heads = min(kTmHeads, a.G - g0);
+        float4 q[kTmHeads][NJ], o[kTmHeads][NJ];
+        float m[kTmHeads], l[kTmHeads];
+#pragma unroll
+        for (int g = 0; g < kTmHeads; ++g) {
+            m[g] = -INFINITY;
+            l[g] = 0.0f;
+            const float* qp = a.q + ((size_t)node * a.n_heads + kvh * a.G + g0 + min(g, heads - 1)) * a.hd;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int col = 4 * (lane + 32 * j);
+                q[g][j] = col < a.hd ? *reinterpret_cast<const float4*>(qp + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                o[g][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+        for (int x = warp; x < n_keys; x += kTmWarps) {
+            const int row = x < n_win ? first + x : a.pos0 + chain[x - n_win];
+            float4 k[NJ], v[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int col = 4 * (lane + 32 * j);
+                k[j] = v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (col < a.hd) {
+                    k[j] = *reinterpret_cast<const float4*>(kb + (size_t)row * pstride + col);
+                    v[j] = *reinterpret_cast<const float4*>(vb + (size_t)row * pstride + col);
+                }
+            }
+            float s[kTmHeads];
+#pragma unroll
+            for (int g = 0; g < kTmHeads; ++g) {
+                s[g] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    s[g] = fmaf(q[g][j].w, k[j].w, fmaf(q[g][j].z, k[j].z, fmaf(q[g][j].y, k[j].y, fmaf(q[g][j].x, k[j].x, s[g]))));
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1)
+#pragma unroll
+                for (int g = 0; g < kTmHeads; ++g) s[g] += __shfl_xor_sync(0xffffffffu, s[g], w);
+#pragma unroll
+            for (int g = 0; g < kTmHeads; ++g) {
+                const float sc = s[g] * a.scale;
+                const float mn = fmaxf(m[g], sc);
+                const float e = sc == -INFINITY ? 0.0f : __expf(sc - mn);
+                const float corr = m[g] == -INFINITY ? 0.0f : __expf(m[g] - mn);
+                m[g] = mn;
+                l[g] = fmaf(l[g], corr, e);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    o[g][j].x = fmaf(e, v[j].x, o[g][j].x * corr);
+                    o[g][j].y = fmaf(e, v[j].y, o[g][j].y * corr);
+                    o[g][j].z = fmaf(e, v[j].z, o[g][j].z * corr);
+                    o[g][j].w = fmaf(e, v[j].w, o[g][j].w * corr);
+                }
+            }
+        }
+        if (lane == 0)
+#pragma unroll
+            for (int g = 0; g < kTmHeads; ++g) {
+                s_m[warp][g] = m[g];
+                s_l[warp][g] = l[g];
+            }
+#pragma unroll
+        for (int g = 0; g < kTmHeads; ++g)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int col = 4 * (lane + 32 * j);
+                if (col < a.hd) *reinterpret_cast<float4*>(os + (warp * kTmHeads + g) * a.hd + col) = o[g][j];
+            }
+        if (!waited) pdl_wait();  // the dense kernel's records
+        waited = true;
+        __syncthreads();
+        // maximum and sum of head g over the records and the warps' states: warp g
+        if (warp < heads) {
+            const float* rec = a.part + ((size_t)kvh * rows + node * a.G + g0 + warp) * a.splits * rl;
+            float M = lane < kTmWarps ? s_m[lane][warp] : -INFINITY;
+            for (int s = lane; s < a.splits; s += 32) M = fmaxf(M, rec[(size_t)s * rl]);
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+            float L = 0.0f;
+            if (lane < kTmWarps) {
+                const float f = s_m[lane][warp] == -INFINITY ? 0.0f : __expf(s_m[lane][warp] - M);
+                L = s_l[lane][warp] * f;
+                s_m[lane][warp] = f;  // from here on the factor
+            }
+            for (int s = lane; s < a.splits; s += 32) {
+                const float rm = rec[(size_t)s * rl];
+                const float f = rm == -INFINITY ? 0.0f : __expf(rm - M);
+                fs[warp * a.splits + s] = f;
+                L = fmaf(rec[(size_t)s * rl + 1], f, L);
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) L += __shfl_xor_sync(0xffffffffu, L, w);
+            if (lane == 0) s_inv[warp] = 1.0f / L;
+        }
+        __syncthreads();
+        for (int t = tid; t < heads * a.hd; t += kTmThreads) {
+            const int g = t / a.hd, d = t - g * a.hd;
+            const float* rec = a.part + ((size_t)kvh * rows + node * a.G + g0 + g) * a.splits * rl;
+            float acc = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kTmWarps; ++w) acc = fmaf(os[(w * kTmHeads + g) * a.hd + d], s_m[w][g], acc);
+#pragma unroll 8
+            for (int s = 0; s < a.splits; ++s) acc = fmaf(rec[(size_t)s * rl + 4 + d], fs[g * a.splits + s], acc);
+            a.out[((size_t)node * a.n_heads + kvh * a.G + g0 + g) * a.hd + d] = acc * s_inv[g];
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- host
+// First row of the dense range, its splits and rows per split.
+static void tree_geometry(TreeArgs& a, int sm_count) {
+    const int64_t lo = a.window > 0 ? (int64_t)a.pos0 + a.n_tok - a.window : 0;
+    a.lo = lo < 0 ? 0 : lo > a.pos0 ? a.pos0 : (int)lo;
+    const int len = a.pos0 - a.lo;
+    const int tiles = (a.n_tok * a.G + kTdRows - 1) / kTdRows;
+    int want = (int)((2 * (int64_t)sm_count + (int64_t)a.n_kv * tiles - 1) / ((int64_t)a.n_kv * tiles));
+    const int most = (len + kTdKeys - 1) / kTdKeys;
+    if (want > most) want = most;
+    a.splits = a.max_splits = want;
+    a.per = 0;
+    if (want > 0) {
+        a.per = ((len + want - 1) / want + kTdKeys - 1) / kTdKeys * kTdKeys;
+        a.splits = (len + a.per - 1) / a.per;
+    }
+}
+
+static TreeArgs tree_args(int pos0, int n_tok, int n_heads, int n_kv, int hd, int window) {
+    TreeArgs a{};
+    a.pos0 = pos0;
+    a.n_tok = n_tok;
+    a.n_heads = n_heads;
+    a.n_kv = n_kv;
+    a.hd = hd;
+    a.G = n_heads / n_kv;
+    a.window = window;
+    tree_geometry(a, device_info().sm_count);
+    return a;
+}
+
+size_t tree_workspace_bytes(int pos0, int n_tok, int n_heads, int n_kv, int hd, int window) {
+    const TreeArgs a = tree_args(pos0, n_tok, n_heads, n_kv, hd, window);
+    return (size_t)n_heads * n_tok * a.max_splits * (hd + 4) * 4;
+}
+
+int tree_launch(const float* q, const float* kc, const float* vc, const int32_t* parents, int pos0, int n_tok,
+                int n_heads, int n_kv, int hd, float scale, int window, float* out, void* ws, int32_t* err,
+                cudaStream_t st) {
+    TreeArgs a = tree_args(pos0, n_tok, n_heads, n_kv, hd, window);
+    a.q = q;
+    a.kc = kc;
+    a.vc = vc;
+    a.parents = parents;
+    a.scale = scale;
+    a.part = static_cast<float*>(ws);
+    a.out = out;
+    a.err = err;
+    if (a.splits > 0) {
+        const size_t smem = tree_dense_smem(hd);
+        if (set_smem_limit(tree_dense_kernel, smem) != cudaSuccess) return kErrCuda;
+        const int tiles = (n_tok * a.G + kTdRows - 1) / kTdRows;
+        tree_dense_kernel<<<dim3(a.splits, n_kv, tiles), kTdThreads, smem, st>>>(a);
+        if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    }
+    const size_t msm = ((size_t)kTmWarps * kTmHeads * hd + kTmHeads * a.splits + 2 * n_tok) * 4;
+    const dim3 grid(n_tok, n_kv);
+    auto go = [&](auto k) {
+        if (set_smem_limit(k, msm) != cudaSuccess) return kErrCuda;
+        if (a.splits > 0) return launch_after(k, grid, dim3(kTmThreads), msm, st, a) == cudaSuccess ? kOk : kErrCuda;
+        k<<<grid, kTmThreads, msm, st>>>(a);
+        return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+    };
+    return hd <= 128 ? go(tree_merge_kernel<1>) : go(tree_merge_kernel<2>);
+}
+
+}  // namespace gncx

@@ -229,6 +229,100 @@ int32_t gncx_mqa_attention_step_noalloc(const float* q_vec, const float* k_vec, 
                                         void* cuda_stream);
 
 /* ------------------------------------------------------------------------ */
+/* Several candidates over one cache, and caches held to a budget            */
+/* (no reference counterparts)                                               */
+/* ------------------------------------------------------------------------ */
+/* Rules these calls share.  They run on gncx_set_stream's stream, wait in
+ * synchronous mode, and return a status (GNCX_OK or the reason, which
+ * gncx_last_error_message() words).  A refused call has written nothing.
+ * Buffers are memory of the current device (or managed / mapped memory); the
+ * vectors and caches start on 16-byte boundaries, the other arrays on 4-byte
+ * ones.  Caches have the reference layout [row][n_kv][head_dim].  `workspace`
+ * is scratch of at least the _workspace query's bytes (16-byte aligned, no
+ * content kept between calls; the size does not shrink when the position
+ * grows); NULL takes the library's own.  Calls that may run at the same time
+ * (on different streams, or replays of different graphs) need workspaces of
+ * their own.  All can be captured into a CUDA graph, in stream-ordered mode
+ * and with a workspace of the caller's.  What only the GPU sees to be wrong
+ * (a parent or an index out of range) is reported as GNCX_ERR_INVALID_ARG by
+ * the call itself in synchronous mode, else by the next gncx_sync(). */
+
+/* Attention of a tree of n_tok (1..1024) drafted tokens, for the verification
+ * step of speculative decoding.  Node i's K/V row is cache row pos0 + i;
+ * parents[i] (device array) is its parent node, below i, or -1 where it
+ * continues cache row pos0 - 1.  It sits at position pos0 + its depth and sees
+ * cache rows 0 .. pos0 - 1, its ancestors and itself; with sliding_window W > 0
+ * only rows whose position is above its own minus W.  q and out are
+ * [n_tok][n_heads * head_dim].  Rows that a node does not see are not read for
+ * it.  A node with an invalid parent is an error; its output is unspecified.
+ * Split softmax, fp32 accuracy (as gncx_mqa_attention_step_ext's default
+ * mode); gncx_set_exact_attention has no effect.  The accepted path's rows are
+ * brought together with gncx_state_reorder. */
+int32_t gncx_attention_tree(const float* q, const float* k_cache, const float* v_cache, const int32_t* parents,
+                            int32_t pos0, int32_t n_tok, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                            float attn_scale, int32_t sliding_window, float* out, void* workspace,
+                            size_t workspace_bytes);
+size_t gncx_attention_tree_workspace(int32_t pos0, int32_t n_tok, int32_t n_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, int32_t sliding_window);
+
+/* gncx_mqa_attention_step_ext without a window, which also adds the weights it
+ * gave: weight_sum[kv][t] += sum over the KV head's query heads of the softmax
+ * weight of row t, t = 0 .. pos.  weight_sum and positions (may be NULL) are
+ * [n_kv][row_stride].  `pos` is the cache row, `token_pos` the token's position
+ * in the sequence (they differ once rows have been evicted).  With write_kv the
+ * row's K/V come from k_vec / v_vec (device memory), its weight sum starts at
+ * this step's weight and positions[kv][pos] = token_pos. */
+int32_t gncx_mqa_attention_step_weights(const float* q_vec, const float* k_vec, const float* v_vec,
+                                        float* k_cache_layer, float* v_cache_layer, int32_t pos, int32_t token_pos,
+                                        int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, float attn_scale,
+                                        int32_t write_kv, float* out_attn_vec, float* weight_sum, int32_t* positions,
+                                        int32_t row_stride, void* workspace, size_t workspace_bytes);
+size_t gncx_mqa_attention_step_weights_workspace(int32_t pos, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
+
+/* Evicts rows from a cache of n_rows rows, each KV head by itself, so that
+ * n_keep rows are left in rows 0 .. n_keep - 1.  The rows that stay: first
+ * those with positions[kv][row] >= recent_pos, then by weight_sum, greatest
+ * first (NaN counts least), then the lowest row.  The i-th evicted row below
+ * n_keep is overwritten by the i-th row that stays from n_keep on; all others,
+ * and the rows from n_keep on, are left as they were, so rows are not in order
+ * of position afterwards.  weight_out / positions_out [n_kv][out_stride] get the
+ * n_keep rows' sums and positions; they may be the input arrays themselves
+ * (then out_stride = row_stride) but not overlap them otherwise.  positions and
+ * positions_out may both be NULL. */
+int32_t gncx_kv_evict(float* k_cache_layer, float* v_cache_layer, const float* weight_sum, const int32_t* positions,
+                      int32_t row_stride, int32_t n_rows, int32_t n_keep, int32_t recent_pos, int32_t n_kv_heads,
+                      int32_t head_dim, float* weight_out, int32_t* positions_out, int32_t out_stride,
+                      void* workspace, size_t workspace_bytes);
+size_t gncx_kv_evict_workspace(int32_t n_rows, int32_t n_keep, int32_t n_kv_heads);
+
+/* One step of beam search: the n_out (1..256) best continuations of n_beam
+ * (1..256) beams.  Candidate (b, t) scores
+ * scores[b] + logits[b][t] - log sum_t exp(logits[b][t]), in double precision;
+ * a beam with finished[b] != 0 has the one candidate (b, eos) with scores[b]
+ * (finished may be NULL).  Ranked by score, then beam, then logit, then token.
+ * A score of -inf or NaN is no candidate (a beam whose logits hold a NaN or
+ * +inf has none); where candidates run out, score -inf, parent -1, token -1.
+ * logits are [n_beam][vocab].  out_finished (may be NULL): the beam had ended
+ * or the token is eos (eos -1: none).  The outputs may be the arrays scores
+ * and finished. */
+int32_t gncx_beam_select(const float* logits, const float* scores, const int32_t* finished, int32_t n_beam,
+                         int32_t vocab, int32_t eos, int32_t n_out, float* out_scores, int32_t* out_parents,
+                         int32_t* out_tokens, int32_t* out_finished, void* workspace, size_t workspace_bytes);
+size_t gncx_beam_select_workspace(int32_t n_beam, int32_t vocab, int32_t n_out);
+
+/* Reorders per-slot state in place: for every state s < n_states and slot
+ * i < n_slots (up to 256) the n_bytes at state + s * state_stride +
+ * i * slot_stride become what slot index[i] (device array) held; -1 leaves the
+ * slot as it is.  Any mapping, repeats included.  Beam search: slots are beams,
+ * index the parents, states the layers' K and V caches.  Accepting a drafted
+ * path: slots are the drafted cache rows (state = row pos0, slot_stride = the
+ * row's bytes), index[i] the path's i-th node, -1 behind its end.  An index
+ * outside [-1, n_slots) is an error and leaves its slot.  Sizes and strides are
+ * multiples of 4 bytes (of 16, with state 16-byte aligned, for full speed). */
+int32_t gncx_state_reorder(void* state, int32_t n_states, size_t state_stride, int32_t n_slots, size_t slot_stride,
+                           size_t n_bytes, const int32_t* index);
+
+/* ------------------------------------------------------------------------ */
 /* Model engine: the reference orchestrator's decode loop on the GPU         */
 /* ------------------------------------------------------------------------ */
 /* A restatement of GNCXStreamer (lua/gncx_streamer.lua) for callers without
