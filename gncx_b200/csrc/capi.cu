@@ -114,7 +114,9 @@ static int32_t ensure_init() {
     }
     if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
     if (g_rt.device != dev) {
+        const bool synchronous = g_rt.synchronous;  // gncx_set_synchronous may come before the first call
         g_rt = Runtime{};
+        g_rt.synchronous = synchronous;
         g_rt.device = dev;
         if ((e = cudaStreamCreateWithFlags(&g_rt.own, cudaStreamNonBlocking)) != cudaSuccess ||
             (e = cudaMalloc(&g_rt.d_err, sizeof(int32_t))) != cudaSuccess ||

@@ -767,6 +767,33 @@ def test_stream_ordered_calls_in_a_row(gpu):
         assert torch.equal(io[i, 0], want_beam[1]) and torch.equal(io[i, 1], want_beam[2])
 
 
+def test_stream_ordered_mode_set_before_the_first_call():
+    """gncx_set_synchronous(0) as a process's first call holds: a call after it does not wait, and can be captured."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    code = """
+import ctypes, torch
+from gncx_b200 import core
+lib = core.load()
+lib.gncx_set_synchronous(0)
+s = torch.cuda.Stream()
+lib.gncx_set_stream(ctypes.c_void_p(s.cuda_stream))
+x = torch.arange(8, device="cuda").float().view(2, 4)
+i = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    st = lib.gncx_state_reorder(x.data_ptr(), 1, 32, 2, 16, 16, i.data_ptr())
+assert st == 0, lib.gncx_last_error_message()
+g.replay()
+torch.cuda.synchronize()
+assert x.tolist() == [[4, 5, 6, 7], [0, 1, 2, 3]], x
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
 # ---------------------------------------------------------------- runs as they would be used
 def test_speculative_decoding_run(gpu):
     """Draft a tree, verify it, accept a path, go on: outputs and caches of plain sequential decoding."""
