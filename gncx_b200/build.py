@@ -18,7 +18,7 @@ OUT_DIR = HERE / "_build"
 LIB = HERE / "libgncx_llm_core.so"
 
 SOURCES = ["gemv.cu", "matbatch.cu", "matbatch_tc.cu", "attention.cu", "ops.cu", "fused.cu", "capi.cu", "engine.cu", "noalloc.cu", "decode_step.cu",
-           "tp.cu", "tree.cu", "evict.cu", "beam.cu"]
+           "tp.cu", "tree.cu", "tree_tc.cu", "evict.cu", "beam.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -23,24 +23,9 @@
 #include "kernels.h"
 #include "launch.cuh"
 #include "tma.cuh"
+#include "tree.cuh"
 
 namespace gncx {
-
-struct TreeArgs {
-    const float* q;
-    const float* kc;
-    const float* vc;
-    const int32_t* parents;
-    int pos0, n_tok, n_heads, n_kv, hd, G;
-    float scale;
-    int window;
-    int lo;            // the dense range is [lo, pos0)
-    int splits, per;   // its splits, and rows per split
-    int max_splits;    // at least splits; does not shrink when the range grows
-    float* part;       // records [kv head][query row][split] of hd + 4 floats
-    float* out;
-    int32_t* err;
-};
 
 // ---------------------------------------------------------------- dense range, CUDA cores
 constexpr int kTdRows = 32;     // query rows (node, head of the group) per CTA
@@ -101,17 +86,17 @@ __global__ void __launch_bounds__(kTdThreads) tree_dense_kernel(const TreeArgs a
         float bm = -INFINITY;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            s[k] = base + c + 8 * k < j1 ? s[k] * a.scale : -INFINITY;
+            s[k] = base + c + 8 * k < j1 ? s[k] * a.scale2 : -INFINITY;
             bm = fmaxf(bm, s[k]);
         }
 #pragma unroll
         for (int x = 4; x > 0; x >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, x));
         const float m_new = fmaxf(m, bm);
-        const float corr = m == -INFINITY ? 0.0f : __expf(m - m_new);
+        const float corr = m == -INFINITY ? 0.0f : ex2(m - m_new);
         float bs = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float e = s[k] == -INFINITY ? 0.0f : __expf(s[k] - m_new);
+            const float e = s[k] == -INFINITY ? 0.0f : ex2(s[k] - m_new);
             bs += e;
             ps[r * (kTdKeys + 1) + c + 8 * k] = e;
         }
@@ -234,10 +219,10 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a
                 for (int g = 0; g < kTmHeads; ++g) s[g] += __shfl_xor_sync(0xffffffffu, s[g], w);
 #pragma unroll
             for (int g = 0; g < kTmHeads; ++g) {
-                const float sc = s[g] * a.scale;
+                const float sc = s[g] * a.scale2;
                 const float mn = fmaxf(m[g], sc);
-                const float e = sc == -INFINITY ? 0.0f : __expf(sc - mn);
-                const float corr = m[g] == -INFINITY ? 0.0f : __expf(m[g] - mn);
+                const float e = sc == -INFINITY ? 0.0f : ex2(sc - mn);
+                const float corr = m[g] == -INFINITY ? 0.0f : ex2(m[g] - mn);
                 m[g] = mn;
                 l[g] = fmaf(l[g], corr, e);
 #pragma unroll
@@ -274,13 +259,13 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a
             for (int w = 16; w > 0; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
             float L = 0.0f;
             if (lane < kTmWarps) {
-                const float f = s_m[lane][warp] == -INFINITY ? 0.0f : __expf(s_m[lane][warp] - M);
+                const float f = s_m[lane][warp] == -INFINITY ? 0.0f : ex2(s_m[lane][warp] - M);
                 L = s_l[lane][warp] * f;
                 s_m[lane][warp] = f;  // from here on the factor
             }
             for (int s = lane; s < a.splits; s += 32) {
                 const float rm = rec[(size_t)s * rl];
-                const float f = rm == -INFINITY ? 0.0f : __expf(rm - M);
+                const float f = rm == -INFINITY ? 0.0f : ex2(rm - M);
                 fs[warp * a.splits + s] = f;
                 L = fmaf(rec[(size_t)s * rl + 1], f, L);
             }
@@ -309,14 +294,18 @@ static void tree_geometry(TreeArgs& a, int sm_count) {
     const int64_t lo = a.window > 0 ? (int64_t)a.pos0 + a.n_tok - a.window : 0;
     a.lo = lo < 0 ? 0 : lo > a.pos0 ? a.pos0 : (int)lo;
     const int len = a.pos0 - a.lo;
-    const int tiles = (a.n_tok * a.G + kTdRows - 1) / kTdRows;
-    int want = (int)((2 * (int64_t)sm_count + (int64_t)a.n_kv * tiles - 1) / ((int64_t)a.n_kv * tiles));
-    const int most = (len + kTdKeys - 1) / kTdKeys;
+    a.tc = tree_tc_ok(a.hd);
+    const int qrows = a.tc ? kTcTreeRows : kTdRows, keys = a.tc ? kTcTreeKeys : kTdKeys;
+    const int64_t ctas = (int64_t)a.n_kv * ((a.n_tok * a.G + qrows - 1) / qrows);  // per split
+    // CUDA cores: about two CTAs per SM; tensor cores: one per SM, in one wave
+    int want = (int)(a.tc ? sm_count / ctas : (2 * (int64_t)sm_count + ctas - 1) / ctas);
+    if (want < 1) want = 1;
+    const int most = (len + keys - 1) / keys;
     if (want > most) want = most;
     a.splits = a.max_splits = want;
     a.per = 0;
     if (want > 0) {
-        a.per = ((len + want - 1) / want + kTdKeys - 1) / kTdKeys * kTdKeys;
+        a.per = ((len + want - 1) / want + keys - 1) / keys * keys;
         a.splits = (len + a.per - 1) / a.per;
     }
 }
@@ -347,11 +336,13 @@ int tree_launch(const float* q, const float* kc, const float* vc, const int32_t*
     a.kc = kc;
     a.vc = vc;
     a.parents = parents;
-    a.scale = scale;
+    a.scale2 = scale * 1.4426950408889634f;
     a.part = static_cast<float*>(ws);
     a.out = out;
     a.err = err;
-    if (a.splits > 0) {
+    if (a.splits > 0 && a.tc) {
+        if (tree_tc_launch(a, st) != cudaSuccess) return kErrCuda;
+    } else if (a.splits > 0) {
         const size_t smem = tree_dense_smem(hd);
         if (set_smem_limit(tree_dense_kernel, smem) != cudaSuccess) return kErrCuda;
         const int tiles = (n_tok * a.G + kTdRows - 1) / kTdRows;

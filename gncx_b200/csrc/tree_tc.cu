@@ -1,0 +1,517 @@
+// tree_tc.cu -- the dense range of tree attention (tree.cu) on the tcgen05
+// tensor cores, with fp32 accuracy.
+//
+// Every fp32 operand x is used as a pair of fp16 values: with a power of two s
+// that brings the largest |x| of its group into [2^11, 2^15),
+//   hi = fp16(x s),  lo = fp16(x s - hi),
+// so that hi + lo keeps 22 bits of x (or 2^-36 of the group's largest value,
+// where that is more), and a b is the sum of the products hi hi, lo hi and
+// hi lo, each exact in the fp32 accumulator; lo lo (2^-22 of the product) is
+// left out.  bf16 pairs would keep 16 bits, a tf32 pair costs twice the tensor
+// time.  Groups: a query row; 8 cache rows of K; 8 cache rows of V; the
+// softmax numerators need none, they are in (0, 1] and used times 2^14.
+//
+// One CTA takes up to 256 query rows of one KV head as two lanes A and B of
+// 128 and walks its split of the cache in tiles of 64 rows, each K and V row
+// read and split once for both lanes:
+//   * loader warps 8-11 bring 8-row chunks in with bulk copies (four in flight
+//     per warp, 64 KB per SM), split them and write the K-major operand tiles;
+//   * warp 12, one thread, issues S = Q K^T (Q pairs stay in TMEM) and, once a
+//     lane's weights are in TMEM over its scores, O = P V into the shared O
+//     columns, so one lane's softmax runs under the other's products;
+//   * warps 0-3 (A) and 4-7 (B), a thread per query row: online softmax, P
+//     pairs, and the sum of the tiles' O in fp32 registers: a sum over all
+//     tiles in TMEM would add up the tensor core's cut-off bits.
+// Every wait is bounded; on a timeout the kernel records an error and leaves.
+#include <cuda_fp16.h>
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+#include "tree.cuh"
+#include "umma.cuh"
+
+namespace gncx {
+
+constexpr int kTtThreads = 512;
+constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12;
+constexpr int kTtKStride = 64 * 16 + 16;  // bytes between 8-column chunks of the K tile: shifted by a bank group
+constexpr int kTtStages = 2;              // K and V operand tiles
+constexpr int kTtScales = 4;              // tiles whose scales are kept
+// TMEM columns
+constexpr int kTtQ = 0, kTtS = 256, kTtO = 384, kTtCols = 512;
+
+template <int HD>
+struct TtLayout {
+    static constexpr int kK = HD / 8 * kTtKStride;  // one of hi, lo
+    static constexpr int kV = 8 * HD * 16;
+    static constexpr int kStage = 2 * (kK + kV);
+    static constexpr int kChunk = 8 * HD * 4;
+    static constexpr int oStaging = kTtStages * kStage;
+    static constexpr int oScale = oStaging + 16 * kChunk;     // int [kTtScales][2][8]
+    static constexpr int oBar = oScale + kTtScales * 2 * 8 * 4;
+    static constexpr int kBars = 16 + 4 * kTtStages + 2 + 6 + 1;
+    static constexpr int kBytes = oBar + kBars * 8 + 16;
+    // more than half of an SM's shared memory, so one CTA per SM owns all of TMEM
+    static constexpr int kAlloc = kBytes > 120 * 1024 ? kBytes : 120 * 1024;
+};
+
+__device__ __forceinline__ float pow2i(int n) { return __int_as_float((n + 127) << 23); }  // -126 <= n <= 127
+
+// Exponent s with max * 2^s in [2^11, 2^15) for the largest magnitude `max`
+// (its bits), a multiple of 4 up to 124.
+__device__ __forceinline__ int scale_exp(uint32_t bits) {
+    const int s = 14 - ((int)(bits >> 23) - 127);
+    return min(s & ~3, 124);
+}
+
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// Bits of the largest finite magnitude of the warp's values; inf(i) is called
+// for an infinite x[i].
+template <int N, class Inf>
+__device__ __forceinline__ uint32_t warp_max_bits(float (&x)[N], Inf inf) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
+    uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    if (b == 0x7F800000u) {
+        m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (fabsf(x[i]) == INFINITY) inf(i);
+            else m = fmaxf(m, fabsf(x[i]));
+        }
+        b = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    }
+    return b;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a) {
+    using L = TtLayout<HD>;
+    extern __shared__ __align__(128) uint8_t sm[];
+    int* scales = reinterpret_cast<int*>(sm + L::oScale);
+    uint64_t* staged = reinterpret_cast<uint64_t*>(sm + L::oBar);  // [loader warp][4]
+    uint64_t* kfull = staged + 16;
+    uint64_t* kempty = kfull + kTtStages;
+    uint64_t* vfull = kempty + kTtStages;
+    uint64_t* vempty = vfull + kTtStages;
+    uint64_t* sfull = vempty + kTtStages;  // [lane]
+    uint64_t* pfull = sfull + 2;
+    uint64_t* ofull = pfull + 2;
+    uint64_t* oempty = ofull + 2;
+    uint64_t* qfull = oempty + 1;
+    uint64_t* done = qfull + 1;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    // columns of V with an infinity (1: +, 2: -): left out of the products, where
+    // its lo part and a zero weight would make it a NaN, and set in the records
+    __shared__ int infinite[HD];
+    __shared__ int any_infinite;
+
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTcTreeRows;
+    const int rows = a.n_tok * a.G;
+    const int nl = rows - r0 > 128 ? 2 : 1;  // lanes in use
+    const int j0 = a.lo + split * a.per, j1 = min(a.pos0, j0 + a.per);
+    const int n_tiles = (j1 - j0 + kTcTreeKeys - 1) / kTcTreeKeys;
+
+    if (tid == 0) {
+        for (int i = 0; i < 16; ++i) mbar_init(&staged[i], 1);
+        for (int i = 0; i < kTtStages; ++i) {
+            mbar_init(&kfull[i], 4);
+            mbar_init(&kempty[i], 1);
+            mbar_init(&vfull[i], 4);
+            mbar_init(&vempty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sfull[i], 2);
+            mbar_init(&pfull[i], 128);
+            mbar_init(&ofull[i], 1);
+        }
+        mbar_init(oempty, 128);
+        mbar_init(qfull, 128 * nl);
+        mbar_init(done, 1);
+        abort_flag = 0;
+        any_infinite = 0;
+        fence_barrier_init();
+    }
+    if (tid < HD) infinite[tid] = 0;
+    if (warp == kTtMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"(kTtCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    // False once any wait of the CTA ran out; the roles then leave their loops.
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!mbar_wait(bar, parity)) {
+            record_error(a.err, kErrTimeout);
+            *(volatile int*)&abort_flag = 1;
+        }
+        return *(volatile int*)&abort_flag == 0;
+    };
+
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+    if (warp >= kTtMmaWarp) {
+        regs_dec<40>();
+        if (warp == kTtMmaWarp && lane == 0) {
+            // ---------------- products ----------------
+            constexpr uint32_t idesc_s = umma_idesc_f16(128, kTcTreeKeys), idesc_o = umma_idesc_f16(128, HD);
+            const uint32_t sbase = smem_u32(sm);
+            auto scores = [&](int x, int t) {  // S_x = Q_x K(t)^T
+                const uint32_t k = sbase + (t & 1) * L::kStage;
+                const uint64_t hi = umma_desc(k, kTtKStride, 128), lo = umma_desc(k + L::kK, kTtKStride, 128);
+                const uint32_t q = tmem + kTtQ + x * 128, d = tmem + kTtS + x * 64;
+                constexpr uint32_t step = 2 * kTtKStride >> 4;
+#pragma unroll 1
+                for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + HD / 2 + 8 * i, hi + i * step, idesc_s, i > 0);
+#pragma unroll 1
+                for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + 8 * i, lo + i * step, idesc_s, true);
+#pragma unroll 1
+                for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + 8 * i, hi + i * step, idesc_s, true);
+                mbar_arrive(&sfull[x]);  // orders the loaders' scales before the lane's reads
+                umma_commit(&sfull[x]);
+            };
+            auto values = [&](int x, int t) {  // O = P_x V(t)
+                const uint32_t v = sbase + (t & 1) * L::kStage + 2 * L::kK;
+                const uint64_t hi = umma_desc(v, HD * 16, 128), lo = umma_desc(v + L::kV, HD * 16, 128);
+                const uint32_t p = tmem + kTtS + x * 64, d = tmem + kTtO;
+                constexpr uint32_t step = 2 * HD * 16 >> 4;
+                // P's block of 16 rows i: columns 16 i .. + 7 hold the hi parts, + 8 .. + 15 the lo parts
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i + 8, hi + i * step, idesc_o, i > 0);
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i, lo + i * step, idesc_o, true);
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i, hi + i * step, idesc_o, true);
+                umma_commit(&ofull[x]);
+            };
+            bool ok = wait(qfull, 0) && wait(&kfull[0], 0);
+            tc_fence_after();
+            if (ok) {
+                for (int x = 0; x < nl; ++x) scores(x, 0);
+                umma_commit(&kempty[0]);
+            }
+            int n_o = 0;  // products into O so far
+            for (int t = 0; ok && t < n_tiles; ++t)
+                for (int x = 0; ok && x < nl; ++x) {
+                    ok = wait(&pfull[x], t & 1);
+                    if (ok && x == 0) ok = wait(&vfull[t & 1], (t >> 1) & 1);
+                    if (ok && n_o > 0) ok = wait(oempty, (n_o - 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(x, t);
+                    ++n_o;
+                    if (x == nl - 1) umma_commit(&vempty[t & 1]);
+                    if (t + 1 < n_tiles) {
+                        if (x == 0) ok = wait(&kfull[(t + 1) & 1], ((t + 1) >> 1) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(x, t + 1);
+                        if (x == nl - 1) umma_commit(&kempty[(t + 1) & 1]);
+                    }
+                }
+            umma_commit(done);  // nothing of this CTA's is in flight when TMEM is freed
+            if (!mbar_wait(done, 0)) record_error(a.err, kErrTimeout);
+        }
+    } else if (warp >= kTtLoadWarp) {
+        // ---------------- loaders: warp w takes rows 16 w .. 16 w + 15 of each tile ----------------
+        regs_dec<104>();
+        const int lw = warp - kTtLoadWarp;
+        const size_t pstride = (size_t)a.n_kv * a.hd;
+        const float* src[2] = {a.kc + (size_t)kvh * a.hd, a.vc + (size_t)kvh * a.hd};
+        const uint32_t row_bytes = (uint32_t)a.hd * 4;
+        uint8_t* staging = sm + L::oStaging + lw * 4 * L::kChunk;
+        // chunk i of tile t: K rows 0-7, 8-15, V rows 0-7, 8-15 of the warp's 16
+        auto row_of = [&](int t, int i) { return j0 + kTcTreeKeys * t + 16 * lw + 8 * (i & 1); };
+        auto issue = [&](int t, int i) {
+            const int row = row_of(t, i), n = max(0, min(8, j1 - row));
+            uint64_t* bar = &staged[lw * 4 + i];
+            if (lane == 0) {
+                if (n > 0) mbar_arrive_expect_tx(bar, n * row_bytes);
+                else mbar_arrive(bar);
+            }
+            __syncwarp();
+            if (lane < n)
+                bulk_g2s(staging + i * L::kChunk + lane * row_bytes, src[i >> 1] + (size_t)(row + lane) * pstride, row_bytes, bar);
+        };
+        for (int i = 0; i < 4; ++i) issue(0, i);
+        bool ok = true;
+        int t = 0, i = 0;
+        for (; t < n_tiles && ok; ++t) {
+            uint8_t* tile = sm + (t & 1) * L::kStage;
+            int* sc = scales + (t & (kTtScales - 1)) * 16;
+#pragma unroll 1
+            for (i = 0; i < 4; ++i) {
+                ok = wait_warp(&staged[lw * 4 + i], t & 1);
+                if (!ok) break;
+                const float* st = reinterpret_cast<const float*>(staging + i * L::kChunk);
+                const int n = min(8, j1 - row_of(t, i)), chunk = 2 * lw + (i & 1);
+                float x[HD / 4];
+                if (i < 2) {
+                    // K: float4 c of a row per lane
+                    constexpr int LPR = HD / 4, RS = 32 / LPR;
+                    const int c = lane % LPR, sub = lane / LPR;
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const int key = sub + RS * k;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (key < n && 4 * c < a.hd) v = *reinterpret_cast<const float4*>(st + key * a.hd + 4 * c);
+                        x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+                    }
+                    const int s = scale_exp(warp_max_bits(x, [](int) {}));
+                    if (t + 1 < n_tiles) issue(t + 1, i);  // the chunk is in registers
+                    const float f = pow2i(s);
+                    if (i == 0 && t >= kTtStages) ok = wait_warp(&kempty[t & 1], ((t >> 1) - 1) & 1);
+                    if (!ok) break;
+                    uint8_t* d = tile + (c >> 1) * kTtKStride + (8 * chunk + sub) * 16 + (c & 1) * 8;
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        uint2 hi, lo;
+                        split2(x[4 * k] * f, x[4 * k + 1] * f, hi.x, lo.x);
+                        split2(x[4 * k + 2] * f, x[4 * k + 3] * f, hi.y, lo.y);
+                        *reinterpret_cast<uint2*>(d + RS * k * 16) = hi;
+                        *reinterpret_cast<uint2*>(d + L::kK + RS * k * 16) = lo;
+                    }
+                    if (lane == 0) sc[chunk] = s;
+                } else {
+                    // V, transposed: the 8 rows of columns lane, lane + 32, ..
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            x[8 * c + k] = k < n && lane + 32 * c < a.hd ? st[k * a.hd + lane + 32 * c] : 0.0f;
+                    const int s = scale_exp(warp_max_bits(x, [&](int e) {
+                        atomicOr(&infinite[lane + 32 * (e / 8)], x[e] > 0.0f ? 1 : 2);
+                        any_infinite = 1;
+                        x[e] = 0.0f;
+                    }));
+                    if (t + 1 < n_tiles) issue(t + 1, i);
+                    const float f = pow2i(s);
+                    if (i == 2 && t >= kTtStages) ok = wait_warp(&vempty[t & 1], ((t >> 1) - 1) & 1);
+                    if (!ok) break;
+                    uint8_t* d = tile + 2 * L::kK + chunk * HD * 16 + lane * 16;
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint4 hi, lo;
+                        split2(x[8 * c] * f, x[8 * c + 1] * f, hi.x, lo.x);
+                        split2(x[8 * c + 2] * f, x[8 * c + 3] * f, hi.y, lo.y);
+                        split2(x[8 * c + 4] * f, x[8 * c + 5] * f, hi.z, lo.z);
+                        split2(x[8 * c + 6] * f, x[8 * c + 7] * f, hi.w, lo.w);
+                        *reinterpret_cast<uint4*>(d + c * 512) = hi;
+                        *reinterpret_cast<uint4*>(d + L::kV + c * 512) = lo;
+                    }
+                    if (lane == 0) sc[8 + chunk] = s;
+                }
+                if (i & 1) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(i == 1 ? &kfull[t & 1] : &vfull[t & 1]);
+                } else {
+                    fence_async_smem();
+                }
+            }
+        }
+        if (!ok) {
+            // leave no copy of this warp's in flight: wait for the chunks that were issued and not yet awaited
+            --t;
+            for (int k = 0; k < 4; ++k) {
+                mbar_wait(&staged[lw * 4 + k], t & 1);
+                if (k < i + 1 && t + 1 < n_tiles) mbar_wait(&staged[lw * 4 + k], (t + 1) & 1);
+            }
+        }
+    } else if ((warp >> 2) < nl) {
+        // ---------------- softmax and output: a thread per query row ----------------
+        regs_inc<184>();
+        const int x = warp >> 2;
+        const int row = r0 + 128 * x + 32 * (warp & 3) + lane;
+        const bool active = r0 + 128 * x + 32 * (warp & 3) < rows;  // of the warp
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t tq = tmem + lanes + kTtQ + x * 128, ts = tmem + lanes + kTtS + x * 64, to = tmem + lanes + kTtO;
+        int sq = 0;
+        if (active) {
+            const bool some = row < rows;
+            const float* qp = a.q + ((size_t)(some ? row / a.G : 0) * a.n_heads + kvh * a.G + (some ? row % a.G : 0)) * a.hd;
+            float m = 0.0f;
+            for (int c = 0; 4 * c < a.hd; ++c) {
+                const float4 v = *reinterpret_cast<const float4*>(qp + 4 * c);
+                const float w[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) m = fmaxf(m, w[k] < INFINITY ? w[k] : 0.0f);
+            }
+            sq = scale_exp(__float_as_uint(m));
+            const float f = some ? pow2i(sq) : 0.0f;
+#pragma unroll 1
+            for (int b = 0; b < HD / 32; ++b) {
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (some && 32 * b + 4 * c < a.hd) v = *reinterpret_cast<const float4*>(qp + 32 * b + 4 * c);
+                    split2(v.x * f, v.y * f, hi[2 * c], lo[2 * c]);
+                    split2(v.z * f, v.w * f, hi[2 * c + 1], lo[2 * c + 1]);
+                }
+                tmem_st16(tq + 16 * b, hi);
+                tmem_st16(tq + HD / 2 + 16 * b, lo);
+            }
+            tmem_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(qfull);
+
+        float T = -INFINITY, l = 0.0f;
+        float o[HD];
+#pragma unroll
+        for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+        for (int t = 0; t < n_tiles; ++t) {
+            if (!wait_warp(&sfull[x], t & 1)) break;
+            float alpha = 1.0f, beta = 1.0f;
+            if (active) {
+                tc_fence_after();
+                const int4* sc = reinterpret_cast<const int4*>(scales + (t & (kTtScales - 1)) * 16);
+                const int valid = j1 - j0 - kTcTreeKeys * t;
+                const int4 k0 = sc[0], k1 = sc[1];
+                // 2^(-sq - sk) may need two factors
+                auto factor = [&](int sk) {
+                    const int n = -sq - sk, h = n >> 1;
+                    return a.scale2 * pow2i(h) * pow2i(n - h);
+                };
+                const bool even_k = k0.x == k0.y && k0.x == k0.z && k0.x == k0.w && k0.x == k1.x && k0.x == k1.y &&
+                                    k0.x == k1.z && k0.x == k1.w;
+                const float c0 = factor(k0.x);
+                float tm = -INFINITY;
+                if (even_k && valid >= kTcTreeKeys) {
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        float s[32];
+                        tmem_ld32f(ts + 32 * h, s);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) tm = fmaxf(tm, s[j] * c0);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int b = 0; b < 4; ++b) {
+                        float s[16];
+                        tmem_ld16f(ts + 16 * b, s);
+                        const int* sk = reinterpret_cast<const int*>(sc) + 2 * b;
+                        const float ca = factor(sk[0]), cb = factor(sk[1]);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (16 * b + j < valid) tm = fmaxf(tm, s[j] * (j < 8 ? ca : cb));
+                    }
+                }
+                const float Tn = fmaxf(T, tm);
+                const float ref = Tn == -INFINITY ? 0.0f : Tn;
+                alpha = T == -INFINITY ? 0.0f : ex2(T - ref);
+                T = Tn;
+                // V's scales: the products of this tile count in units of its largest rows
+                if (!wait_warp(&vfull[t & 1], (t >> 1) & 1)) break;
+                const int4 v0 = sc[2], v1 = sc[3];
+                const int U = min(min(min(v0.x, v0.y), min(v0.z, v0.w)), min(min(v1.x, v1.y), min(v1.z, v1.w)));
+                const bool even_v = U == max(max(max(v0.x, v0.y), max(v0.z, v0.w)), max(max(v1.x, v1.y), max(v1.z, v1.w)));
+                beta = pow2i(-U);
+                const float shift = 14.0f - ref;
+                float sum = 0.0f;
+                if (even_k && even_v && valid >= kTcTreeKeys) {
+#pragma unroll 1
+                    for (int b = 0; b < 4; ++b) {
+                        float s[16];
+                        uint32_t p[16];
+                        tmem_ld16f(ts + 16 * b, s);
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            const float e0 = ex2(fmaf(s[j], c0, shift)), e1 = ex2(fmaf(s[j + 1], c0, shift));
+                            sum += e0 + e1;
+                            split2(e0, e1, p[j / 2], p[8 + j / 2]);
+                        }
+                        tmem_st16(ts + 16 * b, p);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int b = 0; b < 4; ++b) {
+                        float s[16];
+                        uint32_t p[16];
+                        tmem_ld16f(ts + 16 * b, s);
+                        const int* sk = reinterpret_cast<const int*>(sc) + 2 * b;
+                        const float ca = factor(sk[0]), cb = factor(sk[1]);
+                        const float wa = pow2i(max(-126, U - sk[8])), wb = pow2i(max(-126, U - sk[9]));
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            const float c = j < 8 ? ca : cb, w = j < 8 ? wa : wb;
+                            const float e0 = 16 * b + j < valid ? ex2(fmaf(s[j], c, shift)) : 0.0f;
+                            const float e1 = 16 * b + j + 1 < valid ? ex2(fmaf(s[j + 1], c, shift)) : 0.0f;
+                            sum += e0 + e1;
+                            split2(e0 * w, e1 * w, p[j / 2], p[8 + j / 2]);
+                        }
+                        tmem_st16(ts + 16 * b, p);
+                    }
+                }
+                l = fmaf(l, alpha, sum);
+                tmem_wait_st();
+                tc_fence_before();
+            }
+            mbar_arrive(&pfull[x]);
+            if (!wait_warp(&ofull[x], t & 1)) break;
+            if (active) {
+                tc_fence_after();
+#pragma unroll
+                for (int b = 0; b < HD / 32; ++b) {
+                    float v[32];
+                    tmem_ld32f(to + 32 * b, v);
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) o[32 * b + d] = fmaf(v[d], beta, o[32 * b + d] * alpha);
+                }
+                tc_fence_before();
+            }
+            mbar_arrive(oempty);
+        }
+        if (any_infinite) {
+#pragma unroll
+            for (int d = 0; d < HD; ++d)
+                if (infinite[d]) o[d] += infinite[d] == 1 ? INFINITY : infinite[d] == 2 ? -INFINITY : NAN;
+        }
+        if (row < rows) {
+            float* rec = a.part + (((size_t)kvh * rows + row) * a.splits + split) * (a.hd + 4);
+            const float f = pow2i(-14);
+            *reinterpret_cast<float2*>(rec) = make_float2(T, l * f);
+#pragma unroll
+            for (int d = 0; d < HD; d += 4)
+                if (d < a.hd)
+                    *reinterpret_cast<float4*>(rec + 4 + d) =
+                        make_float4(o[d] * f, o[d + 1] * f, o[d + 2] * f, o[d + 3] * f);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kTtMmaWarp)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTtCols));
+}
+
+bool tree_tc_ok(int hd) { return hd <= 128 && hd % 16 == 0; }
+
+cudaError_t tree_tc_launch(const TreeArgs& a, cudaStream_t st) {
+    const dim3 grid(a.splits, a.n_kv, (a.n_tok * a.G + kTcTreeRows - 1) / kTcTreeRows);
+    auto go = [&](auto k, size_t smem) {
+        const cudaError_t e = set_smem_limit(k, smem);
+        if (e != cudaSuccess) return e;
+        k<<<grid, kTtThreads, smem, st>>>(a);
+        return cudaGetLastError();
+    };
+    return a.hd <= 64 ? go(tree_tc_kernel<64>, TtLayout<64>::kAlloc) : go(tree_tc_kernel<128>, TtLayout<128>::kAlloc);
+}
+
+}  // namespace gncx
