@@ -14,8 +14,8 @@
 // One CTA takes up to 256 query rows of one KV head as two lanes A and B of
 // 128 and walks its split of the cache in tiles of 64 rows, each K and V row
 // read and split once for both lanes:
-//   * loader warps 8-11 bring 8-row chunks in with bulk copies (four in flight
-//     per warp, 64 KB per SM), split them and write the K-major operand tiles;
+//   * loader warps 8-11 bring 8-row chunks in with cp.async (four in flight per
+//     warp, 64 KB per SM), split them and write the K-major operand tiles;
 //   * warp 12, one thread, issues S = Q K^T (Q pairs stay in TMEM) and, once a
 //     lane's weights are in TMEM over its scores, O = P V into the shared O
 //     columns, so one lane's softmax runs under the other's products;
@@ -49,11 +49,15 @@ struct TtLayout {
     static constexpr int oStaging = kTtStages * kStage;
     static constexpr int oScale = oStaging + 16 * kChunk;     // int [kTtScales][2][8]
     static constexpr int oBar = oScale + kTtScales * 2 * 8 * 4;
-    static constexpr int kBars = 16 + 4 * kTtStages + 2 + 6 + 1;
+    static constexpr int kBars = 4 * kTtStages + 2 + 6 + 1;
     static constexpr int kBytes = oBar + kBars * 8 + 16;
     // more than half of an SM's shared memory, so one CTA per SM owns all of TMEM
     static constexpr int kAlloc = kBytes > 120 * 1024 ? kBytes : 120 * 1024;
 };
+
+__device__ __forceinline__ void cp_async16_row(void* smem, const void* gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
+}
 
 __device__ __forceinline__ float pow2i(int n) { return __int_as_float((n + 127) << 23); }  // -126 <= n <= 127
 
@@ -64,10 +68,41 @@ __device__ __forceinline__ int scale_exp(uint32_t bits) {
     return min(s & ~3, 124);
 }
 
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(a, b);
+// A pair of fp32 values in one 64-bit register, and two operations at once on it.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// hi = fp16(x), lo = fp16(x - hi) of two values
+__device__ __forceinline__ void split2(f32x2 x, uint32_t& hi, uint32_t& lo) {
+    const float2 v = unpack2(x);
+    const __half2 h = __floats2half2_rn(v.x, v.y);
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    const float2 r = unpack2(fma2(pack2(f.x, f.y), pack2(-1.0f, -1.0f), x));
+    const __half2 l = __floats2half2_rn(r.x, r.y);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -97,8 +132,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     using L = TtLayout<HD>;
     extern __shared__ __align__(128) uint8_t sm[];
     int* scales = reinterpret_cast<int*>(sm + L::oScale);
-    uint64_t* staged = reinterpret_cast<uint64_t*>(sm + L::oBar);  // [loader warp][4]
-    uint64_t* kfull = staged + 16;
+    uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + L::oBar);
     uint64_t* kempty = kfull + kTtStages;
     uint64_t* vfull = kempty + kTtStages;
     uint64_t* vempty = vfull + kTtStages;
@@ -109,7 +143,6 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     uint64_t* qfull = oempty + 1;
     uint64_t* done = qfull + 1;
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
     // columns of V with an infinity (1: +, 2: -): left out of the products, where
     // its lo part and a zero weight would make it a NaN, and set in the records
     __shared__ int infinite[HD];
@@ -124,7 +157,6 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     const int n_tiles = (j1 - j0 + kTcTreeKeys - 1) / kTcTreeKeys;
 
     if (tid == 0) {
-        for (int i = 0; i < 16; ++i) mbar_init(&staged[i], 1);
         for (int i = 0; i < kTtStages; ++i) {
             mbar_init(&kfull[i], 4);
             mbar_init(&kempty[i], 1);
@@ -139,7 +171,6 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         mbar_init(oempty, 128);
         mbar_init(qfull, 128 * nl);
         mbar_init(done, 1);
-        abort_flag = 0;
         any_infinite = 0;
         fence_barrier_init();
     }
@@ -153,22 +184,18 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
-    // False once any wait of the CTA ran out; the roles then leave their loops.
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!mbar_wait(bar, parity)) {
-            record_error(a.err, kErrTimeout);
-            *(volatile int*)&abort_flag = 1;
-        }
-        return *(volatile int*)&abort_flag == 0;
+    constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's, so they start at 0
+    // False when a wait ran out: the role leaves its loop, and the roles that wait for it run out too.
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+        const bool ok = mbar_wait(bar, parity);
+        if (!ok) record_error(a.err, kErrTimeout);
+        return __all_sync(0xffffffffu, ok) != 0;
     };
 
-    auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-
     if (warp >= kTtMmaWarp) {
-        regs_dec<40>();
-        if (warp == kTtMmaWarp && lane == 0) {
-            // ---------------- products ----------------
+        regs_dec<64>();
+        if (warp == kTtMmaWarp) {
+            // ---------------- products: the warp waits, one thread issues ----------------
             constexpr uint32_t idesc_s = umma_idesc_f16(128, kTcTreeKeys), idesc_o = umma_idesc_f16(128, HD);
             const uint32_t sbase = smem_u32(sm);
             auto scores = [&](int x, int t) {  // S_x = Q_x K(t)^T
@@ -176,14 +203,17 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 const uint64_t hi = umma_desc(k, kTtKStride, 128), lo = umma_desc(k + L::kK, kTtKStride, 128);
                 const uint32_t q = tmem + kTtQ + x * 128, d = tmem + kTtS + x * 64;
                 constexpr uint32_t step = 2 * kTtKStride >> 4;
-#pragma unroll 1
-                for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + HD / 2 + 8 * i, hi + i * step, idesc_s, i > 0);
-#pragma unroll 1
-                for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + 8 * i, lo + i * step, idesc_s, true);
-#pragma unroll 1
-                for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + 8 * i, hi + i * step, idesc_s, true);
-                mbar_arrive(&sfull[x]);  // orders the loaders' scales before the lane's reads
-                umma_commit(&sfull[x]);
+                if (elect_one()) {
+                    mbar_arrive(&sfull[x]);  // orders the loaders' scales before the lane's reads
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + HD / 2 + 8 * i, hi + i * step, idesc_s, i > 0);
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + 8 * i, lo + i * step, idesc_s, true);
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + 8 * i, hi + i * step, idesc_s, true);
+                    umma_commit(&sfull[x]);
+                }
+                __syncwarp();
             };
             auto values = [&](int x, int t) {  // O = P_x V(t)
                 const uint32_t v = sbase + (t & 1) * L::kStage + 2 * L::kK;
@@ -191,98 +221,102 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 const uint32_t p = tmem + kTtS + x * 64, d = tmem + kTtO;
                 constexpr uint32_t step = 2 * HD * 16 >> 4;
                 // P's block of 16 rows i: columns 16 i .. + 7 hold the hi parts, + 8 .. + 15 the lo parts
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i + 8, hi + i * step, idesc_o, i > 0);
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i, lo + i * step, idesc_o, true);
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i, hi + i * step, idesc_o, true);
-                umma_commit(&ofull[x]);
+                if (elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i + 8, hi + i * step, idesc_o, i > 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i, lo + i * step, idesc_o, true);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i, hi + i * step, idesc_o, true);
+                    umma_commit(&ofull[x]);
+                }
+                __syncwarp();
             };
-            bool ok = wait(qfull, 0) && wait(&kfull[0], 0);
+            auto commit = [&](uint64_t* bar) {
+                if (elect_one()) umma_commit(bar);
+                __syncwarp();
+            };
+            bool ok = wait_warp(qfull, 0) && wait_warp(&kfull[0], 0);
             tc_fence_after();
             if (ok) {
                 for (int x = 0; x < nl; ++x) scores(x, 0);
-                umma_commit(&kempty[0]);
+                commit(&kempty[0]);
             }
             int n_o = 0;  // products into O so far
             for (int t = 0; ok && t < n_tiles; ++t)
                 for (int x = 0; ok && x < nl; ++x) {
-                    ok = wait(&pfull[x], t & 1);
-                    if (ok && x == 0) ok = wait(&vfull[t & 1], (t >> 1) & 1);
-                    if (ok && n_o > 0) ok = wait(oempty, (n_o - 1) & 1);
+                    ok = wait_warp(&pfull[x], t & 1);
+                    if (ok && x == 0) ok = wait_warp(&vfull[t & 1], (t >> 1) & 1);
+                    if (ok && n_o > 0) ok = wait_warp(oempty, (n_o - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     values(x, t);
                     ++n_o;
-                    if (x == nl - 1) umma_commit(&vempty[t & 1]);
+                    if (x == nl - 1) commit(&vempty[t & 1]);
                     if (t + 1 < n_tiles) {
-                        if (x == 0) ok = wait(&kfull[(t + 1) & 1], ((t + 1) >> 1) & 1);
+                        if (x == 0) ok = wait_warp(&kfull[(t + 1) & 1], ((t + 1) >> 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
                         scores(x, t + 1);
-                        if (x == nl - 1) umma_commit(&kempty[(t + 1) & 1]);
+                        if (x == nl - 1) commit(&kempty[(t + 1) & 1]);
                     }
                 }
-            umma_commit(done);  // nothing of this CTA's is in flight when TMEM is freed
+            commit(done);  // nothing of this CTA's is in flight when TMEM is freed
             if (!mbar_wait(done, 0)) record_error(a.err, kErrTimeout);
         }
     } else if (warp >= kTtLoadWarp) {
         // ---------------- loaders: warp w takes rows 16 w .. 16 w + 15 of each tile ----------------
-        regs_dec<104>();
+        regs_dec<96>();
         const int lw = warp - kTtLoadWarp;
         const size_t pstride = (size_t)a.n_kv * a.hd;
         const float* src[2] = {a.kc + (size_t)kvh * a.hd, a.vc + (size_t)kvh * a.hd};
-        const uint32_t row_bytes = (uint32_t)a.hd * 4;
         uint8_t* staging = sm + L::oStaging + lw * 4 * L::kChunk;
-        // chunk i of tile t: K rows 0-7, 8-15, V rows 0-7, 8-15 of the warp's 16
+        // chunk i of tile t: K rows 0-7, 8-15, V rows 0-7, 8-15 of the warp's 16;
+        // float4 c of a row per lane, rows sub, sub + RS, ..
+        constexpr int LPR = HD / 4, RS = 32 / LPR;
+        const int c = lane % LPR, sub = lane / LPR;
         auto row_of = [&](int t, int i) { return j0 + kTcTreeKeys * t + 16 * lw + 8 * (i & 1); };
         auto issue = [&](int t, int i) {
-            const int row = row_of(t, i), n = max(0, min(8, j1 - row));
-            uint64_t* bar = &staged[lw * 4 + i];
-            if (lane == 0) {
-                if (n > 0) mbar_arrive_expect_tx(bar, n * row_bytes);
-                else mbar_arrive(bar);
-            }
-            __syncwarp();
-            if (lane < n)
-                bulk_g2s(staging + i * L::kChunk + lane * row_bytes, src[i >> 1] + (size_t)(row + lane) * pstride, row_bytes, bar);
+            const int row = row_of(t, i) + sub;
+            const float* g = src[i >> 1] + (size_t)row * pstride + 4 * c;
+            float* d = reinterpret_cast<float*>(staging + i * L::kChunk) + sub * HD + 4 * c;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+                if (t < n_tiles && row + RS * k < j1 && 4 * c < a.hd) cp_async16_row(d + RS * k * HD, g + (size_t)(RS * k) * pstride);
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
         for (int i = 0; i < 4; ++i) issue(0, i);
         bool ok = true;
-        int t = 0, i = 0;
-        for (; t < n_tiles && ok; ++t) {
+        for (int t = 0; t < n_tiles && ok; ++t) {
             uint8_t* tile = sm + (t & 1) * L::kStage;
             int* sc = scales + (t & (kTtScales - 1)) * 16;
 #pragma unroll 1
-            for (i = 0; i < 4; ++i) {
-                ok = wait_warp(&staged[lw * 4 + i], t & 1);
-                if (!ok) break;
+            for (int i = 0; i < 4; ++i) {
+                asm volatile("cp.async.wait_group 3;" ::: "memory");
+                __syncwarp();
                 const float* st = reinterpret_cast<const float*>(staging + i * L::kChunk);
                 const int n = min(8, j1 - row_of(t, i)), chunk = 2 * lw + (i & 1);
                 float x[HD / 4];
                 if (i < 2) {
                     // K: float4 c of a row per lane
-                    constexpr int LPR = HD / 4, RS = 32 / LPR;
-                    const int c = lane % LPR, sub = lane / LPR;
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
                         const int key = sub + RS * k;
                         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (key < n && 4 * c < a.hd) v = *reinterpret_cast<const float4*>(st + key * a.hd + 4 * c);
+                        if (key < n && 4 * c < a.hd) v = *reinterpret_cast<const float4*>(st + key * HD + 4 * c);
                         x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
                     }
                     const int s = scale_exp(warp_max_bits(x, [](int) {}));
-                    if (t + 1 < n_tiles) issue(t + 1, i);  // the chunk is in registers
-                    const float f = pow2i(s);
+                    issue(t + 1, i);  // the chunk is in registers
+                    const f32x2 f = pack2(pow2i(s), pow2i(s));
                     if (i == 0 && t >= kTtStages) ok = wait_warp(&kempty[t & 1], ((t >> 1) - 1) & 1);
                     if (!ok) break;
                     uint8_t* d = tile + (c >> 1) * kTtKStride + (8 * chunk + sub) * 16 + (c & 1) * 8;
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
                         uint2 hi, lo;
-                        split2(x[4 * k] * f, x[4 * k + 1] * f, hi.x, lo.x);
-                        split2(x[4 * k + 2] * f, x[4 * k + 3] * f, hi.y, lo.y);
+                        split2(mul2(pack2(x[4 * k], x[4 * k + 1]), f), hi.x, lo.x);
+                        split2(mul2(pack2(x[4 * k + 2], x[4 * k + 3]), f), hi.y, lo.y);
                         *reinterpret_cast<uint2*>(d + RS * k * 16) = hi;
                         *reinterpret_cast<uint2*>(d + L::kK + RS * k * 16) = lo;
                     }
@@ -293,24 +327,24 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     for (int c = 0; c < HD / 32; ++c)
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            x[8 * c + k] = k < n && lane + 32 * c < a.hd ? st[k * a.hd + lane + 32 * c] : 0.0f;
+                            x[8 * c + k] = k < n && lane + 32 * c < a.hd ? st[k * HD + lane + 32 * c] : 0.0f;
                     const int s = scale_exp(warp_max_bits(x, [&](int e) {
                         atomicOr(&infinite[lane + 32 * (e / 8)], x[e] > 0.0f ? 1 : 2);
                         any_infinite = 1;
                         x[e] = 0.0f;
                     }));
-                    if (t + 1 < n_tiles) issue(t + 1, i);
-                    const float f = pow2i(s);
+                    issue(t + 1, i);
+                    const f32x2 f = pack2(pow2i(s), pow2i(s));
                     if (i == 2 && t >= kTtStages) ok = wait_warp(&vempty[t & 1], ((t >> 1) - 1) & 1);
                     if (!ok) break;
                     uint8_t* d = tile + 2 * L::kK + chunk * HD * 16 + lane * 16;
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c) {
                         uint4 hi, lo;
-                        split2(x[8 * c] * f, x[8 * c + 1] * f, hi.x, lo.x);
-                        split2(x[8 * c + 2] * f, x[8 * c + 3] * f, hi.y, lo.y);
-                        split2(x[8 * c + 4] * f, x[8 * c + 5] * f, hi.z, lo.z);
-                        split2(x[8 * c + 6] * f, x[8 * c + 7] * f, hi.w, lo.w);
+                        split2(mul2(pack2(x[8 * c], x[8 * c + 1]), f), hi.x, lo.x);
+                        split2(mul2(pack2(x[8 * c + 2], x[8 * c + 3]), f), hi.y, lo.y);
+                        split2(mul2(pack2(x[8 * c + 4], x[8 * c + 5]), f), hi.z, lo.z);
+                        split2(mul2(pack2(x[8 * c + 6], x[8 * c + 7]), f), hi.w, lo.w);
                         *reinterpret_cast<uint4*>(d + c * 512) = hi;
                         *reinterpret_cast<uint4*>(d + L::kV + c * 512) = lo;
                     }
@@ -325,17 +359,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 }
             }
         }
-        if (!ok) {
-            // leave no copy of this warp's in flight: wait for the chunks that were issued and not yet awaited
-            --t;
-            for (int k = 0; k < 4; ++k) {
-                mbar_wait(&staged[lw * 4 + k], t & 1);
-                if (k < i + 1 && t + 1 < n_tiles) mbar_wait(&staged[lw * 4 + k], (t + 1) & 1);
-            }
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if ((warp >> 2) < nl) {
         // ---------------- softmax and output: a thread per query row ----------------
-        regs_inc<184>();
+        regs_inc<176>();
         const int x = warp >> 2;
         const int row = r0 + 128 * x + 32 * (warp & 3) + lane;
         const bool active = r0 + 128 * x + 32 * (warp & 3) < rows;  // of the warp
@@ -361,8 +388,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 for (int c = 0; c < 8; ++c) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (some && 32 * b + 4 * c < a.hd) v = *reinterpret_cast<const float4*>(qp + 32 * b + 4 * c);
-                    split2(v.x * f, v.y * f, hi[2 * c], lo[2 * c]);
-                    split2(v.z * f, v.w * f, hi[2 * c + 1], lo[2 * c + 1]);
+                    split2(pack2(v.x * f, v.y * f), hi[2 * c], lo[2 * c]);
+                    split2(pack2(v.z * f, v.w * f), hi[2 * c + 1], lo[2 * c + 1]);
                 }
                 tmem_st16(tq + 16 * b, hi);
                 tmem_st16(tq + HD / 2 + 16 * b, lo);
@@ -373,9 +400,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         mbar_arrive(qfull);
 
         float T = -INFINITY, l = 0.0f;
-        float o[HD];
+        f32x2 o[HD / 2];
 #pragma unroll
-        for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+        for (int d = 0; d < HD / 2; ++d) o[d] = 0;
         for (int t = 0; t < n_tiles; ++t) {
             if (!wait_warp(&sfull[x], t & 1)) break;
             float alpha = 1.0f, beta = 1.0f;
@@ -393,14 +420,15 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                                     k0.x == k1.z && k0.x == k1.w;
                 const float c0 = factor(k0.x);
                 float tm = -INFINITY;
-                if (even_k && valid >= kTcTreeKeys) {
+                if (even_k && valid >= kTcTreeKeys && c0 >= 0.0f) {
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
                         float s[32];
                         tmem_ld32f(ts + 32 * h, s);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) tm = fmaxf(tm, s[j] * c0);
+                        for (int j = 0; j < 32; j += 2) tm = fmaxf(tm, fmaxf(s[j], s[j + 1]));
                     }
+                    tm *= c0;
                 } else {
 #pragma unroll 1
                     for (int b = 0; b < 4; ++b) {
@@ -424,8 +452,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 const bool even_v = U == max(max(max(v0.x, v0.y), max(v0.z, v0.w)), max(max(v1.x, v1.y), max(v1.z, v1.w)));
                 beta = pow2i(-U);
                 const float shift = 14.0f - ref;
-                float sum = 0.0f;
+                f32x2 sum = 0;
                 if (even_k && even_v && valid >= kTcTreeKeys) {
+                    const f32x2 c02 = pack2(c0, c0), shift2 = pack2(shift, shift);
 #pragma unroll 1
                     for (int b = 0; b < 4; ++b) {
                         float s[16];
@@ -433,9 +462,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                         tmem_ld16f(ts + 16 * b, s);
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
-                            const float e0 = ex2(fmaf(s[j], c0, shift)), e1 = ex2(fmaf(s[j + 1], c0, shift));
-                            sum += e0 + e1;
-                            split2(e0, e1, p[j / 2], p[8 + j / 2]);
+                            const float2 z = unpack2(fma2(pack2(s[j], s[j + 1]), c02, shift2));
+                            const f32x2 e = pack2(ex2(z.x), ex2(z.y));
+                            sum = add2(sum, e);
+                            split2(e, p[j / 2], p[8 + j / 2]);
                         }
                         tmem_st16(ts + 16 * b, p);
                     }
@@ -453,13 +483,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                             const float c = j < 8 ? ca : cb, w = j < 8 ? wa : wb;
                             const float e0 = 16 * b + j < valid ? ex2(fmaf(s[j], c, shift)) : 0.0f;
                             const float e1 = 16 * b + j + 1 < valid ? ex2(fmaf(s[j + 1], c, shift)) : 0.0f;
-                            sum += e0 + e1;
-                            split2(e0 * w, e1 * w, p[j / 2], p[8 + j / 2]);
+                            sum = add2(sum, pack2(e0, e1));
+                            split2(pack2(e0 * w, e1 * w), p[j / 2], p[8 + j / 2]);
                         }
                         tmem_st16(ts + 16 * b, p);
                     }
                 }
-                l = fmaf(l, alpha, sum);
+                const float2 parts = unpack2(sum);
+                l = fmaf(l, alpha, parts.x + parts.y);
                 tmem_wait_st();
                 tc_fence_before();
             }
@@ -467,12 +498,18 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             if (!wait_warp(&ofull[x], t & 1)) break;
             if (active) {
                 tc_fence_after();
+                const f32x2 beta2 = pack2(beta, beta);
+                if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+                    const f32x2 alpha2 = pack2(alpha, alpha);
+#pragma unroll
+                    for (int d = 0; d < HD / 2; ++d) o[d] = mul2(o[d], alpha2);
+                }
 #pragma unroll
                 for (int b = 0; b < HD / 32; ++b) {
                     float v[32];
                     tmem_ld32f(to + 32 * b, v);
 #pragma unroll
-                    for (int d = 0; d < 32; ++d) o[32 * b + d] = fmaf(v[d], beta, o[32 * b + d] * alpha);
+                    for (int d = 0; d < 32; d += 2) o[16 * b + d / 2] = fma2(pack2(v[d], v[d + 1]), beta2, o[16 * b + d / 2]);
                 }
                 tc_fence_before();
             }
@@ -480,8 +517,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         }
         if (any_infinite) {
 #pragma unroll
-            for (int d = 0; d < HD; ++d)
-                if (infinite[d]) o[d] += infinite[d] == 1 ? INFINITY : infinite[d] == 2 ? -INFINITY : NAN;
+            for (int d = 0; d < HD / 2; ++d) {
+                auto of = [&](int c) { return infinite[c] == 0 ? 0.0f : infinite[c] == 1 ? INFINITY : infinite[c] == 2 ? -INFINITY : NAN; };
+                o[d] = add2(o[d], pack2(of(2 * d), of(2 * d + 1)));
+            }
         }
         if (row < rows) {
             float* rec = a.part + (((size_t)kvh * rows + row) * a.splits + split) * (a.hd + 4);
@@ -489,9 +528,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             *reinterpret_cast<float2*>(rec) = make_float2(T, l * f);
 #pragma unroll
             for (int d = 0; d < HD; d += 4)
-                if (d < a.hd)
-                    *reinterpret_cast<float4*>(rec + 4 + d) =
-                        make_float4(o[d] * f, o[d + 1] * f, o[d + 2] * f, o[d + 3] * f);
+                if (d < a.hd) {
+                    const float2 x0 = unpack2(o[d / 2]), x1 = unpack2(o[d / 2 + 1]);
+                    *reinterpret_cast<float4*>(rec + 4 + d) = make_float4(x0.x * f, x0.y * f, x1.x * f, x1.y * f);
+                }
         }
     }
     tc_fence_before();
