@@ -8,8 +8,7 @@
 // where that is more), and a b is the sum of the products hi hi, lo hi and
 // hi lo, each exact in the fp32 accumulator; lo lo (2^-22 of the product) is
 // left out.  bf16 pairs would keep 16 bits, a tf32 pair costs twice the tensor
-// time.  Groups: a query row; 8 cache rows of K; 8 cache rows of V; the
-// softmax numerators need none, they are in (0, 1] and used times 2^14.
+// time.  Groups: a query row; 8 cache rows of K; 8 cache rows of V.
 //
 // One CTA takes up to 256 query rows of one KV head as two lanes A and B of
 // 128 and walks its split of the cache in tiles of 64 rows, each K and V row
@@ -37,6 +36,10 @@ constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12;
 constexpr int kTtKStride = 64 * 16 + 16;  // bytes between 8-column chunks of the K tile: shifted by a bank group
 constexpr int kTtStages = 2;              // K and V operand tiles
 constexpr int kTtScales = 4;              // tiles whose scales are kept
+// Weights are held as 2^(score - reference + kTtShift), with the score at most
+// kTtHead above the reference: up to 2^14 in fp16, and 2^-34 of a weight of 1 is
+// still seen.
+constexpr int kTtShift = 10, kTtHead = 4;
 // TMEM columns
 constexpr int kTtQ = 0, kTtS = 256, kTtO = 384, kTtCols = 512;
 
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's, so they start at 0
     // False when a wait ran out: the role leaves its loop, and the roles that wait for it run out too.
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
-        const bool ok = mbar_wait(bar, parity);
+        const bool ok = mbar_wait_idle(bar, parity);
         if (!ok) record_error(a.err, kErrTimeout);
         return __all_sync(0xffffffffu, ok) != 0;
     };
@@ -280,9 +283,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             const int row = row_of(t, i) + sub;
             const float* g = src[i >> 1] + (size_t)row * pstride + 4 * c;
             float* d = reinterpret_cast<float*>(staging + i * L::kChunk) + sub * HD + 4 * c;
+            if (row_of(t, i) + 8 <= j1 && 4 * c < a.hd) {
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k)
-                if (t < n_tiles && row + RS * k < j1 && 4 * c < a.hd) cp_async16_row(d + RS * k * HD, g + (size_t)(RS * k) * pstride);
+                for (int k = 0; k < HD / 16; ++k) cp_async16_row(d + RS * k * HD, g + (size_t)(RS * k) * pstride);
+            } else {
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k)
+                    if (row + RS * k < j1 && 4 * c < a.hd) cp_async16_row(d + RS * k * HD, g + (size_t)(RS * k) * pstride);
+            }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         for (int i = 0; i < 4; ++i) issue(0, i);
@@ -296,15 +304,19 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 __syncwarp();
                 const float* st = reinterpret_cast<const float*>(staging + i * L::kChunk);
                 const int n = min(8, j1 - row_of(t, i)), chunk = 2 * lw + (i & 1);
+                const bool whole = n == 8 && a.hd == HD;
                 float x[HD / 4];
                 if (i < 2) {
                     // K: float4 c of a row per lane
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
-                        const int key = sub + RS * k;
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (key < n && 4 * c < a.hd) v = *reinterpret_cast<const float4*>(st + key * HD + 4 * c);
+                        const float4 v = *reinterpret_cast<const float4*>(st + (sub + RS * k) * HD + 4 * c);
                         x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+                    }
+                    if (!whole) {  // what the copies did not write
+#pragma unroll
+                        for (int k = 0; k < HD / 4; ++k)
+                            if (sub + RS * (k / 4) >= n || 4 * c >= a.hd) x[k] = 0.0f;
                     }
                     const int s = scale_exp(warp_max_bits(x, [](int) {}));
                     issue(t + 1, i);  // the chunk is in registers
@@ -326,8 +338,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c)
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            x[8 * c + k] = k < n && lane + 32 * c < a.hd ? st[k * HD + lane + 32 * c] : 0.0f;
+                        for (int k = 0; k < 8; ++k) x[8 * c + k] = st[k * HD + lane + 32 * c];
+                    if (!whole) {
+#pragma unroll
+                        for (int k = 0; k < HD / 4; ++k)
+                            if (k % 8 >= n || lane + 32 * (k / 8) >= a.hd) x[k] = 0.0f;
+                    }
                     const int s = scale_exp(warp_max_bits(x, [&](int e) {
                         atomicOr(&infinite[lane + 32 * (e / 8)], x[e] > 0.0f ? 1 : 2);
                         any_infinite = 1;
@@ -441,17 +457,21 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                             if (16 * b + j < valid) tm = fmaxf(tm, s[j] * (j < 8 ? ca : cb));
                     }
                 }
-                const float Tn = fmaxf(T, tm);
-                const float ref = Tn == -INFINITY ? 0.0f : Tn;
-                alpha = T == -INFINITY ? 0.0f : ex2(T - ref);
-                T = Tn;
+                // the reference follows the maximum only when that has grown by more
+                // than kTtHead: a rescaling of o for every new maximum would come in
+                // most tiles of 32 rows
+                if (tm > T + kTtHead || T == -INFINITY) {
+                    alpha = T == -INFINITY ? 0.0f : ex2(T - tm);
+                    T = tm;
+                }
+                const float ref = T == -INFINITY ? 0.0f : T;
                 // V's scales: the products of this tile count in units of its largest rows
                 if (!wait_warp(&vfull[t & 1], (t >> 1) & 1)) break;
                 const int4 v0 = sc[2], v1 = sc[3];
                 const int U = min(min(min(v0.x, v0.y), min(v0.z, v0.w)), min(min(v1.x, v1.y), min(v1.z, v1.w)));
                 const bool even_v = U == max(max(max(v0.x, v0.y), max(v0.z, v0.w)), max(max(v1.x, v1.y), max(v1.z, v1.w)));
                 beta = pow2i(-U);
-                const float shift = 14.0f - ref;
+                const float shift = kTtShift - ref;
                 f32x2 sum = 0;
                 if (even_k && even_v && valid >= kTcTreeKeys) {
                     const f32x2 c02 = pack2(c0, c0), shift2 = pack2(shift, shift);
@@ -524,7 +544,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         }
         if (row < rows) {
             float* rec = a.part + (((size_t)kvh * rows + row) * a.splits + split) * (a.hd + 4);
-            const float f = pow2i(-14);
+            const float f = pow2i(-kTtShift);
             *reinterpret_cast<float2*>(rec) = make_float2(T, l * f);
 #pragma unroll
             for (int d = 0; d < HD; d += 4)

@@ -91,6 +91,26 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
         : "memory");
 }
 
+// mbar_wait for roles that wait beside working warps: the hardware holds the
+// warp for up to 100 us per attempt instead of returning to be asked again.
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t parity) {
+    long long t0 = 0;
+    while (true) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+            : "memory");
+        if (ok) return true;
+        const long long t = clock64();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitCycles) return false;
+    }
+}
+
 // True in one thread of the (converged) warp.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
