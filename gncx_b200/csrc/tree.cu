@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kTdThreads) tree_dense_kernel(const TreeArgs a
 }
 
 // ---------------------------------------------------------------- ancestors and merge
-constexpr int kTmThreads = 128;
+constexpr int kTmThreads = 256;
 constexpr int kTmWarps = kTmThreads / 32;
 constexpr int kTmHeads = 4;  // query heads of the group at a time
 
@@ -274,15 +274,50 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a
             if (lane == 0) s_inv[warp] = 1.0f / L;
         }
         __syncthreads();
-        for (int t = tid; t < heads * a.hd; t += kTmThreads) {
-            const int g = t / a.hd, d = t - g * a.hd;
-            const float* rec = a.part + ((size_t)kvh * rows + node * a.G + g0 + g) * a.splits * rl;
-            float acc = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kTmWarps; ++w) acc = fmaf(os[(w * kTmHeads + g) * a.hd + d], s_m[w][g], acc);
+        // four columns per thread; where there are threads to spare, groups of
+        // them take every groups-th record
+        const int hd4 = a.hd / 4, items = heads * hd4;
+        const int groups = min(8, max(1, kTmThreads / items));  // their sums fit where the states were
+        const int grp = tid / items, it = tid - grp * items;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int g = it / hd4, c = it - g * hd4;
+        if (grp < groups) {
+            const float* rec = a.part + ((size_t)kvh * rows + node * a.G + g0 + g) * a.splits * rl + 4 + 4 * c;
 #pragma unroll 8
-            for (int s = 0; s < a.splits; ++s) acc = fmaf(rec[(size_t)s * rl + 4 + d], fs[g * a.splits + s], acc);
-            a.out[((size_t)node * a.n_heads + kvh * a.G + g0 + g) * a.hd + d] = acc * s_inv[g];
+            for (int s = grp; s < a.splits; s += groups) {
+                const float4 v = *reinterpret_cast<const float4*>(rec + (size_t)s * rl);
+                const float f = fs[g * a.splits + s];
+                acc.x = fmaf(v.x, f, acc.x);
+                acc.y = fmaf(v.y, f, acc.y);
+                acc.z = fmaf(v.z, f, acc.z);
+                acc.w = fmaf(v.w, f, acc.w);
+            }
+            if (grp == 0)
+#pragma unroll
+                for (int w = 0; w < kTmWarps; ++w) {
+                    const float4 v = *reinterpret_cast<const float4*>(os + (w * kTmHeads + g) * a.hd + 4 * c);
+                    const float f = s_m[w][g];
+                    acc.x = fmaf(v.x, f, acc.x);
+                    acc.y = fmaf(v.y, f, acc.y);
+                    acc.z = fmaf(v.z, f, acc.z);
+                    acc.w = fmaf(v.w, f, acc.w);
+                }
+        }
+        __syncthreads();
+        float4* sum = reinterpret_cast<float4*>(os);  // the warps' states are merged
+        if (grp > 0 && grp < groups) sum[tid - items] = acc;
+        __syncthreads();
+        if (grp == 0) {
+            for (int k = 0; k < groups - 1; ++k) {
+                const float4 v = sum[k * items + it];
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+            }
+            const float f = s_inv[g];
+            *reinterpret_cast<float4*>(a.out + ((size_t)node * a.n_heads + kvh * a.G + g0 + g) * a.hd + 4 * c) =
+                make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
         }
         __syncthreads();
     }

@@ -388,25 +388,22 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         if (active) {
             const bool some = row < rows;
             const float* qp = a.q + ((size_t)(some ? row / a.G : 0) * a.n_heads + kvh * a.G + (some ? row % a.G : 0)) * a.hd;
-            float m = 0.0f;
-            for (int c = 0; 4 * c < a.hd; ++c) {
-                const float4 v = *reinterpret_cast<const float4*>(qp + 4 * c);
-                const float w[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+            float v[HD];  // the whole row in flight at once
 #pragma unroll
-                for (int k = 0; k < 4; ++k) m = fmaxf(m, w[k] < INFINITY ? w[k] : 0.0f);
+            for (int c = 0; c < HD / 4; ++c) {
+                const float4 w = some && 4 * c < a.hd ? *reinterpret_cast<const float4*>(qp + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[4 * c] = w.x; v[4 * c + 1] = w.y; v[4 * c + 2] = w.z; v[4 * c + 3] = w.w;
             }
+            float m = 0.0f;
+#pragma unroll
+            for (int c = 0; c < HD; ++c) m = fmaxf(m, fabsf(v[c]) < INFINITY ? fabsf(v[c]) : 0.0f);
             sq = scale_exp(__float_as_uint(m));
-            const float f = some ? pow2i(sq) : 0.0f;
-#pragma unroll 1
+            const f32x2 f = pack2(pow2i(sq), pow2i(sq));
+#pragma unroll
             for (int b = 0; b < HD / 32; ++b) {
                 uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (some && 32 * b + 4 * c < a.hd) v = *reinterpret_cast<const float4*>(qp + 32 * b + 4 * c);
-                    split2(pack2(v.x * f, v.y * f), hi[2 * c], lo[2 * c]);
-                    split2(pack2(v.z * f, v.w * f), hi[2 * c + 1], lo[2 * c + 1]);
-                }
+                for (int c = 0; c < 16; ++c) split2(mul2(pack2(v[32 * b + 2 * c], v[32 * b + 2 * c + 1]), f), hi[c], lo[c]);
                 tmem_st16(tq + 16 * b, hi);
                 tmem_st16(tq + HD / 2 + 16 * b, lo);
             }
