@@ -10,14 +10,14 @@
 // then token, so that the chosen parents and tokens do not depend on how the
 // work was split.
 //   * beam_part_kernel: one CTA per (part of the vocabulary, beam) reads its
-//     logits once.  It keeps sum exp(x - m) per thread (terms and sums in
+//     logits once.  It keeps sum exp(x - ref) per thread (terms and sums in
 //     double: an error of 1e-7 in L_b, as fp32 terms give, could swap two
 //     beams' candidates) and a list of the part's best n_out logits: a
-//     threshold T that at least n_out seen elements reach, first the n_out-th
-//     largest of the threads' maxima, filters what is appended.
-//   * beam_merge_kernel: one CTA forms the L_b, scores the parts' lists rank
-//     by rank (they are sorted, so it stops at a rank at which no list beats
-//     the n_out-th best) and writes the best n_out.
+//     threshold T that at least n_out seen elements reach, at first from the
+//     threads' maxima, filters what is appended.  It writes the list sorted.
+//   * beam_merge_kernel: one CTA forms the L_b and walks the sorted lists, a
+//     thread per list, past a threshold from their first entries, until no
+//     list has an entry that reaches it; then it ranks what it found.
 #include <cuda_runtime.h>
 #include "common.cuh"
 #include "kernels.h"
@@ -72,10 +72,42 @@ __device__ __forceinline__ void bitonic_desc(Key* list, int P) {
 }
 
 struct BeamPart {
-    double sum;  // sum of exp(x - max) over the part
-    float max;
+    double sum;  // sum of exp(x - ref) over the part; NaN when a logit is NaN or +inf
+    float ref;   // about the part's largest logit; -inf: all are
     int pad;
 };
+
+// e^y for y in [-700, 700], off by less than 1e-11 of it: y = n ln2 + r with
+// |r| <= ln2 / 2, and the Taylor polynomial of e^r to r^9 (r^10 / 10! < 7e-12).
+__device__ __forceinline__ double exp_taylor(double y) {
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+    const double t = fma(y, 1.4426950408889634, magic);
+    const double r = fma(t - magic, -0.6931471805599453, y);
+    double p = 1.0 / 362880;
+    p = fma(p, r, 1.0 / 40320);
+    p = fma(p, r, 1.0 / 5040);
+    p = fma(p, r, 1.0 / 720);
+    p = fma(p, r, 1.0 / 120);
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+}
+
+// The k-th largest (k = 1..32) of the warp's values, by a bitonic sort over its lanes.
+__device__ __forceinline__ uint32_t warp_kth(uint32_t v, int k, int lane) {
+#pragma unroll
+    for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+        for (int j = n >> 1; j > 0; j >>= 1) {
+            const uint32_t o = __shfl_xor_sync(0xffffffffu, v, j);
+            const bool up = ((lane & n) == 0) == ((lane & j) == 0);  // this lane keeps the larger
+            v = up ? max(v, o) : min(v, o);
+        }
+    return __shfl_sync(0xffffffffu, v, k - 1);
+}
 
 // Keep the n largest of list[0, cnt) (distinct keys, kBsSort < cnt <=
 // kBsList), in any order: the n-th largest is found bit by bit.  Returns it.
@@ -117,23 +149,25 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
                                                                const int32_t* __restrict__ finished, int vocab,
                                                                int parts, int per, int n, u64* __restrict__ keys,
                                                                BeamPart* __restrict__ stats) {
+    constexpr int kWarps = kBsThreads / 32;
     __shared__ __align__(16) u64 list[kBsList];
     __shared__ int s_cnt;
-    __shared__ float s_m[kBsThreads / 32];
-    __shared__ double s_l[kBsThreads / 32];
+    __shared__ uint32_t s_t[kWarps];
+    __shared__ float s_m[kWarps];
+    __shared__ double s_l[kWarps];
     pdl_launch_dependents();
-    const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (finished && finished[b]) return;  // the merge does not look at an ended beam's lists
     const float* x = logits + (size_t)b * vocab;
     const int i0 = part * per, i1 = min(vocab, i0 + per);
-    float m = -INFINITY;
+    float m = -INFINITY;  // reference of l, at most 64 below the thread's maximum
     double l = 0.0;
+    bool bad = false;
     u64 T = 0;
     if (tid == 0) s_cnt = 0;
     for (int base = i0; base < i1; base += kBsTile) {
         float v[kBsPer];
         float tm = -INFINITY;
-        u64 best = 0;
 #pragma unroll
         for (int j = 0; j < kBsPer; ++j) {
             const int i = base + j * kBsThreads + tid;
@@ -141,64 +175,83 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
         }
 #pragma unroll
         for (int j = 0; j < kBsPer; ++j) tm = fmaxf(tm, v[j]);
-        if (tm > m) {
-            l *= exp((double)m - (double)tm);  // m = -inf: l is 0
+        if (base == i0) {
+            // at least n elements reach T: the (n / kWarps)-th largest of each warp's thread maxima
+            const uint32_t t = warp_kth(tid < i1 - base ? ord32(tm) : 0u, (n + kWarps - 1) / kWarps, lane);
+            if (lane == 0) s_t[warp] = t;
+            __syncthreads();
+            uint32_t low = s_t[0];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) low = min(low, s_t[w]);
+            T = (u64)low << 32;
+        }
+        if (ord32(tm) >= (uint32_t)(T >> 32)) {
+#pragma unroll
+            for (int j = 0; j < kBsPer; ++j) {
+                const int i = base + j * kBsThreads + tid;
+                const u64 k = (u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)i);
+                if (k >= T && i < i1) list[atomicAdd(&s_cnt, 1)] = k;
+            }
+        }
+        if (tm > m + 64.0f || m == -INFINITY) {
+            l *= tm - m < 700.0f ? exp_taylor((double)m - (double)tm) : 0.0;  // m = -inf: l is 0
             m = tm;
         }
 #pragma unroll
-        for (int j = 0; j < kBsPer; ++j)
-            l += v[j] == -INFINITY ? 0.0 : exp((double)v[j] - (double)m);
-        auto key = [&](int j) {
-            const int i = base + j * kBsThreads + tid;
-            return i < i1 ? (u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)i) : 0ull;
-        };
-        if (base == i0) {
-#pragma unroll
-            for (int j = 0; j < kBsPer; ++j) {
-                const u64 k = key(j);
-                best = k > best ? k : best;
-            }
-            list[tid] = best;
-            bitonic_desc(list, kBsThreads);
-            T = list[n - 1];  // n <= kBsThreads
-            __syncthreads();
-        }
-#pragma unroll
         for (int j = 0; j < kBsPer; ++j) {
-            const u64 k = key(j);
-            if (k >= T && k != 0) list[atomicAdd(&s_cnt, 1)] = k;
+            bad |= !(v[j] < INFINITY);
+            if (v[j] - m > -700.0f) l += exp_taylor((double)v[j] - (double)m);
         }
         __syncthreads();
         const int cnt = s_cnt;
         __syncthreads();
         if (cnt > kBsSort) T = beam_keep_n(list, &s_cnt, cnt, n);
     }
-    __syncthreads();
-    const int cnt = s_cnt;
-    int P = kBsThreads;
-    while (P < cnt) P <<= 1;
-    for (int i = cnt + tid; i < P; i += kBsThreads) list[i] = 0;
-    bitonic_desc(list, P);
-    u64* out = keys + ((size_t)b * parts + part) * n;
-    for (int i = tid; i < n; i += kBsThreads) out[i] = list[i];
     // the threads' (m, l) as one
     float M = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (m != -INFINITY) l *= exp((double)m - (double)M);
+    if (bad) l = NAN;
+    else l = m - M > -700.0f ? l * exp_taylor((double)m - (double)M) : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if ((tid & 31) == 0) {
-        s_m[tid >> 5] = M;
-        s_l[tid >> 5] = l;
+    if (lane == 0) {
+        s_m[warp] = M;
+        s_l[warp] = l;
     }
     __syncthreads();
+    const int cnt = s_cnt;
+    u64* out = keys + ((size_t)b * parts + part) * n;
+    if (cnt <= 2 * kBsThreads) {  // place by the number of larger keys
+        const u64 k0 = tid < cnt ? list[tid] : 0, k1 = tid + kBsThreads < cnt ? list[tid + kBsThreads] : 0;
+        int r0 = 0, r1 = 0;
+        if (32 * warp < cnt)
+#pragma unroll 4
+            for (int i = 0; i < cnt; ++i) {
+                const u64 k = list[i];
+                r0 += k > k0;
+                r1 += k > k1;
+            }
+        if (k0 && r0 < n) out[r0] = k0;
+        if (k1 && r1 < n) out[r1] = k1;
+    } else {
+        int P = kBsThreads;
+        while (P < cnt) P <<= 1;
+        for (int i = cnt + tid; i < P; i += kBsThreads) list[i] = 0;
+        bitonic_desc(list, P);
+        for (int i = tid; i < n; i += kBsThreads) out[i] = list[i];
+    }
+    for (int i = cnt + tid; i < n; i += kBsThreads) out[i] = 0;
     if (tid == 0) {
         float mm = -INFINITY;
-        for (int w = 0; w < kBsThreads / 32; ++w) mm = fmaxf(mm, s_m[w]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w]);
         double ll = 0.0;
-        for (int w = 0; w < kBsThreads / 32; ++w)
-            ll += s_m[w] == -INFINITY ? s_l[w] : s_l[w] * exp((double)s_m[w] - (double)mm);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const double f = s_m[w] - mm > -700.0f ? exp_taylor((double)s_m[w] - (double)mm) : 0.0;
+            ll += s_l[w] == s_l[w] ? s_l[w] * f : s_l[w];  // a NaN stays
+        }
         stats[(size_t)b * parts + part] = BeamPart{ll, mm, 0};
     }
 }
@@ -209,90 +262,138 @@ struct BeamKey {
     __device__ bool operator<(const BeamKey& o) const { return hi < o.hi || (hi == o.hi && lo < o.lo); }
 };
 
+// The candidate that entry e (0: none) of beam b's list stands for.
+__device__ __forceinline__ BeamKey beam_key(u64 e, int b, double score, double lse) {
+    const uint32_t o = (uint32_t)(e >> 32), token = 0xFFFFFFFFu - (uint32_t)e;
+    const double s = score + ((double)unord32(o) - lse);
+    return BeamKey{e && s > -INFINITY ? ord64(s) : 0, ~((u64)b << 56 | (u64)~o << 24 | token)};
+}
+
 __global__ void __launch_bounds__(kBmThreads) beam_merge_kernel(
     const u64* __restrict__ keys, const BeamPart* __restrict__ stats, const float* scores, const int32_t* finished,
     int n_beam, int parts, int n, int eos, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
     int32_t* out_finished) {
     __shared__ __align__(16) BeamKey list[kBmList];
-    __shared__ double s_lse[kBeamMax];
-    __shared__ int s_cnt;
+    __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
+    __shared__ u64 s_T;
+    __shared__ int s_cnt, s_live;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) s_cnt = s_live = 0, s_T = 0;
+    __syncthreads();
+    // the beams' scores; NaN for a beam without lists (ended, or no candidate can be better than none)
+    for (int b = tid; b < n_beam; b += kBmThreads) {
+        const float s = scores[b];
+        const bool live = !(finished && finished[b]) && s > -INFINITY;
+        s_score[b] = live ? (double)s : NAN;
+        if (live) atomicAdd(&s_live, 1);
+        else if (s > -INFINITY) list[atomicAdd(&s_cnt, 1)] = BeamKey{ord64((double)s), ~((u64)b << 56 | (u64)eos)};
+    }
     pdl_wait();
-    for (int b = warp; b < n_beam; b += kBmThreads / 32) {
-        if (finished && finished[b]) continue;
+    __syncthreads();
+    // a thread per list; the first entries of all lists are on their way while the beams' sums are formed
+    const int lists = n_beam * parts;  // < kBmThreads
+    const int b = min(tid / parts, n_beam - 1);
+    const bool has = tid < lists && s_score[b] == s_score[b];
+    const u64* mine = keys + (size_t)tid * n;
+    u64 next = has ? mine[0] : 0;
+    for (int w = warp; w < n_beam; w += kBmThreads / 32) {
+        if (s_score[w] != s_score[w]) continue;
+        const BeamPart* st = stats + (size_t)w * parts;
         float M = -INFINITY;
-        for (int p = lane; p < parts; p += 32) M = fmaxf(M, stats[(size_t)b * parts + p].max);
+        for (int p = lane; p < parts; p += 32) M = fmaxf(M, st[p].ref);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         double l = 0.0;
         for (int p = lane; p < parts; p += 32) {
-            const BeamPart s = stats[(size_t)b * parts + p];
-            l += s.max == -INFINITY ? s.sum : s.sum * exp((double)s.max - (double)M);
+            const BeamPart s = st[p];
+            const double f = s.ref - M > -700.0f ? exp_taylor((double)s.ref - (double)M) : 0.0;
+            l += s.sum == s.sum ? s.sum * f : s.sum;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) s_lse[b] = (double)M + log(l);
+        if (lane == 0) s_lse[w] = (double)M + log(l);
     }
-    if (tid == 0) s_cnt = 0;
     __syncthreads();
-    const int lists = n_beam * parts;
-    BeamKey T{0, 0};
-    for (int base = 0; base < lists * n; base += kBmThreads) {
-        const int c = base + tid;
-        BeamKey k{0, 0};
-        if (c < lists * n) {
-            const int r = c / lists, li = c - r * lists, b = li / parts;
-            if (finished && finished[b]) {
-                if (r == 0 && li == b * parts) {
-                    const double s = (double)scores[b];
-                    k.hi = s > -INFINITY ? ord64(s) : 0;  // false for NaN
-                    k.lo = ~((u64)b << 56 | (u64)eos);
-                }
-            } else {
-                const u64 e = keys[(size_t)li * n + r];
-                if (e) {
-                    const uint32_t o = (uint32_t)(e >> 32);
-                    const uint32_t token = 0xFFFFFFFFu - (uint32_t)e;
-                    const double s = (double)scores[b] + ((double)unord32(o) - s_lse[b]);
-                    k.hi = s > -INFINITY ? ord64(s) : 0;
-                    k.lo = ~((u64)b << 56 | (u64)~o << 24 | token);
-                }
+    const double score = s_score[b], lse = has ? s_lse[b] : 0.0;
+    // T: a score that n candidates reach, the n-th best of the lists' first R entries (and the ended beams)
+    const int R = min(n, (n + max(1, s_live * parts) - 1) / max(1, s_live * parts));
+    int r = 0;  // entries of this thread's list that are in the list of candidates
+    bool more = has;
+    for (; r < R; ++r) {
+        const BeamKey k = beam_key(next, b, score, lse);
+        more = more && k.hi != 0;  // the list is sorted: nothing follows an entry that is no candidate
+        if (more) list[atomicAdd(&s_cnt, 1)] = k;
+        next = more && r + 1 < n ? mine[r + 1] : 0;
+    }
+    __syncthreads();
+    int cnt = s_cnt;  // <= n_beam + live lists + n
+    if (cnt > n) {
+        for (int i = tid; i < cnt; i += kBmThreads) {
+            const u64 mineh = list[i].hi;
+            int above = 0, ties = 0;
+#pragma unroll 4
+            for (int j = 0; j < cnt; ++j) {
+                above += list[j].hi > mineh;
+                ties += list[j].hi == mineh;
             }
+            if (above < n && n <= above + ties) s_T = mineh;
         }
-        const bool better = k.hi != 0 && T < k;
-        if (better) list[atomicAdd(&s_cnt, 1)] = k;
-        const bool any = __syncthreads_or(better);
-        const int cnt = s_cnt;
         __syncthreads();
-        if (!any && lists <= kBmThreads) break;  // every list's next entry lost, so all later ones do
-        if ((T.hi == 0 && cnt >= n) || cnt > kBmList - kBmThreads) {
-            int P = kBmThreads / 4;
-            while (P < cnt) P <<= 1;
-            for (int i = cnt + tid; i < P; i += kBmThreads) list[i] = BeamKey{0, 0};
-            bitonic_desc(list, P);
+    }
+    BeamKey T{s_T, 0};
+    // the rest, an entry per list and round, until no list has one that reaches T
+    for (; r < n; ++r) {
+        const BeamKey k = beam_key(next, b, score, lse);
+        more = more && k.hi != 0 && !(k < T);
+        if (more) list[atomicAdd(&s_cnt, 1)] = k;
+        next = more && r + 1 < n ? mine[r + 1] : 0;
+        if (!__syncthreads_or(more)) break;
+        cnt = s_cnt;
+        __syncthreads();
+        if (cnt > kBmList - kBmThreads) {
+            for (int i = cnt + tid; i < kBmList; i += kBmThreads) list[i] = BeamKey{0, 0};
+            bitonic_desc(list, kBmList);
             T = list[n - 1];
-            if (tid == 0) s_cnt = n;  // cnt >= n: n <= kBmList - kBmThreads
+            if (tid == 0) s_cnt = n;
             __syncthreads();
         }
     }
     __syncthreads();
-    const int cnt = s_cnt;
-    int P = kBmThreads / 4;
-    while (P < cnt) P <<= 1;
-    for (int i = cnt + tid; i < P; i += kBmThreads) list[i] = BeamKey{0, 0};
-    bitonic_desc(list, P);
-    const BeamKey k = list[tid < n ? tid : 0];
-    const u64 id = ~k.lo;
-    const bool some = tid < n && k.hi != 0;
-    const int b = some ? (int)(id >> 56) : -1;
+    cnt = s_cnt;
+    BeamKey best{0, 0};  // the tid-th best
+    if (cnt <= 384) {
+        // place by the number of better ones
+        BeamKey k{0, 0};
+        int rank = kBmThreads;
+        if (32 * warp < cnt) {
+            k = tid < cnt ? list[tid] : k;
+            int better = 0;
+#pragma unroll 4
+            for (int j = 0; j < cnt; ++j) better += k < list[j];
+            if (tid < cnt) rank = better;
+        }
+        __syncthreads();
+        if (rank < n) list[rank] = k;
+        __syncthreads();
+        if (tid < min(cnt, n)) best = list[tid];
+    } else {
+        int P = 512;
+        while (P < cnt) P <<= 1;
+        for (int i = cnt + tid; i < P; i += kBmThreads) list[i] = BeamKey{0, 0};
+        bitonic_desc(list, P);
+        if (tid < n) best = list[tid];
+    }
+    const u64 id = ~best.lo;
+    const bool some = tid < n && best.hi != 0;
+    const int parent = some ? (int)(id >> 56) : -1;
     const int token = some ? (int)(id & 0xFFFFFFu) : -1;
-    const bool ended = some && ((finished && finished[b]) || token == eos);
+    const bool end = some && ((finished && finished[parent]) || token == eos);
     __syncthreads();  // the inputs are read: the outputs may be the same arrays
     if (tid < n) {
-        out_scores[tid] = some ? (float)unord64(k.hi) : -INFINITY;
-        out_parents[tid] = b;
+        out_scores[tid] = some ? (float)unord64(best.hi) : -INFINITY;
+        out_parents[tid] = parent;
         out_tokens[tid] = token;
-        if (out_finished) out_finished[tid] = ended;
+        if (out_finished) out_finished[tid] = end;
     }
 }
 
