@@ -145,13 +145,71 @@ __device__ u64 beam_keep_n(u64* list, int* s_cnt, int cnt, int n) {
     return t;
 }
 
+// Raise the threshold T of list[0, cnt) (all keys >= T, n < cnt <= kBsSort) to
+// the lower edge of the bucket that holds the n-th largest value, of 256
+// buckets between T and the maximum, and drop the keys below it.
+__device__ u64 beam_tighten(u64* list, int* s_cnt, int cnt, int n, u64 T, int* hist) {
+    constexpr int kPer = kBsSort / kBsThreads;
+    __shared__ uint32_t s_max;
+    __shared__ int s_bucket;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u64 k[kPer];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int p = tid + i * kBsThreads;
+        k[i] = p < cnt ? list[p] : 0;
+        top = max(top, (uint32_t)(k[i] >> 32));
+    }
+    hist[tid] = 0;
+    if (tid == 0) s_max = 0;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) atomicMax(&s_max, top);
+    __syncthreads();
+    const uint32_t low = (uint32_t)(T >> 32);
+    const int shift = max(0, 24 - __clz(s_max - low));  // (max - low) >> shift < 256
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (k[i]) atomicAdd(&hist[((uint32_t)(k[i] >> 32) - low) >> shift], 1);
+    if (tid == 0) *s_cnt = 0;
+    __syncthreads();
+    if (warp == 0) {  // lane L: buckets 255 - 8 L .. 248 - 8 L, from the top
+        int c[8], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            c[i] = hist[255 - 8 * lane - i];
+            mine += c[i];
+        }
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+        }
+        before -= mine;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (before < n && n <= before + c[i]) s_bucket = 255 - 8 * lane - i;
+            before += c[i];
+        }
+    }
+    __syncthreads();
+    T = (u64)(low + ((uint32_t)s_bucket << shift)) << 32;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (k[i] >= T && k[i]) list[atomicAdd(s_cnt, 1)] = k[i];
+    __syncthreads();
+    return T;
+}
+
 __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __restrict__ logits,
                                                                const int32_t* __restrict__ finished, int vocab,
                                                                int parts, int per, int n, u64* __restrict__ keys,
                                                                BeamPart* __restrict__ stats) {
     constexpr int kWarps = kBsThreads / 32;
     __shared__ __align__(16) u64 list[kBsList];
-    __shared__ int s_cnt;
+    __shared__ int s_cnt, s_hist[kBsThreads];
     __shared__ uint32_t s_t[kWarps];
     __shared__ float s_m[kWarps];
     __shared__ double s_l[kWarps];
@@ -165,16 +223,24 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     bool bad = false;
     u64 T = 0;
     if (tid == 0) s_cnt = 0;
+    float ahead[kBsPer];  // the next tile's logits
+    auto load = [&](int base) {
+#pragma unroll
+        for (int j = 0; j < kBsPer; ++j) {
+            const int i = base + j * kBsThreads + tid;
+            ahead[j] = i < i1 ? __ldg(x + i) : -INFINITY;
+        }
+    };
+    load(i0);
     for (int base = i0; base < i1; base += kBsTile) {
         float v[kBsPer];
         float tm = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kBsPer; ++j) {
-            const int i = base + j * kBsThreads + tid;
-            v[j] = i < i1 ? __ldg(x + i) : -INFINITY;
+            v[j] = ahead[j];
+            tm = fmaxf(tm, v[j]);
         }
-#pragma unroll
-        for (int j = 0; j < kBsPer; ++j) tm = fmaxf(tm, v[j]);
+        if (base + kBsTile < i1) load(base + kBsTile);
         if (base == i0) {
             // at least n elements reach T: the (n / kWarps)-th largest of each warp's thread maxima
             const uint32_t t = warp_kth(tid < i1 - base ? ord32(tm) : 0u, (n + kWarps - 1) / kWarps, lane);
@@ -206,6 +272,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
         const int cnt = s_cnt;
         __syncthreads();
         if (cnt > kBsSort) T = beam_keep_n(list, &s_cnt, cnt, n);
+        else if (cnt > n + n / 2 + 64 && base + kBsTile < i1) T = beam_tighten(list, &s_cnt, cnt, n, T, s_hist);
     }
     // the threads' (m, l) as one
     float M = m;
@@ -295,7 +362,19 @@ __global__ void __launch_bounds__(kBmThreads) beam_merge_kernel(
     const int b = min(tid / parts, n_beam - 1);
     const bool has = tid < lists && s_score[b] == s_score[b];
     const u64* mine = keys + (size_t)tid * n;
-    u64 next = has ? mine[0] : 0;
+    constexpr int kAhead = 4;  // entries of the list that are loaded together
+    u64 ahead[kAhead];
+    auto load = [&](int r) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ahead[i] = r + i < n ? mine[r + i] : 0;
+    };
+    auto entry = [&](int r) {
+        u64 e = ahead[0];
+#pragma unroll
+        for (int i = 1; i < kAhead; ++i) e = (r & (kAhead - 1)) == i ? ahead[i] : e;
+        return e;
+    };
+    if (has) load(0);
     for (int w = warp; w < n_beam; w += kBmThreads / 32) {
         if (s_score[w] != s_score[w]) continue;
         const BeamPart* st = stats + (size_t)w * parts;
@@ -320,10 +399,10 @@ __global__ void __launch_bounds__(kBmThreads) beam_merge_kernel(
     int r = 0;  // entries of this thread's list that are in the list of candidates
     bool more = has;
     for (; r < R; ++r) {
-        const BeamKey k = beam_key(next, b, score, lse);
+        if (more && r && (r & (kAhead - 1)) == 0) load(r);
+        const BeamKey k = more ? beam_key(entry(r), b, score, lse) : BeamKey{0, 0};
         more = more && k.hi != 0;  // the list is sorted: nothing follows an entry that is no candidate
         if (more) list[atomicAdd(&s_cnt, 1)] = k;
-        next = more && r + 1 < n ? mine[r + 1] : 0;
     }
     __syncthreads();
     int cnt = s_cnt;  // <= n_beam + live lists + n
@@ -343,10 +422,10 @@ __global__ void __launch_bounds__(kBmThreads) beam_merge_kernel(
     BeamKey T{s_T, 0};
     // the rest, an entry per list and round, until no list has one that reaches T
     for (; r < n; ++r) {
-        const BeamKey k = beam_key(next, b, score, lse);
+        if (more && r && (r & (kAhead - 1)) == 0) load(r);
+        const BeamKey k = more ? beam_key(entry(r), b, score, lse) : BeamKey{0, 0};
         more = more && k.hi != 0 && !(k < T);
         if (more) list[atomicAdd(&s_cnt, 1)] = k;
-        next = more && r + 1 < n ? mine[r + 1] : 0;
         if (!__syncthreads_or(more)) break;
         cnt = s_cnt;
         __syncthreads();
