@@ -263,10 +263,21 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
             l *= tm - m < 700.0f ? exp_taylor((double)m - (double)tm) : 0.0;  // m = -inf: l is 0
             m = tm;
         }
+        if (m > -INFINITY) {
+            // what lies over 700 below counts as e^-700: no branch, so that the
+            // chains of several terms run side by side
+            const float floor = m - 700.0f;
+            const double md = (double)m;
+            double part[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (int j = 0; j < kBsPer; ++j) {
-            bad |= !(v[j] < INFINITY);
-            if (v[j] - m > -700.0f) l += exp_taylor((double)v[j] - (double)m);
+            for (int j = 0; j < kBsPer; ++j) {
+                bad |= !(v[j] < INFINITY);
+                part[j & 3] += exp_taylor((double)fmaxf(v[j], floor) - md);
+            }
+            l += (part[0] + part[1]) + (part[2] + part[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kBsPer; ++j) bad |= !(v[j] < INFINITY);
         }
         __syncthreads();
         const int cnt = s_cnt;
@@ -291,14 +302,22 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     u64* out = keys + ((size_t)b * parts + part) * n;
     if (cnt <= 2 * kBsThreads) {  // place by the number of larger keys
         const u64 k0 = tid < cnt ? list[tid] : 0, k1 = tid + kBsThreads < cnt ? list[tid + kBsThreads] : 0;
+        if (tid == 0) list[cnt] = 0;
+        __syncthreads();
         int r0 = 0, r1 = 0;
-        if (32 * warp < cnt)
-#pragma unroll 4
-            for (int i = 0; i < cnt; ++i) {
-                const u64 k = list[i];
-                r0 += k > k0;
-                r1 += k > k1;
+        if (32 * warp < cnt) {
+#pragma unroll 8
+            for (int i = 0; i < cnt; i += 2) {
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(list + i);
+                r0 += (k.x > k0) + (k.y > k0);
             }
+            if (cnt > kBsThreads)
+#pragma unroll 8
+                for (int i = 0; i < cnt; i += 2) {
+                    const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(list + i);
+                    r1 += (k.x > k1) + (k.y > k1);
+                }
+        }
         if (k0 && r0 < n) out[r0] = k0;
         if (k1 && r1 < n) out[r1] = k1;
     } else {
@@ -335,17 +354,30 @@ __device__ __forceinline__ BeamKey beam_key(u64 e, int b, double score, double l
     const double s = score + ((double)unord32(o) - lse);
     return BeamKey{e && s > -INFINITY ? ord64(s) : 0, ~((u64)b << 56 | (u64)~o << 24 | token)};
 }
+// 32 bits of a score in the same order (equal for near ones), 0 for no candidate.
+__device__ __forceinline__ uint32_t beam_key32(u64 hi) { return (uint32_t)(hi >> 32); }
 
-__global__ void __launch_bounds__(kBmThreads) beam_merge_kernel(
+// A value that at least n of the threads' v reach, as large as its leading 26
+// bits allow; 0 when fewer than n are not 0.  Whole CTA.
+__device__ __forceinline__ uint32_t cta_nth(uint32_t v, int n) {
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 6; --bit) {
+        const uint32_t cand = t | 1u << bit;
+        if (__syncthreads_count(v >= cand) >= n) t = cand;
+    }
+    return t;
+}
+
+__global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     const u64* __restrict__ keys, const BeamPart* __restrict__ stats, const float* scores, const int32_t* finished,
     int n_beam, int parts, int n, int eos, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
     int32_t* out_finished) {
     __shared__ __align__(16) BeamKey list[kBmList];
     __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
-    __shared__ u64 s_T;
-    __shared__ int s_cnt, s_live;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) s_cnt = s_live = 0, s_T = 0;
+    __shared__ int s_rank[kBeamMaxOut * 2];
+    __shared__ int s_cnt, s_live, s_full;
+    const int tid = threadIdx.x;
+    if (tid == 0) s_cnt = s_live = s_full = 0;
     __syncthreads();
     // the beams' scores; NaN for a beam without lists (ended, or no candidate can be better than none)
     for (int b = tid; b < n_beam; b += kBmThreads) {
@@ -375,82 +407,121 @@ __global__ void __launch_bounds__(kBmThreads) beam_merge_kernel(
         return e;
     };
     if (has) load(0);
-    for (int w = warp; w < n_beam; w += kBmThreads / 32) {
-        if (s_score[w] != s_score[w]) continue;
-        const BeamPart* st = stats + (size_t)w * parts;
+    {
+        // 4 to 32 lanes per beam
+        int width = 32;
+        while (width > 4 && n_beam * width > kBmThreads) width >>= 1;
+        const int w = tid / width, wl = tid & (width - 1);
+        const bool on = w < n_beam && s_score[min(w, n_beam - 1)] == s_score[min(w, n_beam - 1)];
+        const BeamPart* st = stats + (size_t)min(w, n_beam - 1) * parts;
         float M = -INFINITY;
-        for (int p = lane; p < parts; p += 32) M = fmaxf(M, st[p].ref);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        for (int p = wl; on && p < parts; p += width) M = fmaxf(M, st[p].ref);
+        for (int o = width / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         double l = 0.0;
-        for (int p = lane; p < parts; p += 32) {
+        for (int p = wl; on && p < parts; p += width) {
             const BeamPart s = st[p];
             const double f = s.ref - M > -700.0f ? exp_taylor((double)s.ref - (double)M) : 0.0;
-            l += s.sum == s.sum ? s.sum * f : s.sum;
+            l += s.sum == s.sum ? s.sum * f : s.sum;  // a NaN stays
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) s_lse[w] = (double)M + log(l);
+        for (int o = width / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (on && wl == 0) s_lse[w] = (double)M + log(l);
     }
     __syncthreads();
     const double score = s_score[b], lse = has ? s_lse[b] : 0.0;
-    // T: a score that n candidates reach, the n-th best of the lists' first R entries (and the ended beams)
+    // the lists' first R entries, which with the ended beams are enough unless many are no candidates
     const int R = min(n, (n + max(1, s_live * parts) - 1) / max(1, s_live * parts));
-    int r = 0;  // entries of this thread's list that are in the list of candidates
+    int r = 0;  // entries of this thread's list that were taken
     bool more = has;
-    for (; r < R; ++r) {
-        if (more && r && (r & (kAhead - 1)) == 0) load(r);
-        const BeamKey k = more ? beam_key(entry(r), b, score, lse) : BeamKey{0, 0};
-        more = more && k.hi != 0;  // the list is sorted: nothing follows an entry that is no candidate
+    for (; r < R && more; ++r) {
+        if (r && (r & (kAhead - 1)) == 0) load(r);
+        const BeamKey k = beam_key(entry(r), b, score, lse);
+        more = k.hi != 0;  // the list is sorted: nothing follows an entry that is no candidate
         if (more) list[atomicAdd(&s_cnt, 1)] = k;
     }
     __syncthreads();
-    int cnt = s_cnt;  // <= n_beam + live lists + n
-    if (cnt > n) {
-        for (int i = tid; i < cnt; i += kBmThreads) {
-            const u64 mineh = list[i].hi;
-            int above = 0, ties = 0;
-#pragma unroll 4
-            for (int j = 0; j < cnt; ++j) {
-                above += list[j].hi > mineh;
-                ties += list[j].hi == mineh;
+    int cnt = s_cnt;  // <= n_beam + live lists + n; where it is over kBmThreads, t1 goes by the first of them
+    const uint32_t t1 = cnt > n ? cta_nth(tid < cnt ? beam_key32(list[tid].hi) : 0u, n) : 0u;
+    // the rest, while it reaches t1: a few entries per list.  Where the lists hold
+    // so many candidates that t1 does not bound them, in rounds with a sort.
+    const bool bounded = t1 != 0;
+    if (bounded) {
+        __syncthreads();
+        while (more && r < n) {
+            if (r && (r & (kAhead - 1)) == 0) load(r);
+            const BeamKey k = beam_key(entry(r), b, score, lse);
+            more = k.hi != 0 && beam_key32(k.hi) >= t1;
+            if (!more) break;
+            const int p = atomicAdd(&s_cnt, 1);
+            if (p >= kBmList) {  // no room: this entry and the later ones are for the rounds
+                s_full = 1;
+                break;
             }
-            if (above < n && n <= above + ties) s_T = mineh;
+            list[p] = k;
+            ++r;
         }
         __syncthreads();
-    }
-    BeamKey T{s_T, 0};
-    // the rest, an entry per list and round, until no list has one that reaches T
-    for (; r < n; ++r) {
-        if (more && r && (r & (kAhead - 1)) == 0) load(r);
-        const BeamKey k = more ? beam_key(entry(r), b, score, lse) : BeamKey{0, 0};
-        more = more && k.hi != 0 && !(k < T);
-        if (more) list[atomicAdd(&s_cnt, 1)] = k;
-        if (!__syncthreads_or(more)) break;
-        cnt = s_cnt;
+        if (s_full && tid == 0) s_cnt = kBmList;
         __syncthreads();
-        if (cnt > kBmList - kBmThreads) {
-            for (int i = cnt + tid; i < kBmList; i += kBmThreads) list[i] = BeamKey{0, 0};
-            bitonic_desc(list, kBmList);
-            T = list[n - 1];
-            if (tid == 0) s_cnt = n;
+    }
+    BeamKey T{0, 0};
+    if (!bounded || s_full) {
+        for (bool go = true; go;) {
+            cnt = s_cnt;
             __syncthreads();
+            if (cnt > kBmList - kBmThreads || (T.hi == 0 && cnt >= n)) {
+                int P = 512;
+                while (P < cnt) P <<= 1;
+                for (int i = cnt + tid; i < P; i += kBmThreads) list[i] = BeamKey{0, 0};
+                bitonic_desc(list, P);
+                T = list[n - 1];
+                if (tid == 0) s_cnt = n;
+                __syncthreads();
+            }
+            more = more && r < n;
+            if (more) {
+                if (r && (r & (kAhead - 1)) == 0) load(r);
+                const BeamKey k = beam_key(entry(r), b, score, lse);
+                more = k.hi != 0 && T < k;
+                if (more) list[atomicAdd(&s_cnt, 1)] = k;
+                ++r;
+            }
+            go = __syncthreads_or(more);
         }
+        __syncthreads();
     }
-    __syncthreads();
     cnt = s_cnt;
     BeamKey best{0, 0};  // the tid-th best
-    if (cnt <= 384) {
-        // place by the number of better ones
-        BeamKey k{0, 0};
-        int rank = kBmThreads;
-        if (32 * warp < cnt) {
-            k = tid < cnt ? list[tid] : k;
+    uint32_t t2 = 0;
+    if (cnt <= kBmThreads) {
+        // only what reaches the n-th best (but for the last bits) is ranked
+        const BeamKey k = tid < cnt ? list[tid] : BeamKey{0, 0};
+        t2 = cnt > n ? cta_nth(beam_key32(k.hi), n) : 0u;
+        __syncthreads();
+        if (tid == 0) s_cnt = 0;
+        __syncthreads();
+        if (k.hi && beam_key32(k.hi) >= t2) list[atomicAdd(&s_cnt, 1)] = k;
+        __syncthreads();
+        cnt = s_cnt;
+    }
+    if (cnt <= 2 * kBeamMaxOut) {
+        // place each by the number of better ones; groups of threads count their shares
+        const int P = max(32, (cnt + 31) & ~31), groups = kBmThreads / P;
+        if (tid < 2 * kBeamMaxOut) s_rank[tid] = 0;
+        __syncthreads();
+        const int i = tid % P, g = tid / P;
+        if (g < groups && i < cnt) {
+            const BeamKey k = list[i];
             int better = 0;
 #pragma unroll 4
-            for (int j = 0; j < cnt; ++j) better += k < list[j];
-            if (tid < cnt) rank = better;
+            for (int j = g; j < cnt; j += groups) {
+                const BeamKey o = list[j];
+                better += (o.hi > k.hi) | ((o.hi == k.hi) & (o.lo > k.lo));
+            }
+            atomicAdd(&s_rank[i], better);
         }
+        __syncthreads();
+        const BeamKey k = list[tid < cnt ? tid : 0];
+        const int rank = tid < cnt ? s_rank[tid] : kBmThreads;
         __syncthreads();
         if (rank < n) list[rank] = k;
         __syncthreads();
