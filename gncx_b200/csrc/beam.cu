@@ -96,6 +96,23 @@ __device__ __forceinline__ double exp_taylor(double y) {
     return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 
+// e^y for the sums over a vocabulary, with fewer double-precision operations:
+// y = n ln2 / 16 + r, |r| <= 0.0217, the polynomial to r^4 (r^5 / 120 < 5e-11)
+// and tab[k] = 2^(k / 16).
+__device__ __forceinline__ double exp_tab(double y, const double* tab) {
+    const double magic = 6755399441055744.0;
+    const double t = fma(y, 16 * 1.4426950408889634, magic);
+    const double r = fma(t - magic, -0.6931471805599453 / 16, y);
+    double p = 1.0 / 24;
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    const int n = __double2loint(t);
+    p *= tab[n & 15];
+    return __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p));
+}
+
 // The k-th largest (k = 1..32) of the warp's values, by a bitonic sort over its lanes.
 __device__ __forceinline__ uint32_t warp_kth(uint32_t v, int k, int lane) {
 #pragma unroll
@@ -209,7 +226,9 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
                                                                BeamPart* __restrict__ stats) {
     constexpr int kWarps = kBsThreads / 32;
     __shared__ __align__(16) u64 list[kBsList];
-    __shared__ int s_cnt, s_hist[kBsThreads];
+    __shared__ int s_cnt;
+    __shared__ __align__(16) int s_hist[2 * kBsThreads + 4];
+    __shared__ double s_tab[16];
     __shared__ uint32_t s_t[kWarps];
     __shared__ float s_m[kWarps];
     __shared__ double s_l[kWarps];
@@ -223,6 +242,8 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     bool bad = false;
     u64 T = 0;
     if (tid == 0) s_cnt = 0;
+    if (tid < 16) s_tab[tid] = exp2(tid / 16.0);
+    __syncthreads();
     float ahead[kBsPer];  // the next tile's logits
     auto load = [&](int base) {
 #pragma unroll
@@ -251,12 +272,31 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
             for (int w = 1; w < kWarps; ++w) low = min(low, s_t[w]);
             T = (u64)low << 32;
         }
-        if (ord32(tm) >= (uint32_t)(T >> 32)) {
+        {
+            // what reaches T goes to the list: a place per warp, then per lane
+            unsigned take = 0;
+            if (ord32(tm) >= (uint32_t)(T >> 32)) {
 #pragma unroll
-            for (int j = 0; j < kBsPer; ++j) {
-                const int i = base + j * kBsThreads + tid;
-                const u64 k = (u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)i);
-                if (k >= T && i < i1) list[atomicAdd(&s_cnt, 1)] = k;
+                for (int j = 0; j < kBsPer; ++j) {
+                    const int i = base + j * kBsThreads + tid;
+                    const u64 k = (u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)i);
+                    take |= (unsigned)(k >= T && i < i1) << j;
+                }
+            }
+            if (__any_sync(0xffffffffu, take != 0)) {
+                int at = __popc(take);
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, at, o);
+                    if (lane >= o) at += y;
+                }
+                int start = 0;
+                if (lane == 31) start = atomicAdd(&s_cnt, at);
+                at += __shfl_sync(0xffffffffu, start, 31) - __popc(take);
+#pragma unroll
+                for (int j = 0; j < kBsPer; ++j)
+                    if (take >> j & 1)
+                        list[at++] = (u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)(base + j * kBsThreads + tid));
             }
         }
         if (tm > m + 64.0f || m == -INFINITY) {
@@ -272,7 +312,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
 #pragma unroll
             for (int j = 0; j < kBsPer; ++j) {
                 bad |= !(v[j] < INFINITY);
-                part[j & 3] += exp_taylor((double)fmaxf(v[j], floor) - md);
+                part[j & 3] += exp_tab((double)fmaxf(v[j], floor) - md, s_tab);
             }
             l += (part[0] + part[1]) + (part[2] + part[3]);
         } else {
@@ -283,7 +323,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
         const int cnt = s_cnt;
         __syncthreads();
         if (cnt > kBsSort) T = beam_keep_n(list, &s_cnt, cnt, n);
-        else if (cnt > n + n / 2 + 64 && base + kBsTile < i1) T = beam_tighten(list, &s_cnt, cnt, n, T, s_hist);
+        else if (cnt > 2 * n + 256 || (cnt > n + n / 4 + 32 && base + kBsTile >= i1)) T = beam_tighten(list, &s_cnt, cnt, n, T, s_hist);
     }
     // the threads' (m, l) as one
     float M = m;
@@ -300,23 +340,40 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     __syncthreads();
     const int cnt = s_cnt;
     u64* out = keys + ((size_t)b * parts + part) * n;
-    if (cnt <= 2 * kBsThreads) {  // place by the number of larger keys
+    if (cnt <= 2 * kBsThreads) {
+        // place by the number of larger keys: by their values, and where two values
+        // are equal once more by the whole keys
+        uint32_t* hi = reinterpret_cast<uint32_t*>(s_hist);  // 2 * kBsThreads values and 4 zeros
         const u64 k0 = tid < cnt ? list[tid] : 0, k1 = tid + kBsThreads < cnt ? list[tid + kBsThreads] : 0;
+        const uint32_t h0 = (uint32_t)(k0 >> 32), h1 = (uint32_t)(k1 >> 32);
+        hi[tid] = h0;
+        hi[tid + kBsThreads] = h1;
+        if (tid < 4) hi[2 * kBsThreads + tid] = 0;
         if (tid == 0) list[cnt] = 0;
         __syncthreads();
-        int r0 = 0, r1 = 0;
+        int r0 = 0, r1 = 0, e0 = 0;
         if (32 * warp < cnt) {
-#pragma unroll 8
+#pragma unroll 4
+            for (int i = 0; i < cnt; i += 4) {
+                const uint4 k = *reinterpret_cast<const uint4*>(hi + i);
+                r0 += (k.x > h0) + (k.y > h0) + (k.z > h0) + (k.w > h0);
+                e0 += (k.x == h0) + (k.y == h0) + (k.z == h0) + (k.w == h0);
+            }
+            if (cnt > kBsThreads)
+#pragma unroll 4
+                for (int i = 0; i < cnt; i += 4) {
+                    const uint4 k = *reinterpret_cast<const uint4*>(hi + i);
+                    r1 += (k.x > h1) + (k.y > h1) + (k.z > h1) + (k.w > h1);
+                    e0 += k1 && ((k.x == h1) | (k.y == h1) | (k.z == h1) | (k.w == h1));
+                }
+        }
+        if (__syncthreads_or((k0 && e0 > (k1 ? 2 : 1)))) {
+            r0 = r1 = 0;
             for (int i = 0; i < cnt; i += 2) {
                 const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(list + i);
                 r0 += (k.x > k0) + (k.y > k0);
+                r1 += (k.x > k1) + (k.y > k1);
             }
-            if (cnt > kBsThreads)
-#pragma unroll 8
-                for (int i = 0; i < cnt; i += 2) {
-                    const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(list + i);
-                    r1 += (k.x > k1) + (k.y > k1);
-                }
         }
         if (k0 && r0 < n) out[r0] = k0;
         if (k1 && r1 < n) out[r1] = k1;
@@ -357,14 +414,53 @@ __device__ __forceinline__ BeamKey beam_key(u64 e, int b, double score, double l
 // 32 bits of a score in the same order (equal for near ones), 0 for no candidate.
 __device__ __forceinline__ uint32_t beam_key32(u64 hi) { return (uint32_t)(hi >> 32); }
 
-// A value that at least n of the threads' v reach, as large as its leading 26
-// bits allow; 0 when fewer than n are not 0.  Whole CTA.
-__device__ __forceinline__ uint32_t cta_nth(uint32_t v, int n) {
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 6; --bit) {
-        const uint32_t cand = t | 1u << bit;
-        if (__syncthreads_count(v >= cand) >= n) t = cand;
+// A value that at least n of the threads' v reach: the lower edge of the bucket
+// with the n-th largest, of 256 between the least and the greatest v that is not
+// 0; 0 when fewer than n are not.  Whole CTA.
+__device__ __forceinline__ uint32_t cta_bound(uint32_t v, int n, int* hist) {
+    __shared__ uint32_t s_low, s_top;
+    __shared__ int s_bucket;
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid < 256) hist[tid] = 0;
+    if (tid == 0) {
+        s_low = 0xFFFFFFFFu;
+        s_top = 0;
+        s_bucket = -1;
     }
+    __syncthreads();
+    const uint32_t low = __reduce_min_sync(0xffffffffu, v ? v : 0xFFFFFFFFu), top = __reduce_max_sync(0xffffffffu, v);
+    if (lane == 0 && top) {
+        atomicMin(&s_low, low);
+        atomicMax(&s_top, top);
+    }
+    __syncthreads();
+    const uint32_t base = s_low;
+    const int shift = s_top ? max(0, 24 - __clz(s_top - base)) : 0;
+    if (v) atomicAdd(&hist[(v - base) >> shift], 1);
+    __syncthreads();
+    if (tid < 32) {  // lane L: buckets 255 - 8 L .. 248 - 8 L, from the top
+        int c[8], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            c[i] = hist[255 - 8 * lane - i];
+            mine += c[i];
+        }
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+        }
+        before -= mine;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (before < n && n <= before + c[i]) s_bucket = 255 - 8 * lane - i;
+            before += c[i];
+        }
+    }
+    __syncthreads();
+    const uint32_t t = s_bucket < 0 ? 0u : base + ((uint32_t)s_bucket << shift);
+    __syncthreads();
     return t;
 }
 
@@ -440,7 +536,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     }
     __syncthreads();
     int cnt = s_cnt;  // <= n_beam + live lists + n; where it is over kBmThreads, t1 goes by the first of them
-    const uint32_t t1 = cnt > n ? cta_nth(tid < cnt ? beam_key32(list[tid].hi) : 0u, n) : 0u;
+    const uint32_t t1 = cnt > n ? cta_bound(tid < cnt ? beam_key32(list[tid].hi) : 0u, n, s_rank) : 0u;
     // the rest, while it reaches t1: a few entries per list.  Where the lists hold
     // so many candidates that t1 does not bound them, in rounds with a sort.
     const bool bounded = t1 != 0;
@@ -495,7 +591,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     if (cnt <= kBmThreads) {
         // only what reaches the n-th best (but for the last bits) is ranked
         const BeamKey k = tid < cnt ? list[tid] : BeamKey{0, 0};
-        t2 = cnt > n ? cta_nth(beam_key32(k.hi), n) : 0u;
+        t2 = cnt > n ? cta_bound(beam_key32(k.hi), n, s_rank) : 0u;
         __syncthreads();
         if (tid == 0) s_cnt = 0;
         __syncthreads();
