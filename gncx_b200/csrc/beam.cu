@@ -31,6 +31,7 @@ constexpr int kBsPer = 16;
 constexpr int kBsTile = kBsThreads * kBsPer;
 constexpr int kBsSort = 1024;             // largest list that is sorted
 constexpr int kBsList = kBsSort + kBsTile;
+constexpr int kBsCtasPerSm = 3;           // that a vocabulary is split for
 constexpr int kBmThreads = 1024;
 constexpr int kBmList = 2 * kBmThreads;
 
@@ -229,6 +230,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     __shared__ int s_cnt;
     __shared__ __align__(16) int s_hist[2 * kBsThreads + 4];
     __shared__ double s_tab[16];
+    __shared__ int s_seen[2 * kBsThreads];
     __shared__ uint32_t s_t[kWarps];
     __shared__ float s_m[kWarps];
     __shared__ double s_l[kWarps];
@@ -293,10 +295,10 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
                 int start = 0;
                 if (lane == 31) start = atomicAdd(&s_cnt, at);
                 at += __shfl_sync(0xffffffffu, start, 31) - __popc(take);
-#pragma unroll
-                for (int j = 0; j < kBsPer; ++j)
-                    if (take >> j & 1)
-                        list[at++] = (u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)(base + j * kBsThreads + tid));
+                for (; take; take &= take - 1) {  // few per thread: read again rather than picked from registers
+                    const int i = base + (__ffs(take) - 1) * kBsThreads + tid;
+                    list[at++] = (u64)ord32(__ldg(x + i)) << 32 | (0xFFFFFFFFu - (uint32_t)i);
+                }
             }
         }
         if (tm > m + 64.0f || m == -INFINITY) {
@@ -310,9 +312,13 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
             const double md = (double)m;
             double part[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-            for (int j = 0; j < kBsPer; ++j) {
-                bad |= !(v[j] < INFINITY);
-                part[j & 3] += exp_tab((double)fmaxf(v[j], floor) - md, s_tab);
+            for (int g = 0; g < kBsPer; g += 4) {
+                if (base + g * kBsThreads >= i1) break;  // of the CTA: the rest of the tile is empty
+#pragma unroll
+                for (int j = g; j < g + 4; ++j) {
+                    bad |= !(v[j] < INFINITY);
+                    part[j & 3] += exp_tab((double)fmaxf(v[j], floor) - md, s_tab);
+                }
             }
             l += (part[0] + part[1]) + (part[2] + part[3]);
         } else {
@@ -350,24 +356,25 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
         hi[tid + kBsThreads] = h1;
         if (tid < 4) hi[2 * kBsThreads + tid] = 0;
         if (tid == 0) list[cnt] = 0;
+        s_seen[tid] = s_seen[tid + kBsThreads] = 0;
         __syncthreads();
-        int r0 = 0, r1 = 0, e0 = 0;
+        int r0 = 0, r1 = 0;
         if (32 * warp < cnt) {
 #pragma unroll 4
             for (int i = 0; i < cnt; i += 4) {
                 const uint4 k = *reinterpret_cast<const uint4*>(hi + i);
                 r0 += (k.x > h0) + (k.y > h0) + (k.z > h0) + (k.w > h0);
-                e0 += (k.x == h0) + (k.y == h0) + (k.z == h0) + (k.w == h0);
             }
             if (cnt > kBsThreads)
 #pragma unroll 4
                 for (int i = 0; i < cnt; i += 4) {
                     const uint4 k = *reinterpret_cast<const uint4*>(hi + i);
                     r1 += (k.x > h1) + (k.y > h1) + (k.z > h1) + (k.w > h1);
-                    e0 += k1 && ((k.x == h1) | (k.y == h1) | (k.z == h1) | (k.w == h1));
                 }
         }
-        if (__syncthreads_or((k0 && e0 > (k1 ? 2 : 1)))) {
+        // equal values have equal ranks
+        const bool tie = (k0 && atomicExch(&s_seen[r0], 1)) || (k1 && atomicExch(&s_seen[r1], 1));
+        if (__syncthreads_or(tie)) {
             r0 = r1 = 0;
             for (int i = 0; i < cnt; i += 2) {
                 const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(list + i);
@@ -470,7 +477,8 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     int32_t* out_finished) {
     __shared__ __align__(16) BeamKey list[kBmList];
     __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
-    __shared__ int s_rank[kBeamMaxOut * 2];
+    __shared__ int s_rank[kBeamMaxOut * 2], s_seen[kBeamMaxOut * 2];
+    __shared__ uint4 s_k32[kBeamMaxOut / 2 + 1];
     __shared__ int s_cnt, s_live, s_full;
     const int tid = threadIdx.x;
     if (tid == 0) s_cnt = s_live = s_full = 0;
@@ -510,15 +518,30 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
         const int w = tid / width, wl = tid & (width - 1);
         const bool on = w < n_beam && s_score[min(w, n_beam - 1)] == s_score[min(w, n_beam - 1)];
         const BeamPart* st = stats + (size_t)min(w, n_beam - 1) * parts;
+        // a lane's parts as one, then the lanes'
         float M = -INFINITY;
-        for (int p = wl; on && p < parts; p += width) M = fmaxf(M, st[p].ref);
-        for (int o = width / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         double l = 0.0;
-        for (int p = wl; on && p < parts; p += width) {
-            const BeamPart s = st[p];
-            const double f = s.ref - M > -700.0f ? exp_taylor((double)s.ref - (double)M) : 0.0;
-            l += s.sum == s.sum ? s.sum * f : s.sum;  // a NaN stays
+        auto join = [&](float m, double sum) {
+            const float top = fmaxf(M, m);
+            // nothing counts for less than e^-700; a NaN sum stays
+            const double a = M - top > -700.0f ? exp_taylor((double)M - (double)top) : 0.0;
+            const double c = m - top > -700.0f ? exp_taylor((double)m - (double)top) : 0.0;
+            l = (l == l ? l * a : l) + (sum == sum ? sum * c : sum);
+            M = top;
+        };
+        if (on && wl < parts) {
+            BeamPart s = st[wl];
+            M = s.ref;
+            l = s.sum;
+            for (int p = wl + width; p < parts; p += width) {
+                s = st[p];
+                join(s.ref, s.sum);
+            }
         }
+        float top = M;
+        for (int o = width / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (l == l) l = M - top > -700.0f ? l * exp_taylor((double)M - (double)top) : 0.0;
+        M = top;
         for (int o = width / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         if (on && wl == 0) s_lse[w] = (double)M + log(l);
     }
@@ -600,22 +623,43 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
         cnt = s_cnt;
     }
     if (cnt <= 2 * kBeamMaxOut) {
-        // place each by the number of better ones; groups of threads count their shares
+        // place each by the number of better ones, groups of threads counting shares
+        // of them: by 32 bits of the scores, where two are equal by the whole keys
         const int P = max(32, (cnt + 31) & ~31), groups = kBmThreads / P;
-        if (tid < 2 * kBeamMaxOut) s_rank[tid] = 0;
-        __syncthreads();
         const int i = tid % P, g = tid / P;
-        if (g < groups && i < cnt) {
-            const BeamKey k = list[i];
-            int better = 0;
-#pragma unroll 4
-            for (int j = g; j < cnt; j += groups) {
-                const BeamKey o = list[j];
-                better += (o.hi > k.hi) | ((o.hi == k.hi) & (o.lo > k.lo));
-            }
-            atomicAdd(&s_rank[i], better);
+        const bool on = g < groups && i < cnt;
+        uint32_t* k32 = reinterpret_cast<uint32_t*>(s_k32);
+        if (tid < 2 * kBeamMaxOut) {
+            s_rank[tid] = 0;
+            k32[tid] = tid < cnt ? beam_key32(list[tid].hi) : 0u;
+            s_seen[tid] = 0;
         }
         __syncthreads();
+        if (on) {
+            const uint32_t k = k32[i];
+            int better = 0;
+            for (int j = 4 * g; j < cnt; j += 4 * groups) {
+                const uint4 o = *reinterpret_cast<const uint4*>(k32 + j);
+                better += (o.x > k) + (o.y > k) + (o.z > k) + (o.w > k);
+            }
+            if (better) atomicAdd(&s_rank[i], better);
+        }
+        __syncthreads();
+        if (__syncthreads_or(tid < cnt && atomicExch(&s_seen[s_rank[tid]], 1))) {
+            if (tid < 2 * kBeamMaxOut) s_rank[tid] = 0;
+            __syncthreads();
+            if (on) {
+                const BeamKey k = list[i];
+                int better = 0;
+#pragma unroll 4
+                for (int j = g; j < cnt; j += groups) {
+                    const BeamKey o = list[j];
+                    better += (o.hi > k.hi) | ((o.hi == k.hi) & (o.lo > k.lo));
+                }
+                if (better) atomicAdd(&s_rank[i], better);
+            }
+            __syncthreads();
+        }
         const BeamKey k = list[tid < cnt ? tid : 0];
         const int rank = tid < cnt ? s_rank[tid] : kBmThreads;
         __syncthreads();
@@ -643,11 +687,11 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     }
 }
 
-// Parts of a beam's vocabulary: about two CTAs per SM over all beams, no part
+// Parts of a beam's vocabulary: about three CTAs per SM over all beams, no part
 // shorter than one tile.
 static int beam_parts(int n_beam, int vocab, int sm_count) {
     const int tiles = (vocab + kBsTile - 1) / kBsTile;
-    const int want = (2 * sm_count + n_beam - 1) / n_beam;
+    const int want = (kBsCtasPerSm * sm_count + n_beam - 1) / n_beam;
     return tiles < want ? tiles : want;
 }
 
