@@ -114,6 +114,15 @@ __device__ __forceinline__ double exp_tab(double y, const double* tab) {
     return __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p));
 }
 
+// log l of a sum of exponentials (e^-700 < l < 1e38): a Newton step in double
+// from the fp32 logarithm y, log l = y + log(l e^-y), with l e^-y near 1.
+__device__ __forceinline__ double log_of_sum(double l) {
+    if (!(l > 0.0)) return l == 0.0 ? -INFINITY : NAN;
+    const double y = (double)logf((float)l);
+    const double d = fma(l, exp_taylor(-y), -1.0);
+    return y + (d - 0.5 * d * d);
+}
+
 // The k-th largest (k = 1..32) of the warp's values, by a bitonic sort over its lanes.
 __device__ __forceinline__ uint32_t warp_kth(uint32_t v, int k, int lane) {
 #pragma unroll
@@ -277,12 +286,16 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
         {
             // what reaches T goes to the list: a place per warp, then per lane
             unsigned take = 0;
-            if (ord32(tm) >= (uint32_t)(T >> 32)) {
+            const float low = T ? unord32((uint32_t)(T >> 32)) : -INFINITY;
+            if (tm >= low) {
 #pragma unroll
-                for (int j = 0; j < kBsPer; ++j) {
-                    const int i = base + j * kBsThreads + tid;
-                    const u64 k = (u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)i);
-                    take |= (unsigned)(k >= T && i < i1) << j;
+                for (int j = 0; j < kBsPer; ++j) take |= (unsigned)(v[j] >= low) << j;
+                if (base + kBsTile > i1 || (uint32_t)T) {  // a part's end; a T that tells equal values apart
+#pragma unroll
+                    for (int j = 0; j < kBsPer; ++j) {
+                        const int i = base + j * kBsThreads + tid;
+                        if (i >= i1 || ((u64)ord32(v[j]) << 32 | (0xFFFFFFFFu - (uint32_t)i)) < T) take &= ~(1u << j);
+                    }
                 }
             }
             if (__any_sync(0xffffffffu, take != 0)) {
@@ -543,7 +556,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
         if (l == l) l = M - top > -700.0f ? l * exp_taylor((double)M - (double)top) : 0.0;
         M = top;
         for (int o = width / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (on && wl == 0) s_lse[w] = (double)M + log(l);
+        if (on && wl == 0) s_lse[w] = (double)M + log_of_sum(l);
     }
     __syncthreads();
     const double score = s_score[b], lse = has ? s_lse[b] : 0.0;
