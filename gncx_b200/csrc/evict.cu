@@ -19,9 +19,11 @@
 // The i-th free row below n_keep takes the i-th row that stays from behind
 // it: rows that are read and rows that are written are disjoint, so the cache
 // is compacted in place, in parallel, and no row moves that need not.
-//   * evict_select_kernel, one CTA per KV head: radix selection of the
-//     n_keep-th key, then the lists of free and of moving rows by prefix sums;
-//   * evict_move_kernel copies the rows.
+//   * evict_select_kernel, a CTA or a cluster of CTAs per KV head: radix
+//     selection of the n_keep-th key over keys in registers, then the lists of
+//     free and of moving rows by prefix sums;
+//   * evict_move_kernel copies the rows (few rows: the selecting kernel does).
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include "common.cuh"
 #include "kernels.h"
@@ -405,6 +407,8 @@ int weights_step_launch(const float* q, const float* new_k, const float* new_v, 
 
 // ---------------------------------------------------------------- eviction
 constexpr int kEvThreads = 1024;
+constexpr int kEvSpread = 8192;  // rows above which a cluster of 8 CTAs selects instead of one CTA
+constexpr int kEvHere = 256;     // moves up to which the selecting kernel makes them
 constexpr int kEvBins = 2048;
 
 struct EvictArgs {
@@ -418,8 +422,9 @@ struct EvictArgs {
     int out_stride;
     int32_t* moves;  // per KV head: count, then max_moves free rows, then max_moves moving rows
     int max_moves;
-    uint32_t* masks;  // per KV head: words of "above the threshold", then of "at the threshold"
+    uint32_t* masks;  // many rows, per KV head: words of "above the threshold", then of "at the threshold"
     int words;
+    bool here;  // the selecting kernel moves the rows too
 };
 
 // Greater keys stay: protected rows, then the weights in order, NaN last.
@@ -457,13 +462,71 @@ __device__ __forceinline__ u_int64_t cta_scan(u_int64_t v, u_int64_t* s_warp, u_
     return x - v + (warp ? s_warp[warp - 1] : 0);
 }
 
+// Copy rows of KV head h: the i-th free row takes the i-th moving row, for i0,
+// i0 + step, .. below n, kEvMoveRows at a time; one warp.
+constexpr int kEvMoveRows = 4;
+__device__ __forceinline__ void evict_move_rows(const EvictArgs& a, int h, const int32_t* to, const int32_t* from, int n,
+                                                int i0, int lane) {
+    const int hd4 = a.hd / 4;
+    const size_t ps = (size_t)a.n_kv * a.hd;
+    int f[kEvMoveRows], t[kEvMoveRows];
+#pragma unroll
+    for (int r = 0; r < kEvMoveRows; ++r) {
+        const int i = min(i0 + r, n - 1);
+        f[r] = from[i];
+        t[r] = to[i];
+    }
+    for (int c = lane; c < hd4; c += 32) {
+        float4 k[kEvMoveRows], v[kEvMoveRows];
+#pragma unroll
+        for (int r = 0; r < kEvMoveRows; ++r) {
+            const size_t at = (size_t)f[r] * ps + (size_t)h * a.hd + 4 * c;
+            k[r] = __ldcs(reinterpret_cast<const float4*>(a.kc + at));
+            v[r] = __ldcs(reinterpret_cast<const float4*>(a.vc + at));
+        }
+#pragma unroll
+        for (int r = 0; r < kEvMoveRows; ++r)
+            if (i0 + r < n) {
+                const size_t at = (size_t)t[r] * ps + (size_t)h * a.hd + 4 * c;
+                *reinterpret_cast<float4*>(a.kc + at) = k[r];
+                *reinterpret_cast<float4*>(a.vc + at) = v[r];
+            }
+    }
+    if (lane < kEvMoveRows && i0 + lane < n) {
+        const int ff = from[i0 + lane], tt = to[i0 + lane];
+        a.weight_out[(size_t)h * a.out_stride + tt] = a.weight[(size_t)h * a.row_stride + ff];
+        if (a.positions) a.positions_out[(size_t)h * a.out_stride + tt] = a.positions[(size_t)h * a.row_stride + ff];
+    }
+}
+
+// One cluster per KV head, each CTA a run of kEvThreads * KPT rows, their keys in
+// registers.  Counts are summed over the cluster through distributed shared
+// memory.
+template <int KPT>
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs a) {
-    __shared__ int hist[kEvBins];
+    constexpr int kWords = 32 * KPT;  // of 32 rows, per CTA
+    __shared__ __align__(16) int hist[kEvBins];
     __shared__ u_int64_t s_warp[32];
+    __shared__ uint32_t s_gt[kWords], s_eq[kWords];
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
+    __shared__ int s_count[3];  // of this CTA: ties, free rows, moving rows
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    auto meet = [&] {
+        if (size > 1) cluster.sync();
+        else __syncthreads();
+    };
     pdl_launch_dependents();
-    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row0 = rank * kEvThreads * KPT;
+    uint32_t key[KPT];
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+        const int row = row0 + i * kEvThreads + tid;
+        key[i] = row < a.n_rows ? evict_key(a, h, row) : 0u;
+    }
     // The n_keep-th largest key by digits of 11, 11 and 10 bits from the top:
     // each pass counts the keys that share the digits found so far.
     uint32_t prefix = 0;
@@ -475,23 +538,151 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         shift -= bits;
         for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = 0;
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const bool in = row0 + i * kEvThreads + tid < a.n_rows && (key[i] & high) == prefix;
+            const uint32_t d = (key[i] >> shift) & ((1u << bits) - 1);
+            const unsigned act = __ballot_sync(0xffffffffu, in);
+            if (!act) continue;
+            // rows of equal digits (equal weights, a shared exponent): one addition for the warp
+            const uint32_t d0 = __shfl_sync(0xffffffffu, d, __ffs(act) - 1);
+            const unsigned same = __ballot_sync(0xffffffffu, in && d == d0);
+            if (lane == 0) atomicAdd(&hist[d0], __popc(same));
+            if (in && d != d0) atomicAdd(&hist[d], 1);
+        }
+        meet();
+        // bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t
+        const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
+        int c1 = hist[b1], c0 = hist[b0];
+        if (size > 1) {
+            c0 = c1 = 0;
+#pragma unroll 8
+            for (int r = 0; r < size; ++r) {
+                const int2 c = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[b0], r));
+                c0 += c.x;
+                c1 += c.y;
+            }
+        }
+        u_int64_t total;
+        const int before = (int)cta_scan((u_int64_t)(c1 + c0), s_warp, total);
+        if (before < need && need <= before + c1) {
+            s_prefix = prefix | (uint32_t)b1 << shift;
+            s_need = need - before;
+        } else if (before + c1 < need && need <= before + c1 + c0) {
+            s_prefix = prefix | (uint32_t)b0 << shift;
+            s_need = need - before - c1;
+        }
+        meet();  // the counts are read
+        prefix = s_prefix;
+        need = s_need;
+        __syncthreads();
+    }
+    // prefix is the n_keep-th largest key; the first `need` rows that have it stay
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+        const bool some = row0 + i * kEvThreads + tid < a.n_rows;
+        const unsigned gt = __ballot_sync(0xffffffffu, some && key[i] > prefix);
+        const unsigned eq = __ballot_sync(0xffffffffu, some && key[i] == prefix);
+        if (lane == 0) {
+            s_gt[32 * i + warp] = gt;
+            s_eq[32 * i + warp] = eq;
+        }
+    }
+    if (a.weight_out != a.weight || (a.positions && a.positions_out != a.positions))
+#pragma unroll 4
+        for (int i = 0; i < KPT; ++i) {
+            const int row = row0 + i * kEvThreads + tid;
+            if (row >= a.n_keep) break;
+            if (a.weight_out != a.weight)
+                a.weight_out[(size_t)h * a.out_stride + row] = a.weight[(size_t)h * a.row_stride + row];
+            if (a.positions && a.positions_out != a.positions)
+                a.positions_out[(size_t)h * a.out_stride + row] = a.positions[(size_t)h * a.row_stride + row];
+        }
+    __syncthreads();
+    // a word per thread; counts of the CTAs before this one
+    uint32_t keep = tid < kWords ? s_gt[tid] : 0u;
+    const uint32_t eq = tid < kWords ? s_eq[tid] : 0u;
+    u_int64_t total;
+    int before = (int)cta_scan((u_int64_t)__popc(eq), s_warp, total);
+    if (size > 1) {
+        if (tid == 0) s_count[0] = (int)total;
+        cluster.sync();
+        for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&s_count[0], r);
+    }
+    uint32_t left = eq;
+    for (int r = min(__popc(eq), max(0, need - before)); r > 0; --r) {
+        keep |= left & (0u - left);
+        left &= left - 1;
+    }
+    // rows of this word below n_keep, and rows that exist
+    const int i0 = row0 + tid * 32;
+    const uint32_t low = i0 >= a.n_keep ? 0u : a.n_keep - i0 >= 32 ? ~0u : (1u << (a.n_keep - i0)) - 1;
+    uint32_t free_bits = tid < kWords ? low & ~keep : 0u;
+    uint32_t move_bits = keep & ~low;
+    const u_int64_t pre = cta_scan((u_int64_t)__popc(free_bits) << 32 | __popc(move_bits), s_warp, total);
+    int pt = (int)(pre >> 32), pf = (int)(uint32_t)pre;
+    int n_to = (int)(total >> 32);  // of the whole head, = the moving rows
+    if (size > 1) {
+        if (tid == 0) {
+            s_count[1] = (int)(total >> 32);
+            s_count[2] = (int)(uint32_t)total;
+        }
+        cluster.sync();
+        n_to = 0;
+        for (int r = 0; r < size; ++r) {
+            const int* c = cluster.map_shared_rank(&s_count[0], r);
+            if (r < rank) {
+                pt += c[1];
+                pf += c[2];
+            }
+            n_to += c[1];
+        }
+    }
+    int32_t* count = a.moves + (size_t)h * (1 + 2 * (size_t)a.max_moves);
+    int32_t* to = count + 1;
+    int32_t* from = to + a.max_moves;
+    for (; free_bits; free_bits &= free_bits - 1) to[pt++] = i0 + __ffs(free_bits) - 1;
+    for (; move_bits; move_bits &= move_bits - 1) from[pf++] = i0 + __ffs(move_bits) - 1;
+    if (tid == 0 && rank == 0) *count = n_to;
+    if (a.here) {  // few rows: moved by the cluster itself
+        meet();
+        for (int i = (warp * size + rank) * kEvMoveRows; i < n_to; i += 32 * size * kEvMoveRows)
+            evict_move_rows(a, h, to, from, n_to, i, lane);
+    } else if (size > 1) {
+        cluster.sync();  // no CTA leaves while another may read its counts
+    }
+}
+
+// Any number of rows: one CTA per KV head, which reads the weights in every pass.
+__global__ void __launch_bounds__(kEvThreads) evict_select_many_kernel(const EvictArgs a) {
+    __shared__ int hist[kEvBins];
+    __shared__ u_int64_t s_warp[32];
+    __shared__ uint32_t s_prefix;
+    __shared__ int s_need;
+    pdl_launch_dependents();
+    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t prefix = 0;
+    int need = a.n_keep;
+    int shift = 32;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int bits = pass < 2 ? 11 : 10;
+        const uint32_t high = shift == 32 ? 0u : ~0u << shift;
+        shift -= bits;
+        for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = 0;
+        __syncthreads();
         for (int base = 0; base < a.n_rows; base += kEvThreads) {
             const int i = base + tid;
             const uint32_t k = i < a.n_rows ? evict_key(a, h, i) : 0u;
             const bool in = i < a.n_rows && (k & high) == prefix;
             const uint32_t d = (k >> shift) & ((1u << bits) - 1);
-            int same;
             const unsigned act = __ballot_sync(0xffffffffu, in);
-            if (!in) continue;
-            __match_all_sync(act, d, &same);
-            if (same) {  // rows of equal weight: one addition for the warp
-                if (lane == __ffs(act) - 1) atomicAdd(&hist[d], __popc(act));
-            } else {
-                atomicAdd(&hist[d], 1);
-            }
+            if (!act) continue;
+            const uint32_t d0 = __shfl_sync(0xffffffffu, d, __ffs(act) - 1);
+            const unsigned same = __ballot_sync(0xffffffffu, in && d == d0);
+            if (lane == 0) atomicAdd(&hist[d0], __popc(same));
+            if (in && d != d0) atomicAdd(&hist[d], 1);
         }
         __syncthreads();
-        // bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t
         const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
         const int c1 = hist[b1], c0 = hist[b0];
         u_int64_t total;
@@ -508,7 +699,6 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         need = s_need;
         __syncthreads();
     }
-    // prefix is the n_keep-th largest key; the first `need` rows that have it stay
     uint32_t* above = a.masks + (size_t)h * 2 * a.words;
     uint32_t* at = above + a.words;
     for (int w = warp; w < a.words; w += kEvThreads / 32) {
@@ -521,12 +711,12 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
             at[w] = eq;
         }
     }
-    if (a.weight_out != a.weight)
-        for (int i = tid; i < a.n_keep; i += kEvThreads)
+    for (int i = tid; i < a.n_keep; i += kEvThreads) {
+        if (a.weight_out != a.weight)
             a.weight_out[(size_t)h * a.out_stride + i] = a.weight[(size_t)h * a.row_stride + i];
-    if (a.positions && a.positions_out != a.positions)
-        for (int i = tid; i < a.n_keep; i += kEvThreads)
+        if (a.positions && a.positions_out != a.positions)
             a.positions_out[(size_t)h * a.out_stride + i] = a.positions[(size_t)h * a.row_stride + i];
+    }
     __syncthreads();
     int32_t* count = a.moves + (size_t)h * (1 + 2 * (size_t)a.max_moves);
     int32_t* to = count + 1;
@@ -544,7 +734,6 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
             keep |= left & (0u - left);
             left &= left - 1;
         }
-        // rows of this word below n_keep, and rows that exist
         const int i0 = w * 32;
         const uint32_t low = i0 >= a.n_keep ? 0u : a.n_keep - i0 >= 32 ? ~0u : (1u << (a.n_keep - i0)) - 1;
         uint32_t free_bits = w < a.words ? low & ~keep : 0u;
@@ -561,7 +750,6 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
 }
 
 constexpr int kEvMoveThreads = 256;
-constexpr int kEvMoveRows = 4;  // rows in flight per warp
 
 __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const EvictArgs a) {
     const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -570,40 +758,9 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const EvictA
     const int32_t* to = count + 1;
     const int32_t* from = to + a.max_moves;
     const int n = *count;
-    const int hd4 = a.hd / 4;
-    const size_t ps = (size_t)a.n_kv * a.hd;
     for (int i0 = (blockIdx.x * (kEvMoveThreads / 32) + warp) * kEvMoveRows; i0 < n;
-         i0 += gridDim.x * (kEvMoveThreads / 32) * kEvMoveRows) {
-        int f[kEvMoveRows], t[kEvMoveRows];
-#pragma unroll
-        for (int r = 0; r < kEvMoveRows; ++r) {
-            const int i = min(i0 + r, n - 1);
-            f[r] = from[i];
-            t[r] = to[i];
-        }
-        for (int c = lane; c < hd4; c += 32) {
-            float4 k[kEvMoveRows], v[kEvMoveRows];
-#pragma unroll
-            for (int r = 0; r < kEvMoveRows; ++r) {
-                const size_t at = (size_t)f[r] * ps + (size_t)h * a.hd + 4 * c;
-                k[r] = __ldcs(reinterpret_cast<const float4*>(a.kc + at));
-                v[r] = __ldcs(reinterpret_cast<const float4*>(a.vc + at));
-            }
-#pragma unroll
-            for (int r = 0; r < kEvMoveRows; ++r)
-                if (i0 + r < n) {
-                    const size_t at = (size_t)t[r] * ps + (size_t)h * a.hd + 4 * c;
-                    *reinterpret_cast<float4*>(a.kc + at) = k[r];
-                    *reinterpret_cast<float4*>(a.vc + at) = v[r];
-                }
-        }
-        if (lane < kEvMoveRows && i0 + lane < n) {
-            const int ff = from[i0 + lane], tt = to[i0 + lane];
-            a.weight_out[(size_t)h * a.out_stride + tt] = a.weight[(size_t)h * a.row_stride + ff];
-            if (a.positions)
-                a.positions_out[(size_t)h * a.out_stride + tt] = a.positions[(size_t)h * a.row_stride + ff];
-        }
-    }
+         i0 += gridDim.x * (kEvMoveThreads / 32) * kEvMoveRows)
+        evict_move_rows(a, h, to, from, n, i0, lane);
 }
 
 static int evict_max_moves(int n_rows, int n_keep) { return n_keep < n_rows - n_keep ? n_keep : n_rows - n_keep; }
@@ -617,11 +774,33 @@ int evict_launch(float* kc, float* vc, const float* weight, const int32_t* posit
                  int n_keep, int recent_pos, int n_kv, int hd, float* weight_out, int32_t* positions_out,
                  int out_stride, void* ws, cudaStream_t st) {
     EvictArgs a{kc, vc, weight, positions, row_stride, n_rows, n_keep, recent_pos, n_kv, hd, weight_out, positions_out,
-                out_stride, static_cast<int32_t*>(ws), evict_max_moves(n_rows, n_keep), nullptr, (n_rows + 31) / 32};
+                out_stride, static_cast<int32_t*>(ws), evict_max_moves(n_rows, n_keep), nullptr, (n_rows + 31) / 32, false};
     a.masks = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(ws) +
                                           ((size_t)n_kv * (1 + 2 * (size_t)a.max_moves) * 4 + 255) / 256 * 256);
-    evict_select_kernel<<<n_kv, kEvThreads, 0, st>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    const int cluster = n_rows <= kEvSpread ? 1 : 8;
+    const int64_t per_thread = ((int64_t)n_rows + cluster * kEvThreads - 1) / (cluster * kEvThreads);
+    if (per_thread > 16) {
+        evict_select_many_kernel<<<n_kv, kEvThreads, 0, st>>>(a);
+        if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    } else {
+        a.here = a.max_moves <= kEvHere;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(cluster, n_kv);
+        cfg.blockDim = dim3(kEvThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = per_thread <= 4   ? cudaLaunchKernelEx(&cfg, evict_select_kernel<4>, a)
+                              : per_thread <= 8 ? cudaLaunchKernelEx(&cfg, evict_select_kernel<8>, a)
+                                                : cudaLaunchKernelEx(&cfg, evict_select_kernel<16>, a);
+        if (e != cudaSuccess) return kErrCuda;
+        if (a.here) return kOk;
+    }
     if (a.max_moves == 0) return kOk;
     const int per_cta = kEvMoveThreads / 32 * kEvMoveRows;
     int gx = (a.max_moves + per_cta - 1) / per_cta;

@@ -388,7 +388,8 @@ def evict_weights(kind, nkv, n, seed):
 
 
 EVICTS = [(1, 4, 1, 1), (1, 4, 2, 1), (2, 64, 33, 32), (2, 64, 64, 33), (3, 80, 100, 7), (8, 128, 1000, 999), (4, 128, 1025, 512),
-          (2, 256, 5000, 1234), (8, 64, 4097, 4096), (1, 128, 40000, 100), (2, 20, 70001, 35001), (5, 12, 31, 31), (1, 300, 96, 48)]
+          (2, 256, 5000, 1234), (8, 64, 4097, 4096), (1, 128, 40000, 100), (2, 20, 70001, 35001), (5, 12, 31, 31), (1, 300, 96, 48),
+          (1, 4, 8192, 5000), (2, 4, 8193, 8192), (1, 4, 140001, 70000), (1, 4, 140001, 140000)]
 
 
 @pytest.mark.parametrize("nkv,hd,n,keep", EVICTS)
