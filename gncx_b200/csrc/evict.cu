@@ -429,37 +429,34 @@ struct EvictArgs {
 
 // Greater keys stay: protected rows, then the weights in order, NaN last.
 __device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, int h, int i) {
-    if (a.positions && a.positions[(size_t)h * a.row_stride + i] >= a.recent_pos) return 0xFFFFFFFFu;
     const float w = a.weight[(size_t)h * a.row_stride + i];
-    if (w != w) return 0u;
+    const bool late = a.positions && a.positions[(size_t)h * a.row_stride + i] >= a.recent_pos;
     const uint32_t u = __float_as_uint(w + 0.0f);  // -0 as +0
-    return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+    return late ? 0xFFFFFFFFu : w != w ? 0u : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-// Exclusive prefix sum of one value per thread over the CTA, and the total.
-__device__ __forceinline__ u_int64_t cta_scan(u_int64_t v, u_int64_t* s_warp, u_int64_t& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    u_int64_t x = v;
+// Exclusive prefix sum of one value per thread over the CTA (32 warps), and the
+// total; s_warp holds 32 values, and the next scan uses another array.
+template <class T>
+__device__ __forceinline__ T cta_scan(T v, T* s_warp, T& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u_int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    __syncthreads();
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        u_int64_t w = lane < nw ? s_warp[lane] : 0;
+    T w = s_warp[lane];  // every warp sums the warps' totals for itself
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u_int64_t y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
-        }
-        s_warp[lane] = w;
+    for (int o = 1; o < 32; o <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
     }
-    __syncthreads();
-    total = s_warp[nw - 1];
-    return x - v + (warp ? s_warp[warp - 1] : 0);
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const T before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+    return x - v + (warp ? before : T(0));
 }
 
 // Copy rows of KV head h: the i-th free row takes the i-th moving row, for i0,
@@ -505,12 +502,15 @@ __device__ __forceinline__ void evict_move_rows(const EvictArgs& a, int h, const
 template <int KPT>
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs a) {
     constexpr int kWords = 32 * KPT;  // of 32 rows, per CTA
-    __shared__ __align__(16) int hist[kEvBins];
-    __shared__ u_int64_t s_warp[32];
+    static_assert(kEvThreads == 1024, "32 warps, and a word per thread where KPT is 32");
+    __shared__ __align__(16) int hist[3][kEvBins];
+    __shared__ int s_scan[4][32];
+    __shared__ u_int64_t s_scan2[32];
     __shared__ uint32_t s_gt[kWords], s_eq[kWords];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_need;
-    __shared__ int s_count[3];  // of this CTA: ties, free rows, moving rows
+    __shared__ uint32_t s_prefix[3];
+    __shared__ int s_need[3], s_ties;  // need of each pass; how many rows have the last key
+    __shared__ int s_count[2];         // of this CTA: free rows, moving rows
+    __shared__ int32_t s_to[kEvHere], s_from[kEvHere];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -527,17 +527,18 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         const int row = row0 + i * kEvThreads + tid;
         key[i] = row < a.n_rows ? evict_key(a, h, row) : 0u;
     }
+    for (int i = tid; i < 3 * kEvBins; i += kEvThreads) hist[0][i] = 0;
+    __syncthreads();
     // The n_keep-th largest key by digits of 11, 11 and 10 bits from the top:
     // each pass counts the keys that share the digits found so far.
     uint32_t prefix = 0;
     int need = a.n_keep;  // how many of the keys that share the prefix stay
     int shift = 32;
+#pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int bits = pass < 2 ? 11 : 10;
         const uint32_t high = shift == 32 ? 0u : ~0u << shift;  // the digits found so far
         shift -= bits;
-        for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = 0;
-        __syncthreads();
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
             const bool in = row0 + i * kEvThreads + tid < a.n_rows && (key[i] & high) == prefix;
@@ -547,37 +548,40 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
             // rows of equal digits (equal weights, a shared exponent): one addition for the warp
             const uint32_t d0 = __shfl_sync(0xffffffffu, d, __ffs(act) - 1);
             const unsigned same = __ballot_sync(0xffffffffu, in && d == d0);
-            if (lane == 0) atomicAdd(&hist[d0], __popc(same));
-            if (in && d != d0) atomicAdd(&hist[d], 1);
+            if (lane == 0) atomicAdd(&hist[pass][d0], __popc(same));
+            if (in && d != d0) atomicAdd(&hist[pass][d], 1);
         }
         meet();
         // bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t
         const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
-        int c1 = hist[b1], c0 = hist[b0];
-        if (size > 1) {
-            c0 = c1 = 0;
+        int c0 = 0, c1 = 0;
+        if (size == 1) {
+            c0 = hist[pass][b0];
+            c1 = hist[pass][b1];
+        } else {
 #pragma unroll 8
             for (int r = 0; r < size; ++r) {
-                const int2 c = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[b0], r));
+                const int2 c = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[pass][b0], r));
                 c0 += c.x;
                 c1 += c.y;
             }
         }
-        u_int64_t total;
-        const int before = (int)cta_scan((u_int64_t)(c1 + c0), s_warp, total);
+        int total;
+        const int before = cta_scan(c1 + c0, s_scan[pass], total);
         if (before < need && need <= before + c1) {
-            s_prefix = prefix | (uint32_t)b1 << shift;
-            s_need = need - before;
+            s_prefix[pass] = prefix | (uint32_t)b1 << shift;
+            s_need[pass] = need - before;
+            s_ties = c1;
         } else if (before + c1 < need && need <= before + c1 + c0) {
-            s_prefix = prefix | (uint32_t)b0 << shift;
-            s_need = need - before - c1;
+            s_prefix[pass] = prefix | (uint32_t)b0 << shift;
+            s_need[pass] = need - before - c1;
+            s_ties = c0;
         }
-        meet();  // the counts are read
-        prefix = s_prefix;
-        need = s_need;
         __syncthreads();
+        prefix = s_prefix[pass];
+        need = s_need[pass];
     }
-    // prefix is the n_keep-th largest key; the first `need` rows that have it stay
+    // prefix is the n_keep-th largest key; the first `need` of the s_ties rows that have it stay
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
         const bool some = row0 + i * kEvThreads + tid < a.n_rows;
@@ -599,48 +603,54 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
                 a.positions_out[(size_t)h * a.out_stride + row] = a.positions[(size_t)h * a.row_stride + row];
         }
     __syncthreads();
-    // a word per thread; counts of the CTAs before this one
+    // a word per thread
     uint32_t keep = tid < kWords ? s_gt[tid] : 0u;
     const uint32_t eq = tid < kWords ? s_eq[tid] : 0u;
-    u_int64_t total;
-    int before = (int)cta_scan((u_int64_t)__popc(eq), s_warp, total);
-    if (size > 1) {
-        if (tid == 0) s_count[0] = (int)total;
-        cluster.sync();
-        for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&s_count[0], r);
-    }
-    uint32_t left = eq;
-    for (int r = min(__popc(eq), max(0, need - before)); r > 0; --r) {
-        keep |= left & (0u - left);
-        left &= left - 1;
+    if (need == s_ties) {
+        keep |= eq;
+    } else {
+        int total;
+        int before = cta_scan(__popc(eq), s_scan[3], total);
+        // the rows of the CTAs before this one that have the key: their bin of the last pass
+        for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&hist[2][prefix & 1023u], r);
+        uint32_t left = eq;
+        for (int r = min(__popc(eq), max(0, need - before)); r > 0; --r) {
+            keep |= left & (0u - left);
+            left &= left - 1;
+        }
     }
     // rows of this word below n_keep, and rows that exist
     const int i0 = row0 + tid * 32;
     const uint32_t low = i0 >= a.n_keep ? 0u : a.n_keep - i0 >= 32 ? ~0u : (1u << (a.n_keep - i0)) - 1;
     uint32_t free_bits = tid < kWords ? low & ~keep : 0u;
     uint32_t move_bits = keep & ~low;
-    const u_int64_t pre = cta_scan((u_int64_t)__popc(free_bits) << 32 | __popc(move_bits), s_warp, total);
+    u_int64_t total;
+    const u_int64_t pre = cta_scan((u_int64_t)__popc(free_bits) << 32 | __popc(move_bits), s_scan2, total);
     int pt = (int)(pre >> 32), pf = (int)(uint32_t)pre;
     int n_to = (int)(total >> 32);  // of the whole head, = the moving rows
     if (size > 1) {
         if (tid == 0) {
-            s_count[1] = (int)(total >> 32);
-            s_count[2] = (int)(uint32_t)total;
+            s_count[0] = (int)(total >> 32);
+            s_count[1] = (int)(uint32_t)total;
         }
         cluster.sync();
         n_to = 0;
         for (int r = 0; r < size; ++r) {
             const int* c = cluster.map_shared_rank(&s_count[0], r);
             if (r < rank) {
-                pt += c[1];
-                pf += c[2];
+                pt += c[0];
+                pf += c[1];
             }
-            n_to += c[1];
+            n_to += c[0];
         }
     }
     int32_t* count = a.moves + (size_t)h * (1 + 2 * (size_t)a.max_moves);
     int32_t* to = count + 1;
     int32_t* from = to + a.max_moves;
+    if (a.here && size == 1) {
+        to = s_to;
+        from = s_from;
+    }
     for (; free_bits; free_bits &= free_bits - 1) to[pt++] = i0 + __ffs(free_bits) - 1;
     for (; move_bits; move_bits &= move_bits - 1) from[pf++] = i0 + __ffs(move_bits) - 1;
     if (tid == 0 && rank == 0) *count = n_to;
@@ -656,7 +666,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
 // Any number of rows: one CTA per KV head, which reads the weights in every pass.
 __global__ void __launch_bounds__(kEvThreads) evict_select_many_kernel(const EvictArgs a) {
     __shared__ int hist[kEvBins];
-    __shared__ u_int64_t s_warp[32];
+    __shared__ int s_warp[32];
+    __shared__ u_int64_t s_warp2[32];
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
     pdl_launch_dependents();
@@ -685,8 +696,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_many_kernel(const Evi
         __syncthreads();
         const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
         const int c1 = hist[b1], c0 = hist[b0];
-        u_int64_t total;
-        const int before = (int)cta_scan((u_int64_t)(c1 + c0), s_warp, total);
+        int total;
+        const int before = cta_scan(c1 + c0, s_warp, total);
         if (before < need && need <= before + c1) {
             s_prefix = prefix | (uint32_t)b1 << shift;
             s_need = need - before;
@@ -726,9 +737,9 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_many_kernel(const Evi
         const int w = base + tid;
         uint32_t keep = w < a.words ? above[w] : 0u;
         const uint32_t eq = w < a.words ? at[w] : 0u;
-        u_int64_t total;
-        const int before = ties + (int)cta_scan((u_int64_t)__popc(eq), s_warp, total);
-        ties += (int)total;
+        int total;
+        const int before = ties + cta_scan(__popc(eq), s_warp, total);
+        ties += total;
         uint32_t left = eq;
         for (int r = min(__popc(eq), max(0, need - before)); r > 0; --r) {
             keep |= left & (0u - left);
@@ -739,10 +750,12 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_many_kernel(const Evi
         uint32_t free_bits = w < a.words ? low & ~keep : 0u;
         uint32_t move_bits = keep & ~low;
         const u_int64_t mine = (u_int64_t)__popc(free_bits) << 32 | __popc(move_bits);
-        const u_int64_t pre = cta_scan(mine, s_warp, total);
+        u_int64_t sum;
+        const u_int64_t pre = cta_scan(mine, s_warp2, sum);
         int pt = n_to + (int)(pre >> 32), pf = n_from + (int)(uint32_t)pre;
-        n_to += (int)(total >> 32);
-        n_from += (int)(uint32_t)total;
+        n_to += (int)(sum >> 32);
+        n_from += (int)(uint32_t)sum;
+        __syncthreads();  // the scans' arrays are read
         for (; free_bits; free_bits &= free_bits - 1) to[pt++] = i0 + __ffs(free_bits) - 1;
         for (; move_bits; move_bits &= move_bits - 1) from[pf++] = i0 + __ffs(move_bits) - 1;
     }
@@ -803,9 +816,7 @@ int evict_launch(float* kc, float* vc, const float* weight, const int32_t* posit
     }
     if (a.max_moves == 0) return kOk;
     const int per_cta = kEvMoveThreads / 32 * kEvMoveRows;
-    int gx = (a.max_moves + per_cta - 1) / per_cta;
-    const int most = (8 * device_info().sm_count + n_kv - 1) / n_kv;
-    if (gx > most) gx = most;
+    const int gx = (a.max_moves + per_cta - 1) / per_cta;
     return launch_after(evict_move_kernel, dim3(gx, n_kv), dim3(kEvMoveThreads), 0, st, a) == cudaSuccess ? kOk : kErrCuda;
 }
 
