@@ -408,6 +408,7 @@ int weights_step_launch(const float* q, const float* new_k, const float* new_v, 
 // ---------------------------------------------------------------- eviction
 constexpr int kEvThreads = 1024;
 constexpr int kEvSpread = 8192;  // rows above which a cluster of 8 CTAs selects instead of one CTA
+constexpr int kEvOne = 65536;    // rows up to which one CTA looks for the one row to evict
 constexpr int kEvHere = 256;     // moves up to which the selecting kernel makes them
 constexpr int kEvBins = 2048;
 
@@ -428,11 +429,37 @@ struct EvictArgs {
 };
 
 // Greater keys stay: protected rows, then the weights in order, NaN last.
-__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, int h, int i) {
-    const float w = a.weight[(size_t)h * a.row_stride + i];
-    const bool late = a.positions && a.positions[(size_t)h * a.row_stride + i] >= a.recent_pos;
+__device__ __forceinline__ uint32_t evict_key(float w, bool late) {
     const uint32_t u = __float_as_uint(w + 0.0f);  // -0 as +0
     return late ? 0xFFFFFFFFu : w != w ? 0u : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, int h, int i) {
+    const float w = a.weight[(size_t)h * a.row_stride + i];
+    return evict_key(w, a.positions && a.positions[(size_t)h * a.row_stride + i] >= a.recent_pos);
+}
+// The keys of rows row0 + i * kEvThreads + thread (0 past the last row); the
+// sums and positions of those below n_keep go to the outputs at once, where
+// the rows that move in write theirs later.
+template <int KPT>
+__device__ __forceinline__ void evict_load(const EvictArgs& a, int h, int row0, uint32_t (&key)[KPT]) {
+    float w[KPT];
+    int32_t p[KPT];
+    const size_t base = (size_t)h * a.row_stride;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+        const int row = row0 + i * kEvThreads + threadIdx.x;
+        w[i] = row < a.n_rows ? a.weight[base + row] : 0.0f;
+        p[i] = row < a.n_rows && a.positions ? a.positions[base + row] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+        const int row = row0 + i * kEvThreads + threadIdx.x;
+        key[i] = row < a.n_rows ? evict_key(w[i], a.positions && p[i] >= a.recent_pos) : 0u;
+        if (row < a.n_keep) {
+            if (a.weight_out != a.weight) a.weight_out[(size_t)h * a.out_stride + row] = w[i];
+            if (a.positions && a.positions_out != a.positions) a.positions_out[(size_t)h * a.out_stride + row] = p[i];
+        }
+    }
 }
 
 // Exclusive prefix sum of one value per thread over the CTA (32 warps), and the
@@ -461,7 +488,7 @@ __device__ __forceinline__ T cta_scan(T v, T* s_warp, T& total) {
 
 // Copy rows of KV head h: the i-th free row takes the i-th moving row, for i0,
 // i0 + step, .. below n, kEvMoveRows at a time; one warp.
-constexpr int kEvMoveRows = 4;
+constexpr int kEvMoveRows = 2;
 __device__ __forceinline__ void evict_move_rows(const EvictArgs& a, int h, const int32_t* to, const int32_t* from, int n,
                                                 int i0, int lane) {
     const int hd4 = a.hd / 4;
@@ -499,7 +526,7 @@ __device__ __forceinline__ void evict_move_rows(const EvictArgs& a, int h, const
 // One cluster per KV head, each CTA a run of kEvThreads * KPT rows, their keys in
 // registers.  Counts are summed over the cluster through distributed shared
 // memory.
-template <int KPT>
+template <int KPT, int SIZE>
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs a) {
     constexpr int kWords = 32 * KPT;  // of 32 rows, per CTA
     static_assert(kEvThreads == 1024, "32 warps, and a word per thread where KPT is 32");
@@ -509,24 +536,21 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
     __shared__ uint32_t s_gt[kWords], s_eq[kWords];
     __shared__ uint32_t s_prefix[3];
     __shared__ int s_need[3], s_ties;  // need of each pass; how many rows have the last key
-    __shared__ int s_count[2];         // of this CTA: free rows, moving rows
+    __shared__ int2 s_count;           // of this CTA: free rows, moving rows
+    __shared__ u_int64_t s_base[kWords];
     __shared__ int32_t s_to[kEvHere], s_from[kEvHere];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int rank = SIZE > 1 ? (int)cluster.block_rank() : 0;
     auto meet = [&] {
-        if (size > 1) cluster.sync();
+        if (SIZE > 1) cluster.sync();
         else __syncthreads();
     };
     pdl_launch_dependents();
     const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row0 = rank * kEvThreads * KPT;
     uint32_t key[KPT];
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-        const int row = row0 + i * kEvThreads + tid;
-        key[i] = row < a.n_rows ? evict_key(a, h, row) : 0u;
-    }
+    evict_load(a, h, row0, key);
     for (int i = tid; i < 3 * kEvBins; i += kEvThreads) hist[0][i] = 0;
     __syncthreads();
     // The n_keep-th largest key by digits of 11, 11 and 10 bits from the top:
@@ -555,15 +579,17 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         // bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t
         const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
         int c0 = 0, c1 = 0;
-        if (size == 1) {
+        if (SIZE == 1) {
             c0 = hist[pass][b0];
             c1 = hist[pass][b1];
         } else {
-#pragma unroll 8
-            for (int r = 0; r < size; ++r) {
-                const int2 c = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[pass][b0], r));
-                c0 += c.x;
-                c1 += c.y;
+            int2 c[SIZE];
+#pragma unroll
+            for (int r = 0; r < SIZE; ++r) c[r] = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[pass][b0], r));
+#pragma unroll
+            for (int r = 0; r < SIZE; ++r) {
+                c0 += c[r].x;
+                c1 += c[r].y;
             }
         }
         int total;
@@ -592,16 +618,6 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
             s_eq[32 * i + warp] = eq;
         }
     }
-    if (a.weight_out != a.weight || (a.positions && a.positions_out != a.positions))
-#pragma unroll 4
-        for (int i = 0; i < KPT; ++i) {
-            const int row = row0 + i * kEvThreads + tid;
-            if (row >= a.n_keep) break;
-            if (a.weight_out != a.weight)
-                a.weight_out[(size_t)h * a.out_stride + row] = a.weight[(size_t)h * a.row_stride + row];
-            if (a.positions && a.positions_out != a.positions)
-                a.positions_out[(size_t)h * a.out_stride + row] = a.positions[(size_t)h * a.row_stride + row];
-        }
     __syncthreads();
     // a word per thread
     uint32_t keep = tid < kWords ? s_gt[tid] : 0u;
@@ -612,7 +628,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         int total;
         int before = cta_scan(__popc(eq), s_scan[3], total);
         // the rows of the CTAs before this one that have the key: their bin of the last pass
-        for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&hist[2][prefix & 1023u], r);
+        if (SIZE > 1)
+            for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&hist[2][prefix & 1023u], r);
         uint32_t left = eq;
         for (int r = min(__popc(eq), max(0, need - before)); r > 0; --r) {
             keep |= left & (0u - left);
@@ -622,45 +639,91 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
     // rows of this word below n_keep, and rows that exist
     const int i0 = row0 + tid * 32;
     const uint32_t low = i0 >= a.n_keep ? 0u : a.n_keep - i0 >= 32 ? ~0u : (1u << (a.n_keep - i0)) - 1;
-    uint32_t free_bits = tid < kWords ? low & ~keep : 0u;
-    uint32_t move_bits = keep & ~low;
+    const uint32_t free_bits = tid < kWords ? low & ~keep : 0u, move_bits = keep & ~low;
     u_int64_t total;
     const u_int64_t pre = cta_scan((u_int64_t)__popc(free_bits) << 32 | __popc(move_bits), s_scan2, total);
-    int pt = (int)(pre >> 32), pf = (int)(uint32_t)pre;
-    int n_to = (int)(total >> 32);  // of the whole head, = the moving rows
-    if (size > 1) {
-        if (tid == 0) {
-            s_count[0] = (int)(total >> 32);
-            s_count[1] = (int)(uint32_t)total;
-        }
+    if (tid < kWords) {
+        s_base[tid] = pre;
+        s_gt[tid] = free_bits;
+        s_eq[tid] = move_bits;
+    }
+    int n_to = (int)(total >> 32), pt0 = 0, pf0 = 0;  // of the whole head (= the moving rows); of the CTAs before
+    if (SIZE > 1) {
+        if (tid == 0) s_count = make_int2((int)(total >> 32), (int)(uint32_t)total);
         cluster.sync();
+        int2 c[SIZE];
+#pragma unroll
+        for (int r = 0; r < SIZE; ++r) c[r] = *cluster.map_shared_rank(&s_count, r);
         n_to = 0;
-        for (int r = 0; r < size; ++r) {
-            const int* c = cluster.map_shared_rank(&s_count[0], r);
+#pragma unroll
+        for (int r = 0; r < SIZE; ++r) {
             if (r < rank) {
-                pt += c[0];
-                pf += c[1];
+                pt0 += c[r].x;
+                pf0 += c[r].y;
             }
-            n_to += c[0];
+            n_to += c[r].x;
         }
+    } else {
+        __syncthreads();
     }
     int32_t* count = a.moves + (size_t)h * (1 + 2 * (size_t)a.max_moves);
     int32_t* to = count + 1;
     int32_t* from = to + a.max_moves;
-    if (a.here && size == 1) {
+    if (a.here && SIZE == 1) {
         to = s_to;
         from = s_from;
     }
-    for (; free_bits; free_bits &= free_bits - 1) to[pt++] = i0 + __ffs(free_bits) - 1;
-    for (; move_bits; move_bits &= move_bits - 1) from[pf++] = i0 + __ffs(move_bits) - 1;
+    for (int w = warp; w < kWords; w += kEvThreads / 32) {  // a word per warp, a row per lane
+        const uint32_t f = s_gt[w], m = s_eq[w], below = (1u << lane) - 1;
+        const u_int64_t at = s_base[w];
+        const int row = row0 + 32 * w + lane;
+        if (f >> lane & 1) to[pt0 + (int)(at >> 32) + __popc(f & below)] = row;
+        if (m >> lane & 1) from[pf0 + (int)(uint32_t)at + __popc(m & below)] = row;
+    }
     if (tid == 0 && rank == 0) *count = n_to;
     if (a.here) {  // few rows: moved by the cluster itself
         meet();
-        for (int i = (warp * size + rank) * kEvMoveRows; i < n_to; i += 32 * size * kEvMoveRows)
+        for (int i = (warp * SIZE + rank) * kEvMoveRows; i < n_to; i += 32 * SIZE * kEvMoveRows)
             evict_move_rows(a, h, to, from, n_to, i, lane);
-    } else if (size > 1) {
+    } else if (SIZE > 1) {
         cluster.sync();  // no CTA leaves while another may read its counts
     }
+}
+
+// One row to evict, the steady state of a full cache: the row with the least key
+// (of equal ones the last) is overwritten by the row behind the first n_keep.
+// One CTA per KV head.
+__global__ void __launch_bounds__(kEvThreads) evict_one_kernel(const EvictArgs a) {
+    constexpr int KPT = 4;
+    __shared__ u_int64_t s_least[32];
+    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u_int64_t least = ~(u_int64_t)0;
+    for (int row0 = 0; row0 < a.n_rows; row0 += kEvThreads * KPT) {
+        uint32_t key[KPT];
+        evict_load(a, h, row0, key);
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) {
+            const int row = row0 + i * kEvThreads + tid;
+            const u_int64_t k = (u_int64_t)key[i] << 32 | (0xFFFFFFFFu - (uint32_t)row);
+            if (row < a.n_rows && k < least) least = k;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const u_int64_t y = __shfl_xor_sync(0xffffffffu, least, o);
+        least = y < least ? y : least;
+    }
+    if (lane == 0) s_least[warp] = least;
+    __syncthreads();
+    if (warp > 0) return;
+    least = s_least[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const u_int64_t y = __shfl_xor_sync(0xffffffffu, least, o);
+        least = y < least ? y : least;
+    }
+    const int32_t to = (int32_t)(0xFFFFFFFFu - (uint32_t)least), from = a.n_keep;
+    if (to < a.n_keep) evict_move_rows(a, h, &to, &from, 1, 0, lane);
 }
 
 // Any number of rows: one CTA per KV head, which reads the weights in every pass.
@@ -790,6 +853,10 @@ int evict_launch(float* kc, float* vc, const float* weight, const int32_t* posit
                 out_stride, static_cast<int32_t*>(ws), evict_max_moves(n_rows, n_keep), nullptr, (n_rows + 31) / 32, false};
     a.masks = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(ws) +
                                           ((size_t)n_kv * (1 + 2 * (size_t)a.max_moves) * 4 + 255) / 256 * 256);
+    if (n_rows - n_keep == 1 && n_rows <= kEvOne) {
+        evict_one_kernel<<<n_kv, kEvThreads, 0, st>>>(a);
+        return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+    }
     const int cluster = n_rows <= kEvSpread ? 1 : 8;
     const int64_t per_thread = ((int64_t)n_rows + cluster * kEvThreads - 1) / (cluster * kEvThreads);
     if (per_thread > 16) {
@@ -808,9 +875,11 @@ int evict_launch(float* kc, float* vc, const float* weight, const int32_t* posit
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        const cudaError_t e = per_thread <= 4   ? cudaLaunchKernelEx(&cfg, evict_select_kernel<4>, a)
-                              : per_thread <= 8 ? cudaLaunchKernelEx(&cfg, evict_select_kernel<8>, a)
-                                                : cudaLaunchKernelEx(&cfg, evict_select_kernel<16>, a);
+        auto go = [&](auto k) { return cudaLaunchKernelEx(&cfg, k, a); };
+        const cudaError_t e = cluster == 1 ? (per_thread <= 4 ? go(evict_select_kernel<4, 1>) : go(evict_select_kernel<8, 1>))
+                              : per_thread <= 4 ? go(evict_select_kernel<4, 8>)
+                              : per_thread <= 8 ? go(evict_select_kernel<8, 8>)
+                                                : go(evict_select_kernel<16, 8>);
         if (e != cudaSuccess) return kErrCuda;
         if (a.here) return kOk;
     }
