@@ -243,8 +243,12 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     __shared__ uint32_t s_t[kWarps];
     __shared__ float s_m[kWarps];
     __shared__ double s_l[kWarps];
-    pdl_launch_dependents();
     const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) s_cnt = 0;
+    if (tid < 16) s_tab[tid] = exp2(tid / 16.0);
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
     if (finished && finished[b]) return;  // the merge does not look at an ended beam's lists
     const float* x = logits + (size_t)b * vocab;
     const int i0 = part * per, i1 = min(vocab, i0 + per);
@@ -252,9 +256,6 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     double l = 0.0;
     bool bad = false;
     u64 T = 0;
-    if (tid == 0) s_cnt = 0;
-    if (tid < 16) s_tab[tid] = exp2(tid / 16.0);
-    __syncthreads();
     float ahead[kBsPer];  // the next tile's logits
     auto load = [&](int base) {
 #pragma unroll
@@ -496,6 +497,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     const int tid = threadIdx.x;
     if (tid == 0) s_cnt = s_live = s_full = 0;
     __syncthreads();
+    pdl_wait();
     // the beams' scores; NaN for a beam without lists (ended, or no candidate can be better than none)
     for (int b = tid; b < n_beam; b += kBmThreads) {
         const float s = scores[b];
@@ -504,7 +506,6 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
         if (live) atomicAdd(&s_live, 1);
         else if (s > -INFINITY) list[atomicAdd(&s_cnt, 1)] = BeamKey{ord64((double)s), ~((u64)b << 56 | (u64)eos)};
     }
-    pdl_wait();
     __syncthreads();
     // a thread per list; the first entries of all lists are on their way while the beams' sums are formed
     const int lists = n_beam * parts;  // < kBmThreads
@@ -722,8 +723,9 @@ int beam_select_launch(const float* logits, const float* scores, const int32_t* 
     u64* keys = static_cast<u64*>(ws);
     const size_t lists = (size_t)n_beam * parts;
     BeamPart* stats = reinterpret_cast<BeamPart*>(static_cast<uint8_t*>(ws) + (lists * n_out * sizeof(u64) + 255) / 256 * 256);
-    beam_part_kernel<<<dim3(parts, n_beam), kBsThreads, 0, st>>>(logits, finished, vocab, parts, per, n_out, keys, stats);
-    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    if (launch_after(beam_part_kernel, dim3(parts, n_beam), dim3(kBsThreads), 0, st, logits, finished, vocab, parts, per,
+                     n_out, keys, stats) != cudaSuccess)
+        return kErrCuda;
     return launch_after(beam_merge_kernel, dim3(1), dim3(kBmThreads), 0, st, (const u64*)keys, (const BeamPart*)stats,
                         scores, finished, n_beam, parts, n_out, eos, out_scores, out_parents, out_tokens,
                         out_finished) == cudaSuccess
@@ -765,6 +767,7 @@ template <class V, int N>
 __global__ void __launch_bounds__(256) reorder_regs_kernel(const ReorderArgs a) {
     __shared__ int2 s_move[N];
     __shared__ int s_n;
+    pdl_wait();
     const int m = reorder_moves(a, s_move, &s_n);
     if (m == 0) return;
     const size_t c = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -786,6 +789,7 @@ __global__ void reorder_smem_kernel(const ReorderArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int2 s_move[kReorderMaxSlots];
     __shared__ int s_n;
+    pdl_wait();
     const int m = reorder_moves(a, s_move, &s_n);
     if (m == 0) return;
     const size_t c = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -808,18 +812,17 @@ static cudaError_t reorder_launch_v(ReorderArgs a, size_t n_bytes, cudaStream_t 
     const int gy = a.n_states < 65535 ? a.n_states : 65535;
     if (a.n_slots <= kReorderRegs) {
         const dim3 grid((unsigned)((a.cols + threads - 1) / threads), gy);
-        if (a.n_slots <= 4) reorder_regs_kernel<V, 4><<<grid, threads, 0, st>>>(a);
-        else if (a.n_slots <= 8) reorder_regs_kernel<V, 8><<<grid, threads, 0, st>>>(a);
-        else reorder_regs_kernel<V, kReorderRegs><<<grid, threads, 0, st>>>(a);
-        return cudaGetLastError();
+        auto go = [&](auto k) { return launch_after(k, grid, dim3(threads), 0, st, a); };
+        return a.n_slots <= 4   ? go(reorder_regs_kernel<V, 4>)
+               : a.n_slots <= 8 ? go(reorder_regs_kernel<V, 8>)
+                                : go(reorder_regs_kernel<V, kReorderRegs>);
     }
     while (threads > 32 && (size_t)threads * a.n_slots * sizeof(V) > 64 * 1024) threads >>= 1;
     const size_t smem = (size_t)threads * a.n_slots * sizeof(V);
     const cudaError_t e = set_smem_limit(reorder_smem_kernel<V>, smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)((a.cols + threads - 1) / threads), gy);
-    reorder_smem_kernel<V><<<grid, threads, smem, st>>>(a);
-    return cudaGetLastError();
+    return launch_after(reorder_smem_kernel<V>, grid, dim3(threads), smem, st, a);
 }
 
 int reorder_launch(void* state, int n_states, size_t state_stride, int n_slots, size_t slot_stride, size_t n_bytes,

@@ -101,7 +101,6 @@ __global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const Weigh
     extern __shared__ __align__(16) float ost[];  // [warp][GT][hd]
     __shared__ float wsh[kWsWarps][SUB * NV + GT];
     __shared__ float mst[kWsWarps][GT], lst[kWsWarps][GT];
-    pdl_launch_dependents();
     const int part = blockIdx.x, kvh = blockIdx.y, h0 = kvh * a.G + blockIdx.z * GT;
     const int heads = min(GT, a.G - (int)blockIdx.z * GT);
     const int len = a.pos + 1;
@@ -118,6 +117,8 @@ __global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const Weigh
         col[j] = 4 * (lr + j * LPR);
         on[j] = col[j] < a.hd;
     }
+    pdl_wait();
+    pdl_launch_dependents();
     float4 q[GT][NJ], o[GT][NJ];
 #pragma unroll
     for (int g = 0; g < GT; ++g)
@@ -302,6 +303,18 @@ __global__ void __launch_bounds__(kWsThreads) weights_merge_kernel(const Weights
     float w[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) w[i] = 0.0f;
+    // the first heads' scores and the sums are on their way while the maxima are formed
+    constexpr int kEarly = 4;
+    const float* s0 = a.scores + (size_t)kvh * a.G * a.score_ld;
+    float* wt = a.weight + (size_t)kvh * a.row_stride;
+    float early[kEarly][kPer], old[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int t = t0 + i * kWsThreads;
+        old[i] = t <= a.pos ? wt[t] : 0.0f;
+#pragma unroll
+        for (int g = 0; g < kEarly; ++g) early[g][i] = t <= a.pos && g < a.G ? s0[g * a.score_ld + t] : 0.0f;
+    }
     for (int g0 = 0; g0 < a.G; g0 += kWsWarps) {
         __syncthreads();
         if (g0 + warp < a.G) {
@@ -313,8 +326,16 @@ __global__ void __launch_bounds__(kWsThreads) weights_merge_kernel(const Weights
             }
         }
         __syncthreads();
-        for (int g = 0; g < min(kWsWarps, a.G - g0); ++g) {
-            const float* s = a.scores + (size_t)(kvh * a.G + g0 + g) * a.score_ld;
+        if (g0 == 0) {
+#pragma unroll
+            for (int g = 0; g < kEarly; ++g)
+                if (g < a.G) {
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) w[i] = fmaf(__expf(early[g][i] - s_M[g]), s_inv[g], w[i]);
+                }
+        }
+        for (int g = g0 == 0 ? kEarly : 0; g < min(kWsWarps, a.G - g0); ++g) {
+            const float* s = s0 + (size_t)(g0 + g) * a.score_ld;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int t = t0 + i * kWsThreads;
@@ -322,13 +343,12 @@ __global__ void __launch_bounds__(kWsThreads) weights_merge_kernel(const Weights
             }
         }
     }
-    float* wt = a.weight + (size_t)kvh * a.row_stride;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int t = t0 + i * kWsThreads;
         if (t > a.pos) continue;
         const bool fresh = a.new_k && t == a.pos;  // the new row's sum starts here
-        wt[t] = fresh ? w[i] : wt[t] + w[i];
+        wt[t] = fresh ? w[i] : old[i] + w[i];
         if (fresh && a.positions) a.positions[(size_t)kvh * a.row_stride + t] = a.token_pos;
     }
 }
@@ -356,8 +376,7 @@ static cudaError_t launch_weights_part(const WeightsArgs& a, dim3 grid, int GT, 
     auto go = [&](auto k) {
         const cudaError_t e = set_smem_limit(k, smem);
         if (e != cudaSuccess) return e;
-        k<<<grid, kWsThreads, smem, st>>>(a);
-        return cudaGetLastError();
+        return launch_after(k, grid, dim3(kWsThreads), smem, st, a);
     };
     constexpr int B = NJ == 1 ? 4 : 2;
     switch (GT) {
@@ -546,12 +565,13 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         if (SIZE > 1) cluster.sync();
         else __syncthreads();
     };
-    pdl_launch_dependents();
     const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row0 = rank * kEvThreads * KPT;
+    for (int i = tid; i < 3 * kEvBins; i += kEvThreads) hist[0][i] = 0;
+    pdl_wait();
+    pdl_launch_dependents();
     uint32_t key[KPT];
     evict_load(a, h, row0, key);
-    for (int i = tid; i < 3 * kEvBins; i += kEvThreads) hist[0][i] = 0;
     __syncthreads();
     // The n_keep-th largest key by digits of 11, 11 and 10 bits from the top:
     // each pass counts the keys that share the digits found so far.
@@ -697,6 +717,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_one_kernel(const EvictArgs a
     constexpr int KPT = 4;
     __shared__ u_int64_t s_least[32];
     const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
     u_int64_t least = ~(u_int64_t)0;
     for (int row0 = 0; row0 < a.n_rows; row0 += kEvThreads * KPT) {
         uint32_t key[KPT];
@@ -854,8 +875,7 @@ int evict_launch(float* kc, float* vc, const float* weight, const int32_t* posit
     a.masks = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(ws) +
                                           ((size_t)n_kv * (1 + 2 * (size_t)a.max_moves) * 4 + 255) / 256 * 256);
     if (n_rows - n_keep == 1 && n_rows <= kEvOne) {
-        evict_one_kernel<<<n_kv, kEvThreads, 0, st>>>(a);
-        return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+        return launch_after(evict_one_kernel, dim3(n_kv), dim3(kEvThreads), 0, st, a) == cudaSuccess ? kOk : kErrCuda;
     }
     const int cluster = n_rows <= kEvSpread ? 1 : 8;
     const int64_t per_thread = ((int64_t)n_rows + cluster * kEvThreads - 1) / (cluster * kEvThreads);
@@ -864,18 +884,7 @@ int evict_launch(float* kc, float* vc, const float* weight, const int32_t* posit
         if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     } else {
         a.here = a.max_moves <= kEvHere;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(cluster, n_kv);
-        cfg.blockDim = dim3(kEvThreads);
-        cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = cluster;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        auto go = [&](auto k) { return cudaLaunchKernelEx(&cfg, k, a); };
+        auto go = [&](auto k) { return launch_early(k, dim3(cluster, n_kv), dim3(kEvThreads), 0, st, cluster, a); };
         const cudaError_t e = cluster == 1 ? (per_thread <= 4 ? go(evict_select_kernel<4, 1>) : go(evict_select_kernel<8, 1>))
                               : per_thread <= 4 ? go(evict_select_kernel<4, 8>)
                               : per_thread <= 8 ? go(evict_select_kernel<8, 8>)

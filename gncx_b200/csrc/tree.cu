@@ -43,7 +43,8 @@ __global__ void __launch_bounds__(kTdThreads) tree_dense_kernel(const TreeArgs a
     float* ks = qs + kTdRows * ld;
     float* vs = ks + kTdKeys * ld;
     float* ps = vs + kTdKeys * ld;
-    pdl_launch_dependents();
+    pdl_wait();
+    pdl_launch_dependents();  // after the wait: the second kernel reads inputs before it waits for this one
     const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTdRows;
     const int rows = a.n_tok * a.G;
     const int tid = threadIdx.x, r = tid >> 3, c = tid & 7;
@@ -381,8 +382,8 @@ int tree_launch(const float* q, const float* kc, const float* vc, const int32_t*
         const size_t smem = tree_dense_smem(hd);
         if (set_smem_limit(tree_dense_kernel, smem) != cudaSuccess) return kErrCuda;
         const int tiles = (n_tok * a.G + kTdRows - 1) / kTdRows;
-        tree_dense_kernel<<<dim3(a.splits, n_kv, tiles), kTdThreads, smem, st>>>(a);
-        if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+        if (launch_after(tree_dense_kernel, dim3(a.splits, n_kv, tiles), dim3(kTdThreads), smem, st, a) != cudaSuccess)
+            return kErrCuda;
     }
     const size_t msm = ((size_t)kTmWarps * kTmHeads * hd + kTmHeads * a.splits + 2 * n_tok) * 4;
     const dim3 grid(n_tok, n_kv);

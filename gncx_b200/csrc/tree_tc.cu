@@ -151,7 +151,6 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     __shared__ int infinite[HD];
     __shared__ int any_infinite;
 
-    pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTcTreeRows;
     const int rows = a.n_tok * a.G;
@@ -187,6 +186,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_wait();
+    pdl_launch_dependents();  // after the wait: the second kernel reads inputs before it waits for this one
     constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's, so they start at 0
     // False when a wait ran out: the role leaves its loop, and the roles that wait for it run out too.
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
@@ -565,8 +566,7 @@ cudaError_t tree_tc_launch(const TreeArgs& a, cudaStream_t st) {
     auto go = [&](auto k, size_t smem) {
         const cudaError_t e = set_smem_limit(k, smem);
         if (e != cudaSuccess) return e;
-        k<<<grid, kTtThreads, smem, st>>>(a);
-        return cudaGetLastError();
+        return launch_after(k, grid, dim3(kTtThreads), smem, st, a);
     };
     return a.hd <= 64 ? go(tree_tc_kernel<64>, TtLayout<64>::kAlloc) : go(tree_tc_kernel<128>, TtLayout<128>::kAlloc);
 }
