@@ -33,6 +33,10 @@ namespace gncx {
 
 constexpr int kTtThreads = 512;
 constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12;
+// Registers per thread: softmax, loaders, products (whose warpgroup is filled
+// up by idle warps); together the 512 x 128 that the block is launched with.
+constexpr int kTtSoftmaxRegs = 184, kTtLoadRegs = 96, kTtMmaRegs = 48;
+static_assert(2 * kTtSoftmaxRegs + kTtLoadRegs + kTtMmaRegs <= 4 * 128, "a split that can be had");
 constexpr int kTtKStride = 64 * 16 + 16;  // bytes between 8-column chunks of the K tile: shifted by a bank group
 constexpr int kTtStages = 2;              // K and V operand tiles
 constexpr int kTtScales = 4;              // tiles whose scales are kept
@@ -45,9 +49,8 @@ constexpr int kTtQ = 0, kTtS = 256, kTtO = 384, kTtCols = 512;
 
 template <int HD>
 struct TtLayout {
-    static constexpr int kK = HD / 8 * kTtKStride;  // one of hi, lo
-    static constexpr int kV = 8 * HD * 16;
-    static constexpr int kStage = 2 * (kK + kV);
+    static constexpr int kPart = HD / 8 * kTtKStride;  // one of K hi, K lo, V hi, V lo
+    static constexpr int kStage = 4 * kPart;
     static constexpr int kChunk = 8 * HD * 4;
     static constexpr int oStaging = kTtStages * kStage;
     static constexpr int oScale = oStaging + 16 * kChunk;     // int [kTtScales][2][8]
@@ -60,6 +63,10 @@ struct TtLayout {
 
 __device__ __forceinline__ void cp_async16_row(void* smem, const void* gmem) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
+}
+// The first `bytes` of 16, zeros behind them.
+__device__ __forceinline__ void cp_async16_row(void* smem, const void* gmem, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ float pow2i(int n) { return __int_as_float((n + 127) << 23); }  // -126 <= n <= 127
@@ -114,9 +121,13 @@ __device__ __forceinline__ void split2(f32x2 x, uint32_t& hi, uint32_t& lo) {
 // for an infinite x[i].
 template <int N, class Inf>
 __device__ __forceinline__ uint32_t warp_max_bits(float (&x)[N], Inf inf) {
-    float m = 0.0f;
+    float m = 0.0f, m1 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
+    for (int i = 0; i < N; i += 4) {
+        m = fmaxf(m, fmaxf(fabsf(x[i]), fabsf(x[i + 1])));
+        m1 = fmaxf(m1, fmaxf(fabsf(x[i + 2]), fabsf(x[i + 3])));
+    }
+    m = fmaxf(m, m1);
     uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
     if (b == 0x7F800000u) {
         m = 0.0f;
@@ -146,9 +157,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     uint64_t* qfull = oempty + 1;
     uint64_t* done = qfull + 1;
     __shared__ uint32_t tmem_slot;
-    // columns of V with an infinity (1: +, 2: -): left out of the products, where
-    // its lo part and a zero weight would make it a NaN, and set in the records
-    __shared__ int infinite[HD];
+    // columns of V with an infinity, positive and negative ones: left out of the
+    // products, where its lo part and a zero weight would make it a NaN, and set
+    // in the records
+    __shared__ unsigned infinite[2][HD / 32];
     __shared__ int any_infinite;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -176,7 +188,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         any_infinite = 0;
         fence_barrier_init();
     }
-    if (tid < HD) infinite[tid] = 0;
+    if (tid < HD / 16) infinite[0][tid] = 0;
     if (warp == kTtMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                      "r"(kTtCols)
@@ -191,47 +203,60 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's, so they start at 0
     // False when a wait ran out: the role leaves its loop, and the roles that wait for it run out too.
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
-        const bool ok = mbar_wait_idle(bar, parity);
+        if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+        const bool ok = mbar_wait(bar, parity);
         if (!ok) record_error(a.err, kErrTimeout);
         return __all_sync(0xffffffffu, ok) != 0;
     };
+    // Several barriers, asked at once; the slow path one by one.
+    auto wait_all3 = [&](uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2) {
+        const bool r0 = mbar_test(b0, p0), r1 = mbar_test(b1, p1), r2 = mbar_test(b2, p2);
+        if (__all_sync(0xffffffffu, r0 && r1 && r2)) return true;
+        return wait_warp(b0, p0) && wait_warp(b1, p1) && wait_warp(b2, p2);
+    };
+    auto wait_all2 = [&](uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1) {
+        const bool r0 = mbar_test(b0, p0), r1 = mbar_test(b1, p1);
+        if (__all_sync(0xffffffffu, r0 && r1)) return true;
+        return wait_warp(b0, p0) && wait_warp(b1, p1);
+    };
 
     if (warp >= kTtMmaWarp) {
-        regs_dec<64>();
+        regs_dec<kTtMmaRegs>();
         if (warp == kTtMmaWarp) {
             // ---------------- products: the warp waits, one thread issues ----------------
-            constexpr uint32_t idesc_s = umma_idesc_f16(128, kTcTreeKeys), idesc_o = umma_idesc_f16(128, HD);
+            constexpr uint32_t idesc_s = umma_idesc_f16(128, kTcTreeKeys), idesc_o = umma_idesc_f16(128, HD) | kUmmaTransB;
             const uint32_t sbase = smem_u32(sm);
             auto scores = [&](int x, int t) {  // S_x = Q_x K(t)^T
-                const uint32_t k = sbase + (t & 1) * L::kStage;
-                const uint64_t hi = umma_desc(k, kTtKStride, 128), lo = umma_desc(k + L::kK, kTtKStride, 128);
+                const uint32_t hi = umma_desc_lo(sbase + (t & 1) * L::kStage, kTtKStride), lo = hi + (L::kPart >> 4);
                 const uint32_t q = tmem + kTtQ + x * 128, d = tmem + kTtS + x * 64;
-                constexpr uint32_t step = 2 * kTtKStride >> 4;
+                constexpr uint32_t step = 2 * kTtKStride >> 4, rest = umma_desc_hi(128);
                 if (elect_one()) {
                     mbar_arrive(&sfull[x]);  // orders the loaders' scales before the lane's reads
+                    umma_f16_ts<false>(d, q + HD / 2, hi, rest, idesc_s);
 #pragma unroll
-                    for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + HD / 2 + 8 * i, hi + i * step, idesc_s, i > 0);
+                    for (int i = 1; i < HD / 16; ++i) umma_f16_ts<true>(d, q + HD / 2 + 8 * i, hi + i * step, rest, idesc_s);
 #pragma unroll
-                    for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + 8 * i, lo + i * step, idesc_s, true);
+                    for (int i = 0; i < HD / 16; ++i) umma_f16_ts<true>(d, q + 8 * i, lo + i * step, rest, idesc_s);
 #pragma unroll
-                    for (int i = 0; i < HD / 16; ++i) umma_f16_ts(d, q + 8 * i, hi + i * step, idesc_s, true);
+                    for (int i = 0; i < HD / 16; ++i) umma_f16_ts<true>(d, q + 8 * i, hi + i * step, rest, idesc_s);
                     umma_commit(&sfull[x]);
                 }
                 __syncwarp();
             };
             auto values = [&](int x, int t) {  // O = P_x V(t)
-                const uint32_t v = sbase + (t & 1) * L::kStage + 2 * L::kK;
-                const uint64_t hi = umma_desc(v, HD * 16, 128), lo = umma_desc(v + L::kV, HD * 16, 128);
+                // V's rows are the reduction here: 8 x 16-byte core matrices as K's, transposed
+                const uint32_t hi = umma_desc_lo(sbase + (t & 1) * L::kStage + 2 * L::kPart, 128), lo = hi + (L::kPart >> 4);
                 const uint32_t p = tmem + kTtS + x * 64, d = tmem + kTtO;
-                constexpr uint32_t step = 2 * HD * 16 >> 4;
+                constexpr uint32_t step = 16 * 16 >> 4, rest = umma_desc_hi(kTtKStride);
                 // P's block of 16 rows i: columns 16 i .. + 7 hold the hi parts, + 8 .. + 15 the lo parts
                 if (elect_one()) {
+                    umma_f16_ts<false>(d, p + 8, hi, rest, idesc_o);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i + 8, hi + i * step, idesc_o, i > 0);
+                    for (int i = 1; i < 4; ++i) umma_f16_ts<true>(d, p + 16 * i + 8, hi + i * step, rest, idesc_o);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i, lo + i * step, idesc_o, true);
+                    for (int i = 0; i < 4; ++i) umma_f16_ts<true>(d, p + 16 * i, lo + i * step, rest, idesc_o);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) umma_f16_ts(d, p + 16 * i, hi + i * step, idesc_o, true);
+                    for (int i = 0; i < 4; ++i) umma_f16_ts<true>(d, p + 16 * i, hi + i * step, rest, idesc_o);
                     umma_commit(&ofull[x]);
                 }
                 __syncwarp();
@@ -249,9 +274,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             int n_o = 0;  // products into O so far
             for (int t = 0; ok && t < n_tiles; ++t)
                 for (int x = 0; ok && x < nl; ++x) {
-                    ok = wait_warp(&pfull[x], t & 1);
-                    if (ok && x == 0) ok = wait_warp(&vfull[t & 1], (t >> 1) & 1);
-                    if (ok && n_o > 0) ok = wait_warp(oempty, (n_o - 1) & 1);
+                    // before the first product into O, oempty's phase "before 0" counts as complete
+                    ok = wait_all3(&pfull[x], t & 1, &vfull[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     values(x, t);
@@ -270,7 +294,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         }
     } else if (warp >= kTtLoadWarp) {
         // ---------------- loaders: warp w takes rows 16 w .. 16 w + 15 of each tile ----------------
-        regs_dec<96>();
+        regs_dec<kTtLoadRegs>();
         const int lw = warp - kTtLoadWarp;
         const size_t pstride = (size_t)a.n_kv * a.hd;
         const float* src[2] = {a.kc + (size_t)kvh * a.hd, a.vc + (size_t)kvh * a.hd};
@@ -284,13 +308,15 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             const int row = row_of(t, i) + sub;
             const float* g = src[i >> 1] + (size_t)row * pstride + 4 * c;
             float* d = reinterpret_cast<float*>(staging + i * L::kChunk) + sub * HD + 4 * c;
-            if (row_of(t, i) + 8 <= j1 && 4 * c < a.hd) {
+            if (t < n_tiles && row_of(t, i) + 8 <= j1 && 4 * c < a.hd) {
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) cp_async16_row(d + RS * k * HD, g + (size_t)(RS * k) * pstride);
-            } else {
-#pragma unroll
-                for (int k = 0; k < HD / 16; ++k)
-                    if (row + RS * k < j1 && 4 * c < a.hd) cp_async16_row(d + RS * k * HD, g + (size_t)(RS * k) * pstride);
+            } else if (t < n_tiles) {  // zeros past the last row and column
+#pragma unroll 1
+                for (int k = 0; k < HD / 16; ++k) {
+                    const bool some = row + RS * k < j1 && 4 * c < a.hd;
+                    cp_async16_row(d + RS * k * HD, some ? g + (size_t)(RS * k) * pstride : src[0], some ? 16 : 0);
+                }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -304,82 +330,45 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 asm volatile("cp.async.wait_group 3;" ::: "memory");
                 __syncwarp();
                 const float* st = reinterpret_cast<const float*>(staging + i * L::kChunk);
-                const int n = min(8, j1 - row_of(t, i)), chunk = 2 * lw + (i & 1);
-                const bool whole = n == 8 && a.hd == HD;
+                const int chunk = 2 * lw + (i & 1);
                 float x[HD / 4];
-                if (i < 2) {
-                    // K: float4 c of a row per lane
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k) {
-                        const float4 v = *reinterpret_cast<const float4*>(st + (sub + RS * k) * HD + 4 * c);
-                        x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
-                    }
-                    if (!whole) {  // what the copies did not write
-#pragma unroll
-                        for (int k = 0; k < HD / 4; ++k)
-                            if (sub + RS * (k / 4) >= n || 4 * c >= a.hd) x[k] = 0.0f;
-                    }
-                    const int s = scale_exp(warp_max_bits(x, [](int) {}));
-                    issue(t + 1, i);  // the chunk is in registers
-                    const f32x2 f = pack2(pow2i(s), pow2i(s));
-                    if (i == 0 && t >= kTtStages) ok = wait_warp(&kempty[t & 1], ((t >> 1) - 1) & 1);
-                    if (!ok) break;
-                    uint8_t* d = tile + (c >> 1) * kTtKStride + (8 * chunk + sub) * 16 + (c & 1) * 8;
-#pragma unroll
-                    for (int k = 0; k < HD / 16; ++k) {
-                        uint2 hi, lo;
-                        split2(mul2(pack2(x[4 * k], x[4 * k + 1]), f), hi.x, lo.x);
-                        split2(mul2(pack2(x[4 * k + 2], x[4 * k + 3]), f), hi.y, lo.y);
-                        *reinterpret_cast<uint2*>(d + RS * k * 16) = hi;
-                        *reinterpret_cast<uint2*>(d + L::kK + RS * k * 16) = lo;
-                    }
-                    if (lane == 0) sc[chunk] = s;
-                } else {
-                    // V, transposed: the 8 rows of columns lane, lane + 32, ..
-#pragma unroll
-                    for (int c = 0; c < HD / 32; ++c)
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) x[8 * c + k] = st[k * HD + lane + 32 * c];
-                    if (!whole) {
-#pragma unroll
-                        for (int k = 0; k < HD / 4; ++k)
-                            if (k % 8 >= n || lane + 32 * (k / 8) >= a.hd) x[k] = 0.0f;
-                    }
-                    const int s = scale_exp(warp_max_bits(x, [&](int e) {
-                        atomicOr(&infinite[lane + 32 * (e / 8)], x[e] > 0.0f ? 1 : 2);
-                        any_infinite = 1;
-                        x[e] = 0.0f;
-                    }));
-                    issue(t + 1, i);
-                    const f32x2 f = pack2(pow2i(s), pow2i(s));
-                    if (i == 2 && t >= kTtStages) ok = wait_warp(&vempty[t & 1], ((t >> 1) - 1) & 1);
-                    if (!ok) break;
-                    uint8_t* d = tile + 2 * L::kK + chunk * HD * 16 + lane * 16;
-#pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-                        uint4 hi, lo;
-                        split2(mul2(pack2(x[8 * c], x[8 * c + 1]), f), hi.x, lo.x);
-                        split2(mul2(pack2(x[8 * c + 2], x[8 * c + 3]), f), hi.y, lo.y);
-                        split2(mul2(pack2(x[8 * c + 4], x[8 * c + 5]), f), hi.z, lo.z);
-                        split2(mul2(pack2(x[8 * c + 6], x[8 * c + 7]), f), hi.w, lo.w);
-                        *reinterpret_cast<uint4*>(d + c * 512) = hi;
-                        *reinterpret_cast<uint4*>(d + L::kV + c * 512) = lo;
-                    }
-                    if (lane == 0) sc[8 + chunk] = s;
+                for (int k = 0; k < HD / 16; ++k) {
+                    const float4 v = *reinterpret_cast<const float4*>(st + (sub + RS * k) * HD + 4 * c);
+                    x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
                 }
+                const int s = scale_exp(warp_max_bits(x, [&](int e) {
+                    if (i < 2) return;
+                    const int col = 4 * c + (e & 3);
+                    atomicOr(&infinite[x[e] < 0.0f][col >> 5], 1u << (col & 31));
+                    any_infinite = 1;
+                    x[e] = 0.0f;
+                }));
+                issue(t + 1, i);  // the chunk is in registers
+                const f32x2 f = pack2(pow2i(s), pow2i(s));
+                if ((i & 1) == 0 && t >= kTtStages) ok = wait_warp(i ? &vempty[t & 1] : &kempty[t & 1], ((t >> 1) - 1) & 1);
+                if (!ok) break;
+                uint8_t* d = tile + (i >> 1) * 2 * L::kPart + (c >> 1) * kTtKStride + (8 * chunk + sub) * 16 + (c & 1) * 8;
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    uint2 hi, lo;
+                    split2(mul2(pack2(x[4 * k], x[4 * k + 1]), f), hi.x, lo.x);
+                    split2(mul2(pack2(x[4 * k + 2], x[4 * k + 3]), f), hi.y, lo.y);
+                    *reinterpret_cast<uint2*>(d + RS * k * 16) = hi;
+                    *reinterpret_cast<uint2*>(d + L::kPart + RS * k * 16) = lo;
+                }
+                if (lane == 0) sc[8 * (i >> 1) + chunk] = s;
                 if (i & 1) {
                     fence_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(i == 1 ? &kfull[t & 1] : &vfull[t & 1]);
-                } else {
-                    fence_async_smem();
                 }
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if ((warp >> 2) < nl) {
         // ---------------- softmax and output: a thread per query row ----------------
-        regs_inc<176>();
+        regs_inc<kTtSoftmaxRegs>();
         const int x = warp >> 2;
         const int row = r0 + 128 * x + 32 * (warp & 3) + lane;
         const bool active = r0 + 128 * x + 32 * (warp & 3) < rows;  // of the warp
@@ -536,7 +525,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         if (any_infinite) {
 #pragma unroll
             for (int d = 0; d < HD / 2; ++d) {
-                auto of = [&](int c) { return infinite[c] == 0 ? 0.0f : infinite[c] == 1 ? INFINITY : infinite[c] == 2 ? -INFINITY : NAN; };
+                auto of = [&](int c) {
+                    const float up = infinite[0][c >> 5] >> (c & 31) & 1 ? INFINITY : 0.0f;
+                    return infinite[1][c >> 5] >> (c & 31) & 1 ? up - INFINITY : up;
+                };
                 o[d] = add2(o[d], pack2(of(2 * d), of(2 * d + 1)));
             }
         }
