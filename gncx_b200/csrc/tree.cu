@@ -146,11 +146,11 @@ constexpr int kTmHeads = 4;  // query heads of the group at a time
 template <int NJ>
 __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a) {
     extern __shared__ __align__(16) float sm[];
-    float* os = sm;                                             // [warp][kTmHeads][hd]
-    float* fs = os + kTmWarps * kTmHeads * a.hd;                // [kTmHeads][splits]
-    int* up = reinterpret_cast<int*>(fs + kTmHeads * a.splits); // parents, then
-    int* chain = up + a.n_tok;                                  // the path from the node up
-    __shared__ float s_m[kTmWarps][kTmHeads], s_l[kTmWarps][kTmHeads], s_inv[kTmHeads];
+    float* os = sm;                                                // [warp][kTmHeads][hd]
+    int* up = reinterpret_cast<int*>(os + kTmWarps * kTmHeads * a.hd); // parents, then
+    int* chain = up + a.n_tok;                                     // the path from the node up
+    __shared__ float s_m[kTmWarps][kTmHeads], s_l[kTmWarps][kTmHeads];
+    __shared__ float2 ml_g[kTmThreads];
     __shared__ int s_len;
     const int node = blockIdx.x, kvh = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -248,75 +248,63 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a
                 const int col = 4 * (lane + 32 * j);
                 if (col < a.hd) *reinterpret_cast<float4*>(os + (warp * kTmHeads + g) * a.hd + col) = o[g][j];
             }
+        __syncthreads();
         if (!waited) pdl_wait();  // the dense kernel's records
         waited = true;
-        __syncthreads();
-        // maximum and sum of head g over the records and the warps' states: warp g
-        if (warp < heads) {
-            const float* rec = a.part + ((size_t)kvh * rows + node * a.G + g0 + warp) * a.splits * rl;
-            float M = lane < kTmWarps ? s_m[lane][warp] : -INFINITY;
-            for (int s = lane; s < a.splits; s += 32) M = fmaxf(M, rec[(size_t)s * rl]);
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
-            float L = 0.0f;
-            if (lane < kTmWarps) {
-                const float f = s_m[lane][warp] == -INFINITY ? 0.0f : ex2(s_m[lane][warp] - M);
-                L = s_l[lane][warp] * f;
-                s_m[lane][warp] = f;  // from here on the factor
-            }
-            for (int s = lane; s < a.splits; s += 32) {
-                const float rm = rec[(size_t)s * rl];
-                const float f = rm == -INFINITY ? 0.0f : ex2(rm - M);
-                fs[warp * a.splits + s] = f;
-                L = fmaf(rec[(size_t)s * rl + 1], f, L);
-            }
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) L += __shfl_xor_sync(0xffffffffu, L, w);
-            if (lane == 0) s_inv[warp] = 1.0f / L;
-        }
-        __syncthreads();
-        // four columns per thread; where there are threads to spare, groups of
-        // them take every groups-th record
+        // Four columns per thread; where there are threads to spare, groups of them
+        // take every groups-th record, group 0 the warps' states too.  Each thread
+        // merges with a maximum of its own, so that all its loads are in flight at once.
         const int hd4 = a.hd / 4, items = heads * hd4;
-        const int groups = min(8, max(1, kTmThreads / items));  // their sums fit where the states were
+        const int groups = min(8, max(1, kTmThreads / items));
         const int grp = tid / items, it = tid - grp * items;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         const int g = it / hd4, c = it - g * hd4;
+        float M = -INFINITY, sum = 0.0f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto join = [&](float m, float l, const float4& v) {
+            const float Mn = fmaxf(M, m);
+            const float f = M == -INFINITY ? 0.0f : ex2(M - Mn), e = m == -INFINITY ? 0.0f : ex2(m - Mn);
+            // a record without a weight may hold no number: NaN sums (and no others) count all the same
+            M = Mn;
+            sum = fmaf(sum, f, l * e);
+            acc.x = fmaf(acc.x, f, v.x * e);
+            acc.y = fmaf(acc.y, f, v.y * e);
+            acc.z = fmaf(acc.z, f, v.z * e);
+            acc.w = fmaf(acc.w, f, v.w * e);
+        };
         if (grp < groups) {
-            const float* rec = a.part + ((size_t)kvh * rows + node * a.G + g0 + g) * a.splits * rl + 4 + 4 * c;
-#pragma unroll 8
-            for (int s = grp; s < a.splits; s += groups) {
-                const float4 v = *reinterpret_cast<const float4*>(rec + (size_t)s * rl);
-                const float f = fs[g * a.splits + s];
-                acc.x = fmaf(v.x, f, acc.x);
-                acc.y = fmaf(v.y, f, acc.y);
-                acc.z = fmaf(v.z, f, acc.z);
-                acc.w = fmaf(v.w, f, acc.w);
+            constexpr int kBatch = 8;
+            const float* rec = a.part + ((size_t)kvh * rows + node * a.G + g0 + g) * a.splits * rl;
+            for (int s0 = grp; s0 < a.splits; s0 += kBatch * groups) {
+                float2 ml[kBatch];
+                float4 v[kBatch];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int s = min(s0 + i * groups, a.splits - 1);
+                    ml[i] = *reinterpret_cast<const float2*>(rec + (size_t)s * rl);
+                    v[i] = *reinterpret_cast<const float4*>(rec + (size_t)s * rl + 4 + 4 * c);
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    if (s0 + i * groups < a.splits) join(ml[i].x, ml[i].y, v[i]);
             }
             if (grp == 0)
 #pragma unroll
-                for (int w = 0; w < kTmWarps; ++w) {
-                    const float4 v = *reinterpret_cast<const float4*>(os + (w * kTmHeads + g) * a.hd + 4 * c);
-                    const float f = s_m[w][g];
-                    acc.x = fmaf(v.x, f, acc.x);
-                    acc.y = fmaf(v.y, f, acc.y);
-                    acc.z = fmaf(v.z, f, acc.z);
-                    acc.w = fmaf(v.w, f, acc.w);
-                }
+                for (int w = 0; w < kTmWarps; ++w)
+                    join(s_m[w][g], s_l[w][g], *reinterpret_cast<const float4*>(os + (w * kTmHeads + g) * a.hd + 4 * c));
         }
-        __syncthreads();
-        float4* sum = reinterpret_cast<float4*>(os);  // the warps' states are merged
-        if (grp > 0 && grp < groups) sum[tid - items] = acc;
-        __syncthreads();
-        if (grp == 0) {
-            for (int k = 0; k < groups - 1; ++k) {
-                const float4 v = sum[k * items + it];
-                acc.x += v.x;
-                acc.y += v.y;
-                acc.z += v.z;
-                acc.w += v.w;
+        if (groups > 1) {
+            __syncthreads();  // the warps' states are merged: their place holds the groups'
+            float4* sums = reinterpret_cast<float4*>(os);
+            if (grp > 0 && grp < groups) {
+                sums[tid - items] = acc;
+                ml_g[tid - items] = make_float2(M, sum);
             }
-            const float f = s_inv[g];
+            __syncthreads();
+            if (grp == 0)
+                for (int k = 0; k < groups - 1; ++k) join(ml_g[k * items + it].x, ml_g[k * items + it].y, sums[k * items + it]);
+        }
+        if (grp == 0) {
+            const float f = 1.0f / sum;
             *reinterpret_cast<float4*>(a.out + ((size_t)node * a.n_heads + kvh * a.G + g0 + g) * a.hd + 4 * c) =
                 make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
         }
@@ -385,7 +373,7 @@ int tree_launch(const float* q, const float* kc, const float* vc, const int32_t*
         if (launch_after(tree_dense_kernel, dim3(a.splits, n_kv, tiles), dim3(kTdThreads), smem, st, a) != cudaSuccess)
             return kErrCuda;
     }
-    const size_t msm = ((size_t)kTmWarps * kTmHeads * hd + kTmHeads * a.splits + 2 * n_tok) * 4;
+    const size_t msm = ((size_t)kTmWarps * kTmHeads * hd + 2 * n_tok) * 4;
     const dim3 grid(n_tok, n_kv);
     auto go = [&](auto k) {
         if (set_smem_limit(k, msm) != cudaSuccess) return kErrCuda;
