@@ -498,19 +498,10 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     if (tid == 0) s_cnt = s_live = s_full = 0;
     __syncthreads();
     pdl_wait();
-    // the beams' scores; NaN for a beam without lists (ended, or no candidate can be better than none)
-    for (int b = tid; b < n_beam; b += kBmThreads) {
-        const float s = scores[b];
-        const bool live = !(finished && finished[b]) && s > -INFINITY;
-        s_score[b] = live ? (double)s : NAN;
-        if (live) atomicAdd(&s_live, 1);
-        else if (s > -INFINITY) list[atomicAdd(&s_cnt, 1)] = BeamKey{ord64((double)s), ~((u64)b << 56 | (u64)eos)};
-    }
-    __syncthreads();
-    // a thread per list; the first entries of all lists are on their way while the beams' sums are formed
+    // Everything that is read first is asked for at once: the first entries of the
+    // lists, a thread per list; the parts' sums, 4 to 32 lanes per beam; the beams' scores.
     const int lists = n_beam * parts;  // < kBmThreads
     const int b = min(tid / parts, n_beam - 1);
-    const bool has = tid < lists && s_score[b] == s_score[b];
     const u64* mine = keys + (size_t)tid * n;
     constexpr int kAhead = 4;  // entries of the list that are loaded together
     u64 ahead[kAhead];
@@ -524,14 +515,24 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
         for (int i = 1; i < kAhead; ++i) e = (r & (kAhead - 1)) == i ? ahead[i] : e;
         return e;
     };
-    if (has) load(0);
+    if (tid < lists) load(0);  // of ended beams too, whose entries are not used
+    int width = 32;
+    while (width > 4 && n_beam * width > kBmThreads) width >>= 1;
+    const int w = tid / width, wl = tid & (width - 1);
+    const BeamPart* st = stats + (size_t)min(w, n_beam - 1) * parts;
+    const BeamPart part0 = st[min(wl, parts - 1)];
+    // the scores; NaN for a beam without lists (ended, or no candidate can be better than none)
+    if (tid < n_beam) {
+        const float s = scores[tid];
+        const bool live = !(finished && finished[tid]) && s > -INFINITY;
+        s_score[tid] = live ? (double)s : NAN;
+        if (live) atomicAdd(&s_live, 1);
+        else if (s > -INFINITY) list[atomicAdd(&s_cnt, 1)] = BeamKey{ord64((double)s), ~((u64)tid << 56 | (u64)eos)};
+    }
+    __syncthreads();
+    const bool has = tid < lists && s_score[b] == s_score[b];
     {
-        // 4 to 32 lanes per beam
-        int width = 32;
-        while (width > 4 && n_beam * width > kBmThreads) width >>= 1;
-        const int w = tid / width, wl = tid & (width - 1);
         const bool on = w < n_beam && s_score[min(w, n_beam - 1)] == s_score[min(w, n_beam - 1)];
-        const BeamPart* st = stats + (size_t)min(w, n_beam - 1) * parts;
         // a lane's parts as one, then the lanes'
         float M = -INFINITY;
         double l = 0.0;
@@ -544,11 +545,10 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
             M = top;
         };
         if (on && wl < parts) {
-            BeamPart s = st[wl];
-            M = s.ref;
-            l = s.sum;
+            M = part0.ref;
+            l = part0.sum;
             for (int p = wl + width; p < parts; p += width) {
-                s = st[p];
+                const BeamPart s = st[p];
                 join(s.ref, s.sum);
             }
         }
