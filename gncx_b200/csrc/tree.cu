@@ -178,8 +178,9 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a
     const float* kb = a.kc + (size_t)kvh * a.hd;
     const float* vb = a.vc + (size_t)kvh * a.hd;
     bool waited = false;
-    for (int g0 = 0; g0 < a.G; g0 += kTmHeads) {
-        const int heads = min(kTmHeads, a.G - g0);
+    const int g_end = min(a.G, ((int)blockIdx.z + 1) * a.merge_heads);
+    for (int g0 = blockIdx.z * a.merge_heads; g0 < g_end; g0 += kTmHeads) {
+        const int heads = min(kTmHeads, g_end - g0);
         float4 q[kTmHeads][NJ], o[kTmHeads][NJ];
         float m[kTmHeads], l[kTmHeads];
 #pragma unroll
@@ -374,7 +375,14 @@ int tree_launch(const float* q, const float* kc, const float* vc, const int32_t*
             return kErrCuda;
     }
     const size_t msm = ((size_t)kTmWarps * kTmHeads * hd + 2 * n_tok) * 4;
-    const dim3 grid(n_tok, n_kv);
+    // Heads of a group share the CTA that walks a node's rows; spread over more
+    // CTAs only as far as these fit the SMs (8 heads on one KV head, 16 nodes,
+    // 65536 rows, 147 records each: 64 us with the 8 together, 34 apart; 16 heads, 4
+    // KV heads, 25 nodes, window 1024: 10.2 us as it is, 13.0 with 200 CTAs).
+    a.merge_heads = a.G;
+    const auto ctas = [&](int heads) { return (int64_t)n_tok * n_kv * ((a.G + heads - 1) / heads); };
+    while (a.merge_heads > 1 && ctas((a.merge_heads + 1) / 2) <= device_info().sm_count) a.merge_heads = (a.merge_heads + 1) / 2;
+    const dim3 grid(n_tok, n_kv, (a.G + a.merge_heads - 1) / a.merge_heads);
     auto go = [&](auto k) {
         if (set_smem_limit(k, msm) != cudaSuccess) return kErrCuda;
         if (a.splits > 0) return launch_after(k, grid, dim3(kTmThreads), msm, st, a) == cudaSuccess ? kOk : kErrCuda;

@@ -16,6 +16,7 @@ struct TreeArgs {
     int lo;            // the dense range is [lo, pos0)
     int splits, per;   // its splits, and rows per split
     int max_splits;    // at least splits; does not shrink when the range grows
+    int merge_heads;   // heads of a group per CTA of the merge
     bool tc;           // the dense range runs on the tensor cores
     float* part;       // records [kv head][query row][split] of hd + 4 floats: max, sum, -, -, o
     float* out;

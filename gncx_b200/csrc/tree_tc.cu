@@ -12,7 +12,9 @@
 //
 // One CTA takes up to 256 query rows of one KV head as two lanes A and B of
 // 128 and walks its split of the cache in tiles of 64 rows, each K and V row
-// read and split once for both lanes:
+// read and split once for both lanes; with at most 128 query rows and several
+// tiles both lanes serve the same rows, tile t on lane t & 1 (ALT), and join
+// their sums at the end:
 //   * loader warps 8-11 bring 8-row chunks in with cp.async (four in flight per
 //     warp, 64 KB per SM), split them and write the K-major operand tiles;
 //   * warp 12, one thread, issues S = Q K^T (Q pairs stay in TMEM) and, once a
@@ -44,6 +46,11 @@ constexpr int kTtScales = 4;              // tiles whose scales are kept
 // kTtHead above the reference: up to 2^14 in fp16, and 2^-34 of a weight of 1 is
 // still seen.
 constexpr int kTtShift = 10, kTtHead = 4;
+// ALT from so many tiles per CTA.  16 heads, 8 KV heads of 128, 16 nodes: 8192
+// rows (7 tiles) 28.5 us with both lanes, 30.5 with one; 32 heads, 32 nodes, 32768
+// rows (28 tiles) 80.4 and 90; with 4 tiles the joining costs as much as it saves
+// (32 heads, 24 nodes, 4096 rows: 24.3 and 23.8).
+constexpr int kTtAltTiles = 6;
 // TMEM columns
 constexpr int kTtQ = 0, kTtS = 256, kTtO = 384, kTtCols = 512;
 
@@ -55,8 +62,10 @@ struct TtLayout {
     static constexpr int oStaging = kTtStages * kStage;
     static constexpr int oScale = oStaging + 16 * kChunk;     // int [kTtScales][2][8]
     static constexpr int oBar = oScale + kTtScales * 2 * 8 * 4;
-    static constexpr int kBars = 4 * kTtStages + 2 + 6 + 1;
-    static constexpr int kBytes = oBar + kBars * 8 + 16;
+    static constexpr int kBars = 4 * kTtStages + 2 + 6 + 2;
+    static constexpr int oState = oBar + kBars * 8;    // lane 1's reference and sum of each row: float [2][128]
+    static constexpr int kBytes = oState + 2 * 128 * 4;
+    static_assert(kStage >= 128 * HD * 4, "a lane's output fits an operand stage");
     // more than half of an SM's shared memory, so one CTA per SM owns all of TMEM
     static constexpr int kAlloc = kBytes > 120 * 1024 ? kBytes : 120 * 1024;
 };
@@ -141,7 +150,8 @@ __device__ __forceinline__ uint32_t warp_max_bits(float (&x)[N], Inf inf) {
     return b;
 }
 
-template <int HD>
+// ALT: at most 128 query rows, both lanes on them, tile t on lane t & 1.
+template <int HD, bool ALT>
 __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a) {
     using L = TtLayout<HD>;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -155,7 +165,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     uint64_t* ofull = pfull + 2;
     uint64_t* oempty = ofull + 2;
     uint64_t* qfull = oempty + 1;
-    uint64_t* done = qfull + 1;
+    uint64_t* joined = qfull + 1;
+    uint64_t* done = joined + 1;
     __shared__ uint32_t tmem_slot;
     // columns of V with an infinity, positive and negative ones: left out of the
     // products, where its lo part and a zero weight would make it a NaN, and set
@@ -166,9 +177,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTcTreeRows;
     const int rows = a.n_tok * a.G;
-    const int nl = rows - r0 > 128 ? 2 : 1;  // lanes in use
+    const int nl = !ALT && rows - r0 > 128 ? 2 : 1;  // row blocks of 128
     const int j0 = a.lo + split * a.per, j1 = min(a.pos0, j0 + a.per);
     const int n_tiles = (j1 - j0 + kTcTreeKeys - 1) / kTcTreeKeys;
+    auto phase = [](int t) { return (uint32_t)(ALT ? t >> 1 : t) & 1; };  // of a lane's barriers
 
     if (tid == 0) {
         for (int i = 0; i < kTtStages; ++i) {
@@ -184,6 +196,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         }
         mbar_init(oempty, 128);
         mbar_init(qfull, 128 * nl);
+        mbar_init(joined, 128);
         mbar_init(done, 1);
         any_infinite = 0;
         fence_barrier_init();
@@ -214,11 +227,6 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         if (__all_sync(0xffffffffu, r0 && r1 && r2)) return true;
         return wait_warp(b0, p0) && wait_warp(b1, p1) && wait_warp(b2, p2);
     };
-    auto wait_all2 = [&](uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1) {
-        const bool r0 = mbar_test(b0, p0), r1 = mbar_test(b1, p1);
-        if (__all_sync(0xffffffffu, r0 && r1)) return true;
-        return wait_warp(b0, p0) && wait_warp(b1, p1);
-    };
 
     if (warp >= kTtMmaWarp) {
         regs_dec<kTtMmaRegs>();
@@ -228,7 +236,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             const uint32_t sbase = smem_u32(sm);
             auto scores = [&](int x, int t) {  // S_x = Q_x K(t)^T
                 const uint32_t hi = umma_desc_lo(sbase + (t & 1) * L::kStage, kTtKStride), lo = hi + (L::kPart >> 4);
-                const uint32_t q = tmem + kTtQ + x * 128, d = tmem + kTtS + x * 64;
+                const uint32_t q = tmem + kTtQ + (ALT ? 0 : x * 128), d = tmem + kTtS + x * 64;
                 constexpr uint32_t step = 2 * kTtKStride >> 4, rest = umma_desc_hi(128);
                 if (elect_one()) {
                     mbar_arrive(&sfull[x]);  // orders the loaders' scales before the lane's reads
@@ -265,28 +273,33 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 if (elect_one()) umma_commit(bar);
                 __syncwarp();
             };
-            bool ok = wait_warp(qfull, 0) && wait_warp(&kfull[0], 0);
-            tc_fence_after();
-            if (ok) {
-                for (int x = 0; x < nl; ++x) scores(x, 0);
-                commit(&kempty[0]);
+            constexpr int kAhead = ALT ? 2 : 1;  // a lane's next tile
+            bool ok = wait_warp(qfull, 0);
+            for (int t = 0; ok && t < min(kAhead, n_tiles); ++t) {
+                ok = wait_warp(&kfull[t], 0);
+                if (!ok) break;
+                tc_fence_after();
+                for (int x = 0; x < nl; ++x) scores(ALT ? t : x, t);
+                commit(&kempty[t]);
             }
-            int n_o = 0;  // products into O so far
+            int n_o = 0;                    // products into O so far
             for (int t = 0; ok && t < n_tiles; ++t)
-                for (int x = 0; ok && x < nl; ++x) {
+                for (int i = 0; ok && i < nl; ++i) {
+                    const int x = ALT ? t & 1 : i;
                     // before the first product into O, oempty's phase "before 0" counts as complete
-                    ok = wait_all3(&pfull[x], t & 1, &vfull[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
+                    ok = wait_all3(&pfull[x], phase(t), &vfull[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     values(x, t);
                     ++n_o;
-                    if (x == nl - 1) commit(&vempty[t & 1]);
-                    if (t + 1 < n_tiles) {
-                        if (x == 0) ok = wait_warp(&kfull[(t + 1) & 1], ((t + 1) >> 1) & 1);
+                    if (i == nl - 1) commit(&vempty[t & 1]);
+                    const int t2 = t + kAhead;
+                    if (t2 < n_tiles) {
+                        if (i == 0) ok = wait_warp(&kfull[t2 & 1], (t2 >> 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
-                        scores(x, t + 1);
-                        if (x == nl - 1) commit(&kempty[(t + 1) & 1]);
+                        scores(x, t2);
+                        if (i == nl - 1) commit(&kempty[t2 & 1]);
                     }
                 }
             commit(done);  // nothing of this CTA's is in flight when TMEM is freed
@@ -366,12 +379,12 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if ((warp >> 2) < nl) {
-        // ---------------- softmax and output: a thread per query row ----------------
+    } else if ((warp >> 2) < nl || ALT) {
+        // ---------------- softmax and output: a thread per query row (and lane) ----------------
         regs_inc<kTtSoftmaxRegs>();
         const int x = warp >> 2;
-        const int row = r0 + 128 * x + 32 * (warp & 3) + lane;
-        const bool active = r0 + 128 * x + 32 * (warp & 3) < rows;  // of the warp
+        const int first = r0 + (ALT ? 0 : 128 * x) + 32 * (warp & 3), row = first + lane;
+        const bool active = first < rows;  // of the warp
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t tq = tmem + lanes + kTtQ + x * 128, ts = tmem + lanes + kTtS + x * 64, to = tmem + lanes + kTtO;
         int sq = 0;
@@ -388,26 +401,31 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
 #pragma unroll
             for (int c = 0; c < HD; ++c) m = fmaxf(m, fabsf(v[c]) < INFINITY ? fabsf(v[c]) : 0.0f);
             sq = scale_exp(__float_as_uint(m));
-            const f32x2 f = pack2(pow2i(sq), pow2i(sq));
+            if (x == 0 || !ALT) {
+                const f32x2 f = pack2(pow2i(sq), pow2i(sq));
 #pragma unroll
-            for (int b = 0; b < HD / 32; ++b) {
-                uint32_t hi[16], lo[16];
+                for (int b = 0; b < HD / 32; ++b) {
+                    uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int c = 0; c < 16; ++c) split2(mul2(pack2(v[32 * b + 2 * c], v[32 * b + 2 * c + 1]), f), hi[c], lo[c]);
-                tmem_st16(tq + 16 * b, hi);
-                tmem_st16(tq + HD / 2 + 16 * b, lo);
+                    for (int c = 0; c < 16; ++c) split2(mul2(pack2(v[32 * b + 2 * c], v[32 * b + 2 * c + 1]), f), hi[c], lo[c]);
+                    tmem_st16(tq + 16 * b, hi);
+                    tmem_st16(tq + HD / 2 + 16 * b, lo);
+                }
+                tmem_wait_st();
             }
-            tmem_wait_st();
         }
         tc_fence_before();
-        mbar_arrive(qfull);
+        if (x == 0 || !ALT) mbar_arrive(qfull);
 
         float T = -INFINITY, l = 0.0f;
         f32x2 o[HD / 2];
 #pragma unroll
         for (int d = 0; d < HD / 2; ++d) o[d] = 0;
-        for (int t = 0; t < n_tiles; ++t) {
-            if (!wait_warp(&sfull[x], t & 1)) break;
+        bool ok = true;
+#pragma unroll 1
+        for (int t = ALT ? x : 0; t < n_tiles; t += ALT ? 2 : 1) {
+            ok = wait_warp(&sfull[x], phase(t));
+            if (!ok) break;
             float alpha = 1.0f, beta = 1.0f;
             if (active) {
                 tc_fence_after();
@@ -453,7 +471,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 }
                 const float ref = T == -INFINITY ? 0.0f : T;
                 // V's scales: the products of this tile count in units of its largest rows
-                if (!wait_warp(&vfull[t & 1], (t >> 1) & 1)) break;
+                ok = wait_warp(&vfull[t & 1], (t >> 1) & 1);
+                if (!ok) break;
                 const int4 v0 = sc[2], v1 = sc[3];
                 const int U = min(min(min(v0.x, v0.y), min(v0.z, v0.w)), min(min(v1.x, v1.y), min(v1.z, v1.w)));
                 const bool even_v = U == max(max(max(v0.x, v0.y), max(v0.z, v0.w)), max(max(v1.x, v1.y), max(v1.z, v1.w)));
@@ -502,7 +521,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 tc_fence_before();
             }
             mbar_arrive(&pfull[x]);
-            if (!wait_warp(&ofull[x], t & 1)) break;
+            ok = wait_warp(&ofull[x], phase(t));
+            if (!ok) break;
             if (active) {
                 tc_fence_after();
                 const f32x2 beta2 = pack2(beta, beta);
@@ -522,6 +542,37 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             }
             mbar_arrive(oempty);
         }
+        if (ALT && ok) {
+            // lane 1's state of each row joins lane 0's, its output through the second
+            // operand stage: the odd tiles', whose products are through
+            float* other = reinterpret_cast<float*>(sm + L::kStage) + 32 * (warp & 3) + lane;
+            float* state = reinterpret_cast<float*>(sm + L::oState) + 32 * (warp & 3) + lane;
+            if (x == 1) {
+                if (active) {
+                    state[0] = T;
+                    state[128] = l;
+#pragma unroll
+                    for (int d = 0; d < HD / 2; ++d) {
+                        const float2 v = unpack2(o[d]);
+                        other[2 * d * 128] = v.x;
+                        other[(2 * d + 1) * 128] = v.y;
+                    }
+                }
+                mbar_arrive(joined);
+            } else {
+                ok = wait_warp(joined, 0);
+                if (active && ok) {
+                    const float T1 = state[0], Tn = fmaxf(T, T1);
+                    const float f = T == -INFINITY ? 0.0f : ex2(T - Tn), g = T1 == -INFINITY ? 0.0f : ex2(T1 - Tn);
+                    T = Tn;
+                    l = fmaf(l, f, state[128] * g);
+                    const f32x2 f2 = pack2(f, f), g2 = pack2(g, g);
+#pragma unroll
+                    for (int d = 0; d < HD / 2; ++d)
+                        o[d] = fma2(o[d], f2, mul2(pack2(other[2 * d * 128], other[(2 * d + 1) * 128]), g2));
+                }
+            }
+        }
         if (any_infinite) {
 #pragma unroll
             for (int d = 0; d < HD / 2; ++d) {
@@ -532,7 +583,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 o[d] = add2(o[d], pack2(of(2 * d), of(2 * d + 1)));
             }
         }
-        if (row < rows) {
+        if (row < rows && !(ALT && x == 1)) {
             float* rec = a.part + (((size_t)kvh * rows + row) * a.splits + split) * (a.hd + 4);
             const float f = pow2i(-kTtShift);
             *reinterpret_cast<float2*>(rec) = make_float2(T, l * f);
@@ -560,7 +611,9 @@ cudaError_t tree_tc_launch(const TreeArgs& a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         return launch_after(k, grid, dim3(kTtThreads), smem, st, a);
     };
-    return a.hd <= 64 ? go(tree_tc_kernel<64>, TtLayout<64>::kAlloc) : go(tree_tc_kernel<128>, TtLayout<128>::kAlloc);
+    const bool alt = a.n_tok * a.G <= 128 && a.per >= kTtAltTiles * kTcTreeKeys;
+    if (a.hd <= 64) return alt ? go(tree_tc_kernel<64, true>, TtLayout<64>::kAlloc) : go(tree_tc_kernel<64, false>, TtLayout<64>::kAlloc);
+    return alt ? go(tree_tc_kernel<128, true>, TtLayout<128>::kAlloc) : go(tree_tc_kernel<128, false>, TtLayout<128>::kAlloc);
 }
 
 }  // namespace gncx

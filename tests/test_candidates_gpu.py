@@ -178,6 +178,46 @@ def test_tree_peaked_softmax(gpu, hd):
     check_tree(run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0), q, k, v, up, pos0, hd**-0.5, 0)
 
 
+# Several tiles of 64 rows per CTA and at most 128 query rows (148 SMs), where two
+# lanes share the rows: whole and odd numbers of tiles, a last split of one row,
+# the largest such group, one beyond it.
+LANES = [(32, 32, 64, 1700, 9), (32, 32, 128, 1999, 11), (64, 32, 96, 3333, 40), (30, 30, 80, 2700, 3), (148, 148, 64, 450, 5),
+         (148, 148, 128, 385, 2), (148, 148, 128, 400, 1), (20, 10, 128, 4993, 7), (64, 16, 128, 5000, 32), (64, 16, 128, 5000, 33),
+         (8, 1, 128, 70001, 16)]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,pos0,n", LANES)
+@pytest.mark.parametrize("size", [1.0, 5.0])
+def test_tree_lanes(gpu, nh, nkv, hd, pos0, n, size):
+    rows = pos0 + n
+    q, k, v = randn(40, n, nh, hd) * size, randn(41, rows + 3, nkv, hd), randn(42, rows + 3, nkv, hd)
+    k[rows:], v[rows:] = float("nan"), float("nan")
+    for row in (0, 63, 64, 127, 128, 200, pos0 - 1):  # heavy rows on both sides of the tiles' borders
+        k[row] *= 4
+    up = make_tree("random", n, 11)
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0)
+    heads = sorted({0, nh // 2, nh - 1})
+    for i in sorted({0, n // 2, n - 1}):
+        rs = torch.tensor(tree_seen(up, i, pos0, 0), device="cuda")
+        for h in heads:
+            g = h // (nh // nkv)
+            ref, tol, _, _ = attend(q[i, h], k[rs][:, g], v[rs][:, g], hd**-0.5)
+            assert bool(((out[i, h].double() - ref).abs() <= tol).all()), (i, h)
+    assert bool(out.isfinite().all())
+    assert torch.equal(out, run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0))
+
+
+@pytest.mark.parametrize("row", [3, 70, 388, 1750, 1799])
+def test_tree_lanes_infinite_and_nan_rows_show(gpu, row):
+    nh, nkv, hd, pos0, n = 32, 32, 128, 1800, 6
+    q, k, v = randn(43, n, nh, hd), randn(44, pos0 + n, nkv, hd), randn(45, pos0 + n, nkv, hd)
+    v[row, 4, 9], k[row, 7, 2] = float("-inf"), float("nan")
+    out = run_tree(gpu, q, k, v, make_tree("random", n, 12), pos0, hd**-0.5, 0)
+    assert bool((out[:, 4, 9] == float("-inf")).all()) and bool(out[:, 7].isnan().all())
+    out[:, 4, 9], out[:, 7] = 0, 0
+    assert bool(out.isfinite().all())
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_tree_other_branches_do_not_leak(gpu, bad):
     nh, nkv, hd, pos0, n = 8, 2, 128, 300, 40
