@@ -32,6 +32,10 @@ constexpr int kBsTile = kBsThreads * kBsPer;
 constexpr int kBsSort = 1024;             // largest list that is sorted
 constexpr int kBsList = kBsSort + kBsTile;
 constexpr int kBsCtasPerSm = 3;           // that a vocabulary is split for
+// From fewer than so many parts for each beam the division follows the number of
+// beams that have not ended: 64 beams, 9 of them ended, 33.3 us against 37.1 (none
+// ended: 38.7 and 36.9); with more parts it gains less than reading the flags costs.
+constexpr int kBsShare = 16;
 constexpr int kBmThreads = 1024;
 constexpr int kBmList = 2 * kBmThreads;
 
@@ -70,6 +74,39 @@ __device__ __forceinline__ void bitonic_desc(Key* list, int P) {
             }
         }
     __syncthreads();
+}
+
+// How the vocabulary is divided: into `parts` for each beam or, where `share` is
+// set, on the device into as many as give at most `room` lists of the beams that
+// have not ended.
+struct BeamSplit {
+    int room, parts, per;
+    bool share;
+};
+__host__ __device__ inline int beam_parts(int live, int vocab, int room) {
+    const int tiles = (vocab + kBsTile - 1) / kBsTile, most = room / (live > 1 ? live : 1);
+    return tiles < most ? tiles : most > 1 ? most : 1;
+}
+
+// The beams that have not ended: their number, and s_beam[i] the i-th of them.
+// Whole CTA of at least kBeamMax threads.
+__device__ __forceinline__ int beam_live(const int32_t* finished, int n_beam, int* s_beam) {
+    __shared__ unsigned s_on[kBeamMax / 32];
+    const int tid = threadIdx.x;
+    const bool on = tid < n_beam && !finished[tid];
+    const unsigned mine = __ballot_sync(0xffffffffu, on);
+    if (tid < kBeamMax && (tid & 31) == 0) s_on[tid >> 5] = mine;
+    __syncthreads();
+    int total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kBeamMax / 32; ++w) {
+        const int c = __popc(s_on[w]);
+        if (w < tid >> 5) before += c;
+        total += c;
+    }
+    if (on) s_beam[before + __popc(mine & ((1u << (tid & 31)) - 1))] = tid;
+    __syncthreads();
+    return total;
 }
 
 struct BeamPart {
@@ -231,11 +268,13 @@ __device__ u64 beam_tighten(u64* list, int* s_cnt, int cnt, int n, u64 T, int* h
 }
 
 __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __restrict__ logits,
-                                                               const int32_t* __restrict__ finished, int vocab,
-                                                               int parts, int per, int n, u64* __restrict__ keys,
+                                                               const int32_t* __restrict__ finished, int n_beam,
+                                                               int vocab, const BeamSplit split, int n,
+                                                               u64* __restrict__ keys,
                                                                BeamPart* __restrict__ stats) {
     constexpr int kWarps = kBsThreads / 32;
-    __shared__ __align__(16) u64 list[kBsList];
+    extern __shared__ __align__(16) u64 list[];                  // [kBsList]
+    float* s_tile = reinterpret_cast<float*>(list + kBsList);    // [kBsTile]
     __shared__ int s_cnt;
     __shared__ __align__(16) int s_hist[2 * kBsThreads + 4];
     __shared__ double s_tab[16];
@@ -243,13 +282,25 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     __shared__ uint32_t s_t[kWarps];
     __shared__ float s_m[kWarps];
     __shared__ double s_l[kWarps];
-    const int part = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ int s_beam[kBeamMax];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) s_cnt = 0;
     if (tid < 16) s_tab[tid] = exp2(tid / 16.0);
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    if (finished && finished[b]) return;  // the merge does not look at an ended beam's lists
+    int b = blockIdx.y, part = blockIdx.x, per = split.per, at = b * split.parts + part;
+    if (split.share) {
+        const int live = beam_live(finished, n_beam, s_beam), parts = beam_parts(live, vocab, split.room);
+        at = blockIdx.x;
+        const int rank = at / parts;
+        if (rank >= live) return;
+        b = s_beam[rank];
+        part = at - rank * parts;
+        per = (vocab + parts - 1) / parts;
+    } else if (finished && finished[b]) {
+        return;  // the merge does not look at an ended beam's lists
+    }
     const float* x = logits + (size_t)b * vocab;
     const int i0 = part * per, i1 = min(vocab, i0 + per);
     float m = -INFINITY;  // reference of l, at most 64 below the thread's maximum
@@ -300,18 +351,20 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
                 }
             }
             if (__any_sync(0xffffffffu, take != 0)) {
-                int at = __popc(take);
+#pragma unroll
+                for (int j = 0; j < kBsPer; ++j) s_tile[j * kBsThreads + tid] = v[j];  // to be picked by index
+                int to = __popc(take);
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, at, o);
-                    if (lane >= o) at += y;
+                    const int y = __shfl_up_sync(0xffffffffu, to, o);
+                    if (lane >= o) to += y;
                 }
                 int start = 0;
-                if (lane == 31) start = atomicAdd(&s_cnt, at);
-                at += __shfl_sync(0xffffffffu, start, 31) - __popc(take);
-                for (; take; take &= take - 1) {  // few per thread: read again rather than picked from registers
-                    const int i = base + (__ffs(take) - 1) * kBsThreads + tid;
-                    list[at++] = (u64)ord32(__ldg(x + i)) << 32 | (0xFFFFFFFFu - (uint32_t)i);
+                if (lane == 31) start = atomicAdd(&s_cnt, to);
+                to += __shfl_sync(0xffffffffu, start, 31) - __popc(take);
+                for (; take; take &= take - 1) {  // few per thread
+                    const int j = __ffs(take) - 1;
+                    list[to++] = (u64)ord32(s_tile[j * kBsThreads + tid]) << 32 | (0xFFFFFFFFu - (uint32_t)(base + j * kBsThreads + tid));
                 }
             }
         }
@@ -359,7 +412,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     }
     __syncthreads();
     const int cnt = s_cnt;
-    u64* out = keys + ((size_t)b * parts + part) * n;
+    u64* out = keys + (size_t)at * n;
     if (cnt <= 2 * kBsThreads) {
         // place by the number of larger keys: by their values, and where two values
         // are equal once more by the whole keys
@@ -416,7 +469,7 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
             const double f = s_m[w] - mm > -700.0f ? exp_taylor((double)s_m[w] - (double)mm) : 0.0;
             ll += s_l[w] == s_l[w] ? s_l[w] * f : s_l[w];  // a NaN stays
         }
-        stats[(size_t)b * parts + part] = BeamPart{ll, mm, 0};
+        stats[at] = BeamPart{ll, mm, 0};
     }
 }
 
@@ -487,21 +540,24 @@ __device__ __forceinline__ uint32_t cta_bound(uint32_t v, int n, int* hist) {
 
 __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     const u64* __restrict__ keys, const BeamPart* __restrict__ stats, const float* scores, const int32_t* finished,
-    int n_beam, int parts, int n, int eos, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
+    int n_beam, int vocab, const BeamSplit split, int n, int eos, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
     int32_t* out_finished) {
     __shared__ __align__(16) BeamKey list[kBmList];
     __shared__ double s_lse[kBeamMax], s_score[kBeamMax];
     __shared__ int s_rank[kBeamMaxOut * 2], s_seen[kBeamMaxOut * 2];
     __shared__ uint4 s_k32[kBeamMaxOut / 2 + 1];
     __shared__ int s_cnt, s_live, s_full;
+    __shared__ int s_beam[kBeamMax];
     const int tid = threadIdx.x;
     if (tid == 0) s_cnt = s_live = s_full = 0;
-    __syncthreads();
+    // read before the wait: the first kernel has let this one start after its own
+    const int n_live = split.share ? beam_live(finished, n_beam, s_beam) : n_beam;
+    const int parts = split.share ? beam_parts(n_live, vocab, split.room) : split.parts;
     pdl_wait();
     // Everything that is read first is asked for at once: the first entries of the
     // lists, a thread per list; the parts' sums, 4 to 32 lanes per beam; the beams' scores.
-    const int lists = n_beam * parts;  // < kBmThreads
-    const int b = min(tid / parts, n_beam - 1);
+    const int lists = n_live * parts;  // <= kBmThreads
+    const int at = tid / parts;
     const u64* mine = keys + (size_t)tid * n;
     constexpr int kAhead = 4;  // entries of the list that are loaded together
     u64 ahead[kAhead];
@@ -515,12 +571,13 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
         for (int i = 1; i < kAhead; ++i) e = (r & (kAhead - 1)) == i ? ahead[i] : e;
         return e;
     };
-    if (tid < lists) load(0);  // of ended beams too, whose entries are not used
+    if (tid < lists) load(0);
     int width = 32;
-    while (width > 4 && n_beam * width > kBmThreads) width >>= 1;
+    while (width > 4 && n_live * width > kBmThreads) width >>= 1;
     const int w = tid / width, wl = tid & (width - 1);
-    const BeamPart* st = stats + (size_t)min(w, n_beam - 1) * parts;
-    const BeamPart part0 = st[min(wl, parts - 1)];
+    const BeamPart* st = stats + (size_t)w * parts;
+    BeamPart part0{0.0, -INFINITY, 0};
+    if (w < n_live && wl < parts) part0 = st[wl];
     // the scores; NaN for a beam without lists (ended, or no candidate can be better than none)
     if (tid < n_beam) {
         const float s = scores[tid];
@@ -530,9 +587,10 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
         else if (s > -INFINITY) list[atomicAdd(&s_cnt, 1)] = BeamKey{ord64((double)s), ~((u64)tid << 56 | (u64)eos)};
     }
     __syncthreads();
+    const int b = tid < lists ? split.share ? s_beam[at] : at : 0;
     const bool has = tid < lists && s_score[b] == s_score[b];
     {
-        const bool on = w < n_beam && s_score[min(w, n_beam - 1)] == s_score[min(w, n_beam - 1)];
+        const bool on = w < n_live;
         // a lane's parts as one, then the lanes'
         float M = -INFINITY;
         double l = 0.0;
@@ -560,7 +618,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
         if (on && wl == 0) s_lse[w] = (double)M + log_of_sum(l);
     }
     __syncthreads();
-    const double score = s_score[b], lse = has ? s_lse[b] : 0.0;
+    const double score = s_score[b], lse = has ? s_lse[at] : 0.0;
     // the lists' first R entries, which with the ended beams are enough unless many are no candidates
     const int R = min(n, (n + max(1, s_live * parts) - 1) / max(1, s_live * parts));
     int r = 0;  // entries of this thread's list that were taken
@@ -701,16 +759,16 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     }
 }
 
-// Parts of a beam's vocabulary: about three CTAs per SM over all beams, no part
-// shorter than one tile.
-static int beam_parts(int n_beam, int vocab, int sm_count) {
+// The most lists: kBsCtasPerSm CTAs per SM, twice that where the beams outnumber
+// the SMs.
+static int beam_room(int n_beam, int vocab, int sm_count) {
     const int tiles = (vocab + kBsTile - 1) / kBsTile;
-    const int want = (kBsCtasPerSm * sm_count + n_beam - 1) / n_beam;
-    return tiles < want ? tiles : want;
+    const int room = min(kBmThreads, (n_beam > sm_count ? 2 : 1) * kBsCtasPerSm * sm_count);
+    return max(n_beam, min(room, n_beam * tiles));
 }
 
 size_t beam_workspace_bytes(int n_beam, int vocab, int n_out, int sm_count) {
-    const size_t lists = (size_t)n_beam * beam_parts(n_beam, vocab, sm_count);
+    const size_t lists = beam_room(n_beam, vocab, sm_count);
     return (lists * n_out * sizeof(u64) + 255) / 256 * 256 + lists * sizeof(BeamPart);
 }
 
@@ -718,16 +776,19 @@ int beam_select_launch(const float* logits, const float* scores, const int32_t* 
                        int eos, int n_out, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
                        int32_t* out_finished, void* ws, cudaStream_t st) {
     static_assert(kBeamMaxOut <= kBsThreads && kBeamMaxOut <= kBmThreads / 4, "the lists' capacities");
-    const int parts = beam_parts(n_beam, vocab, device_info().sm_count);
-    const int per = (vocab + parts - 1) / parts;
+    static_assert(kBeamMax <= kBsThreads && kBeamMax <= kBmThreads, "a thread per beam");
+    const int room = beam_room(n_beam, vocab, device_info().sm_count);
+    BeamSplit split{room, beam_parts(n_beam, vocab, room), 0, finished && n_beam * kBsShare > room};
+    split.per = (vocab + split.parts - 1) / split.parts;
     u64* keys = static_cast<u64*>(ws);
-    const size_t lists = (size_t)n_beam * parts;
-    BeamPart* stats = reinterpret_cast<BeamPart*>(static_cast<uint8_t*>(ws) + (lists * n_out * sizeof(u64) + 255) / 256 * 256);
-    if (launch_after(beam_part_kernel, dim3(parts, n_beam), dim3(kBsThreads), 0, st, logits, finished, vocab, parts, per,
-                     n_out, keys, stats) != cudaSuccess)
+    BeamPart* stats = reinterpret_cast<BeamPart*>(static_cast<uint8_t*>(ws) + ((size_t)room * n_out * sizeof(u64) + 255) / 256 * 256);
+    constexpr size_t smem = kBsList * sizeof(u64) + kBsTile * sizeof(float);
+    if (set_smem_limit(beam_part_kernel, smem) != cudaSuccess) return kErrCuda;
+    if (launch_after(beam_part_kernel, split.share ? dim3(room) : dim3(split.parts, n_beam), dim3(kBsThreads), smem, st,
+                     logits, finished, n_beam, vocab, split, n_out, keys, stats) != cudaSuccess)
         return kErrCuda;
     return launch_after(beam_merge_kernel, dim3(1), dim3(kBmThreads), 0, st, (const u64*)keys, (const BeamPart*)stats,
-                        scores, finished, n_beam, parts, n_out, eos, out_scores, out_parents, out_tokens,
+                        scores, finished, n_beam, vocab, split, n_out, eos, out_scores, out_parents, out_tokens,
                         out_finished) == cudaSuccess
                ? kOk
                : kErrCuda;

@@ -531,6 +531,18 @@ def test_beam(gpu, b, vocab, n):
         check_beam(run_beam(gpu, x, s, None, -1, n), beam_ref(x, s, None, -1, n))
 
 
+@pytest.mark.parametrize("ended", ["none", "all", "all but one", "first half", "every third", "the last"])
+@pytest.mark.parametrize("b,vocab,n", [(29, 40001, 58), (64, 9001, 128), (100, 17000, 200), (149, 8200, 256), (256, 4097, 256), (256, 30000, 7)])
+def test_beam_ended_beams_leave_their_share(gpu, b, vocab, n, ended):
+    """Many beams: the vocabulary is divided by the number of those that have not ended."""
+    x, s = randn(65, b, vocab) * 2, -torch.rand(b, device="cuda", generator=gen(66)) * 4
+    i = torch.arange(b, device="cuda")
+    fin = {"none": i < 0, "all": i >= 0, "all but one": i != b // 2, "first half": i < b // 2, "every third": i % 3 == 0, "the last": i == b - 1}[ended]
+    fin = fin.int()
+    s[b // 3] = float("-inf")
+    check_beam(run_beam(gpu, x, s, fin, 11, n), beam_ref(x, s, fin, 11, n))
+
+
 @pytest.mark.parametrize("kind", ["equal", "few", "rising", "falling", "masked", "one", "huge", "zeros", "tiny"])
 @pytest.mark.parametrize("b,vocab,n", [(3, 20000, 64), (1, 9000, 256), (2, 70001, 5)])
 def test_beam_hard_logits(gpu, kind, b, vocab, n):
