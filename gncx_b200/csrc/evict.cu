@@ -549,7 +549,9 @@ template <int KPT, int SIZE>
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs a) {
     constexpr int kWords = 32 * KPT;  // of 32 rows, per CTA
     static_assert(kEvThreads == 1024, "32 warps, and a word per thread where KPT is 32");
-    __shared__ __align__(16) int hist[3][kEvBins];
+    // counts of two bins per word, bin 2 i in the low half: at most 16384 rows per CTA
+    __shared__ uint32_t hist[3][kEvBins / 2];
+    static_assert(kEvThreads * KPT < 65536, "a count fits 16 bits");
     __shared__ int s_scan[4][32];
     __shared__ u_int64_t s_scan2[32];
     __shared__ uint32_t s_gt[kWords], s_eq[kWords];
@@ -567,7 +569,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
     };
     const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row0 = rank * kEvThreads * KPT;
-    for (int i = tid; i < 3 * kEvBins; i += kEvThreads) hist[0][i] = 0;
+    for (int i = tid; i < 3 * kEvBins / 2; i += kEvThreads) hist[0][i] = 0;
     pdl_wait();
     pdl_launch_dependents();
     uint32_t key[KPT];
@@ -592,25 +594,24 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
             // rows of equal digits (equal weights, a shared exponent): one addition for the warp
             const uint32_t d0 = __shfl_sync(0xffffffffu, d, __ffs(act) - 1);
             const unsigned same = __ballot_sync(0xffffffffu, in && d == d0);
-            if (lane == 0) atomicAdd(&hist[pass][d0], __popc(same));
-            if (in && d != d0) atomicAdd(&hist[pass][d], 1);
+            if (lane == 0) atomicAdd(&hist[pass][d0 >> 1], (uint32_t)__popc(same) << 16 * (d0 & 1));
+            if (in && d != d0) atomicAdd(&hist[pass][d >> 1], 1u << 16 * (d & 1));
         }
         meet();
         // bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t
         const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
         int c0 = 0, c1 = 0;
+        uint32_t c[SIZE];
         if (SIZE == 1) {
-            c0 = hist[pass][b0];
-            c1 = hist[pass][b1];
+            c[0] = hist[pass][b0 / 2];
         } else {
-            int2 c[SIZE];
 #pragma unroll
-            for (int r = 0; r < SIZE; ++r) c[r] = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&hist[pass][b0], r));
+            for (int r = 0; r < SIZE; ++r) c[r] = *cluster.map_shared_rank(&hist[pass][b0 / 2], r);
+        }
 #pragma unroll
-            for (int r = 0; r < SIZE; ++r) {
-                c0 += c[r].x;
-                c1 += c[r].y;
-            }
+        for (int r = 0; r < SIZE; ++r) {
+            c0 += c[r] & 0xFFFFu;
+            c1 += c[r] >> 16;
         }
         int total;
         const int before = cta_scan(c1 + c0, s_scan[pass], total);
@@ -649,7 +650,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         int before = cta_scan(__popc(eq), s_scan[3], total);
         // the rows of the CTAs before this one that have the key: their bin of the last pass
         if (SIZE > 1)
-            for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&hist[2][prefix & 1023u], r);
+            for (int r = 0; r < rank; ++r)
+                before += *cluster.map_shared_rank(&hist[2][(prefix & 1023u) >> 1], r) >> 16 * (prefix & 1) & 0xFFFFu;
         uint32_t left = eq;
         for (int r = min(__popc(eq), max(0, need - before)); r > 0; --r) {
             keep |= left & (0u - left);
