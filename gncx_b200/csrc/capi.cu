@@ -896,11 +896,12 @@ static int32_t pick_workspace(const char* fn, void* given, size_t given_bytes, s
     } while (0)
 
 static bool tree_shape_ok(int32_t pos0, int32_t n_tok, int32_t n_heads, int32_t n_kv, int32_t hd) {
-    return pos0 >= 0 && n_tok > 0 && n_tok <= kTreeMaxTok && pos0 <= INT32_MAX - n_tok && n_kv <= 65535 &&
-           attention_shape_ok(n_heads, n_kv, hd);
+    return pos0 >= 0 && n_tok > 0 && n_tok <= kTreeMaxTok && pos0 <= kMaxCacheRows - n_tok && n_kv <= 65535 &&
+           attention_shape_ok(n_heads, n_kv, hd) && n_heads / n_kv <= (1 << 20) / n_tok;
 }
 static const char* const kTreeShape =
-    "pos0 >= 0, n_tok in 1..1024, n_heads a multiple of n_kv_heads, head_dim a multiple of 4 up to 256 are needed";
+    "pos0 >= 0, n_tok in 1..1024, at most 2^30 rows, n_heads a multiple of n_kv_heads, at most 2^20 query rows per KV head, "
+    "head_dim a multiple of 4 up to 256 are needed";
 
 size_t gncx_attention_tree_workspace(int32_t pos0, int32_t n_tok, int32_t n_heads, int32_t n_kv, int32_t hd,
                                      int32_t window) {
@@ -931,10 +932,11 @@ int32_t gncx_attention_tree(const float* q, const float* k_cache, const float* v
 }
 
 static bool step_shape_ok(int32_t pos, int32_t n_heads, int32_t n_kv, int32_t hd) {
-    return pos >= 0 && pos < INT32_MAX - 1024 && n_kv <= 65535 && attention_shape_ok(n_heads, n_kv, hd);
+    return pos >= 0 && pos < kMaxCacheRows && n_kv <= 65535 && attention_shape_ok(n_heads, n_kv, hd) && n_heads / n_kv <= 1 << 16;
 }
 static const char* const kStepShape =
-    "pos >= 0, n_heads a multiple of n_kv_heads, head_dim a multiple of 4 up to 256 are needed";
+    "pos in 0..2^30 - 1, n_heads a multiple of n_kv_heads, at most 65536 of them per KV head, head_dim a multiple of 4 up to "
+    "256 are needed";
 
 size_t gncx_mqa_attention_step_weights_workspace(int32_t pos, int32_t n_heads, int32_t n_kv, int32_t hd) {
     if (!step_shape_ok(pos, n_heads, n_kv, hd)) {
@@ -973,10 +975,10 @@ int32_t gncx_mqa_attention_step_weights(const float* q_vec, const float* k_vec, 
 }
 
 static bool evict_shape_ok(int32_t n_rows, int32_t n_keep, int32_t n_kv, int32_t hd) {
-    return n_rows >= 0 && n_rows < INT32_MAX - 1024 && n_keep >= 0 && n_keep <= n_rows && n_kv > 0 && n_kv <= 65535 && hd > 0 &&
+    return n_rows >= 0 && n_rows <= kMaxCacheRows && n_keep >= 0 && n_keep <= n_rows && n_kv > 0 && n_kv <= 65535 && hd > 0 &&
            hd % 4 == 0;
 }
-static const char* const kEvictShape = "0 <= n_keep <= n_rows, n_kv_heads > 0, head_dim a positive multiple of 4 are needed";
+static const char* const kEvictShape = "0 <= n_keep <= n_rows <= 2^30, n_kv_heads > 0, head_dim a positive multiple of 4 are needed";
 
 size_t gncx_kv_evict_workspace(int32_t n_rows, int32_t n_keep, int32_t n_kv) {
     if (!evict_shape_ok(n_rows, n_keep, n_kv, 4)) {

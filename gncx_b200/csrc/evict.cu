@@ -259,7 +259,8 @@ __device__ __forceinline__ void head_max_sum(const WeightsArgs& a, int h, int la
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     for (int p = lane; p < a.parts; p += 32) {
         const float m = rec[(size_t)p * (a.hd + 4)];
-        if (m != -INFINITY) L = fmaf(rec[(size_t)p * (a.hd + 4) + 1], __expf(m - M), L);
+        // the sum of a range without a maximum is 0, or NaN, which stays
+        L = fmaf(rec[(size_t)p * (a.hd + 4) + 1], m == -INFINITY ? 0.0f : __expf(m - M), L);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);

@@ -149,6 +149,7 @@ int32_t attention_scratch_records(int32_t pos, int32_t n_heads, int32_t window);
 // ---- several candidates, bounded caches (tree.cu, evict.cu, beam.cu) ----
 // Workspaces are 16-byte aligned; their content need not survive or be set.
 constexpr int kTreeMaxTok = 1024;       // drafted nodes per call
+constexpr int kMaxCacheRows = 1 << 30;
 constexpr int kBeamMax = 256;           // beams
 constexpr int kBeamMaxOut = 256;        // candidates kept
 constexpr int kBeamMaxVocab = 1 << 24;  // tokens

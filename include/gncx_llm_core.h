@@ -237,7 +237,9 @@ int32_t gncx_mqa_attention_step_noalloc(const float* q_vec, const float* k_vec, 
  * gncx_last_error_message() words).  A refused call has written nothing.
  * Buffers are memory of the current device (or managed / mapped memory); the
  * vectors and caches start on 16-byte boundaries, the other arrays on 4-byte
- * ones.  Caches have the reference layout [row][n_kv][head_dim].  `workspace`
+ * ones.  Caches have the reference layout [row][n_kv][head_dim] and up to 2^30
+ * rows; an infinity or NaN in a K row that a query sees may make that query's
+ * output NaN, one in a V row shows in that column.  `workspace`
  * is scratch of at least the _workspace query's bytes (16-byte aligned, no
  * content kept between calls; the size does not shrink when the position
  * grows); NULL takes the library's own.  Calls that may run at the same time

@@ -356,6 +356,18 @@ def test_step_weights(gpu, nh, nkv, hd, pos, write):
         assert bool((err <= (tol_w + (group + 1) * U) * add + U * ref_w + 1e-38).all()), c
 
 
+@pytest.mark.parametrize("rows", [(0, 401), (31, 62), (100, 300), (17, 18), (400, 401)])
+def test_step_weights_nan_rows_show(gpu, rows):
+    """A NaN among a KV head's scores makes its weights and outputs NaN, also where it fills a whole range of rows."""
+    nh, nkv, hd, pos = 4, 2, 64, 400
+    q, k, v = randn(49, nh, hd), randn(50, pos + 1, nkv, hd), randn(51, pos + 1, nkv, hd)
+    k[rows[0]:rows[1], 0, 5] = float("nan")
+    weight = torch.ones(nkv, pos + 1, device="cuda")
+    out = run_step(gpu, q, None, None, k, v, pos, pos, hd**-0.5, 0, weight, None)
+    assert bool(out[:2].isnan().all()) and bool(weight[0].isnan().all())
+    assert bool(out[2:].isfinite().all()) and bool(weight[1].isfinite().all())
+
+
 def test_step_weights_without_positions_and_own_workspace(gpu):
     nh, nkv, hd, pos = 8, 4, 128, 777
     q, k, v = randn(46, nh, hd), randn(47, pos + 1, nkv, hd), randn(48, pos + 1, nkv, hd)

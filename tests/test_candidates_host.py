@@ -23,7 +23,8 @@ def tree(lib, pos0=4, n_tok=3, nh=4, nkv=2, hd=64):
 
 
 @pytest.mark.parametrize("bad", [dict(pos0=-1), dict(n_tok=0), dict(n_tok=-3), dict(n_tok=1025), dict(nh=3), dict(nkv=0),
-                                 dict(nh=0), dict(hd=0), dict(hd=66), dict(hd=260), dict(pos0=2**31 - 2, n_tok=8)])
+                                 dict(nh=0), dict(hd=0), dict(hd=66), dict(hd=260), dict(pos0=2**31 - 2, n_tok=8),
+                                 dict(pos0=2**30 - 7, n_tok=8), dict(nh=1025, nkv=1, n_tok=1024), dict(nkv=65536, nh=65536)])
 def test_tree_refuses(lib, bad):
     assert tree(lib, **bad) == INVALID
     assert lib.gncx_last_error() == INVALID
@@ -32,7 +33,8 @@ def test_tree_refuses(lib, bad):
     assert lib.gncx_attention_tree_workspace(a["pos0"], a["n_tok"], a["nh"], a["nkv"], a["hd"], 0) == 0
 
 
-@pytest.mark.parametrize("bad", [dict(pos=-1), dict(nh=3), dict(nkv=0), dict(hd=62), dict(hd=512), dict(stride=7)])
+@pytest.mark.parametrize("bad", [dict(pos=-1), dict(nh=3), dict(nkv=0), dict(hd=62), dict(hd=512), dict(stride=7),
+                                 dict(pos=2**30, stride=2**31 - 1), dict(nh=65537, nkv=1)])
 def test_step_refuses(lib, bad):
     a = dict(pos=7, nh=4, nkv=2, hd=64, stride=8) | bad
     assert lib.gncx_mqa_attention_step_weights(FAKE, FAKE, FAKE, FAKE, FAKE, a["pos"], a["pos"], a["nh"], a["nkv"], a["hd"],
@@ -40,7 +42,7 @@ def test_step_refuses(lib, bad):
     assert lib.gncx_last_error() == INVALID
 
 
-@pytest.mark.parametrize("bad", [dict(rows=-1, keep=-1), dict(keep=9), dict(keep=-1), dict(nkv=0), dict(hd=0), dict(hd=6),
+@pytest.mark.parametrize("bad", [dict(rows=-1, keep=-1), dict(rows=2**30 + 1, stride=2**31 - 1), dict(keep=9), dict(keep=-1), dict(nkv=0), dict(hd=0), dict(hd=6),
                                  dict(stride=7), dict(out_stride=3), dict(pos=None), dict(pos_out=None),
                                  dict(w_out=FAKE), dict(pos_out=FAKE + 4096)])
 def test_evict_refuses(lib, bad):
