@@ -320,7 +320,7 @@ static void tree_geometry(TreeArgs& a, int sm_count) {
     a.lo = lo < 0 ? 0 : lo > a.pos0 ? a.pos0 : (int)lo;
     const int len = a.pos0 - a.lo;
     a.tc = tree_tc_ok(a.hd);
-    const int qrows = a.tc ? kTcTreeRows : kTdRows, keys = a.tc ? kTcTreeKeys : kTdKeys;
+    const int qrows = a.tc ? tree_tc_rows(a.hd) : kTdRows, keys = a.tc ? tree_tc_keys(a.hd) : kTdKeys;
     const int64_t ctas = (int64_t)a.n_kv * ((a.n_tok * a.G + qrows - 1) / qrows);  // per split
     // CUDA cores: about two CTAs per SM; tensor cores: one per SM, in one wave
     int want = (int)(a.tc ? sm_count / ctas : (2 * (int64_t)sm_count + ctas - 1) / ctas);

@@ -29,10 +29,11 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Dense range on the tensor cores: head sizes it takes, query rows per CTA, launch.
+// Dense range on the tensor cores: head sizes it takes, query rows per CTA, cache
+// rows per tile, launch.
 bool tree_tc_ok(int hd);
-constexpr int kTcTreeRows = 256;
-constexpr int kTcTreeKeys = 64;
+__host__ __device__ constexpr int tree_tc_rows(int hd) { return hd > 128 ? 128 : 256; }
+__host__ __device__ constexpr int tree_tc_keys(int hd) { return hd > 128 ? 32 : 64; }
 cudaError_t tree_tc_launch(const TreeArgs& a, cudaStream_t st);
 
 }  // namespace gncx

@@ -8,14 +8,15 @@
 // where that is more), and a b is the sum of the products hi hi, lo hi and
 // hi lo, each exact in the fp32 accumulator; lo lo (2^-22 of the product) is
 // left out.  bf16 pairs would keep 16 bits, a tf32 pair costs twice the tensor
-// time.  Groups: a query row; 8 cache rows of K; 8 cache rows of V.
+// time.  Groups: a query row; 8 cache rows of K; 8 cache rows of V (4 rows each
+// for head sizes above 128).
 //
 // One CTA takes up to 256 query rows of one KV head as two lanes A and B of
 // 128 and walks its split of the cache in tiles of 64 rows, each K and V row
 // read and split once for both lanes; with at most 128 query rows and several
 // tiles both lanes serve the same rows, tile t on lane t & 1 (ALT), and join
 // their sums at the end:
-//   * loader warps 8-11 bring 8-row chunks in with cp.async (four in flight per
+//   * loader warps 8-11 bring chunks of 8 rows in with cp.async (four in flight per
 //     warp, 64 KB per SM), split them and write the K-major operand tiles;
 //   * warp 12, one thread, issues S = Q K^T (Q pairs stay in TMEM) and, once a
 //     lane's weights are in TMEM over its scores, O = P V into the shared O
@@ -23,7 +24,20 @@
 //   * warps 0-3 (A) and 4-7 (B), a thread per query row: online softmax, P
 //     pairs, and the sum of the tiles' O in fp32 registers: a sum over all
 //     tiles in TMEM would add up the tensor core's cut-off bits.
+// Head sizes above 128 (WIDE): 128 query rows and tiles of 32 rows, as Q's pairs
+// take all of its TMEM columns and a tile as much shared memory; lane A computes
+// the weights, and each lane sums half of the output's columns.
 // Every wait is bounded; on a timeout the kernel records an error and leaves.
+//
+// What bounds it: latency, with the tensor pipe, shared memory and the issue slots
+// each about half busy.  64 nodes, 32 heads, 8 KV heads of 128, 32768 rows: 118 us
+// with the merge (2.3 TB/s; three fp16 products at 870 TFLOP/s, of which the
+// pipe alone would need 60 us), tensor pipe 43 % busy, issue 46 %.  1 node:
+// 70 us, 3.8 TB/s.  16 heads, 4 KV heads of 256, 64 nodes, 32768 rows: 162 us (tree.cu's
+// CUDA-core kernel: 3799 us).  Slower: two threads per row with 16 softmax warps
+// (128 us for the first case), lanes of different tiles in CTAs of 128 rows with 8
+// loader warps (147 us), Q's lo parts in shared memory for a second S buffer
+// (121 us), a weight reference without the pass for the maximum (118 us).
 #include <cuda_fp16.h>
 #include "common.cuh"
 #include "kernels.h"
@@ -36,10 +50,14 @@ namespace gncx {
 constexpr int kTtThreads = 512;
 constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12;
 // Registers per thread: softmax, loaders, products (whose warpgroup is filled
-// up by idle warps); together the 512 x 128 that the block is launched with.
-constexpr int kTtSoftmaxRegs = 184, kTtLoadRegs = 96, kTtMmaRegs = 48;
-static_assert(2 * kTtSoftmaxRegs + kTtLoadRegs + kTtMmaRegs <= 4 * 128, "a split that can be had");
-constexpr int kTtKStride = 64 * 16 + 16;  // bytes between 8-column chunks of the K tile: shifted by a bank group
+// up by idle warps); together at most the 512 x 128 that the block is launched
+// with.  With 184 for head size 256 the softmax spills in its loop: 346 us instead
+// of 193 (16 heads, 4 KV heads, 64 nodes, 32768 rows).
+template <int HD>
+struct TtRegs {
+    static constexpr int kSoftmax = HD > 128 ? 192 : 184, kLoad = HD > 128 ? 88 : 96, kMma = HD > 128 ? 40 : 48;
+    static_assert(2 * kSoftmax + kLoad + kMma <= 4 * 128, "a split that can be had");
+};
 constexpr int kTtStages = 2;              // K and V operand tiles
 constexpr int kTtScales = 4;              // tiles whose scales are kept
 // Weights are held as 2^(score - reference + kTtShift), with the score at most
@@ -51,21 +69,24 @@ constexpr int kTtShift = 10, kTtHead = 4;
 // rows (28 tiles) 80.4 and 90; with 4 tiles the joining costs as much as it saves
 // (32 heads, 24 nodes, 4096 rows: 24.3 and 23.8).
 constexpr int kTtAltTiles = 6;
-// TMEM columns
-constexpr int kTtQ = 0, kTtS = 256, kTtO = 384, kTtCols = 512;
+// TMEM columns: Q pairs, scores, (head sizes above 128: weights), outputs
+constexpr int kTtQ = 0, kTtS = 256, kTtP = 320, kTtO = 384, kTtCols = 512;
 
 template <int HD>
 struct TtLayout {
-    static constexpr int kPart = HD / 8 * kTtKStride;  // one of K hi, K lo, V hi, V lo
+    static constexpr int kKeys = tree_tc_keys(HD);
+    static constexpr int kRows = kKeys / 8;             // of a chunk: the rows that share a scale
+    static constexpr int kStride = kKeys * 16 + 16;     // bytes between 8-column chunks of a tile: shifted by a bank group
+    static constexpr int kPart = HD / 8 * kStride;      // one of K hi, K lo, V hi, V lo
     static constexpr int kStage = 4 * kPart;
-    static constexpr int kChunk = 8 * HD * 4;
+    static constexpr int kChunk = kRows * HD * 4;
     static constexpr int oStaging = kTtStages * kStage;
     static constexpr int oScale = oStaging + 16 * kChunk;     // int [kTtScales][2][8]
     static constexpr int oBar = oScale + kTtScales * 2 * 8 * 4;
     static constexpr int kBars = 4 * kTtStages + 2 + 6 + 2;
-    static constexpr int oState = oBar + kBars * 8;    // lane 1's reference and sum of each row: float [2][128]
+    static constexpr int oState = oBar + kBars * 8;    // what the lanes tell each other of each row: float [2][128]
     static constexpr int kBytes = oState + 2 * 128 * 4;
-    static_assert(kStage >= 128 * HD * 4, "a lane's output fits an operand stage");
+    static_assert(HD > 128 || kStage >= 128 * HD * 4, "a lane's output fits an operand stage");
     // more than half of an SM's shared memory, so one CTA per SM owns all of TMEM
     static constexpr int kAlloc = kBytes > 120 * 1024 ? kBytes : 120 * 1024;
 };
@@ -151,9 +172,16 @@ __device__ __forceinline__ uint32_t warp_max_bits(float (&x)[N], Inf inf) {
 }
 
 // ALT: at most 128 query rows, both lanes on them, tile t on lane t & 1.
+// HD 256 (WIDE): both lanes on 128 rows, lane 0 with columns 0-127 of the output,
+// lane 1 with the others.
 template <int HD, bool ALT>
 __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a) {
     using L = TtLayout<HD>;
+    constexpr bool WIDE = HD > 128;
+    static_assert(!(WIDE && ALT), "one way to share rows");
+    constexpr int KEYS = L::kKeys, CR = L::kRows;
+    constexpr int HO = WIDE ? 128 : HD;  // columns of a lane's output
+    constexpr bool kShared = ALT || WIDE;  // both lanes on the same rows, S of tile t in block t & 1
     extern __shared__ __align__(128) uint8_t sm[];
     int* scales = reinterpret_cast<int*>(sm + L::oScale);
     uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + L::oBar);
@@ -175,12 +203,13 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     __shared__ int any_infinite;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * kTcTreeRows;
+    const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * tree_tc_rows(HD);
     const int rows = a.n_tok * a.G;
-    const int nl = !ALT && rows - r0 > 128 ? 2 : 1;  // row blocks of 128
+    const int nl = WIDE || (!ALT && rows - r0 > 128) ? 2 : 1;  // products into O per tile
     const int j0 = a.lo + split * a.per, j1 = min(a.pos0, j0 + a.per);
-    const int n_tiles = (j1 - j0 + kTcTreeKeys - 1) / kTcTreeKeys;
-    auto phase = [](int t) { return (uint32_t)(ALT ? t >> 1 : t) & 1; };  // of a lane's barriers
+    const int n_tiles = (j1 - j0 + KEYS - 1) / KEYS;
+    auto phase = [](int t) { return (uint32_t)(ALT ? t >> 1 : t) & 1; };        // of a lane's barriers
+    auto phase_s = [](int t) { return (uint32_t)(kShared ? t >> 1 : t) & 1; };  // of the scores'
 
     if (tid == 0) {
         for (int i = 0; i < kTtStages; ++i) {
@@ -229,15 +258,15 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     };
 
     if (warp >= kTtMmaWarp) {
-        regs_dec<kTtMmaRegs>();
+        regs_dec<TtRegs<HD>::kMma>();
         if (warp == kTtMmaWarp) {
             // ---------------- products: the warp waits, one thread issues ----------------
-            constexpr uint32_t idesc_s = umma_idesc_f16(128, kTcTreeKeys), idesc_o = umma_idesc_f16(128, HD) | kUmmaTransB;
+            constexpr uint32_t idesc_s = umma_idesc_f16(128, KEYS), idesc_o = umma_idesc_f16(128, HO) | kUmmaTransB;
             const uint32_t sbase = smem_u32(sm);
-            auto scores = [&](int x, int t) {  // S_x = Q_x K(t)^T
-                const uint32_t hi = umma_desc_lo(sbase + (t & 1) * L::kStage, kTtKStride), lo = hi + (L::kPart >> 4);
-                const uint32_t q = tmem + kTtQ + (ALT ? 0 : x * 128), d = tmem + kTtS + x * 64;
-                constexpr uint32_t step = 2 * kTtKStride >> 4, rest = umma_desc_hi(128);
+            auto scores = [&](int x, int t) {  // S_x = Q_x K(t)^T, or Q K(t)^T
+                const uint32_t hi = umma_desc_lo(sbase + (t & 1) * L::kStage, L::kStride), lo = hi + (L::kPart >> 4);
+                const uint32_t q = tmem + kTtQ + (kShared ? 0 : x * 128), d = tmem + kTtS + x * KEYS;
+                constexpr uint32_t step = 2 * L::kStride >> 4, rest = umma_desc_hi(128);
                 if (elect_one()) {
                     mbar_arrive(&sfull[x]);  // orders the loaders' scales before the lane's reads
                     umma_f16_ts<false>(d, q + HD / 2, hi, rest, idesc_s);
@@ -251,20 +280,20 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 }
                 __syncwarp();
             };
-            auto values = [&](int x, int t) {  // O = P_x V(t)
+            auto values = [&](int x, int t) {  // O = P_x V(t), or P V(t)'s columns 128 x ..
                 // V's rows are the reduction here: 8 x 16-byte core matrices as K's, transposed
-                const uint32_t hi = umma_desc_lo(sbase + (t & 1) * L::kStage + 2 * L::kPart, 128), lo = hi + (L::kPart >> 4);
-                const uint32_t p = tmem + kTtS + x * 64, d = tmem + kTtO;
-                constexpr uint32_t step = 16 * 16 >> 4, rest = umma_desc_hi(kTtKStride);
+                const uint32_t hi = umma_desc_lo(sbase + (t & 1) * L::kStage + 2 * L::kPart + (WIDE ? x * 16 * L::kStride : 0), 128), lo = hi + (L::kPart >> 4);
+                const uint32_t p = tmem + (WIDE ? kTtP + (t & 1) * KEYS : kTtS + x * 64), d = tmem + kTtO;
+                constexpr uint32_t step = 16 * 16 >> 4, rest = umma_desc_hi(L::kStride);
                 // P's block of 16 rows i: columns 16 i .. + 7 hold the hi parts, + 8 .. + 15 the lo parts
                 if (elect_one()) {
                     umma_f16_ts<false>(d, p + 8, hi, rest, idesc_o);
 #pragma unroll
-                    for (int i = 1; i < 4; ++i) umma_f16_ts<true>(d, p + 16 * i + 8, hi + i * step, rest, idesc_o);
+                    for (int i = 1; i < KEYS / 16; ++i) umma_f16_ts<true>(d, p + 16 * i + 8, hi + i * step, rest, idesc_o);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) umma_f16_ts<true>(d, p + 16 * i, lo + i * step, rest, idesc_o);
+                    for (int i = 0; i < KEYS / 16; ++i) umma_f16_ts<true>(d, p + 16 * i, lo + i * step, rest, idesc_o);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) umma_f16_ts<true>(d, p + 16 * i, hi + i * step, rest, idesc_o);
+                    for (int i = 0; i < KEYS / 16; ++i) umma_f16_ts<true>(d, p + 16 * i, hi + i * step, rest, idesc_o);
                     umma_commit(&ofull[x]);
                 }
                 __syncwarp();
@@ -273,13 +302,13 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 if (elect_one()) umma_commit(bar);
                 __syncwarp();
             };
-            constexpr int kAhead = ALT ? 2 : 1;  // a lane's next tile
+            constexpr int kAhead = ALT ? 2 : 1;  // the next tile into the same S
             bool ok = wait_warp(qfull, 0);
             for (int t = 0; ok && t < min(kAhead, n_tiles); ++t) {
                 ok = wait_warp(&kfull[t], 0);
                 if (!ok) break;
                 tc_fence_after();
-                for (int x = 0; x < nl; ++x) scores(ALT ? t : x, t);
+                for (int x = 0; x < (kShared ? 1 : nl); ++x) scores(kShared ? t : x, t);
                 commit(&kempty[t]);
             }
             int n_o = 0;                    // products into O so far
@@ -287,48 +316,49 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 for (int i = 0; ok && i < nl; ++i) {
                     const int x = ALT ? t & 1 : i;
                     // before the first product into O, oempty's phase "before 0" counts as complete
-                    ok = wait_all3(&pfull[x], phase(t), &vfull[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
+                    ok = wait_all3(&pfull[WIDE ? 0 : x], phase(t), &vfull[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     values(x, t);
                     ++n_o;
                     if (i == nl - 1) commit(&vempty[t & 1]);
                     const int t2 = t + kAhead;
-                    if (t2 < n_tiles) {
+                    if (t2 < n_tiles && !(WIDE && i == 1)) {  // WIDE: lane 1 was through with tile t2 - 2 before oempty
                         if (i == 0) ok = wait_warp(&kfull[t2 & 1], (t2 >> 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
-                        scores(x, t2);
-                        if (i == nl - 1) commit(&kempty[t2 & 1]);
+                        scores(WIDE ? t2 & 1 : x, t2);
+                        if (WIDE || i == nl - 1) commit(&kempty[t2 & 1]);
                     }
                 }
             commit(done);  // nothing of this CTA's is in flight when TMEM is freed
             if (!mbar_wait(done, 0)) record_error(a.err, kErrTimeout);
         }
     } else if (warp >= kTtLoadWarp) {
-        // ---------------- loaders: warp w takes rows 16 w .. 16 w + 15 of each tile ----------------
-        regs_dec<kTtLoadRegs>();
+        // ---------------- loaders: warp w takes two of the eight chunks of rows of each tile ----------------
+        regs_dec<TtRegs<HD>::kLoad>();
         const int lw = warp - kTtLoadWarp;
         const size_t pstride = (size_t)a.n_kv * a.hd;
         const float* src[2] = {a.kc + (size_t)kvh * a.hd, a.vc + (size_t)kvh * a.hd};
         uint8_t* staging = sm + L::oStaging + lw * 4 * L::kChunk;
-        // chunk i of tile t: K rows 0-7, 8-15, V rows 0-7, 8-15 of the warp's 16;
-        // float4 c of a row per lane, rows sub, sub + RS, ..
-        constexpr int LPR = HD / 4, RS = 32 / LPR;
-        const int c = lane % LPR, sub = lane / LPR;
-        auto row_of = [&](int t, int i) { return j0 + kTcTreeKeys * t + 16 * lw + 8 * (i & 1); };
+        // chunk i of tile t: the warp's first and second rows of K, of V; a lane's
+        // k-th float4 of a chunk is float4 col(k) of its row at(k)
+        constexpr int LPR = HD / 4, NK = CR * HD / 128;
+        auto at = [&](int k) { return WIDE ? k >> 1 : lane / LPR + 32 / LPR * k; };
+        auto col = [&](int k) { return WIDE ? lane + 32 * (k & 1) : lane % LPR; };
+        auto row_of = [&](int t, int i) { return j0 + KEYS * t + 2 * CR * lw + CR * (i & 1); };
         auto issue = [&](int t, int i) {
-            const int row = row_of(t, i) + sub;
-            const float* g = src[i >> 1] + (size_t)row * pstride + 4 * c;
-            float* d = reinterpret_cast<float*>(staging + i * L::kChunk) + sub * HD + 4 * c;
-            if (t < n_tiles && row_of(t, i) + 8 <= j1 && 4 * c < a.hd) {
+            const int row = row_of(t, i);
+            const float* g = src[i >> 1] + (size_t)row * pstride;
+            float* d = reinterpret_cast<float*>(staging + i * L::kChunk);
+            if (t < n_tiles && row + CR <= j1 && 4 * col(NK - 1) < a.hd) {
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) cp_async16_row(d + RS * k * HD, g + (size_t)(RS * k) * pstride);
+                for (int k = 0; k < NK; ++k) cp_async16_row(d + at(k) * HD + 4 * col(k), g + (size_t)at(k) * pstride + 4 * col(k));
             } else if (t < n_tiles) {  // zeros past the last row and column
 #pragma unroll 1
-                for (int k = 0; k < HD / 16; ++k) {
-                    const bool some = row + RS * k < j1 && 4 * c < a.hd;
-                    cp_async16_row(d + RS * k * HD, some ? g + (size_t)(RS * k) * pstride : src[0], some ? 16 : 0);
+                for (int k = 0; k < NK; ++k) {
+                    const bool some = row + at(k) < j1 && 4 * col(k) < a.hd;
+                    cp_async16_row(d + at(k) * HD + 4 * col(k), some ? g + (size_t)at(k) * pstride + 4 * col(k) : src[0], some ? 16 : 0);
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -344,16 +374,16 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 __syncwarp();
                 const float* st = reinterpret_cast<const float*>(staging + i * L::kChunk);
                 const int chunk = 2 * lw + (i & 1);
-                float x[HD / 4];
+                float x[4 * NK];
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const float4 v = *reinterpret_cast<const float4*>(st + (sub + RS * k) * HD + 4 * c);
+                for (int k = 0; k < NK; ++k) {
+                    const float4 v = *reinterpret_cast<const float4*>(st + at(k) * HD + 4 * col(k));
                     x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
                 }
                 const int s = scale_exp(warp_max_bits(x, [&](int e) {
                     if (i < 2) return;
-                    const int col = 4 * c + (e & 3);
-                    atomicOr(&infinite[x[e] < 0.0f][col >> 5], 1u << (col & 31));
+                    const int c = 4 * col(e >> 2) + (e & 3);
+                    atomicOr(&infinite[x[e] < 0.0f][c >> 5], 1u << (c & 31));
                     any_infinite = 1;
                     x[e] = 0.0f;
                 }));
@@ -361,14 +391,15 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 const f32x2 f = pack2(pow2i(s), pow2i(s));
                 if ((i & 1) == 0 && t >= kTtStages) ok = wait_warp(i ? &vempty[t & 1] : &kempty[t & 1], ((t >> 1) - 1) & 1);
                 if (!ok) break;
-                uint8_t* d = tile + (i >> 1) * 2 * L::kPart + (c >> 1) * kTtKStride + (8 * chunk + sub) * 16 + (c & 1) * 8;
+                uint8_t* d = tile + (i >> 1) * 2 * L::kPart + CR * chunk * 16;
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
+                for (int k = 0; k < NK; ++k) {
+                    uint8_t* dk = d + (col(k) >> 1) * L::kStride + at(k) * 16 + (col(k) & 1) * 8;
                     uint2 hi, lo;
                     split2(mul2(pack2(x[4 * k], x[4 * k + 1]), f), hi.x, lo.x);
                     split2(mul2(pack2(x[4 * k + 2], x[4 * k + 3]), f), hi.y, lo.y);
-                    *reinterpret_cast<uint2*>(d + RS * k * 16) = hi;
-                    *reinterpret_cast<uint2*>(d + L::kPart + RS * k * 16) = lo;
+                    *reinterpret_cast<uint2*>(dk) = hi;
+                    *reinterpret_cast<uint2*>(dk + L::kPart) = lo;
                 }
                 if (lane == 0) sc[8 * (i >> 1) + chunk] = s;
                 if (i & 1) {
@@ -379,37 +410,47 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if ((warp >> 2) < nl || ALT) {
+    } else if ((warp >> 2) < nl || kShared) {
         // ---------------- softmax and output: a thread per query row (and lane) ----------------
-        regs_inc<kTtSoftmaxRegs>();
+        regs_inc<TtRegs<HD>::kSoftmax>();
         const int x = warp >> 2;
-        const int first = r0 + (ALT ? 0 : 128 * x) + 32 * (warp & 3), row = first + lane;
+        const int first = r0 + (kShared ? 0 : 128 * x) + 32 * (warp & 3), row = first + lane;
         const bool active = first < rows;  // of the warp
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t tq = tmem + lanes + kTtQ + x * 128, ts = tmem + lanes + kTtS + x * 64, to = tmem + lanes + kTtO;
+        const uint32_t tq = tmem + lanes + kTtQ + x * (WIDE ? 64 : 128), to = tmem + lanes + kTtO;
+        constexpr int kQlo = HD / 2;  // columns from Q's hi to its lo parts
+        const int c0 = WIDE ? 128 * x : 0;  // the lane's first column
         int sq = 0;
+        float v[HO];  // the lane's columns of the row, in flight at once
+        float qm = 0.0f;
         if (active) {
             const bool some = row < rows;
-            const float* qp = a.q + ((size_t)(some ? row / a.G : 0) * a.n_heads + kvh * a.G + (some ? row % a.G : 0)) * a.hd;
-            float v[HD];  // the whole row in flight at once
+            const float* qp = a.q + ((size_t)(some ? row / a.G : 0) * a.n_heads + kvh * a.G + (some ? row % a.G : 0)) * a.hd + c0;
 #pragma unroll
-            for (int c = 0; c < HD / 4; ++c) {
-                const float4 w = some && 4 * c < a.hd ? *reinterpret_cast<const float4*>(qp + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c = 0; c < HO / 4; ++c) {
+                const float4 w = some && c0 + 4 * c < a.hd ? *reinterpret_cast<const float4*>(qp + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
                 v[4 * c] = w.x; v[4 * c + 1] = w.y; v[4 * c + 2] = w.z; v[4 * c + 3] = w.w;
             }
-            float m = 0.0f;
 #pragma unroll
-            for (int c = 0; c < HD; ++c) m = fmaxf(m, fabsf(v[c]) < INFINITY ? fabsf(v[c]) : 0.0f);
-            sq = scale_exp(__float_as_uint(m));
+            for (int c = 0; c < HO; ++c) qm = fmaxf(qm, fabsf(v[c]) < INFINITY ? fabsf(v[c]) : 0.0f);
+        }
+        if (WIDE) {  // the other columns' maximum
+            float* most = reinterpret_cast<float*>(sm + L::oState) + 32 * (warp & 3) + lane;
+            most[128 * x] = qm;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            qm = fmaxf(qm, most[128 * (x ^ 1)]);
+        }
+        if (active) {
+            sq = scale_exp(__float_as_uint(qm));
             if (x == 0 || !ALT) {
                 const f32x2 f = pack2(pow2i(sq), pow2i(sq));
 #pragma unroll
-                for (int b = 0; b < HD / 32; ++b) {
+                for (int b = 0; b < HO / 32; ++b) {
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) split2(mul2(pack2(v[32 * b + 2 * c], v[32 * b + 2 * c + 1]), f), hi[c], lo[c]);
                     tmem_st16(tq + 16 * b, hi);
-                    tmem_st16(tq + HD / 2 + 16 * b, lo);
+                    tmem_st16(tq + kQlo + 16 * b, lo);
                 }
                 tmem_wait_st();
             }
@@ -418,19 +459,23 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         if (x == 0 || !ALT) mbar_arrive(qfull);
 
         float T = -INFINITY, l = 0.0f;
-        f32x2 o[HD / 2];
+        f32x2 o[HO / 2];
 #pragma unroll
-        for (int d = 0; d < HD / 2; ++d) o[d] = 0;
+        for (int d = 0; d < HO / 2; ++d) o[d] = 0;
         bool ok = true;
 #pragma unroll 1
         for (int t = ALT ? x : 0; t < n_tiles; t += ALT ? 2 : 1) {
-            ok = wait_warp(&sfull[x], phase(t));
+            ok = wait_warp(&sfull[WIDE ? t & 1 : x], phase_s(t));
             if (!ok) break;
             float alpha = 1.0f, beta = 1.0f;
+            const uint32_t ts = tmem + lanes + kTtS + (WIDE ? (t & 1) * KEYS : x * 64), tp = WIDE ? tmem + lanes + kTtP + (t & 1) * KEYS : ts;
+            // the weights; WIDE: by lane 0, the other needs their reference alone.  The products of tile t - 2 have read this block of it, as they
+            // were issued before the one of tile t - 1 that lane 0 has waited for
+            const bool writes = !WIDE || x == 0;
             if (active) {
                 tc_fence_after();
                 const int4* sc = reinterpret_cast<const int4*>(scales + (t & (kTtScales - 1)) * 16);
-                const int valid = j1 - j0 - kTcTreeKeys * t;
+                const int valid = j1 - j0 - KEYS * t;
                 const int4 k0 = sc[0], k1 = sc[1];
                 // 2^(-sq - sk) may need two factors
                 auto factor = [&](int sk) {
@@ -439,27 +484,29 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 };
                 const bool even_k = k0.x == k0.y && k0.x == k0.z && k0.x == k0.w && k0.x == k1.x && k0.x == k1.y &&
                                     k0.x == k1.z && k0.x == k1.w;
-                const float c0 = factor(k0.x);
+                const float f0 = factor(k0.x);
                 float tm = -INFINITY;
-                if (even_k && valid >= kTcTreeKeys && c0 >= 0.0f) {
+                if (even_k && valid >= KEYS && f0 >= 0.0f) {
 #pragma unroll 1
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < KEYS / 32; ++h) {
                         float s[32];
                         tmem_ld32f(ts + 32 * h, s);
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) tm = fmaxf(tm, fmaxf(s[j], s[j + 1]));
                     }
-                    tm *= c0;
+                    tm *= f0;
                 } else {
 #pragma unroll 1
-                    for (int b = 0; b < 4; ++b) {
+                    for (int b = 0; b < KEYS / 16; ++b) {
                         float s[16];
                         tmem_ld16f(ts + 16 * b, s);
-                        const int* sk = reinterpret_cast<const int*>(sc) + 2 * b;
-                        const float ca = factor(sk[0]), cb = factor(sk[1]);
+                        const int* sk = reinterpret_cast<const int*>(sc) + 16 / CR * b;
+                        float f[16 / CR];
+#pragma unroll
+                        for (int i = 0; i < 16 / CR; ++i) f[i] = factor(sk[i]);
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
-                            if (16 * b + j < valid) tm = fmaxf(tm, s[j] * (j < 8 ? ca : cb));
+                            if (16 * b + j < valid) tm = fmaxf(tm, s[j] * f[j / CR]);
                     }
                 }
                 // the reference follows the maximum only when that has grown by more
@@ -479,40 +526,44 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 beta = pow2i(-U);
                 const float shift = kTtShift - ref;
                 f32x2 sum = 0;
-                if (even_k && even_v && valid >= kTcTreeKeys) {
-                    const f32x2 c02 = pack2(c0, c0), shift2 = pack2(shift, shift);
+                if (writes && even_k && even_v && valid >= KEYS) {
+                    const f32x2 f02 = pack2(f0, f0), shift2 = pack2(shift, shift);
 #pragma unroll 1
-                    for (int b = 0; b < 4; ++b) {
+                    for (int b = 0; b < KEYS / 16; ++b) {
                         float s[16];
                         uint32_t p[16];
                         tmem_ld16f(ts + 16 * b, s);
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
-                            const float2 z = unpack2(fma2(pack2(s[j], s[j + 1]), c02, shift2));
+                            const float2 z = unpack2(fma2(pack2(s[j], s[j + 1]), f02, shift2));
                             const f32x2 e = pack2(ex2(z.x), ex2(z.y));
                             sum = add2(sum, e);
                             split2(e, p[j / 2], p[8 + j / 2]);
                         }
-                        tmem_st16(ts + 16 * b, p);
+                        tmem_st16(tp + 16 * b, p);
                     }
-                } else {
+                } else if (writes) {
 #pragma unroll 1
-                    for (int b = 0; b < 4; ++b) {
+                    for (int b = 0; b < KEYS / 16; ++b) {
                         float s[16];
                         uint32_t p[16];
                         tmem_ld16f(ts + 16 * b, s);
-                        const int* sk = reinterpret_cast<const int*>(sc) + 2 * b;
-                        const float ca = factor(sk[0]), cb = factor(sk[1]);
-                        const float wa = pow2i(max(-126, U - sk[8])), wb = pow2i(max(-126, U - sk[9]));
+                        const int* sk = reinterpret_cast<const int*>(sc) + 16 / CR * b;
+                        float f[16 / CR], fw[16 / CR];
+#pragma unroll
+                        for (int i = 0; i < 16 / CR; ++i) {
+                            f[i] = factor(sk[i]);
+                            fw[i] = pow2i(max(-126, U - sk[8 + i]));
+                        }
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
-                            const float c = j < 8 ? ca : cb, w = j < 8 ? wa : wb;
+                            const float c = f[j / CR], w = fw[j / CR];
                             const float e0 = 16 * b + j < valid ? ex2(fmaf(s[j], c, shift)) : 0.0f;
                             const float e1 = 16 * b + j + 1 < valid ? ex2(fmaf(s[j + 1], c, shift)) : 0.0f;
                             sum = add2(sum, pack2(e0, e1));
                             split2(pack2(e0 * w, e1 * w), p[j / 2], p[8 + j / 2]);
                         }
-                        tmem_st16(ts + 16 * b, p);
+                        tmem_st16(tp + 16 * b, p);
                     }
                 }
                 const float2 parts = unpack2(sum);
@@ -520,7 +571,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 tmem_wait_st();
                 tc_fence_before();
             }
-            mbar_arrive(&pfull[x]);
+            if (writes) mbar_arrive(&pfull[x]);
             ok = wait_warp(&ofull[x], phase(t));
             if (!ok) break;
             if (active) {
@@ -529,14 +580,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 if (__any_sync(0xffffffffu, alpha != 1.0f)) {
                     const f32x2 alpha2 = pack2(alpha, alpha);
 #pragma unroll
-                    for (int d = 0; d < HD / 2; ++d) o[d] = mul2(o[d], alpha2);
+                    for (int d = 0; d < HO / 2; ++d) o[d] = mul2(o[d], alpha2);
                 }
 #pragma unroll
-                for (int b = 0; b < HD / 32; ++b) {
-                    float v[32];
-                    tmem_ld32f(to + 32 * b, v);
+                for (int b = 0; b < HO / 32; ++b) {
+                    float w[32];
+                    tmem_ld32f(to + 32 * b, w);
 #pragma unroll
-                    for (int d = 0; d < 32; d += 2) o[16 * b + d / 2] = fma2(pack2(v[d], v[d + 1]), beta2, o[16 * b + d / 2]);
+                    for (int d = 0; d < 32; d += 2) o[16 * b + d / 2] = fma2(pack2(w[d], w[d + 1]), beta2, o[16 * b + d / 2]);
                 }
                 tc_fence_before();
             }
@@ -575,23 +626,23 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         }
         if (any_infinite) {
 #pragma unroll
-            for (int d = 0; d < HD / 2; ++d) {
+            for (int d = 0; d < HO / 2; ++d) {
                 auto of = [&](int c) {
                     const float up = infinite[0][c >> 5] >> (c & 31) & 1 ? INFINITY : 0.0f;
                     return infinite[1][c >> 5] >> (c & 31) & 1 ? up - INFINITY : up;
                 };
-                o[d] = add2(o[d], pack2(of(2 * d), of(2 * d + 1)));
+                o[d] = add2(o[d], pack2(of(c0 + 2 * d), of(c0 + 2 * d + 1)));
             }
         }
         if (row < rows && !(ALT && x == 1)) {
             float* rec = a.part + (((size_t)kvh * rows + row) * a.splits + split) * (a.hd + 4);
             const float f = pow2i(-kTtShift);
-            *reinterpret_cast<float2*>(rec) = make_float2(T, l * f);
+            if (!WIDE || x == 0) *reinterpret_cast<float2*>(rec) = make_float2(T, l * f);
 #pragma unroll
-            for (int d = 0; d < HD; d += 4)
-                if (d < a.hd) {
+            for (int d = 0; d < HO; d += 4)
+                if (c0 + d < a.hd) {
                     const float2 x0 = unpack2(o[d / 2]), x1 = unpack2(o[d / 2 + 1]);
-                    *reinterpret_cast<float4*>(rec + 4 + d) = make_float4(x0.x * f, x0.y * f, x1.x * f, x1.y * f);
+                    *reinterpret_cast<float4*>(rec + 4 + c0 + d) = make_float4(x0.x * f, x0.y * f, x1.x * f, x1.y * f);
                 }
         }
     }
@@ -602,18 +653,20 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTtCols));
 }
 
-bool tree_tc_ok(int hd) { return hd <= 128 && hd % 16 == 0; }
+bool tree_tc_ok(int hd) { return hd <= 256 && hd % 16 == 0; }
 
 cudaError_t tree_tc_launch(const TreeArgs& a, cudaStream_t st) {
-    const dim3 grid(a.splits, a.n_kv, (a.n_tok * a.G + kTcTreeRows - 1) / kTcTreeRows);
+    const int block = tree_tc_rows(a.hd);
+    const dim3 grid(a.splits, a.n_kv, (a.n_tok * a.G + block - 1) / block);
     auto go = [&](auto k, size_t smem) {
         const cudaError_t e = set_smem_limit(k, smem);
         if (e != cudaSuccess) return e;
         return launch_after(k, grid, dim3(kTtThreads), smem, st, a);
     };
-    const bool alt = a.n_tok * a.G <= 128 && a.per >= kTtAltTiles * kTcTreeKeys;
-    if (a.hd <= 64) return alt ? go(tree_tc_kernel<64, true>, TtLayout<64>::kAlloc) : go(tree_tc_kernel<64, false>, TtLayout<64>::kAlloc);
-    return alt ? go(tree_tc_kernel<128, true>, TtLayout<128>::kAlloc) : go(tree_tc_kernel<128, false>, TtLayout<128>::kAlloc);
+    if (a.hd > 128) return go(tree_tc_kernel<256, false>, TtLayout<256>::kAlloc);
+    const bool alt = a.n_tok * a.G <= 128 && a.per >= kTtAltTiles * tree_tc_keys(a.hd);
+    if (a.hd > 64) return alt ? go(tree_tc_kernel<128, true>, TtLayout<128>::kAlloc) : go(tree_tc_kernel<128, false>, TtLayout<128>::kAlloc);
+    return alt ? go(tree_tc_kernel<64, true>, TtLayout<64>::kAlloc) : go(tree_tc_kernel<64, false>, TtLayout<64>::kAlloc);
 }
 
 }  // namespace gncx

@@ -6,9 +6,10 @@ sum of n rounded terms is off by at most LAM sqrt(n) u times the sum of their
 magnitudes but for a probability below 2 exp(-LAM^2 / 2) (Higham and Mary's
 probabilistic rounding analysis); LAM = 8.  Products of fp32 values split into
 fp16 pairs keep 22 bits of each factor and drop one product: 3 * 2^-22 = 12 u; a
-tensor-core sum that is cut instead of rounded is off by 2 u an addition, at
-most 24 + 12 of them in a score and in a tile's output.  So a score is off by
-  ds = (LAM sqrt(hd) + 12 + 2 * 24 + 2) u * scale * sum |q k|,
+tensor-core sum that is cut instead of rounded is off by 2 u an addition: one
+per 16 columns and product, so C = 3 hd / 16 of them in a score (24 is taken
+for the smaller heads too), at most 12 in a tile's output.  So a score is off by
+  ds = (LAM sqrt(hd) + 12 + 2 C + 2) u * scale * sum |q k|,
 a weight by the factor 1 + 2 ds (its numerator and its sum), the exponentials
 (2 + |x|) u each with |x| <= 40 where the weight counts, and an output by
   (2 max ds + (LAM sqrt(n) + 12 + 2 * 12 + 42) u) * sum_j p_j |v_j|.
@@ -58,7 +59,7 @@ def attend(q, k, v, scale):
     q, k, v = q.double(), k.double(), v.double()
     n, hd = k.shape
     s = (k @ q) * scale
-    ds = (LAM * hd**0.5 + 62) * U * abs(scale) * float((k.abs() @ q.abs()).max())
+    ds = (LAM * hd**0.5 + 14 + 2 * max(24, 3 * ((hd + 15) // 16))) * U * abs(scale) * float((k.abs() @ q.abs()).max())
     p = torch.softmax(s, 0)
     rel = 2 * ds + (LAM * n**0.5 + 78) * U
     return p @ v, rel * (p @ v.abs()) + 1e-30, p, rel
@@ -215,6 +216,57 @@ def test_tree_lanes_infinite_and_nan_rows_show(gpu, row):
     out = run_tree(gpu, q, k, v, make_tree("random", n, 12), pos0, hd**-0.5, 0)
     assert bool((out[:, 4, 9] == float("-inf")).all()) and bool(out[:, 7].isnan().all())
     out[:, 4, 9], out[:, 7] = 0, 0
+    assert bool(out.isfinite().all())
+
+
+# Head sizes above 128: tiles of 32 rows, 128 query rows at a time.
+WIDE = [(1, 1, 256, 1, 1, 0), (1, 1, 256, 31, 1, 0), (2, 1, 256, 32, 3, 0), (2, 1, 256, 33, 3, 0), (4, 2, 144, 200, 9, 0), (8, 4, 256, 1000, 31, 0),
+        (8, 2, 160, 777, 33, 0), (16, 4, 256, 2500, 32, 0), (4, 1, 192, 1537, 64, 0), (12, 4, 240, 5000, 11, 0), (148, 148, 256, 230, 3, 0),
+        (74, 74, 256, 417, 2, 0), (4, 1, 256, 5000, 20, 700), (8, 2, 208, 300, 90, 33), (16, 4, 256, 9001, 64, 0)]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,pos0,n,window", WIDE)
+@pytest.mark.parametrize("size", [1.0, 5.0])
+def test_tree_wide(gpu, nh, nkv, hd, pos0, n, window, size):
+    rows = pos0 + n
+    q, k, v = randn(52, n, nh, hd) * size, randn(53, rows + 3, nkv, hd), randn(54, rows + 3, nkv, hd)
+    k[rows:], v[rows:] = float("nan"), float("nan")
+    lo = max(0, pos0 - window + 1) if window else 0
+    k[:min(lo, pos0)], v[:min(lo, pos0)] = float("nan"), float("inf")
+    for row in {min(lo, pos0 - 1), pos0 // 2, pos0 - 1}:
+        k[row] *= 3
+    up = make_tree("random", n, 13)
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, window)
+    assert bool(out.isfinite().all())
+    for i in sorted({0, n // 2, n - 1}):
+        rs = torch.tensor(tree_seen(up, i, pos0, window), device="cuda")
+        for h in sorted({0, nh // 2, nh - 1}):
+            g = h // (nh // nkv)
+            ref, tol, _, _ = attend(q[i, h], k[rs][:, g], v[rs][:, g], hd**-0.5)
+            err = (out[i, h].double() - ref).abs()
+            assert bool((err <= tol).all()), (i, h, float((err / tol).max()))
+    assert torch.equal(out, run_tree(gpu, q, k, v, up, pos0, hd**-0.5, window))
+
+
+@pytest.mark.parametrize("qs,ks,vs", [(1e-3, 1e-6, 1e-20), (1e4, 1e-3, 1e20), (1e-18, 1e18, 1e30), (1.0, 1.0, 1e-30)])
+def test_tree_wide_scales(gpu, qs, ks, vs):
+    nh, nkv, hd, pos0, n = 8, 2, 256, 700, 24
+    q, k, v = randn(55, n, nh, hd) * qs, randn(56, pos0 + n, nkv, hd) * ks, randn(57, pos0 + n, nkv, hd) * vs
+    k *= 2.0 ** torch.randint(-20, 3, (pos0 + n, nkv, 1), device="cuda", generator=gen(58))
+    v *= 2.0 ** torch.randint(-20, 1, (pos0 + n, nkv, 1), device="cuda", generator=gen(59))
+    up = make_tree("random", n, 5)
+    check_tree(run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0), q, k, v, up, pos0, hd**-0.5, 0, [0, 5, 23])
+
+
+@pytest.mark.parametrize("row", [0, 45, 1290, 1301])
+@pytest.mark.parametrize("col", [9, 128, 255])
+def test_tree_wide_infinite_and_nan_rows_show(gpu, row, col):
+    nh, nkv, hd, pos0, n = 16, 16, 256, 1302, 6
+    q, k, v = randn(60, n, nh, hd), randn(61, pos0 + n, nkv, hd), randn(62, pos0 + n, nkv, hd)
+    v[row, 4, col], k[row, 7, col] = float("inf"), float("nan")
+    out = run_tree(gpu, q, k, v, make_tree("random", n, 14), pos0, hd**-0.5, 0)
+    assert bool((out[:, 4, col] == float("inf")).all()) and bool(out[:, 7].isnan().all())
+    out[:, 4, col], out[:, 7] = 0, 0
     assert bool(out.isfinite().all())
 
 
