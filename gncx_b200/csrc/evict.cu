@@ -37,6 +37,7 @@ constexpr int kWsThreads = 256;
 constexpr int kWsWarps = kWsThreads / 32;
 constexpr int kWsRows = 1024;      // rows per CTA of the merge kernel's weight part
 constexpr int kWsMaxParts = 256;
+constexpr int kWsCluster = 8;      // CTAs per KV head that do the whole step for few rows
 
 struct WeightsArgs {
     const float* q;
@@ -88,9 +89,73 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
     return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c))));
 }
 
+// The rest of the step in one cluster: the warps' states as the CTA's record, the
+// records' maxima and sums through distributed shared memory, then this CTA's
+// share of the outputs and the weights of its rows.
+template <int GT>
+__device__ __forceinline__ void weights_cluster_end(const WeightsArgs& a, float* ost, const float* scores, const float (&mst)[kWsWarps][GT],
+                                                    const float (&lst)[kWsWarps][GT], int kvh, int rank, int heads, int p0, int p1) {
+    __shared__ float2 s_ml[GT];
+    __shared__ float s_M[GT], s_inv[GT], s_f[GT][kWsCluster];
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float* wt = a.weight + (size_t)kvh * a.row_stride;
+    const int t0 = p0 + tid;
+    const float old = t0 < p1 ? wt[t0] : 0.0f;  // on its way while the records are merged
+    for (int t = tid; t < heads * a.hd; t += kWsThreads) {
+        const int g = t / a.hd, d = t - g * a.hd;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWsWarps; ++w) M = fmaxf(M, mst[w][g]);
+        float L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWsWarps; ++w) {
+            const float f = mst[w][g] == -INFINITY ? 0.0f : __expf(mst[w][g] - M);
+            L = fmaf(lst[w][g], f, L);
+            O = fmaf(ost[(size_t)(w * GT + g) * a.hd + d], f, O);
+        }
+        ost[(size_t)g * a.hd + d] = O;  // in place of warp 0's, which this thread alone reads
+        if (d == 0) s_ml[g] = make_float2(M, L);
+    }
+    cluster.sync();
+    if (warp < heads) {
+        const float2 ml = lane < kWsCluster ? *cluster.map_shared_rank(&s_ml[warp], lane) : make_float2(-INFINITY, 0.0f);
+        float M = ml.x;
+#pragma unroll
+        for (int o = kWsCluster / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float f = ml.x == -INFINITY ? 0.0f : __expf(ml.x - M);
+        float L = ml.y * f;  // a NaN stays
+#pragma unroll
+        for (int o = kWsCluster / 2; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (lane < kWsCluster) s_f[warp][lane] = f;
+        if (lane == 0) {
+            s_M[warp] = M;
+            s_inv[warp] = 1.0f / L;
+        }
+    }
+    __syncthreads();
+    for (int t = rank * kWsThreads + tid; t < heads * a.hd; t += kWsCluster * kWsThreads) {
+        const int g = t / a.hd;
+        float o = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kWsCluster; ++r) o = fmaf(*cluster.map_shared_rank(&ost[t], r), s_f[g][r], o);
+        a.out[(size_t)kvh * a.G * a.hd + t] = o * s_inv[g];
+    }
+    for (int t = t0; t < p1; t += kWsThreads) {
+        float w = 0.0f;
+        for (int g = 0; g < heads; ++g) w = fmaf(__expf(scores[g * a.ppc + t - p0] - s_M[g]), s_inv[g], w);
+        const bool fresh = a.new_k && t == a.pos;  // the new row's sum starts here
+        wt[t] = fresh ? w : (t == t0 ? old : wt[t]) + w;
+        if (fresh && a.positions) a.positions[(size_t)kvh * a.row_stride + t] = a.token_pos;
+    }
+    cluster.sync();  // no CTA leaves while another may read its shared memory
+}
+
 // LPR lanes hold a row (NJ float4 each; columns past hd are zero), 32 / LPR
-// rows side by side in a warp, B rows per lane and batch, GT query heads.
-template <int LPR, int NJ, int GT, int B>
+// rows side by side in a warp, B rows per lane and batch, GT query heads.  ONE: a
+// cluster of kWsCluster CTAs per KV head does the whole step, the scores and
+// records in its shared memory.
+template <int LPR, int NJ, int GT, int B, bool ONE>
 __global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const WeightsArgs a) {
     constexpr int SUB = 32 / LPR;
     constexpr int NV = B * GT;
@@ -98,7 +163,8 @@ __global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const Weigh
     constexpr int LG = ilog2(GT);
     constexpr int RB = B * SUB;  // rows per warp and batch
     static_assert(NV <= LPR, "one total per lane");
-    extern __shared__ __align__(16) float ost[];  // [warp][GT][hd]
+    extern __shared__ __align__(16) float ost[];  // [warp][GT][hd], with ONE also scores [GT][ppc]
+    float* own_scores = ost + (size_t)kWsWarps * GT * a.hd;
     __shared__ float wsh[kWsWarps][SUB * NV + GT];
     __shared__ float mst[kWsWarps][GT], lst[kWsWarps][GT];
     const int part = blockIdx.x, kvh = blockIdx.y, h0 = kvh * a.G + blockIdx.z * GT;
@@ -118,7 +184,7 @@ __global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const Weigh
         on[j] = col[j] < a.hd;
     }
     pdl_wait();
-    pdl_launch_dependents();
+    if (!ONE) pdl_launch_dependents();
     float4 q[GT][NJ], o[GT][NJ];
 #pragma unroll
     for (int g = 0; g < GT; ++g)
@@ -167,7 +233,10 @@ __global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const Weigh
         const int mp = my / GT, mg = my % GT;
         const bool live = r0 + mp < p1;
         const bool lead = (lr & ((1 << SH) - 1)) == 0;
-        if (live && lead && mg < heads) a.scores[(size_t)(h0 + mg) * a.score_ld + r0 + mp] = sc;
+        if (live && lead && mg < heads) {
+            if (ONE) own_scores[mg * a.ppc + r0 + mp - p0] = sc;
+            else a.scores[(size_t)(h0 + mg) * a.score_ld + r0 + mp] = sc;
+        }
         if (!live) sc = -INFINITY;
         float bm = sc;
 #pragma unroll
@@ -228,6 +297,10 @@ __global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const Weigh
             if (sub == 0 && on[j]) *reinterpret_cast<float4*>(ost + (size_t)(warp * GT + g) * a.hd + col[j]) = c;
         }
     __syncthreads();
+    if constexpr (ONE) {
+        weights_cluster_end<GT>(a, ost, own_scores, mst, lst, kvh, part, heads, p0, p1);
+        return;
+    }
     for (int t = threadIdx.x; t < heads * a.hd; t += kWsThreads) {
         const int g = t / a.hd, d = t - g * a.hd;
         float M = -INFINITY;
@@ -362,6 +435,13 @@ static int weights_parts(int len, int n_kv, int zgroups, int sm_count) {
     if (parts > kWsMaxParts) parts = kWsMaxParts;
     return parts < 1 ? 1 : parts;
 }
+// Whether one launch, a cluster per KV head, does the step: 16 heads, 8 KV heads of
+// 128, 512 rows 4.8 us against 5.2 with two kernels (called one by one 6.9 against
+// 8.9, a launch less); 2048 rows 8.2 against 9.4; 64 columns, 2048 rows on one KV head
+// 5.6 against 7.4; 256 columns, 2048 rows on one KV head 15.4 against 10.4.
+static bool weights_one(int len, int hd, int zgroups) {
+    return zgroups == 1 && len <= 4096 && len * hd <= (hd > 128 ? 1 << 17 : 1 << 18);
+}
 static int weights_group(int G) { return G >= 3 ? 4 : G; }  // query heads a CTA serves
 
 size_t weights_workspace_bytes(int pos, int n_heads, int n_kv, int hd, int sm_count) {
@@ -372,18 +452,18 @@ size_t weights_workspace_bytes(int pos, int n_heads, int n_kv, int hd, int sm_co
 }
 
 template <int LPR, int NJ>
-static cudaError_t launch_weights_part(const WeightsArgs& a, dim3 grid, int GT, cudaStream_t st) {
-    const size_t smem = (size_t)kWsWarps * GT * a.hd * 4;
-    auto go = [&](auto k) {
-        const cudaError_t e = set_smem_limit(k, smem);
+static cudaError_t launch_weights_part(const WeightsArgs& a, dim3 grid, int GT, bool one, cudaStream_t st) {
+    const size_t smem = ((size_t)kWsWarps * GT * a.hd + (one ? GT * a.ppc : 0)) * 4;
+    auto go = [&](auto k, auto k_one) {
+        const cudaError_t e = set_smem_limit(one ? k_one : k, smem);
         if (e != cudaSuccess) return e;
-        return launch_after(k, grid, dim3(kWsThreads), smem, st, a);
+        return launch_early(one ? k_one : k, grid, dim3(kWsThreads), smem, st, one ? kWsCluster : 1, a);
     };
     constexpr int B = NJ == 1 ? 4 : 2;
     switch (GT) {
-        case 1: return go(weights_part_kernel<LPR, NJ, 1, B>);
-        case 2: return go(weights_part_kernel<LPR, NJ, 2, B>);
-        default: return go(weights_part_kernel<LPR, NJ, 4, B>);
+        case 1: return go(weights_part_kernel<LPR, NJ, 1, B, false>, weights_part_kernel<LPR, NJ, 1, B, true>);
+        case 2: return go(weights_part_kernel<LPR, NJ, 2, B, false>, weights_part_kernel<LPR, NJ, 2, B, true>);
+        default: return go(weights_part_kernel<LPR, NJ, 4, B, false>, weights_part_kernel<LPR, NJ, 4, B, true>);
     }
 }
 
@@ -408,17 +488,19 @@ int weights_step_launch(const float* q, const float* new_k, const float* new_v, 
     a.weight = weight;
     a.positions = positions;
     a.row_stride = row_stride;
-    a.parts = weights_parts(len, n_kv, z, device_info().sm_count);
+    const bool one = weights_one(len, hd, z);
+    a.parts = one ? kWsCluster : weights_parts(len, n_kv, z, device_info().sm_count);
     a.ppc = (len + a.parts - 1) / a.parts;
-    a.parts = (len + a.ppc - 1) / a.ppc;
+    if (!one) a.parts = (len + a.ppc - 1) / a.ppc;
     a.part = static_cast<float*>(ws);
     a.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + ((size_t)n_heads * a.parts * (hd + 4) * 4 + 255) / 256 * 256);
     a.score_ld = ((size_t)len + 31) / 32 * 32;
     const dim3 grid(a.parts, n_kv, z);
-    const cudaError_t e = hd <= 64    ? launch_weights_part<16, 1>(a, grid, GT, st)
-                          : hd <= 128 ? launch_weights_part<32, 1>(a, grid, GT, st)
-                                      : launch_weights_part<32, 2>(a, grid, GT, st);
+    const cudaError_t e = hd <= 64    ? launch_weights_part<16, 1>(a, grid, GT, one, st)
+                          : hd <= 128 ? launch_weights_part<32, 1>(a, grid, GT, one, st)
+                                      : launch_weights_part<32, 2>(a, grid, GT, one, st);
     if (e != cudaSuccess) return kErrCuda;
+    if (one) return kOk;
     const int row_ctas = (len + kWsRows - 1) / kWsRows;
     return launch_after(weights_merge_kernel, dim3(row_ctas + G, n_kv), dim3(kWsThreads), 0, st, a, row_ctas) == cudaSuccess
                ? kOk

@@ -55,7 +55,7 @@ constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12;
 // of 193 (16 heads, 4 KV heads, 64 nodes, 32768 rows).
 template <int HD>
 struct TtRegs {
-    static constexpr int kSoftmax = HD > 128 ? 192 : 184, kLoad = HD > 128 ? 88 : 96, kMma = HD > 128 ? 40 : 48;
+    static constexpr int kSoftmax = HD > 128 ? 192 : 176, kLoad = HD > 128 ? 88 : 112, kMma = HD > 128 ? 40 : 48;
     static_assert(2 * kSoftmax + kLoad + kMma <= 4 * 128, "a split that can be had");
 };
 constexpr int kTtStages = 2;              // K and V operand tiles

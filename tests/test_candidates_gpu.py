@@ -370,7 +370,10 @@ def run_step(lib, q, k_new, v_new, k, v, pos, token_pos, scale, write, weight, p
 
 STEPS = [(1, 1, 4, 0), (4, 2, 64, 0), (4, 2, 64, 1), (4, 4, 128, 30), (4, 4, 128, 31), (4, 4, 128, 32), (6, 2, 96, 33), (8, 1, 256, 100),
          (16, 8, 128, 511), (32, 8, 128, 1000), (3, 1, 80, 1023), (12, 4, 64, 1024), (10, 2, 128, 1025), (7, 7, 20, 2500),
-         (40, 2, 64, 300), (32, 8, 128, 20011), (24, 1, 128, 4100)]
+         (40, 2, 64, 300), (32, 8, 128, 20011), (24, 1, 128, 4100),
+         # the last of one launch, the first of two; groups of 1 to 5 heads
+         (4, 2, 64, 4095), (4, 2, 64, 4096), (8, 4, 128, 2047), (8, 4, 128, 2048), (4, 1, 256, 511), (4, 1, 256, 512), (3, 1, 96, 2729),
+         (3, 1, 96, 2730), (5, 1, 64, 500), (2, 2, 4, 4095), (6, 3, 60, 7), (8, 2, 128, 8)]
 
 
 @pytest.mark.parametrize("nh,nkv,hd,pos", STEPS)
