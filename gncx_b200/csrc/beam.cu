@@ -18,6 +18,12 @@
 //   * beam_merge_kernel: one CTA forms the L_b and walks the sorted lists, a
 //     thread per list, past a threshold from their first entries, until no
 //     list has an entry that reaches it; then it ranks what it found.
+// The first kernel is bound by instruction issue (62 % busy, about 50 instructions a
+// logit, a third of them the exponential; 21 % of the fp64 pipe): 27.6 us for 64
+// beams of 151936 logits, 9 of them ended, 1.2 TB/s.  The merge is one CTA's chain
+// of dependent reads and barriers, 8 to 11 us alone and cold.  Both: 33.3 us;
+// 4 beams 13.1 us.  Slower: appending by a ballot per logit (48.7 us against 34.7
+// then), 2, 4 or 5 CTAs per SM (within 3 %).
 #include <cuda_runtime.h>
 #include "common.cuh"
 #include "kernels.h"
@@ -799,7 +805,11 @@ int beam_select_launch(const float* logits, const float* scores, const int32_t* 
 // column (16 or 4 bytes at one offset of every slot), reads the sources of
 // all slots that change before it writes any, so no second buffer and no
 // barrier is needed; slots that stay (-1, or their own index) are not touched.
-// An index outside [-1, n_slots) leaves its slot and records an error.
+// An index outside [-1, n_slots) leaves its slot and records an error.  Bound by
+// HBM: 16 states of 8 slots of 4 MB, every slot's row read once and written once,
+// 138 us for 0.88 GB, 6.4 TB/s; where small by latency: 33 slots of 4 KB in 56
+// states 3.3 us.  Up to 16 slots a thread's columns are in registers, else in shared
+// memory.
 struct ReorderArgs {
     uint8_t* state;
     size_t state_stride, slot_stride;
