@@ -37,6 +37,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.cuh"
+#include "rows.cuh"
 #include "tma.cuh"
 
 namespace gncx {
@@ -66,37 +67,6 @@ struct WeightsArgs {
     float* scores;       // [head][score_ld]
     size_t score_ld;
 };
-
-// Sum each v[i] over the LPR lanes of a row, NV sums at once (NV, LPR powers
-// of two, NV <= LPR): lane l ends with the total of v[(l % LPR) >> SH].
-template <int NV, int LPR>
-__device__ __forceinline__ float lanes_reduce(float (&v)[NV], int lane) {
-    int off = LPR / 2;
-#pragma unroll
-    for (int n = NV; n > 1; n >>= 1) {
-        const bool up = (lane & off) != 0;
-#pragma unroll
-        for (int i = 0; i < n / 2; ++i) {
-            const float send = up ? v[i] : v[i + n / 2];
-            const float keep = up ? v[i + n / 2] : v[i];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
-        }
-        off >>= 1;
-    }
-    float s = v[0];
-#pragma unroll
-    for (; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    return s;
-}
-
-__host__ __device__ constexpr int ilog2(int n) { return n <= 1 ? 0 : 1 + ilog2(n / 2); }
-
-__device__ __forceinline__ float4 ld_row(const float* p, bool ok) {
-    return ok ? __ldcs(reinterpret_cast<const float4*>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
-}
-__device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
-    return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c))));
-}
 
 // The rest of the step in one cluster: the warps' states as the CTA's record, the
 // records' maxima and sums through distributed shared memory, then this CTA's

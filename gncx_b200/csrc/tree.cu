@@ -27,10 +27,16 @@
 // alone and cold for 33 nodes and 8 KV heads), so all that comes before the
 // records runs before it waits for the dense kernel, and a thread has eight
 // records in flight: 5 nodes over 511 rows, both kernels 10.4 us.
+//
+// Few query rows over a short cache take one launch, tree_one_kernel, a cluster
+// of CTAs on the CUDA cores: bound by its chain of reads, sums over lanes and
+// cluster barriers, and by 0.9 us for each 2 (4) cache rows of a warp.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.cuh"
+#include "rows.cuh"
 #include "tma.cuh"
 #include "tree.cuh"
 
@@ -144,6 +150,230 @@ __global__ void __launch_bounds__(kTdThreads) tree_dense_kernel(const TreeArgs a
         const int col = c + 8 * x;
         if (col < hd4) *reinterpret_cast<float4*>(rec + 4 + 4 * col) = o[x];
     }
+}
+
+// ---------------------------------------------------------------- few rows: everything in one launch
+constexpr int kToThreads = 256;
+constexpr int kToWarps = kToThreads / 32;
+constexpr int kToCluster = 8;  // CTAs per KV head and GT query rows
+constexpr int kToTok = 64;     // nodes: a bit each
+
+// A cluster takes GT query rows (node, head of the group) of a KV head and all
+// rows that any of them sees, the drafted ones too.  A warp holds B cache rows
+// across its lanes (NJ float4 each) and scores them against the GT query rows,
+// one (cache row, query row) score per lane; what a query row does not see gets
+// no weight, and no product with V.  The warps' and the CTAs' sums are joined in
+// shared memory.
+template <int NJ, int GT, int B>
+__global__ void __launch_bounds__(kToThreads, 1) tree_one_kernel(const TreeArgs a) {
+    static_assert(GT * B == 32, "a score per lane");
+    extern __shared__ __align__(16) float sm[];  // [warp][GT][hd]
+    __shared__ int s_up[kToTok], s_first[GT];
+    __shared__ unsigned long long s_path[GT];
+    __shared__ __align__(16) float wsh[kToWarps][32 + GT];
+    __shared__ float mst[kToWarps][GT], lst[kToWarps][GT];
+    __shared__ float2 s_ml[GT];
+    __shared__ float s_inv[GT], s_f[GT][kToCluster];
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int rank = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * GT;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rows = a.n_tok * a.G, heads = min(GT, rows - r0);
+    auto row_at = [&](int g) {  // of q and out; the last row again behind the last
+        const int r = min(r0 + g, rows - 1);
+        return ((size_t)(r / a.G) * a.n_heads + kvh * a.G + r % a.G) * a.hd;
+    };
+    pdl_wait();
+    if (tid < a.n_tok) s_up[tid] = a.parents[tid];
+    f32x2 q[GT][2 * NJ], o[GT][2 * NJ];
+    {
+        int head = r0 % a.G;
+        const float* qp = a.q + row_at(0);
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int col = 4 * (lane + 32 * j);
+                const float4 x = ld_row(qp + col, col < a.hd);
+                q[g][2 * j] = pack2(x.x, x.y);
+                q[g][2 * j + 1] = pack2(x.z, x.w);
+                o[g][2 * j] = o[g][2 * j + 1] = 0;
+            }
+            if (g + 1 < heads) {
+                qp += a.hd;
+                if (++head == a.G) {
+                    head = 0;
+                    qp += (size_t)(a.n_heads - a.G) * a.hd;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (tid < GT) {  // what the query row sees: cache rows from `first` on, drafted rows by their bits
+        int depth = -1, i = min(r0 + tid, rows - 1) / a.G;
+        unsigned long long path = 0;
+        while (true) {
+            ++depth;
+            if (a.window <= 0 || depth < a.window) path |= 1ull << i;
+            const int p = s_up[i];
+            if (p < -1 || p >= i) record_error(a.err, kErrInvalidArg);
+            if (p < 0 || p >= i) break;
+            i = p;
+        }
+        s_path[tid] = path;
+        s_first[tid] = a.window > 0 ? max(0, a.pos0 + depth - a.window + 1) : 0;
+    }
+    __syncthreads();
+    const int g_me = lane % GT, p_me = lane / GT, first = s_first[g_me];
+    const unsigned long long path = s_path[g_me];
+    const int k0 = a.window > 0 ? min(a.pos0, max(0, a.pos0 - a.window + 1)) : 0, k1 = a.pos0 + a.n_tok;
+    const int per = (k1 - k0 + kToCluster - 1) / kToCluster;
+    const int p0 = k0 + rank * per, p1 = min(k1, p0 + per);
+    const size_t ps = (size_t)a.n_kv * a.hd;
+    const float* kb = a.kc + (size_t)kvh * a.hd;
+    const float* vb = a.vc + (size_t)kvh * a.hd;
+    float m = -INFINITY, l = 0.0f;  // of query row g_me
+    // the scores of batch b0 that count, and the rows that any of them needs
+    auto seen_at = [&](int b0) {
+        const int key = b0 + p_me;
+        return key < p1 && (key < a.pos0 ? key >= first : (path >> (key - a.pos0) & 1) != 0);
+    };
+    float4 k[B][NJ], v[B][NJ];
+    auto load = [&](int b0, unsigned mask) {
+#pragma unroll
+        for (int p = 0; p < B; ++p)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int col = 4 * (lane + 32 * j);
+                const bool some = col < a.hd && (mask >> (p * GT) & ((1u << GT) - 1));
+                k[p][j] = ld_row(kb + (size_t)(b0 + p) * ps + col, some);
+                v[p][j] = ld_row(vb + (size_t)(b0 + p) * ps + col, some);
+            }
+    };
+    bool seen = seen_at(p0 + warp * B);
+    unsigned mask = __ballot_sync(0xffffffffu, seen);
+    load(p0 + warp * B, mask);
+#pragma unroll 1
+    for (int b0 = p0 + warp * B; b0 < p1;) {
+        f32x2 kk[B][2 * NJ], vv[B][2 * NJ];
+#pragma unroll
+        for (int p = 0; p < B; ++p)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                kk[p][2 * j] = pack2(k[p][j].x, k[p][j].y);
+                kk[p][2 * j + 1] = pack2(k[p][j].z, k[p][j].w);
+                vv[p][2 * j] = pack2(v[p][j].x, v[p][j].y);
+                vv[p][2 * j + 1] = pack2(v[p][j].z, v[p][j].w);
+            }
+        const bool seen_now = seen;
+        const unsigned now = mask;
+        b0 += kToWarps * B;
+        seen = seen_at(b0);
+        mask = __ballot_sync(0xffffffffu, seen);
+        load(b0, mask);  // the next batch, under this one's arithmetic
+        if (!now) continue;
+        float d[32];
+#pragma unroll
+        for (int p = 0; p < B; ++p)
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                f32x2 c = mul2(q[g][0], kk[p][0]);
+#pragma unroll
+                for (int j = 1; j < 2 * NJ; ++j) c = fma2(q[g][j], kk[p][j], c);
+                const float2 s = unpack2(c);
+                d[p * GT + g] = s.x + s.y;
+            }
+        float sc = lanes_reduce<32, 32>(d, lane) * a.scale2;
+        if (!seen_now) sc = -INFINITY;
+        float bm = sc;
+#pragma unroll
+        for (int off = 16; off >= GT; off >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, off));
+        const float m_new = fmaxf(m, bm);
+        const float e = sc == -INFINITY ? 0.0f : ex2(sc - m_new);
+        const float corr = m == -INFINITY ? 0.0f : ex2(m - m_new);
+        float bs = e;
+#pragma unroll
+        for (int off = 16; off >= GT; off >>= 1) bs += __shfl_xor_sync(0xffffffffu, bs, off);
+        l = fmaf(l, corr, bs);
+        m = m_new;
+        float* wr = wsh[warp];
+        wr[lane] = e;
+        if (lane < GT) wr[32 + lane] = corr;
+        __syncwarp();
+        if (__any_sync(0xffffffffu, corr != 1.0f)) {
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                const f32x2 c = pack2(wr[32 + g], wr[32 + g]);
+#pragma unroll
+                for (int j = 0; j < 2 * NJ; ++j) o[g][j] = mul2(o[g][j], c);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < B; ++p)
+#pragma unroll
+            for (int g = 0; g < GT; g += 4) {
+                const float4 w4 = *reinterpret_cast<const float4*>(wr + p * GT + g);
+                const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (now >> (p * GT + g + x) & 1) {  // of the warp
+                        const f32x2 w2 = pack2(w[x], w[x]);
+#pragma unroll
+                        for (int j = 0; j < 2 * NJ; ++j) o[g + x][j] = fma2(w2, vv[p][j], o[g + x][j]);
+                    }
+            }
+        __syncwarp();
+    }
+    if (lane < GT) {
+        mst[warp][lane] = m;
+        lst[warp][lane] = l;
+    }
+#pragma unroll
+    for (int g = 0; g < GT; ++g)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int col = 4 * (lane + 32 * j);
+            const float2 x = unpack2(o[g][2 * j]), y = unpack2(o[g][2 * j + 1]);
+            if (col < a.hd) *reinterpret_cast<float4*>(sm + (size_t)(warp * GT + g) * a.hd + col) = make_float4(x.x, x.y, y.x, y.y);
+        }
+    __syncthreads();
+    // the warps' states as the CTA's record, in place of warp 0's outputs
+    for (int t = tid; t < heads * a.hd; t += kToThreads) {
+        const int g = t / a.hd;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kToWarps; ++w) M = fmaxf(M, mst[w][g]);
+        float L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kToWarps; ++w) {
+            const float f = mst[w][g] == -INFINITY ? 0.0f : ex2(mst[w][g] - M);
+            L = fmaf(lst[w][g], f, L);  // a NaN stays
+            O = fmaf(sm[(size_t)w * GT * a.hd + t], f, O);
+        }
+        sm[t] = O;
+        if (t == g * a.hd) s_ml[g] = make_float2(M, L);
+    }
+    cluster.sync();
+    for (int g = warp; g < heads; g += kToWarps) {
+        const float2 ml = lane < kToCluster ? *cluster.map_shared_rank(&s_ml[g], lane) : make_float2(-INFINITY, 0.0f);
+        float M = ml.x;
+#pragma unroll
+        for (int off = kToCluster / 2; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+        float L = ml.y * f;
+#pragma unroll
+        for (int off = kToCluster / 2; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+        if (lane < kToCluster) s_f[g][lane] = f;
+        if (lane == 0) s_inv[g] = 1.0f / L;
+    }
+    __syncthreads();
+    for (int t = rank * kToThreads + tid; t < heads * a.hd; t += kToCluster * kToThreads) {
+        const int g = t / a.hd;
+        float out = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kToCluster; ++r) out = fmaf(*cluster.map_shared_rank(&sm[t], r), s_f[g][r], out);
+        a.out[row_at(g) + t - g * a.hd] = out * s_inv[g];
+    }
+    cluster.sync();  // no CTA leaves while another may read its shared memory
 }
 
 // ---------------------------------------------------------------- ancestors and merge
@@ -344,6 +574,22 @@ static void tree_geometry(TreeArgs& a, int sm_count) {
     }
 }
 
+// Query rows per cluster where one launch does everything, 0 where not: the clusters
+// run side by side (15 of 8 CTAs do, 16 took twice the time) and the cache is short.
+// One launch against the two kernels: 16 heads, 8 KV heads of 128, 4 nodes (8 query
+// rows): 10 cache rows 6.0 us and 10.6, 511 rows 8.4 and 10.6, 1600 rows 12.8 and 13.4; on 2 KV
+// heads of 64 it loses from about 750 rows (1000: 9.1 and 8.2).  5 nodes (16 rows per
+// cluster): 256 rows 8.8 and 9.8, 511 rows 10.8 and 10.8.  Head size 256: 128 rows 9.2 and 10.9, 384
+// rows 11.7 and 11.0.
+static int tree_one_rows(const TreeArgs& a, int sm_count) {
+    const int64_t len = (int64_t)a.pos0 + a.n_tok - (a.window > 0 ? max(0, a.pos0 - a.window + 1) : 0);
+    const int64_t fit = sm_count * 13 / 16 / kToCluster / a.n_kv;  // clusters per KV head
+    const int rows = a.n_tok * a.G;
+    if (a.n_tok > kToTok) return 0;
+    if (rows <= 8 * fit) return len <= (a.hd > 128 ? 256 : 768) ? 8 : 0;
+    return rows <= 16 * fit && a.hd <= 128 && len <= 384 ? 16 : 0;
+}
+
 static TreeArgs tree_args(int pos0, int n_tok, int n_heads, int n_kv, int hd, int window) {
     TreeArgs a{};
     a.pos0 = pos0;
@@ -374,6 +620,15 @@ int tree_launch(const float* q, const float* kc, const float* vc, const int32_t*
     a.part = static_cast<float*>(ws);
     a.out = out;
     a.err = err;
+    if (const int gt = tree_one_rows(a, device_info().sm_count)) {
+        auto one = [&](auto k) {
+            const size_t smem = (size_t)kToWarps * gt * hd * 4;
+            if (set_smem_limit(k, smem) != cudaSuccess) return kErrCuda;
+            const dim3 grid(kToCluster, n_kv, (n_tok * a.G + gt - 1) / gt);
+            return launch_early(k, grid, dim3(kToThreads), smem, st, kToCluster, a) == cudaSuccess ? kOk : kErrCuda;
+        };
+        return hd > 128 ? one(tree_one_kernel<2, 8, 4>) : gt == 8 ? one(tree_one_kernel<1, 8, 4>) : one(tree_one_kernel<1, 16, 2>);
+    }
     if (a.splits > 0 && a.tc) {
         if (tree_tc_launch(a, st) != cudaSuccess) return kErrCuda;
     } else if (a.splits > 0) {

@@ -42,6 +42,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.cuh"
+#include "rows.cuh"
 #include "tree.cuh"
 #include "umma.cuh"
 
@@ -106,34 +107,6 @@ __device__ __forceinline__ float pow2i(int n) { return __int_as_float((n + 127) 
 __device__ __forceinline__ int scale_exp(uint32_t bits) {
     const int s = 14 - ((int)(bits >> 23) - 127);
     return min(s & ~3, 124);
-}
-
-// A pair of fp32 values in one 64-bit register, and two operations at once on it.
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(f32x2 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
 }
 
 // hi = fp16(x), lo = fp16(x - hi) of two values

@@ -270,6 +270,54 @@ def test_tree_wide_infinite_and_nan_rows_show(gpu, row, col):
     assert bool(out.isfinite().all())
 
 
+# Few query rows and a short cache, one launch of clusters: on both sides of its limits
+# of query rows (8 and 16 per cluster, 15 clusters), nodes (64) and cache rows.
+FEW = [(1, 1, 128, 0, 1, 0), (1, 1, 128, 0, 64, 0), (1, 1, 128, 0, 65, 0), (2, 1, 64, 3, 60, 5), (16, 8, 128, 764, 4, 0), (16, 8, 128, 765, 4, 0),
+       (16, 8, 128, 379, 5, 0), (16, 8, 128, 380, 5, 0), (16, 8, 128, 300, 8, 0), (16, 8, 128, 300, 9, 0), (4, 4, 256, 250, 6, 0),
+       (4, 4, 256, 251, 6, 0), (15, 15, 128, 200, 8, 0), (16, 16, 128, 200, 8, 0), (24, 8, 128, 5000, 2, 200), (8, 1, 20, 90, 14, 0),
+       (12, 4, 252, 200, 2, 90), (3, 1, 36, 7, 5, 2), (4, 2, 128, 600, 4, 1), (5, 1, 64, 40, 24, 0)]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,pos0,n,window", FEW)
+@pytest.mark.parametrize("kind", ["random", "chain", "star"])
+def test_tree_few(gpu, nh, nkv, hd, pos0, n, window, kind):
+    rows = pos0 + n
+    q, k, v = randn(63, n, nh, hd) * 2, randn(64, rows + 3, nkv, hd), randn(65, rows + 3, nkv, hd)
+    k[rows:], v[rows:] = float("nan"), float("nan")
+    lo = max(0, pos0 - window + 1) if window else 0
+    k[:min(lo, pos0)], v[:min(lo, pos0)] = float("nan"), float("inf")
+    up = make_tree(kind, n, pos0 + n + 1)
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, window)
+    check_tree(out, q, k, v, up, pos0, hd**-0.5, window)
+    assert torch.equal(out, run_tree(gpu, q, k, v, up, pos0, hd**-0.5, window))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("pos0,n", [(40, 7), (0, 16), (300, 8)])
+def test_tree_few_other_branches_do_not_leak(gpu, bad, pos0, n):
+    nh, nkv, hd = 4, 4, 64
+    q, k, v = randn(66, n, nh, hd), randn(67, pos0 + n, nkv, hd), randn(68, pos0 + n, nkv, hd)
+    up = make_tree("random", n, 7)
+    k[pos0 + 3], v[pos0 + 3] = bad, bad
+    clean = [i for i in range(n) if 3 not in tree_path(up, i)]
+    assert 1 < len(clean) < n
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0)
+    check_tree(out, q, k, v, up, pos0, hd**-0.5, 0, clean)
+    assert not bool(out[3].isfinite().any())
+
+
+def test_tree_few_bad_parents_are_an_error(gpu):
+    q, k, v = randn(69, 4, 2, 64), randn(70, 24, 2, 64), randn(71, 24, 2, 64)
+    out = torch.zeros_like(q)
+    for up in ([-1, 1, 0, 0], [-1, 0, 3, 0], [-1, 0, -2, 0], [5, 0, 0, 0], [-1, 0, 0, 2**31 - 1]):
+        parents = torch.tensor(up, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        st = gpu.gncx_attention_tree(P(q), P(k), P(v), P(parents), 20, 4, 2, 2, 64, 0.1, 0, P(out), None, 0)
+        assert st == INVALID and gpu.gncx_last_error() == INVALID, up
+        gpu.gncx_clear_error()
+    ok(gpu, gpu.gncx_sync())
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_tree_other_branches_do_not_leak(gpu, bad):
     nh, nkv, hd, pos0, n = 8, 2, 128, 300, 40
