@@ -92,7 +92,16 @@ cudaError_t set_smem_limit(const void* k, size_t bytes) {
     if (cudaGetDevice(&dev) != cudaSuccess) return cudaErrorNoDevice;
     std::lock_guard<std::mutex> lock(mu);
     size_t& have = done[std::make_pair(k, dev)];
-    if (bytes <= have || bytes <= 48 * 1024) return cudaSuccess;
+    if (bytes <= have) return cudaSuccess;
+    if (bytes <= 48 * 1024) {  // allowed as it is, unless the kernel's own variables leave too little of 48 KB
+        cudaFuncAttributes f;
+        const cudaError_t e = cudaFuncGetAttributes(&f, k);
+        if (e != cudaSuccess) return e;
+        if (bytes + f.sharedSizeBytes <= 48 * 1024) {
+            have = bytes;
+            return cudaSuccess;
+        }
+    }
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e == cudaSuccess) have = bytes;
     return e;

@@ -736,6 +736,27 @@ def test_reorder(gpu, slots, words):
         assert torch.equal(y, x[:, src])
 
 
+@pytest.mark.parametrize("slots", [22, 23, 24, 25, 45, 46, 47, 48, 49, 93, 94, 95, 96, 97])
+@pytest.mark.parametrize("words", [1024, 1023])
+def test_reorder_shared_memory_near_48_kb(gpu, slots, words):
+    """Slots whose columns and the kernel's own variables together cross what a launch gets without asking."""
+    idx = np.roll(np.arange(slots), 5)
+    x = randn(72, 2, slots, words)
+    y, index = x.clone(), torch.tensor(idx, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    ok(gpu, gpu.gncx_state_reorder(P(y), 2, slots * words * 4, slots, words * 4, words * 4, P(index)))
+    torch.cuda.synchronize()
+    assert torch.equal(y, x[:, torch.tensor(idx, device="cuda")])
+
+
+@pytest.mark.parametrize("hd", [88, 92, 96, 100])
+def test_tree_shared_memory_near_48_kb(gpu, hd):
+    nh, nkv, pos0, n = 30, 10, 9, 5
+    q, k, v = randn(73, n, nh, hd), randn(74, pos0 + n, nkv, hd), randn(75, pos0 + n, nkv, hd)
+    up = make_tree("random", n, 1)
+    check_tree(run_tree(gpu, q, k, v, up, pos0, 0.1, 0), q, k, v, up, pos0, 0.1, 0)
+
+
 def test_reorder_strides(gpu):
     """Part of each slot, slots innermost, and a start off 16 bytes."""
     idx = torch.tensor([2, 0, 0, -1, 1], dtype=torch.int32, device="cuda")
