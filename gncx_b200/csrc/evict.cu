@@ -278,25 +278,25 @@ __global__ void __launch_bounds__(kWsThreads, 2) weights_part_kernel(const Weigh
     __syncthreads();
     if constexpr (ONE) {
         weights_cluster_end<GT>(a, ost, own_scores, mst, lst, kvh, part, heads, p0, p1);
-        return;
-    }
-    for (int t = threadIdx.x; t < heads * a.hd; t += kWsThreads) {
-        const int g = t / a.hd, d = t - g * a.hd;
-        float M = -INFINITY;
+    } else {
+        for (int t = threadIdx.x; t < heads * a.hd; t += kWsThreads) {
+            const int g = t / a.hd, d = t - g * a.hd;
+            float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWsWarps; ++w) M = fmaxf(M, mst[w][g]);
-        float L = 0.0f, O = 0.0f;
+            for (int w = 0; w < kWsWarps; ++w) M = fmaxf(M, mst[w][g]);
+            float L = 0.0f, O = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWsWarps; ++w) {
-            const float f = mst[w][g] == -INFINITY ? 0.0f : __expf(mst[w][g] - M);
-            L = fmaf(lst[w][g], f, L);
-            O = fmaf(ost[(size_t)(w * GT + g) * a.hd + d], f, O);
-        }
-        float* rec = a.part + ((size_t)(h0 + g) * a.parts + part) * (a.hd + 4);
-        rec[4 + d] = O;
-        if (d == 0) {
-            rec[0] = M;
-            rec[1] = L;
+            for (int w = 0; w < kWsWarps; ++w) {
+                const float f = mst[w][g] == -INFINITY ? 0.0f : __expf(mst[w][g] - M);
+                L = fmaf(lst[w][g], f, L);
+                O = fmaf(ost[(size_t)(w * GT + g) * a.hd + d], f, O);
+            }
+            float* rec = a.part + ((size_t)(h0 + g) * a.parts + part) * (a.hd + 4);
+            rec[4 + d] = O;
+            if (d == 0) {
+                rec[0] = M;
+                rec[1] = L;
+            }
         }
     }
 }
