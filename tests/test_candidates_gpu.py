@@ -929,6 +929,62 @@ def test_captured_and_replayed(gpu):
         lib.gncx_set_synchronous(1)
 
 
+def test_captured_small_and_wide_forms(gpu):
+    """The forms for few rows, one evicted row, head size 256 and ended beams, replayed with other parents, rows and beams."""
+    lib, home = gpu, torch.cuda.current_stream()
+    q, k, v = randn(110, 5, 8, 64), randn(111, 205, 4, 64), randn(112, 205, 4, 64)
+    qw, kw, vw = randn(113, 20, 8, 256), randn(114, 1220, 2, 256), randn(115, 1220, 2, 256)
+    up, upw = (torch.zeros(i, dtype=torch.int32, device="cuda") for i in (5, 20))
+    out, outw = torch.zeros_like(q), torch.zeros_like(qw)
+    x, fin = randn(116, 40, 9000), torch.zeros(40, dtype=torch.int32, device="cuda")
+    s, so, io = torch.zeros(40, device="cuda"), torch.zeros(80, device="cuda"), torch.zeros(3, 80, dtype=torch.int32, device="cuda")
+    w, pos = torch.zeros(4, 205, device="cuda"), torch.zeros(4, 205, dtype=torch.int32, device="cuda")
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    wa, step = (P(ws), ws.numel()), torch.zeros(8, 64, device="cuda")
+
+    def call():
+        assert lib.gncx_attention_tree(P(q), P(k), P(v), P(up), 200, 5, 8, 4, 64, 0.1, 0, P(out), *wa) == 0
+        assert lib.gncx_attention_tree(P(qw), P(kw), P(vw), P(upw), 1200, 20, 8, 2, 256, 0.06, 0, P(outw), *wa) == 0
+        assert lib.gncx_beam_select(P(x), P(s), P(fin), 40, 9000, 3, 80, P(so), P(io), P(io[1]), P(io[2]), *wa) == 0
+        assert lib.gncx_mqa_attention_step_weights(P(q), P(k), P(v), P(k), P(v), 204, 7, 8, 4, 64, 0.1, 0, P(step), P(w), P(pos), 205, *wa) == 0
+        assert lib.gncx_kv_evict(P(k), P(v), P(w), P(pos), 205, 205, 204, 9, 4, 64, P(w), P(pos), 205, *wa) == 0
+
+    def fill(seed):
+        r = np.random.default_rng(seed)
+        for t, n in ((up, 5), (upw, 20)):
+            t.copy_(torch.tensor(make_tree("random", n, seed), dtype=torch.int32))
+        fin.copy_(torch.tensor(r.integers(0, 2, 40), dtype=torch.int32))
+        pos.copy_(torch.tensor(r.integers(0, 12, (4, 205)), dtype=torch.int32))
+        for i, t in enumerate((q, k, v, qw, kw, vw, x, w)):
+            t.copy_(randn(1000 * seed + i, *t.shape))
+
+    outs = (out, outw, so, io, step, w, pos, k, v)
+    wants = []
+    for seed in (1, 2, 3):
+        fill(seed)
+        torch.cuda.synchronize()
+        call()
+        torch.cuda.synchronize()
+        wants.append([t.clone() for t in outs])
+    stream, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    try:
+        lib.gncx_set_synchronous(0)
+        lib.gncx_set_stream(ctypes.c_void_p(stream.cuda_stream))
+        with torch.cuda.graph(g, stream=stream):
+            call()
+        for seed in (3, 1, 2, 1):
+            fill(seed)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                g.replay()
+            torch.cuda.synchronize()
+            for got, want in zip(outs, wants[seed - 1]):
+                assert torch.equal(got, want)
+    finally:
+        lib.gncx_set_stream(ctypes.c_void_p(home.cuda_stream))
+        lib.gncx_set_synchronous(1)
+
+
 def test_stream_ordered_calls_in_a_row(gpu):
     """Stream-ordered, the library's workspace, on a stream of the caller's: each call waits for the one before."""
     home = torch.cuda.current_stream()
