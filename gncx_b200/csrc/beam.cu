@@ -55,6 +55,12 @@ __device__ __forceinline__ uint32_t ord32(float x) {
 __device__ __forceinline__ float unord32(uint32_t o) {
     return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
+// The greater value; NaN if one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
 __device__ __forceinline__ u64 ord64(double x) {
     const u64 u = (u64)__double_as_longlong(x + 0.0);
     return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
@@ -315,6 +321,11 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     u64 T = 0;
     float ahead[kBsPer];  // the next tile's logits
     auto load = [&](int base) {
+        if (base + kBsTile <= i1) {
+#pragma unroll
+            for (int j = 0; j < kBsPer; ++j) ahead[j] = __ldg(x + base + tid + j * kBsThreads);
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < kBsPer; ++j) {
             const int i = base + j * kBsThreads + tid;
@@ -328,8 +339,9 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
 #pragma unroll
         for (int j = 0; j < kBsPer; ++j) {
             v[j] = ahead[j];
-            tm = fmaxf(tm, v[j]);
+            tm = max_nan(tm, v[j]);
         }
+        bad |= !(tm < INFINITY);
         if (base + kBsTile < i1) load(base + kBsTile);
         if (base == i0) {
             // at least n elements reach T: the (n / kWarps)-th largest of each warp's thread maxima
@@ -389,14 +401,10 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
                 if (base + g * kBsThreads >= i1) break;  // of the CTA: the rest of the tile is empty
 #pragma unroll
                 for (int j = g; j < g + 4; ++j) {
-                    bad |= !(v[j] < INFINITY);
                     part[j & 3] += exp_tab((double)fmaxf(v[j], floor) - md, s_tab);
                 }
             }
             l += (part[0] + part[1]) + (part[2] + part[3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kBsPer; ++j) bad |= !(v[j] < INFINITY);
         }
         __syncthreads();
         const int cnt = s_cnt;
