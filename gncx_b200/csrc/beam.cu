@@ -18,12 +18,12 @@
 //   * beam_merge_kernel: one CTA forms the L_b and walks the sorted lists, a
 //     thread per list, past a threshold from their first entries, until no
 //     list has an entry that reaches it; then it ranks what it found.
-// The first kernel is bound by instruction issue (62 % busy, about 50 instructions a
-// logit, a third of them the exponential; 21 % of the fp64 pipe): 27.6 us for 64
-// beams of 151936 logits, 9 of them ended, 1.2 TB/s.  The merge is one CTA's chain
-// of dependent reads and barriers, 8 to 11 us alone and cold.  Both: 33.3 us;
-// 4 beams 13.1 us.  Slower: appending by a ballot per logit (48.7 us against 34.7
-// then), 2, 4 or 5 CTAs per SM (within 3 %).
+// The first kernel is bound by instruction issue (about 60 % busy, 45 instructions a
+// logit, a third of them the exponential): 25.8 us for 64 beams of 151936 logits, 9
+// of them ended, 1.3 TB/s.  The merge is one CTA's chain of dependent reads and
+// barriers, 8 to 11 us alone and cold.  Both: 30.7 us; 4 beams 12.8 us.  Slower:
+// appending by a ballot per logit (48.7 us against 34.7 then), two CTAs per SM
+// (31.3 us), more than fit it (4: 9 % slower).
 #include <cuda_runtime.h>
 #include "common.cuh"
 #include "kernels.h"
@@ -39,8 +39,8 @@ constexpr int kBsSort = 1024;             // largest list that is sorted
 constexpr int kBsList = kBsSort + kBsTile;
 constexpr int kBsCtasPerSm = 3;           // that a vocabulary is split for
 // From fewer than so many parts for each beam the division follows the number of
-// beams that have not ended: 64 beams, 9 of them ended, 33.3 us against 37.1 (none
-// ended: 38.7 and 36.9); with more parts it gains less than reading the flags costs.
+// beams that have not ended: 64 beams, 9 of them ended, 30.7 us against 34.4 (none
+// ended: 34.8 and 34.0); with more parts it gains less than reading the flags costs.
 constexpr int kBsShare = 16;
 constexpr int kBmThreads = 1024;
 constexpr int kBmList = 2 * kBmThreads;

@@ -415,9 +415,9 @@ static int weights_parts(int len, int n_kv, int zgroups, int sm_count) {
     return parts < 1 ? 1 : parts;
 }
 // Whether one launch, a cluster per KV head, does the step: 16 heads, 8 KV heads of
-// 128, 512 rows 4.8 us against 5.2 with two kernels (called one by one 6.9 against
-// 8.9, a launch less); 2048 rows 8.2 against 9.4; 64 columns, 2048 rows on one KV head
-// 5.6 against 7.4; 256 columns, 2048 rows on one KV head 15.4 against 10.4.
+// 128, 512 rows 4.8 us against 5.2 with two kernels (called one by one 6.8 against
+// 9.3, a launch less); 2048 rows 8.2 against 9.1; 64 columns, 2048 rows on one KV head
+// 5.8 against 7.4; 256 columns, 2048 rows on one KV head 15.4 against 10.4.
 static bool weights_one(int len, int hd, int zgroups) {
     return zgroups == 1 && len <= 4096 && len * hd <= (hd > 128 ? 1 << 17 : 1 << 18);
 }

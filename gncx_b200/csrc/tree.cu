@@ -577,10 +577,10 @@ static void tree_geometry(TreeArgs& a, int sm_count) {
 // Query rows per cluster where one launch does everything, 0 where not: the clusters
 // run side by side (15 of 8 CTAs do, 16 took twice the time) and the cache is short.
 // One launch against the two kernels: 16 heads, 8 KV heads of 128, 4 nodes (8 query
-// rows): 10 cache rows 6.0 us and 10.6, 511 rows 8.4 and 10.6, 1600 rows 12.8 and 13.4; on 2 KV
-// heads of 64 it loses from about 750 rows (1000: 9.1 and 8.2).  5 nodes (16 rows per
-// cluster): 256 rows 8.8 and 9.8, 511 rows 10.8 and 10.8.  Head size 256: 128 rows 9.2 and 10.9, 384
-// rows 11.7 and 11.0.
+// rows): 10 cache rows 6.0 us and 11.3, 511 rows 8.4 and 11.6, 700 rows 8.8 and
+// 12.2; on 2 KV heads of 64, 700 rows 7.9 and 8.7, 1000 rows 9.1 and 8.2.  5 nodes
+// (16 rows per cluster): 256 rows 8.8 and 10.8, 511 rows 10.8 and 10.8.  Head size
+// 256: 128 rows 9.2 and 10.8, 384 rows 11.7 and 11.0.
 static int tree_one_rows(const TreeArgs& a, int sm_count) {
     const int64_t len = (int64_t)a.pos0 + a.n_tok - (a.window > 0 ? max(0, a.pos0 - a.window + 1) : 0);
     const int64_t fit = sm_count * 13 / 16 / kToCluster / a.n_kv;  // clusters per KV head

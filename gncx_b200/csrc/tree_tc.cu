@@ -30,9 +30,9 @@
 // Every wait is bounded; on a timeout the kernel records an error and leaves.
 //
 // What bounds it: latency, with the tensor pipe, shared memory and the issue slots
-// each about half busy.  64 nodes, 32 heads, 8 KV heads of 128, 32768 rows: 118 us
-// with the merge (2.3 TB/s; three fp16 products at 870 TFLOP/s, of which the
-// pipe alone would need 60 us), tensor pipe 43 % busy, issue 46 %.  1 node:
+// each about half busy.  64 nodes, 32 heads, 8 KV heads of 128, 32768 rows: 117 us
+// with the merge (2.3 TB/s; three fp16 products at 880 TFLOP/s, of which the
+// pipe alone would need 60 us), tensor pipe 45 % busy, issue 46 %.  1 node:
 // 70 us, 3.8 TB/s.  16 heads, 4 KV heads of 256, 64 nodes, 32768 rows: 162 us (tree.cu's
 // CUDA-core kernel: 3799 us).  Slower: two threads per row with 16 softmax warps
 // (128 us for the first case), lanes of different tiles in CTAs of 128 rows with 8
@@ -66,9 +66,9 @@ constexpr int kTtScales = 4;              // tiles whose scales are kept
 // still seen.
 constexpr int kTtShift = 10, kTtHead = 4;
 // ALT from so many tiles per CTA.  16 heads, 8 KV heads of 128, 16 nodes: 8192
-// rows (7 tiles) 28.5 us with both lanes, 30.5 with one; 32 heads, 32 nodes, 32768
-// rows (28 tiles) 80.4 and 90; with 4 tiles the joining costs as much as it saves
-// (32 heads, 24 nodes, 4096 rows: 24.3 and 23.8).
+// rows (7 tiles) 27.4 us with both lanes, 29.8 with one; 32 heads, 32 nodes, 32768
+// rows (28 tiles) 79.8 and 88.3; with 4 tiles the joining costs more than it saves
+// (32 heads, 24 nodes, 4096 rows: 24.0 and 23.3).
 constexpr int kTtAltTiles = 6;
 // TMEM columns: Q pairs, scores, (head sizes above 128: weights), outputs
 constexpr int kTtQ = 0, kTtS = 256, kTtP = 320, kTtO = 384, kTtCols = 512;
