@@ -37,7 +37,7 @@ constexpr int kBsPer = 16;
 constexpr int kBsTile = kBsThreads * kBsPer;
 constexpr int kBsSort = 1024;             // largest list that is sorted
 constexpr int kBsList = kBsSort + kBsTile;
-constexpr int kBsCtasPerSm = 3;           // that a vocabulary is split for
+constexpr int kBsCtasPerSm = 3;           // that a vocabulary is split for, and that fit one
 // From fewer than so many parts for each beam the division follows the number of
 // beams that have not ended: 64 beams, 9 of them ended, 30.7 us against 34.4 (none
 // ended: 34.8 and 34.0); with more parts it gains less than reading the flags costs.
