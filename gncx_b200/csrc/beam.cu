@@ -279,11 +279,13 @@ __device__ u64 beam_tighten(u64* list, int* s_cnt, int cnt, int n, u64 T, int* h
     return T;
 }
 
-__global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __restrict__ logits,
-                                                               const int32_t* __restrict__ finished, int n_beam,
+// Plain pointers and loads: the kernel may be set up while its predecessor still
+// writes the inputs, so they are not constant over its lifetime.
+__global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* logits,
+                                                               const int32_t* finished, int n_beam,
                                                                int vocab, const BeamSplit split, int n,
-                                                               u64* __restrict__ keys,
-                                                               BeamPart* __restrict__ stats) {
+                                                               u64* keys,
+                                                               BeamPart* stats) {
     constexpr int kWarps = kBsThreads / 32;
     extern __shared__ __align__(16) u64 list[];                  // [kBsList]
     float* s_tile = reinterpret_cast<float*>(list + kBsList);    // [kBsTile]
@@ -323,13 +325,13 @@ __global__ void __launch_bounds__(kBsThreads) beam_part_kernel(const float* __re
     auto load = [&](int base) {
         if (base + kBsTile <= i1) {
 #pragma unroll
-            for (int j = 0; j < kBsPer; ++j) ahead[j] = __ldg(x + base + tid + j * kBsThreads);
+            for (int j = 0; j < kBsPer; ++j) ahead[j] = x[base + tid + j * kBsThreads];
             return;
         }
 #pragma unroll
         for (int j = 0; j < kBsPer; ++j) {
             const int i = base + j * kBsThreads + tid;
-            ahead[j] = i < i1 ? __ldg(x + i) : -INFINITY;
+            ahead[j] = i < i1 ? x[i] : -INFINITY;
         }
     };
     load(i0);
@@ -553,7 +555,7 @@ __device__ __forceinline__ uint32_t cta_bound(uint32_t v, int n, int* hist) {
 }
 
 __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
-    const u64* __restrict__ keys, const BeamPart* __restrict__ stats, const float* scores, const int32_t* finished,
+    const u64* keys, const BeamPart* stats, const float* scores, const int32_t* finished,
     int n_beam, int vocab, const BeamSplit split, int n, int eos, float* out_scores, int32_t* out_parents, int32_t* out_tokens,
     int32_t* out_finished) {
     __shared__ __align__(16) BeamKey list[kBmList];
