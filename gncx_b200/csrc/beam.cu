@@ -105,7 +105,7 @@ __host__ __device__ inline int beam_parts(int live, int vocab, int room) {
 __device__ __forceinline__ int beam_live(const int32_t* finished, int n_beam, int* s_beam) {
     __shared__ unsigned s_on[kBeamMax / 32];
     const int tid = threadIdx.x;
-    const bool on = tid < n_beam && !finished[tid];
+    const bool on = tid < n_beam && !__ldcg(finished + tid);
     const unsigned mine = __ballot_sync(0xffffffffu, on);
     if (tid < kBeamMax && (tid & 31) == 0) s_on[tid >> 5] = mine;
     __syncthreads();
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     __shared__ int s_beam[kBeamMax];
     const int tid = threadIdx.x;
     if (tid == 0) s_cnt = s_live = s_full = 0;
-    // read before the wait: the first kernel has let this one start after its own
+    // read before the wait, from L2: the first kernel has let this one start after its own
     const int n_live = split.share ? beam_live(finished, n_beam, s_beam) : n_beam;
     const int parts = split.share ? beam_parts(n_live, vocab, split.room) : split.parts;
     pdl_wait();

@@ -394,7 +394,9 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a
     const int node = blockIdx.x, kvh = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rows = a.n_tok * a.G, rl = a.hd + 4;
-    for (int i = tid; i <= node; i += kTmThreads) up[i] = a.parents[i];
+    // What is read before the wait is read from L2: the kernels before the dense one
+    // have completed, as it has waited for them before it let this one start.
+    for (int i = tid; i <= node; i += kTmThreads) up[i] = __ldcg(a.parents + i);
     __syncthreads();
     if (tid == 0) {  // parents are below their children, so the walk ends
         int n = 0, i = node;
@@ -430,7 +432,7 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int col = 4 * (lane + 32 * j);
-                q[g][j] = col < a.hd ? *reinterpret_cast<const float4*>(qp + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                q[g][j] = col < a.hd ? __ldcg(reinterpret_cast<const float4*>(qp + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 o[g][j] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
@@ -442,8 +444,8 @@ __global__ void __launch_bounds__(kTmThreads) tree_merge_kernel(const TreeArgs a
                 const int col = 4 * (lane + 32 * j);
                 k[j] = v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (col < a.hd) {
-                    k[j] = *reinterpret_cast<const float4*>(kb + (size_t)row * pstride + col);
-                    v[j] = *reinterpret_cast<const float4*>(vb + (size_t)row * pstride + col);
+                    k[j] = __ldcg(reinterpret_cast<const float4*>(kb + (size_t)row * pstride + col));
+                    v[j] = __ldcg(reinterpret_cast<const float4*>(vb + (size_t)row * pstride + col));
                 }
             }
             float s[kTmHeads];
