@@ -16,7 +16,7 @@
 //     threshold T that at least n_out seen elements reach, at first from the
 //     threads' maxima, filters what is appended.  It writes the list sorted.
 //   * beam_merge_kernel: one CTA forms the L_b and walks the sorted lists, a
-//     thread per list, past a threshold from their first entries, until no
+//     thread (or several) per list, past a threshold from their first entries, until no
 //     list has an entry that reaches it; then it ranks what it found.
 // The first kernel is bound by instruction issue (about 60 % busy, 45 instructions a
 // logit, a third of them the exponential): 25.8 us for 64 beams of 151936 logits, 9
@@ -572,14 +572,21 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     pdl_wait();
     // Everything that is read first is asked for at once: the first entries of the
     // lists, a thread per list; the parts' sums, 4 to 32 lanes per beam; the beams' scores.
-    const int lists = n_live * parts;  // <= kBmThreads
-    const int at = tid / parts;
-    const u64* mine = keys + (size_t)tid * n;
+    // Few lists are shared by 2^sh threads each, which take every 2^sh-th entry:
+    // sorted lists again (3 beams of 1000 logits, 200 out: 15.1 us; a thread per list
+    // 33.3).
+    const int whole = n_live * parts;
+    int sh = 0;
+    if (whole > 0)
+        while (whole << sh < n && whole << (sh + 1) <= kBmThreads) ++sh;
+    const int lists = whole << sh;  // <= kBmThreads
+    const int at = (tid >> sh) / parts, sub = tid & ((1 << sh) - 1), len = (n - sub + (1 << sh) - 1) >> sh;
+    const u64* mine = keys + (size_t)(tid >> sh) * n + sub;
     constexpr int kAhead = 4;  // entries of the list that are loaded together
     u64 ahead[kAhead];
     auto load = [&](int r) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) ahead[i] = r + i < n ? mine[r + i] : 0;
+        for (int i = 0; i < kAhead; ++i) ahead[i] = r + i < len ? mine[(r + i) << sh] : 0;
     };
     auto entry = [&](int r) {
         u64 e = ahead[0];
@@ -636,7 +643,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     __syncthreads();
     const double score = s_score[b], lse = has ? s_lse[at] : 0.0;
     // the lists' first R entries, which with the ended beams are enough unless many are no candidates
-    const int R = min(n, (n + max(1, s_live * parts) - 1) / max(1, s_live * parts));
+    const int live_lists = max(1, s_live * parts << sh), R = min(len, (n + live_lists - 1) / live_lists);
     int r = 0;  // entries of this thread's list that were taken
     bool more = has;
     for (; r < R && more; ++r) {
@@ -647,13 +654,13 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
     }
     __syncthreads();
     int cnt = s_cnt;  // <= n_beam + live lists + n; where it is over kBmThreads, t1 goes by the first of them
-    const uint32_t t1 = cnt > n ? cta_bound(tid < cnt ? beam_key32(list[tid].hi) : 0u, n, s_rank) : 0u;
+    const uint32_t t1 = cnt >= n ? cta_bound(tid < cnt ? beam_key32(list[tid].hi) : 0u, n, s_rank) : 0u;
     // the rest, while it reaches t1: a few entries per list.  Where the lists hold
     // so many candidates that t1 does not bound them, in rounds with a sort.
     const bool bounded = t1 != 0;
     if (bounded) {
         __syncthreads();
-        while (more && r < n) {
+        while (more && r < len) {
             if (r && (r & (kAhead - 1)) == 0) load(r);
             const BeamKey k = beam_key(entry(r), b, score, lse);
             more = k.hi != 0 && beam_key32(k.hi) >= t1;
@@ -684,7 +691,7 @@ __global__ void __launch_bounds__(kBmThreads, 1) beam_merge_kernel(
                 if (tid == 0) s_cnt = n;
                 __syncthreads();
             }
-            more = more && r < n;
+            more = more && r < len;
             if (more) {
                 if (r && (r & (kAhead - 1)) == 0) load(r);
                 const BeamKey k = beam_key(entry(r), b, score, lse);

@@ -631,7 +631,9 @@ def check_beam(got, ref):
 
 
 BEAMS = [(1, 1, 1), (1, 5, 9), (3, 7, 40), (1, 151936, 1), (4, 151936, 8), (2, 4095, 16), (2, 4096, 16), (2, 4097, 16),
-         (5, 8193, 10), (16, 32000, 32), (64, 151936, 128), (7, 50257, 256), (256, 1000, 256), (1, 300001, 256), (3, 262144, 200)]
+         (5, 8193, 10), (16, 32000, 32), (64, 151936, 128), (7, 50257, 256), (256, 1000, 256), (1, 300001, 256), (3, 262144, 200),
+         # few lists, of which several threads read each
+         (1, 4096, 256), (2, 300, 256), (5, 4000, 129), (1, 200, 256), (3, 1000, 200), (16, 4000, 32), (31, 900, 33), (7, 3106, 7), (9, 5000, 255)]
 
 
 @pytest.mark.parametrize("b,vocab,n", BEAMS)
