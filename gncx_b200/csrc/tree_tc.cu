@@ -30,10 +30,10 @@
 // Every wait is bounded; on a timeout the kernel records an error and leaves.
 //
 // What bounds it: latency, with the tensor pipe, shared memory and the issue slots
-// each about half busy.  64 nodes, 32 heads, 8 KV heads of 128, 32768 rows: 117 us
-// with the merge (2.3 TB/s; three fp16 products at 880 TFLOP/s, of which the
+// each about half busy.  64 nodes, 32 heads, 8 KV heads of 128, 32768 rows: 114 us
+// with the merge (2.4 TB/s; three fp16 products at 910 TFLOP/s, of which the
 // pipe alone would need 60 us), tensor pipe 45 % busy, issue 46 %.  1 node:
-// 70 us, 3.8 TB/s.  16 heads, 4 KV heads of 256, 64 nodes, 32768 rows: 162 us (tree.cu's
+// 70 us, 3.8 TB/s.  16 heads, 4 KV heads of 256, 64 nodes, 32768 rows: 157 us (tree.cu's
 // CUDA-core kernel: 3799 us).  Slower: two threads per row with 16 softmax warps
 // (128 us for the first case), lanes of different tiles in CTAs of 128 rows with 8
 // loader warps (147 us), Q's lo parts in shared memory for a second S buffer
@@ -70,6 +70,12 @@ constexpr int kTtShift = 10, kTtHead = 4;
 // rows (28 tiles) 79.8 and 88.3; with 4 tiles the joining costs more than it saves
 // (32 heads, 24 nodes, 4096 rows: 24.0 and 23.3).
 constexpr int kTtAltTiles = 6;
+// Rows of a warp above which Q and the records go through shared memory, so that a
+// load or store touches 8 rows or fewer: 33 nodes, 32 heads, 8 KV heads of 128, 4097
+// rows 25.9 us against 26.8 without, 58 nodes, 3 heads, one KV head of 256, 102 rows
+// 16.4 against 22.5; with few rows it costs more than it saves (5 nodes, 16 heads, 8
+// KV heads, 511 rows: 11.6 against 10.8).
+constexpr int kTtTurn = 16;
 // TMEM columns: Q pairs, scores, (head sizes above 128: weights), outputs
 constexpr int kTtQ = 0, kTtS = 256, kTtP = 320, kTtO = 384, kTtCols = 512;
 
@@ -86,7 +92,10 @@ struct TtLayout {
     static constexpr int oBar = oScale + kTtScales * 2 * 8 * 4;
     static constexpr int kBars = 4 * kTtStages + 2 + 6 + 2;
     static constexpr int oState = oBar + kBars * 8;    // what the lanes tell each other of each row: float [2][128]
-    static constexpr int kBytes = oState + 2 * 128 * 4;
+    static constexpr int oTurn = oState + 2 * 128 * 4;  // per softmax warp: 16 columns of its 32 rows of Q
+    static constexpr int kTurn = 32 * 20 * 4;
+    static constexpr int kBytes = oTurn + 8 * kTurn;
+    static_assert(kBytes <= 227 * 1024 - 1024, "shared memory");
     static_assert(HD > 128 || kStage >= 128 * HD * 4, "a lane's output fits an operand stage");
     // more than half of an SM's shared memory, so one CTA per SM owns all of TMEM
     static constexpr int kAlloc = kBytes > 120 * 1024 ? kBytes : 120 * 1024;
@@ -389,14 +398,43 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         const int x = warp >> 2;
         const int first = r0 + (kShared ? 0 : 128 * x) + 32 * (warp & 3), row = first + lane;
         const bool active = first < rows;  // of the warp
+        const bool many = rows - first > kTtTurn;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t tq = tmem + lanes + kTtQ + x * (WIDE ? 64 : 128), to = tmem + lanes + kTtO;
         constexpr int kQlo = HD / 2;  // columns from Q's hi to its lo parts
         const int c0 = WIDE ? 128 * x : 0;  // the lane's first column
         int sq = 0;
-        float v[HO];  // the lane's columns of the row, in flight at once
+        float v[HO];  // the lane's columns of the row
         float qm = 0.0f;
-        if (active) {
+        if (active && many) {
+            // four lanes per row, 16 columns at a time, then turned into a row per thread:
+            // a load touches 8 rows' lines instead of 32
+            float4 w[HO / 4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int of = first + 8 * k + lane / 4;
+                const bool some = of < rows;
+                const float* qp = a.q + ((size_t)(some ? of / a.G : 0) * a.n_heads + kvh * a.G + (some ? of % a.G : 0)) * a.hd + c0;
+#pragma unroll
+                for (int b = 0; b < HO / 16; ++b) {
+                    const int col = 16 * b + 4 * (lane % 4);
+                    w[4 * b + k] = some && c0 + col < a.hd ? *reinterpret_cast<const float4*>(qp + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+            float* turn = reinterpret_cast<float*>(sm + L::oTurn + L::kTurn * warp);
+#pragma unroll
+            for (int b = 0; b < HO / 16; ++b) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) *reinterpret_cast<float4*>(turn + (8 * k + lane / 4) * 20 + 4 * (lane % 4)) = w[4 * b + k];
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 y = *reinterpret_cast<const float4*>(turn + lane * 20 + 4 * i);
+                    v[16 * b + 4 * i] = y.x; v[16 * b + 4 * i + 1] = y.y; v[16 * b + 4 * i + 2] = y.z; v[16 * b + 4 * i + 3] = y.w;
+                }
+                __syncwarp();
+            }
+        } else if (active) {
             const bool some = row < rows;
             const float* qp = a.q + ((size_t)(some ? row / a.G : 0) * a.n_heads + kvh * a.G + (some ? row % a.G : 0)) * a.hd + c0;
 #pragma unroll
@@ -404,6 +442,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 const float4 w = some && c0 + 4 * c < a.hd ? *reinterpret_cast<const float4*>(qp + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
                 v[4 * c] = w.x; v[4 * c + 1] = w.y; v[4 * c + 2] = w.z; v[4 * c + 3] = w.w;
             }
+        }
+        if (active) {
 #pragma unroll
             for (int c = 0; c < HO; ++c) qm = fmaxf(qm, fabsf(v[c]) < INFINITY ? fabsf(v[c]) : 0.0f);
         }
@@ -607,16 +647,42 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 o[d] = add2(o[d], pack2(of(c0 + 2 * d), of(c0 + 2 * d + 1)));
             }
         }
-        if (row < rows && !(ALT && x == 1)) {
-            float* rec = a.part + (((size_t)kvh * rows + row) * a.splits + split) * (a.hd + 4);
+        if (active && !(ALT && x == 1)) {
+            constexpr int C = HD > 64 ? 32 : 16, LR = C / 4;  // columns at a time, lanes per row
+            static_assert(32 * (C + 4) * 4 <= 2 * L::kChunk, "a warp's share of the staging");
             const float f = pow2i(-kTtShift);
-            if (!WIDE || x == 0) *reinterpret_cast<float2*>(rec) = make_float2(T, l * f);
+            auto record = [&](int of) { return a.part + (((size_t)kvh * rows + of) * a.splits + split) * (a.hd + 4); };
+            if (row < rows && (!WIDE || x == 0)) *reinterpret_cast<float2*>(record(row)) = make_float2(T, l * f);
+            if (many) {
+                // a thread's row is turned into rows of the warp through its part of the loaders'
+                // staging, which they are through with: whole lines are written
+                float* turn = reinterpret_cast<float*>(sm + L::oStaging + 2 * L::kChunk * warp);
 #pragma unroll
-            for (int d = 0; d < HO; d += 4)
-                if (c0 + d < a.hd) {
-                    const float2 x0 = unpack2(o[d / 2]), x1 = unpack2(o[d / 2 + 1]);
-                    *reinterpret_cast<float4*>(rec + 4 + c0 + d) = make_float4(x0.x * f, x0.y * f, x1.x * f, x1.y * f);
+                for (int b = 0; b < HO / C; ++b) {
+#pragma unroll
+                    for (int i = 0; i < LR; ++i) {
+                        const float2 x0 = unpack2(o[b * C / 2 + 2 * i]), x1 = unpack2(o[b * C / 2 + 2 * i + 1]);
+                        *reinterpret_cast<float4*>(turn + lane * (C + 4) + 4 * i) = make_float4(x0.x * f, x0.y * f, x1.x * f, x1.y * f);
+                    }
+                    __syncwarp();
+                    const int col = c0 + b * C + 4 * (lane % LR);
+#pragma unroll
+                    for (int k = 0; k < LR; ++k) {
+                        const int of = 32 / LR * k + lane / LR;
+                        if (first + of < rows && col < a.hd)
+                            *reinterpret_cast<float4*>(record(first + of) + 4 + col) =
+                                *reinterpret_cast<const float4*>(turn + of * (C + 4) + 4 * (lane % LR));
+                    }
+                    __syncwarp();
                 }
+            } else if (row < rows) {
+#pragma unroll
+                for (int d = 0; d < HO; d += 4)
+                    if (c0 + d < a.hd) {
+                        const float2 x0 = unpack2(o[d / 2]), x1 = unpack2(o[d / 2 + 1]);
+                        *reinterpret_cast<float4*>(record(row) + 4 + c0 + d) = make_float4(x0.x * f, x0.y * f, x1.x * f, x1.y * f);
+                    }
+            }
         }
     }
     tc_fence_before();
