@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 for (int i = 0; ok && i < nl; ++i) {
                     const int x = ALT ? t & 1 : i;
                     // before the first product into O, oempty's phase "before 0" counts as complete
-                    ok = wait_all3(&pfull[WIDE ? 0 : x], phase(t), &vfull[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
+                    ok = wait_all3(&pfull[x], phase(t), &vfull[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     values(x, t);
@@ -584,7 +584,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 tmem_wait_st();
                 tc_fence_before();
             }
-            if (writes) mbar_arrive(&pfull[x]);
+            // WIDE: lane 1's arrival says that it has asked for this tile's barriers, which may
+            // go on to their next phases once its products are through
+            mbar_arrive(&pfull[x]);
             ok = wait_warp(&ofull[x], phase(t));
             if (!ok) break;
             if (active) {
