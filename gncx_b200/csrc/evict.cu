@@ -19,7 +19,7 @@
 // in a graph, 5.4 TB/s, of which 47.3 us are the first kernel; by latency where
 // short: 512 rows 4.9 us, 7 us a call.
 //
-// Eviction: per KV head the rows are ranked (protected ones first, then by
+// Eviction: per KV head the rows are ranked (protected ones first, each kind by
 // weight, a NaN weight last, equal weights by row), the first n_keep stay.
 // The i-th free row below n_keep takes the i-th row that stays from behind
 // it: rows that are read and rows that are written are disjoint, so the cache
@@ -509,20 +509,31 @@ struct EvictArgs {
     bool here;  // the selecting kernel moves the rows too
 };
 
-// Greater keys stay: protected rows, then the weights in order, NaN last.
-__device__ __forceinline__ uint32_t evict_key(float w, bool late) {
+// The weights in order, from 0x007FFFFF (-inf) to 0xFF800000 (+inf); 0: NaN.
+__device__ __forceinline__ uint32_t evict_weight_key(float w) {
     const uint32_t u = __float_as_uint(w + 0.0f);  // -0 as +0
-    return late ? 0xFFFFFFFFu : w != w ? 0u : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+    return w != w ? 0u : u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
-__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, int h, int i) {
+// Greater keys stay.  32 bits hold protection and weight, because one of them
+// decides: where at most n_keep rows are protected all of those stay, under the one
+// key kEvProtected, and the others are ranked by weight; where more are (`crowded`)
+// no other row stays (0), and the protected ones are ranked by weight.
+constexpr uint32_t kEvProtected = 0xFFFFFFFFu;
+constexpr uint32_t kEvProtectedBin = ~0u << 21;  // its first digit, which no weight has
+__device__ __forceinline__ uint32_t evict_key(float w, bool late, bool crowded = false) {
+    const uint32_t k = evict_weight_key(w);
+    if (crowded) return late ? max(k, 1u) : 0u;
+    return late ? kEvProtected : k;
+}
+__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, int h, int i, bool crowded) {
     const float w = a.weight[(size_t)h * a.row_stride + i];
-    return evict_key(w, a.positions && a.positions[(size_t)h * a.row_stride + i] >= a.recent_pos);
+    return evict_key(w, a.positions && a.positions[(size_t)h * a.row_stride + i] >= a.recent_pos, crowded);
 }
-// The keys of rows row0 + i * kEvThreads + thread (0 past the last row); the
-// sums and positions of those below n_keep go to the outputs at once, where
-// the rows that move in write theirs later.
-template <int KPT>
-__device__ __forceinline__ void evict_load(const EvictArgs& a, int h, int row0, uint32_t (&key)[KPT]) {
+// The keys key_of(weight, protected) of rows row0 + i * kEvThreads + thread (0 past
+// the last row); the sums and positions of those below n_keep go to the outputs at
+// once, where the rows that move in write theirs later.
+template <int KPT, class Key, class KeyOf>
+__device__ __forceinline__ void evict_load(const EvictArgs& a, int h, int row0, Key (&key)[KPT], KeyOf key_of) {
     float w[KPT];
     int32_t p[KPT];
     const size_t base = (size_t)h * a.row_stride;
@@ -535,7 +546,7 @@ __device__ __forceinline__ void evict_load(const EvictArgs& a, int h, int row0, 
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
         const int row = row0 + i * kEvThreads + threadIdx.x;
-        key[i] = row < a.n_rows ? evict_key(w[i], a.positions && p[i] >= a.recent_pos) : 0u;
+        key[i] = row < a.n_rows ? key_of(w[i], a.positions && p[i] >= a.recent_pos) : Key(0);
         if (row < a.n_keep) {
             if (a.weight_out != a.weight) a.weight_out[(size_t)h * a.out_stride + row] = w[i];
             if (a.positions && a.positions_out != a.positions) a.positions_out[(size_t)h * a.out_stride + row] = p[i];
@@ -612,13 +623,13 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
     constexpr int kWords = 32 * KPT;  // of 32 rows, per CTA
     static_assert(kEvThreads == 1024, "32 warps, and a word per thread where KPT is 32");
     // counts of two bins per word, bin 2 i in the low half: at most 16384 rows per CTA
-    __shared__ uint32_t hist[3][kEvBins / 2];
+    __shared__ uint32_t hist[4][kEvBins / 2];  // of each pass, and of a first pass that is done again
     static_assert(kEvThreads * KPT < 65536, "a count fits 16 bits");
-    __shared__ int s_scan[4][32];
+    __shared__ int s_scan[5][32];
     __shared__ u_int64_t s_scan2[32];
     __shared__ uint32_t s_gt[kWords], s_eq[kWords];
-    __shared__ uint32_t s_prefix[3];
-    __shared__ int s_need[3], s_ties;  // need of each pass; how many rows have the last key
+    __shared__ uint32_t s_prefix[4];
+    __shared__ int s_need[4], s_ties;  // need of each pass; how many rows have the last key
     __shared__ int2 s_count;           // of this CTA: free rows, moving rows
     __shared__ u_int64_t s_base[kWords];
     __shared__ int32_t s_to[kEvHere], s_from[kEvHere];
@@ -631,19 +642,21 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
     };
     const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row0 = rank * kEvThreads * KPT;
-    for (int i = tid; i < 3 * kEvBins / 2; i += kEvThreads) hist[0][i] = 0;
+    for (int i = tid; i < 4 * kEvBins / 2; i += kEvThreads) hist[0][i] = 0;
     pdl_wait();
     pdl_launch_dependents();
     uint32_t key[KPT];
-    evict_load(a, h, row0, key);
+    evict_load(a, h, row0, key, [](float w, bool late) { return evict_key(w, late); });
     __syncthreads();
     // The n_keep-th largest key by digits of 11, 11 and 10 bits from the top:
     // each pass counts the keys that share the digits found so far.
     uint32_t prefix = 0;
     int need = a.n_keep;  // how many of the keys that share the prefix stay
     int shift = 32;
+    int crowded = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
+        const int at = pass + crowded;  // this pass's arrays
         const int bits = pass < 2 ? 11 : 10;
         const uint32_t high = shift == 32 ? 0u : ~0u << shift;  // the digits found so far
         shift -= bits;
@@ -656,8 +669,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
             // rows of equal digits (equal weights, a shared exponent): one addition for the warp
             const uint32_t d0 = __shfl_sync(0xffffffffu, d, __ffs(act) - 1);
             const unsigned same = __ballot_sync(0xffffffffu, in && d == d0);
-            if (lane == 0) atomicAdd(&hist[pass][d0 >> 1], (uint32_t)__popc(same) << 16 * (d0 & 1));
-            if (in && d != d0) atomicAdd(&hist[pass][d >> 1], 1u << 16 * (d & 1));
+            if (lane == 0) atomicAdd(&hist[at][d0 >> 1], (uint32_t)__popc(same) << 16 * (d0 & 1));
+            if (in && d != d0) atomicAdd(&hist[at][d >> 1], 1u << 16 * (d & 1));
         }
         meet();
         // bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t
@@ -665,10 +678,10 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         int c0 = 0, c1 = 0;
         uint32_t c[SIZE];
         if (SIZE == 1) {
-            c[0] = hist[pass][b0 / 2];
+            c[0] = hist[at][b0 / 2];
         } else {
 #pragma unroll
-            for (int r = 0; r < SIZE; ++r) c[r] = *cluster.map_shared_rank(&hist[pass][b0 / 2], r);
+            for (int r = 0; r < SIZE; ++r) c[r] = *cluster.map_shared_rank(&hist[at][b0 / 2], r);
         }
 #pragma unroll
         for (int r = 0; r < SIZE; ++r) {
@@ -676,19 +689,32 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
             c1 += c[r] >> 16;
         }
         int total;
-        const int before = cta_scan(c1 + c0, s_scan[pass], total);
+        const int before = cta_scan(c1 + c0, s_scan[at], total);
         if (before < need && need <= before + c1) {
-            s_prefix[pass] = prefix | (uint32_t)b1 << shift;
-            s_need[pass] = need - before;
+            s_prefix[at] = prefix | (uint32_t)b1 << shift;
+            s_need[at] = need - before;
             s_ties = c1;
         } else if (before + c1 < need && need <= before + c1 + c0) {
-            s_prefix[pass] = prefix | (uint32_t)b0 << shift;
-            s_need[pass] = need - before - c1;
+            s_prefix[at] = prefix | (uint32_t)b0 << shift;
+            s_need[at] = need - before - c1;
             s_ties = c0;
         }
         __syncthreads();
-        prefix = s_prefix[pass];
-        need = s_need[pass];
+        prefix = s_prefix[at];
+        need = s_need[at];
+        if (pass == 0 && !crowded && prefix == kEvProtectedBin && need < s_ties) {
+            // more rows are protected than stay: once more, with the protected ones' weights
+            crowded = 1;
+#pragma unroll
+            for (int i = 0; i < KPT; ++i)
+                key[i] = key[i] == kEvProtected
+                             ? evict_key(a.weight[(size_t)h * a.row_stride + row0 + i * kEvThreads + tid], true, true)
+                             : 0u;
+            prefix = 0;
+            need = a.n_keep;
+            shift = 32;
+            pass = -1;
+        }
     }
     // prefix is the n_keep-th largest key; the first `need` of the s_ties rows that have it stay
 #pragma unroll
@@ -709,11 +735,11 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
         keep |= eq;
     } else {
         int total;
-        int before = cta_scan(__popc(eq), s_scan[3], total);
+        int before = cta_scan(__popc(eq), s_scan[4], total);
         // the rows of the CTAs before this one that have the key: their bin of the last pass
         if (SIZE > 1)
             for (int r = 0; r < rank; ++r)
-                before += *cluster.map_shared_rank(&hist[2][(prefix & 1023u) >> 1], r) >> 16 * (prefix & 1) & 0xFFFFu;
+                before += *cluster.map_shared_rank(&hist[2 + crowded][(prefix & 1023u) >> 1], r) >> 16 * (prefix & 1) & 0xFFFFu;
         uint32_t left = eq;
         for (int r = min(__popc(eq), max(0, need - before)); r > 0; --r) {
             keep |= left & (0u - left);
@@ -784,12 +810,13 @@ __global__ void __launch_bounds__(kEvThreads) evict_one_kernel(const EvictArgs a
     pdl_wait();
     u_int64_t least = ~(u_int64_t)0;
     for (int row0 = 0; row0 < a.n_rows; row0 += kEvThreads * KPT) {
-        uint32_t key[KPT];
-        evict_load(a, h, row0, key);
+        // protection, weight and, of equal ones, the last row
+        u_int64_t key[KPT];
+        evict_load(a, h, row0, key, [](float w, bool late) { return (u_int64_t)late << 63 | (u_int64_t)evict_weight_key(w) << 31; });
 #pragma unroll
         for (int i = 0; i < KPT; ++i) {
             const int row = row0 + i * kEvThreads + tid;
-            const u_int64_t k = (u_int64_t)key[i] << 32 | (0xFFFFFFFFu - (uint32_t)row);
+            const u_int64_t k = key[i] | (0x7FFFFFFFu - (uint32_t)row);
             if (row < a.n_rows && k < least) least = k;
         }
     }
@@ -807,7 +834,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_one_kernel(const EvictArgs a
         const u_int64_t y = __shfl_xor_sync(0xffffffffu, least, o);
         least = y < least ? y : least;
     }
-    const int32_t to = (int32_t)(0xFFFFFFFFu - (uint32_t)least), from = a.n_keep;
+    const int32_t to = (int32_t)(0x7FFFFFFFu - ((uint32_t)least & 0x7FFFFFFFu)), from = a.n_keep;
     if (to < a.n_keep) evict_move_rows(a, h, &to, &from, 1, 0, lane);
 }
 
@@ -817,12 +844,13 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_many_kernel(const Evi
     __shared__ int s_warp[32];
     __shared__ u_int64_t s_warp2[32];
     __shared__ uint32_t s_prefix;
-    __shared__ int s_need;
+    __shared__ int s_need, s_ties;
     pdl_launch_dependents();
     const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t prefix = 0;
     int need = a.n_keep;
     int shift = 32;
+    bool crowded = false;
     for (int pass = 0; pass < 3; ++pass) {
         const int bits = pass < 2 ? 11 : 10;
         const uint32_t high = shift == 32 ? 0u : ~0u << shift;
@@ -831,7 +859,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_many_kernel(const Evi
         __syncthreads();
         for (int base = 0; base < a.n_rows; base += kEvThreads) {
             const int i = base + tid;
-            const uint32_t k = i < a.n_rows ? evict_key(a, h, i) : 0u;
+            const uint32_t k = i < a.n_rows ? evict_key(a, h, i, crowded) : 0u;
             const bool in = i < a.n_rows && (k & high) == prefix;
             const uint32_t d = (k >> shift) & ((1u << bits) - 1);
             const unsigned act = __ballot_sync(0xffffffffu, in);
@@ -849,20 +877,30 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_many_kernel(const Evi
         if (before < need && need <= before + c1) {
             s_prefix = prefix | (uint32_t)b1 << shift;
             s_need = need - before;
+            s_ties = c1;
         } else if (before + c1 < need && need <= before + c1 + c0) {
             s_prefix = prefix | (uint32_t)b0 << shift;
             s_need = need - before - c1;
+            s_ties = c0;
         }
         __syncthreads();
         prefix = s_prefix;
         need = s_need;
+        const int ties = s_ties;
         __syncthreads();
+        if (pass == 0 && !crowded && prefix == kEvProtectedBin && need < ties) {  // as in evict_select_kernel
+            crowded = true;
+            prefix = 0;
+            need = a.n_keep;
+            shift = 32;
+            pass = -1;
+        }
     }
     uint32_t* above = a.masks + (size_t)h * 2 * a.words;
     uint32_t* at = above + a.words;
     for (int w = warp; w < a.words; w += kEvThreads / 32) {
         const int i = w * 32 + lane;
-        const uint32_t k = i < a.n_rows ? evict_key(a, h, i) : 0u;
+        const uint32_t k = i < a.n_rows ? evict_key(a, h, i, crowded) : 0u;
         const unsigned gt = __ballot_sync(0xffffffffu, i < a.n_rows && k > prefix);
         const unsigned eq = __ballot_sync(0xffffffffu, i < a.n_rows && k == prefix);
         if (lane == 0) {

@@ -18,6 +18,19 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: long-running")
 
 
+def pytest_collection_modifyitems(items):
+    """test_evict's reference ranks protected rows by their row alone.  The header, and the
+    operator's plain form, rank them by weight, then row: of five protected rows with
+    weights 5, 1, 9, 2, 7 the two that stay are 2 and 4, not 0 and 1.  Where more rows are
+    protected than stay and their weights differ, its expected rows are wrong;
+    test_evict_in_documented_order has the same cases with the documented order."""
+    for item in items:
+        if getattr(item, "originalname", "") == "test_evict":
+            p = item.callspec.params
+            if p["kind"] != "equal" and p["n"] > max(2, p["keep"]):
+                item.add_marker(pytest.mark.xfail(strict=True, reason="expects protected rows ranked by row, not by weight"))
+
+
 @pytest.fixture(scope="session")
 def oracle():
     from oracle.oracle import Oracle
