@@ -9,7 +9,9 @@
 // hi lo, each exact in the fp32 accumulator; lo lo (2^-22 of the product) is
 // left out.  bf16 pairs would keep 16 bits, a tf32 pair costs twice the tensor
 // time.  Groups: a query row; 8 cache rows of K; 8 cache rows of V (4 rows each
-// for head sizes above 128).
+// for head sizes above 128), of which a row below 2^-8 of the largest is a group
+// of its own (so 2^-28 of a row's largest value are kept at least).  The weights
+// are split in a unit that goes by the largest weight times V of the tile.
 //
 // One CTA takes up to 256 query rows of one KV head as two lanes A and B of
 // 128 and walks its split of the cache in tiles of 64 rows, each K and V row
@@ -18,6 +20,8 @@
 // their sums at the end:
 //   * loader warps 8-11 bring chunks of 8 rows in with cp.async (four in flight per
 //     warp, 64 KB per SM), split them and write the K-major operand tiles;
+//   * warp 13 gives V's small rows their scales, in the chunks whose loader found a
+//     thread without a large value in one of its rows (hardly any of ordinary data);
 //   * warp 12, one thread, issues S = Q K^T (Q pairs stay in TMEM) and, once a
 //     lane's weights are in TMEM over its scores, O = P V into the shared O
 //     columns, so one lane's softmax runs under the other's products;
@@ -49,22 +53,29 @@
 namespace gncx {
 
 constexpr int kTtThreads = 512;
-constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12;
+constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12, kTtSizeWarp = 13;
 // Registers per thread: softmax, loaders, products (whose warpgroup is filled
 // up by idle warps); together at most the 512 x 128 that the block is launched
 // with.  With 184 for head size 256 the softmax spills in its loop: 346 us instead
 // of 193 (16 heads, 4 KV heads, 64 nodes, 32768 rows).
 template <int HD>
 struct TtRegs {
-    static constexpr int kSoftmax = HD > 128 ? 192 : 176, kLoad = HD > 128 ? 88 : 112, kMma = HD > 128 ? 40 : 48;
+    static constexpr int kSoftmax = HD > 128 ? 192 : 176, kLoad = HD > 128 ? 96 : 112, kMma = HD > 128 ? 32 : 48;
     static_assert(2 * kSoftmax + kLoad + kMma <= 4 * 128, "a split that can be had");
 };
 constexpr int kTtStages = 2;              // K and V operand tiles
 constexpr int kTtScales = 4;              // tiles whose scales are kept
-// Weights are held as 2^(score - reference + kTtShift), with the score at most
-// kTtHead above the reference: up to 2^14 in fp16, and 2^-34 of a weight of 1 is
-// still seen.
-constexpr int kTtShift = 10, kTtHead = 4;
+// Weights are 2^(score - reference), with the score at most kTtHead above the
+// reference.  A tile's product with V
+// has a unit of its own for each query row: 2^-n with the weights times 2^(n - V's
+// scale), the largest of them about 2^kTtTop.  So fp16 pairs lose
+// nothing of the rows that make up the tile's output, whatever the weights and
+// sizes of V's other rows are: what is below 2^-30 of the largest weight times V is cut.
+constexpr int kTtHead = 4, kTtTop = 14;
+// A V row whose largest value is below kTtSmall in its chunk's scale has a scale of
+// its own.  It is looked for where a value of a lane is 2^-kTtSpan of the chunk's largest.
+constexpr float kTtSmall = 8.0f;
+constexpr int kTtSpan = 8;
 // ALT from so many tiles per CTA.  16 heads, 8 KV heads of 128, 16 nodes: 8192
 // rows (7 tiles) 27.4 us with both lanes, 29.8 with one; 32 heads, 32 nodes, 32768
 // rows (28 tiles) 79.8 and 88.3; with 4 tiles the joining costs more than it saves
@@ -89,8 +100,9 @@ struct TtLayout {
     static constexpr int kChunk = kRows * HD * 4;
     static constexpr int oStaging = kTtStages * kStage;
     static constexpr int oScale = oStaging + 16 * kChunk;     // int [kTtScales][2][8]
-    static constexpr int oBar = oScale + kTtScales * 2 * 8 * 4;
-    static constexpr int kBars = 4 * kTtStages + 2 + 6 + 2;
+    static constexpr int oRows = oScale + kTtScales * 2 * 8 * 4;  // of V's rows, in flagged tiles: int [kTtScales][kKeys], and whether they differ [kTtScales]
+    static constexpr int oBar = oRows + kTtScales * (kKeys + 1) * 4;
+    static constexpr int kBars = 5 * kTtStages + 2 + 6 + 2;
     static constexpr int oState = oBar + kBars * 8;    // what the lanes tell each other of each row: float [2][128]
     static constexpr int oTurn = oState + 2 * 128 * 4;  // per softmax warp: 16 columns of its 32 rows of Q
     static constexpr int kTurn = 32 * 20 * 4;
@@ -129,17 +141,26 @@ __device__ __forceinline__ void split2(f32x2 x, uint32_t& hi, uint32_t& lo) {
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// Bits of the largest finite magnitude of the warp's values; inf(i) is called
-// for an infinite x[i].
-template <int N, class Inf>
-__device__ __forceinline__ uint32_t warp_max_bits(float (&x)[N], Inf inf) {
-    float m = 0.0f, m1 = 0.0f;
+__device__ __forceinline__ float abs_max4(const float* x) {
+    return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+}
+// The largest magnitude of this lane's values; `least`: the least of its fours' largest.
+template <int N>
+__device__ __forceinline__ float lane_max(const float (&x)[N], float& least) {
+    float m = abs_max4(x);
+    least = m;
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        m = fmaxf(m, fmaxf(fabsf(x[i]), fabsf(x[i + 1])));
-        m1 = fmaxf(m1, fmaxf(fabsf(x[i + 2]), fabsf(x[i + 3])));
+    for (int i = 4; i < N; i += 4) {
+        const float y = abs_max4(x + i);
+        m = fmaxf(m, y);
+        least = fminf(least, y);
     }
-    m = fmaxf(m, m1);
+    return m;
+}
+// Bits of the largest finite magnitude of the warp's values, from the lanes'; inf(i)
+// is called for an infinite x[i].
+template <int N, class Inf>
+__device__ __forceinline__ uint32_t warp_max_bits(float m, float (&x)[N], Inf inf) {
     uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
     if (b == 0x7F800000u) {
         m = 0.0f;
@@ -165,12 +186,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     constexpr int HO = WIDE ? 128 : HD;  // columns of a lane's output
     constexpr bool kShared = ALT || WIDE;  // both lanes on the same rows, S of tile t in block t & 1
     extern __shared__ __align__(128) uint8_t sm[];
-    int* scales = reinterpret_cast<int*>(sm + L::oScale);
+    int* scales = reinterpret_cast<int*>(sm + L::oScale);  // of the chunks; | 1: V's rows may differ
+    int* row_scales = reinterpret_cast<int*>(sm + L::oRows);
     uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + L::oBar);
     uint64_t* kempty = kfull + kTtStages;
     uint64_t* vfull = kempty + kTtStages;
     uint64_t* vempty = vfull + kTtStages;
-    uint64_t* sfull = vempty + kTtStages;  // [lane]
+    uint64_t* vsized = vempty + kTtStages;  // V's small rows have scales of their own
+    uint64_t* sfull = vsized + kTtStages;  // [lane]
     uint64_t* pfull = sfull + 2;
     uint64_t* ofull = pfull + 2;
     uint64_t* oempty = ofull + 2;
@@ -199,6 +222,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             mbar_init(&kempty[i], 1);
             mbar_init(&vfull[i], 4);
             mbar_init(&vempty[i], 1);
+            mbar_init(&vsized[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sfull[i], 2);
@@ -298,7 +322,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 for (int i = 0; ok && i < nl; ++i) {
                     const int x = ALT ? t & 1 : i;
                     // before the first product into O, oempty's phase "before 0" counts as complete
-                    ok = wait_all3(&pfull[x], phase(t), &vfull[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
+                    ok = wait_all3(&pfull[x], phase(t), &vsized[t & 1], (t >> 1) & 1, oempty, (n_o - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     values(x, t);
@@ -315,6 +339,61 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 }
             commit(done);  // nothing of this CTA's is in flight when TMEM is freed
             if (!mbar_wait(done, 0)) record_error(a.err, kErrTimeout);
+        } else if (warp == kTtSizeWarp) {
+            // ---------------- small rows of V get scales of their own, in the chunks that are flagged ----------------
+            for (int t = 0; t < n_tiles && wait_warp(&vfull[t & 1], (t >> 1) & 1); ++t) {
+                const int* sv = scales + (t & (kTtScales - 1)) * 16 + 8;
+                const unsigned flags = __ballot_sync(0xffffffffu, lane < 8 && (sv[lane & 7] & 1));
+                if (flags) {
+                    int* row_v = row_scales + (t & (kTtScales - 1)) * KEYS;
+                    for (int j = lane; j < KEYS; j += 32) row_v[j] = sv[j / CR] & ~1;
+                    __syncwarp();
+                    uint8_t* tile = sm + (t & 1) * L::kStage + 2 * L::kPart;
+                    const int valid = j1 - j0 - KEYS * t;
+                    bool apart = false;
+#pragma unroll 1
+                    for (unsigned left = flags; left; left &= left - 1) {
+                        const int c = __ffs(left) - 1;
+                        constexpr int G = 32 / CR;  // lanes per row
+                        bool large = CR * c + lane / G >= valid;
+#pragma unroll 1
+                        for (int p = lane % G; p < HD / 8; p += G) {
+                            const uint4 h = *reinterpret_cast<const uint4*>(tile + p * L::kStride + (CR * c + lane / G) * 16);
+                            auto abs2 = [](uint32_t u) { u &= 0x7FFF7FFFu; return *reinterpret_cast<const __half2*>(&u); };
+                            const float2 m = __half22float2(__hmax2(__hmax2(abs2(h.x), abs2(h.y)), __hmax2(abs2(h.z), abs2(h.w))));
+                            large |= fmaxf(m.x, m.y) >= kTtSmall;
+                        }
+                        const unsigned larges = __ballot_sync(0xffffffffu, large);
+#pragma unroll 1
+                        for (int r = 0; r < CR; ++r) {
+                            if (larges >> r * G & ((1u << G) - 1)) continue;
+                            const float* g = a.vc + ((size_t)(j0 + KEYS * t + CR * c + r) * a.n_kv + kvh) * a.hd;
+                            auto value = [&](int d) {
+                                const float y = d < a.hd ? g[d] : 0.0f;
+                                return fabsf(y) == INFINITY ? 0.0f : y;
+                            };
+                            float m = 0.0f;
+#pragma unroll 1
+                            for (int d = lane; d < HD; d += 32) m = fmaxf(m, fabsf(value(d)));
+                            const int s = scale_exp(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+#pragma unroll 1
+                            for (int d = lane; d < HD; d += 32) {
+                                const float y = value(d) * pow2i(s);
+                                const __half h = __float2half_rn(y);
+                                __half* to = reinterpret_cast<__half*>(tile + (d >> 3) * L::kStride + (CR * c + r) * 16) + (d & 7);
+                                to[0] = h;
+                                to[L::kPart / 2] = __float2half_rn(y - __half2float(h));
+                            }
+                            if (lane == 0) row_v[CR * c + r] = s;
+                            apart = true;
+                        }
+                    }
+                    if (lane == 0) row_scales[kTtScales * KEYS + (t & (kTtScales - 1))] = apart;
+                    fence_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive(&vsized[t & 1]);
+            }
         }
     } else if (warp >= kTtLoadWarp) {
         // ---------------- loaders: warp w takes two of the eight chunks of rows of each tile ----------------
@@ -336,11 +415,11 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             if (t < n_tiles && row + CR <= j1 && 4 * col(NK - 1) < a.hd) {
 #pragma unroll
                 for (int k = 0; k < NK; ++k) cp_async16_row(d + at(k) * HD + 4 * col(k), g + (size_t)at(k) * pstride + 4 * col(k));
-            } else if (t < n_tiles) {  // zeros past the last row and column
+            } else if (t < n_tiles) {  // zeros past the last column; past the last row that row again, which keeps the scales even
 #pragma unroll 1
                 for (int k = 0; k < NK; ++k) {
-                    const bool some = row + at(k) < j1 && 4 * col(k) < a.hd;
-                    cp_async16_row(d + at(k) * HD + 4 * col(k), some ? g + (size_t)at(k) * pstride + 4 * col(k) : src[0], some ? 16 : 0);
+                    const bool some = 4 * col(k) < a.hd;
+                    cp_async16_row(d + at(k) * HD + 4 * col(k), some ? src[i >> 1] + (size_t)min(row + at(k), j1 - 1) * pstride + 4 * col(k) : src[0], some ? 16 : 0);
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -362,13 +441,15 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     const float4 v = *reinterpret_cast<const float4*>(st + at(k) * HD + 4 * col(k));
                     x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
                 }
-                const int s = scale_exp(warp_max_bits(x, [&](int e) {
+                float least;
+                const uint32_t top = warp_max_bits(lane_max(x, least), x, [&](int e) {
                     if (i < 2) return;
                     const int c = 4 * col(e >> 2) + (e & 3);
                     atomicOr(&infinite[x[e] < 0.0f][c >> 5], 1u << (c & 31));
                     any_infinite = 1;
                     x[e] = 0.0f;
-                }));
+                });
+                const int s = scale_exp(top);
                 issue(t + 1, i);  // the chunk is in registers
                 const f32x2 f = pack2(pow2i(s), pow2i(s));
                 if ((i & 1) == 0 && t >= kTtStages) ok = wait_warp(i ? &vempty[t & 1] : &kempty[t & 1], ((t >> 1) - 1) & 1);
@@ -383,7 +464,10 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     *reinterpret_cast<uint2*>(dk) = hi;
                     *reinterpret_cast<uint2*>(dk + L::kPart) = lo;
                 }
-                if (lane == 0) sc[8 * (i >> 1) + chunk] = s;
+                // rows that may be much smaller than the largest one (or not there): in most chunks each lane sees
+                // in each of its rows a value that is not small, and one vote tells
+                const bool apart = i >= 2 && __any_sync(0xffffffffu, __float_as_uint(least) + (kTtSpan << 23) < top);
+                if (lane == 0) sc[8 * (i >> 1) + chunk] = s | (int)apart;
                 if (i & 1) {
                     fence_async_smem();
                     __syncwarp();
@@ -478,6 +562,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         bool ok = true;
 #pragma unroll 1
         for (int t = ALT ? x : 0; t < n_tiles; t += ALT ? 2 : 1) {
+            // V is mostly there when the scores are: its scales are then looked at under the first pass
+            bool v_in = __all_sync(0xffffffffu, mbar_test(&vfull[t & 1], (t >> 1) & 1));
             ok = wait_warp(&sfull[WIDE ? t & 1 : x], phase_s(t));
             if (!ok) break;
             float alpha = 1.0f, beta = 1.0f;
@@ -495,8 +581,22 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     const int n = -sq - sk, h = n >> 1;
                     return a.scale2 * pow2i(h) * pow2i(n - h);
                 };
-                const bool even_k = k0.x == k0.y && k0.x == k0.z && k0.x == k0.w && k0.x == k1.x && k0.x == k1.y &&
-                                    k0.x == k1.z && k0.x == k1.w;
+                auto differ = [](const int4& p, const int4& q) {
+                    const int c = p.x;
+                    return ((p.y ^ c) | (p.z ^ c)) | ((p.w ^ c) | (q.x ^ c)) | ((q.y ^ c) | (q.z ^ c)) | (q.w ^ c);
+                };
+                const bool even_k = differ(k0, k1) == 0;
+                int V = 0, flagged = 0;
+                bool even_v = false;
+                // The words are not written again before this warp is through with the tile, so that its
+                // threads agree.
+                auto look = [&] {
+                    const int4 v0 = sc[2], v1 = sc[3];
+                    V = v0.x & ~1;
+                    flagged = ((v0.x | v0.y) | (v0.z | v0.w) | (v1.x | v1.y) | (v1.z | v1.w)) & 1;
+                    even_v = (differ(v0, v1) & ~1) == 0;
+                };
+                if (v_in) look();
                 const float f0 = factor(k0.x);
                 float tm = -INFINITY;
                 if (even_k && valid >= KEYS && f0 >= 0.0f) {
@@ -530,57 +630,104 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     T = tm;
                 }
                 const float ref = T == -INFINITY ? 0.0f : T;
-                // V's scales: the products of this tile count in units of its largest rows
-                ok = wait_warp(&vfull[t & 1], (t >> 1) & 1);
-                if (!ok) break;
-                const int4 v0 = sc[2], v1 = sc[3];
-                const int U = min(min(min(v0.x, v0.y), min(v0.z, v0.w)), min(min(v1.x, v1.y), min(v1.z, v1.w)));
-                const bool even_v = U == max(max(max(v0.x, v0.y), max(v0.z, v0.w)), max(max(v1.x, v1.y), max(v1.z, v1.w)));
-                beta = pow2i(-U);
-                const float shift = kTtShift - ref;
+                if (!v_in) {
+                    ok = wait_warp(&vfull[t & 1], (t >> 1) & 1);
+                    if (!ok) break;
+                    look();
+                }
+                if (flagged) {
+                    ok = wait_warp(&vsized[t & 1], (t >> 1) & 1);
+                    if (!ok) break;
+                    even_v = even_v && !row_scales[kTtScales * KEYS + (t & (kTtScales - 1))];
+                }
+                // The unit 2^-n.  With one scale 2^V for all of V's rows the weights are taken
+                // times 2^m, m = n - V; else each times 2^(n - its row's scale).
+                float back = 1.0f;  // 2^-m
                 f32x2 sum = 0;
-                if (writes && even_k && even_v && valid >= KEYS) {
-                    const f32x2 f02 = pack2(f0, f0), shift2 = pack2(shift, shift);
+                if (even_v) {
+                    // a whole number by rounding in the last place of 1.5 * 2^23; at most what 2^-m and 2^-n can be
+                    const float magic = 12582912.0f;
+                    const int zero = __float_as_int(magic), r = min(__float_as_int(fmaxf((float)kTtTop + ref - tm, 0.0f) + magic), zero + 126 - max(V, 0));
+                    const int m = r - zero;
+                    const float shift = (__int_as_float(r) - magic) - ref;
+                    back = pow2i(-m);
+                    beta = pow2i(-m - V);
+                    if (writes && even_k && valid >= KEYS) {
+                        const f32x2 f02 = pack2(f0, f0), shift2 = pack2(shift, shift);
 #pragma unroll 1
-                    for (int b = 0; b < KEYS / 16; ++b) {
-                        float s[16];
-                        uint32_t p[16];
-                        tmem_ld16f(ts + 16 * b, s);
+                        for (int b = 0; b < KEYS / 16; ++b) {
+                            float s[16];
+                            uint32_t p[16];
+                            tmem_ld16f(ts + 16 * b, s);
 #pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float2 z = unpack2(fma2(pack2(s[j], s[j + 1]), f02, shift2));
-                            const f32x2 e = pack2(ex2(z.x), ex2(z.y));
-                            sum = add2(sum, e);
-                            split2(e, p[j / 2], p[8 + j / 2]);
+                            for (int j = 0; j < 16; j += 2) {
+                                const float2 z = unpack2(fma2(pack2(s[j], s[j + 1]), f02, shift2));
+                                const f32x2 e = pack2(ex2(z.x), ex2(z.y));
+                                sum = add2(sum, e);
+                                split2(e, p[j / 2], p[8 + j / 2]);
+                            }
+                            tmem_st16(tp + 16 * b, p);
                         }
-                        tmem_st16(tp + 16 * b, p);
-                    }
-                } else if (writes) {
+                    } else if (writes) {
 #pragma unroll 1
-                    for (int b = 0; b < KEYS / 16; ++b) {
-                        float s[16];
-                        uint32_t p[16];
-                        tmem_ld16f(ts + 16 * b, s);
-                        const int* sk = reinterpret_cast<const int*>(sc) + 16 / CR * b;
-                        float f[16 / CR], fw[16 / CR];
+                        for (int b = 0; b < KEYS / 16; ++b) {
+                            float s[16];
+                            uint32_t p[16];
+                            tmem_ld16f(ts + 16 * b, s);
+                            const int* sk = reinterpret_cast<const int*>(sc) + 16 / CR * b;
+                            float f[16 / CR];
 #pragma unroll
-                        for (int i = 0; i < 16 / CR; ++i) {
-                            f[i] = factor(sk[i]);
-                            fw[i] = pow2i(max(-126, U - sk[8 + i]));
-                        }
+                            for (int i = 0; i < 16 / CR; ++i) f[i] = factor(sk[i]);
 #pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float c = f[j / CR], w = fw[j / CR];
-                            const float e0 = 16 * b + j < valid ? ex2(fmaf(s[j], c, shift)) : 0.0f;
-                            const float e1 = 16 * b + j + 1 < valid ? ex2(fmaf(s[j + 1], c, shift)) : 0.0f;
-                            sum = add2(sum, pack2(e0, e1));
-                            split2(pack2(e0 * w, e1 * w), p[j / 2], p[8 + j / 2]);
+                            for (int j = 0; j < 16; j += 2) {
+                                const float c = f[j / CR];
+                                const float e0 = 16 * b + j < valid ? ex2(fmaf(s[j], c, shift)) : 0.0f;
+                                const float e1 = 16 * b + j + 1 < valid ? ex2(fmaf(s[j + 1], c, shift)) : 0.0f;
+                                sum = add2(sum, pack2(e0, e1));
+                                split2(pack2(e0, e1), p[j / 2], p[8 + j / 2]);
+                            }
+                            tmem_st16(tp + 16 * b, p);
                         }
-                        tmem_st16(tp + 16 * b, p);
                     }
+                } else {
+                    const int* sk = reinterpret_cast<const int*>(sc);
+                    const int* row_v = row_scales + (t & (kTtScales - 1)) * KEYS;
+                    auto scale_v = [&](int j) { return (float)(flagged ? row_v[j] : sk[8 + j / CR]); };
+                    float most = -INFINITY;  // exponent of the largest weight times V, in V's units
+#pragma unroll 1
+                    for (int b = 0; b < KEYS; b += 16) {
+                        float s[16];
+                        tmem_ld16f(ts + b, s);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (b + j < valid) most = fmaxf(most, s[j] * factor(sk[(b + j) / CR]) - scale_v(b + j));
+                    }
+                    const float n = floorf(fminf(fmaxf((float)kTtTop + ref - most, -126.0f), 126.0f));
+                    beta = pow2i(-(int)n);
+                    if (writes)
+#pragma unroll 1
+                        for (int b = 0; b < KEYS; b += 16) {
+                            float s[16];
+                            uint32_t p[16];
+                            tmem_ld16f(ts + b, s);
+#pragma unroll
+                            for (int j = 0; j < 16; j += 2) {
+                                float e[2] = {0.0f, 0.0f}, w[2] = {0.0f, 0.0f};
+#pragma unroll
+                                for (int y = j; y < j + 2; ++y)
+                                    if (b + y < valid) {
+                                        const float z = fmaf(s[y], factor(sk[(b + y) / CR]), -ref);
+                                        e[y - j] = ex2(z);
+                                        w[y - j] = ex2(z + (n - scale_v(b + y)));
+                                    }
+                                sum = add2(sum, pack2(e[0], e[1]));
+                                split2(pack2(w[0], w[1]), p[j / 2], p[8 + j / 2]);
+                            }
+                            tmem_st16(tp + b, p);
+                        }
                 }
                 const float2 parts = unpack2(sum);
-                l = fmaf(l, alpha, parts.x + parts.y);
+                l = fmaf(l, alpha, (parts.x + parts.y) * back);
                 tmem_wait_st();
                 tc_fence_before();
             }
@@ -652,9 +799,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         if (active && !(ALT && x == 1)) {
             constexpr int C = HD > 64 ? 32 : 16, LR = C / 4;  // columns at a time, lanes per row
             static_assert(32 * (C + 4) * 4 <= 2 * L::kChunk, "a warp's share of the staging");
-            const float f = pow2i(-kTtShift);
             auto record = [&](int of) { return a.part + (((size_t)kvh * rows + of) * a.splits + split) * (a.hd + 4); };
-            if (row < rows && (!WIDE || x == 0)) *reinterpret_cast<float2*>(record(row)) = make_float2(T, l * f);
+            if (row < rows && (!WIDE || x == 0)) *reinterpret_cast<float2*>(record(row)) = make_float2(T, l);
             if (many) {
                 // a thread's row is turned into rows of the warp through its part of the loaders'
                 // staging, which they are through with: whole lines are written
@@ -664,7 +810,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
 #pragma unroll
                     for (int i = 0; i < LR; ++i) {
                         const float2 x0 = unpack2(o[b * C / 2 + 2 * i]), x1 = unpack2(o[b * C / 2 + 2 * i + 1]);
-                        *reinterpret_cast<float4*>(turn + lane * (C + 4) + 4 * i) = make_float4(x0.x * f, x0.y * f, x1.x * f, x1.y * f);
+                        *reinterpret_cast<float4*>(turn + lane * (C + 4) + 4 * i) = make_float4(x0.x, x0.y, x1.x, x1.y);
                     }
                     __syncwarp();
                     const int col = c0 + b * C + 4 * (lane % LR);
@@ -682,7 +828,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 for (int d = 0; d < HO; d += 4)
                     if (c0 + d < a.hd) {
                         const float2 x0 = unpack2(o[d / 2]), x1 = unpack2(o[d / 2 + 1]);
-                        *reinterpret_cast<float4*>(record(row) + 4 + c0 + d) = make_float4(x0.x * f, x0.y * f, x1.x * f, x1.y * f);
+                        *reinterpret_cast<float4*>(record(row) + 4 + c0 + d) = make_float4(x0.x, x0.y, x1.x, x1.y);
                     }
             }
         }

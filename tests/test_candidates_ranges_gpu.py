@@ -105,3 +105,128 @@ def test_evict_one_of_protected_rows_keeps_the_new_token(gpu):
     check_evict(gpu, w, pos, n, n - 1, 0)
     w_out, p_out = run_evict(gpu, randn(35, n, 3, 4), randn(36, n, 3, 4), w, pos, n, n - 1, 0)
     assert p_out[0, 11] == n - 1 and p_out[1].tolist() == list(range(n - 1)) and p_out[2, 0] == n - 1
+
+
+# ---------------------------------------------------------------- values of very different size
+U, LAM = 2.0**-24, 8.0
+
+
+def attend_rows(q, k, v, scale):
+    """q [hd], k and v [n, hd] -> (output, its tolerance) in 64 bits, with each row's own error instead of the largest.
+
+    A score is off by ds_j = (LAM sqrt(hd) + 14 + 2 C) u scale sum |q k_j| (the terms of test_candidates_gpu.py), its
+    weight by that and the exponential's (2 + |x_j|) u, x_j its distance from the maximum in powers of two, and the sum
+    of the weights by the weights' errors and its own rounding: D.  Each term p_j v_j of an output is off by its weight's
+    error, D, the pairs' 12 u and the output's sum, (LAM sqrt(n) + 24) u.  What the pairs cut: less than 2^-30 of the
+    largest p_j max |v_j| a row; in K less than 2^-32 of max |k_j| an element."""
+    q, k, v = q.double(), k.double(), v.double()
+    n, hd = k.shape
+    s = (k @ q) * scale
+    c = LAM * hd**0.5 + 14 + 2 * max(24, 3 * ((hd + 15) // 16))
+    p = torch.softmax(s, 0)
+    ds = abs(scale) * (c * U * (k.abs() @ q.abs()) + 2.0**-32 * q.abs().sum() * k.abs().amax(1))
+    r = ds + (2 + (s.max() - s) / np.log(2.0)) * U
+    off = r + (p * r).sum() + (2 * LAM * n**0.5 + 36) * U
+    cut = 2.0**-30 * (LAM * n**0.5 + 8) * (p * v.abs().amax(1)).max()
+    return p @ v, (p * off) @ v.abs() + cut + 1e-36
+
+
+def check_rows(out, q, k, v, up, pos0, scale, window, nodes, heads):
+    group = q.shape[1] // k.shape[1]
+    worst = 0.0
+    for i in nodes:
+        rows = torch.tensor(tree_seen(up, i, pos0, window), device="cuda")
+        for h in heads:
+            ref, tol = attend_rows(q[i, h], k[rows][:, h // group], v[rows][:, h // group], scale)
+            err = (out[i, h].double() - ref).abs()
+            worst = max(worst, float((err / tol).max()))
+            assert bool((err <= tol).all()), (i, h, float((err / tol).max()), float((err / ref.abs().clamp_min(1e-30)).max()))
+    return worst
+
+
+# Forms of the tensor-core kernel: one lane, two lanes, lanes on alternating tiles, and columns above 128; on the CUDA
+# cores: few query rows, other head sizes.
+FORMS = {"one lane": (8, 2, 128, 700, 24), "one lane of 64": (8, 2, 64, 700, 24), "two lanes": (32, 4, 128, 900, 20), "two lanes of 64": (32, 4, 64, 900, 20),
+         "alternating": (32, 32, 128, 1800, 6), "alternating, of 64": (32, 32, 64, 1800, 6), "wide": (16, 4, 256, 700, 24), "wide, many tiles": (148, 148, 256, 400, 2),
+         "one launch": (8, 2, 128, 300, 3), "columns of 36": (8, 2, 36, 900, 30), "columns of 252": (8, 2, 252, 900, 30)}
+
+
+def uneven(seed, n, nh, nkv, hd, pos0):
+    """Scores within about a unit of each other, except where `bias` (one column of K) lowers them."""
+    q, k, v = randn(seed, n, nh, hd) * 0.1, randn(seed + 1, pos0 + n, nkv, hd) * 0.1, randn(seed + 2, pos0 + n, nkv, hd)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    return q, k, v
+
+
+# the row of another size: in the same chunk of 8 rows (or 4), the same tile, another tile, the first, the last
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("r", [6, 13, 17, 20, 24, 30, 36, 60, 100])
+def test_tree_rows_without_weight_do_not_blur_v(gpu, form, r):
+    """Rows that get next to no weight have V 2^r larger than the rows that get it all."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = uneven(40, n, nh, nkv, hd, pos0)
+    large = torch.zeros(pos0 + n, dtype=torch.bool, device="cuda")
+    for row in (0, 5, 70, 130, 200, 201, 202, 203, 204, 205, 206, 207, 290, pos0 - 1):
+        large[row] = True
+    v[large] *= 2.0**r
+    k[large, :, 0] = -(r * 0.75 + 40) / 1.0  # a weight of e^-(..): its product with V is small too
+    up = make_tree("random", n, 41)
+    out = run_tree(gpu, q, k, v, up, pos0, 1.0, 0)
+    check_rows(out, q, k, v, up, pos0, 1.0, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("r", [6, 13, 20, 30, 40, 60])
+def test_tree_small_weights_of_large_v(gpu, form, r):
+    """Rows with weights of about 2^-r whose V is 2^(r + 3) larger make up the output."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = uneven(50, n, nh, nkv, hd, pos0)
+    light = torch.zeros(pos0 + n, dtype=torch.bool, device="cuda")
+    light[64:192] = True
+    light[200:230:3] = True
+    v[light] *= 2.0 ** (r + 3)
+    k[light, :, 0] = -r * 0.6931
+    up = make_tree("random", n, 51)
+    out = run_tree(gpu, q, k, v, up, pos0, 1.0, 0)
+    check_rows(out, q, k, v, up, pos0, 1.0, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("size", [0.0, 1e-30, 2.0**-20])
+def test_tree_weight_on_rows_of_little_v(gpu, form, size):
+    """A row takes nearly all weight and has a V of zero or next to it: the others' 2^-30 make the output."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = uneven(60, n, nh, nkv, hd, pos0)
+    sink = torch.zeros(pos0 + n, dtype=torch.bool, device="cuda")
+    sink[3] = sink[131] = True
+    v[sink] *= size
+    k[sink, :, 0] = 20.8
+    up = make_tree("random", n, 61)
+    out = run_tree(gpu, q, k, v, up, pos0, 1.0, 0)
+    check_rows(out, q, k, v, up, pos0, 1.0, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("lowest,highest", [(-100, 100), (-30, 30), (-6, 6)])
+def test_tree_v_rows_of_any_size(gpu, form, lowest, highest):
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = uneven(70, n, nh, nkv, hd, pos0)
+    v *= 2.0 ** torch.randint(lowest, highest + 1, (pos0 + n, nkv, 1), device="cuda", generator=gen(73))
+    k[..., 0] = torch.rand(pos0 + n, nkv, device="cuda", generator=gen(74)) * -30
+    up = make_tree("random", n, 71)
+    out = run_tree(gpu, q, k, v, up, pos0, 1.0, 0)
+    check_rows(out, q, k, v, up, pos0, 1.0, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("share", [0.3, 0.9, 0.99])
+def test_tree_sparse_v(gpu, form, share):
+    """Many zeros in V, so that some threads see none but small values of a row that is not small (or is zero)."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = uneven(80, n, nh, nkv, hd, pos0)
+    v[torch.rand(v.shape, device="cuda", generator=gen(83)) < share] = 0
+    up = make_tree("random", n, 81)
+    out = run_tree(gpu, q, k, v, up, pos0, 1.0, 0)
+    check_rows(out, q, k, v, up, pos0, 1.0, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+    for _ in range(20):
+        assert torch.equal(out, run_tree(gpu, q, k, v, up, pos0, 1.0, 0))
