@@ -8,10 +8,10 @@
 // where that is more), and a b is the sum of the products hi hi, lo hi and
 // hi lo, each exact in the fp32 accumulator; lo lo (2^-22 of the product) is
 // left out.  bf16 pairs would keep 16 bits, a tf32 pair costs twice the tensor
-// time.  Groups: a query row; 8 cache rows of K; 8 cache rows of V (4 rows each
-// for head sizes above 128), of which a row below 2^-8 of the largest is a group
-// of its own (so 2^-28 of a row's largest value are kept at least).  The weights
-// are split in a unit that goes by the largest weight times V of the tile.
+// time.  Groups: a query row; 8 cache rows of K or V (4 for head sizes above 128), of
+// which a row below 2^-8 of the largest is a group of its own (so 2^-28 of a row's
+// largest value are kept at least).  The weights are split in a unit that goes by the
+// largest weight times V of the tile.
 //
 // One CTA takes up to 256 query rows of one KV head as two lanes A and B of
 // 128 and walks its split of the cache in tiles of 64 rows, each K and V row
@@ -20,8 +20,9 @@
 // their sums at the end:
 //   * loader warps 8-11 bring chunks of 8 rows in with cp.async (four in flight per
 //     warp, 64 KB per SM), split them and write the K-major operand tiles;
-//   * warp 13 gives V's small rows their scales, in the chunks whose loader found a
-//     thread without a large value in one of its rows (hardly any of ordinary data);
+//   * warps 13 and 14 give K's and V's small rows their scales, in the chunks whose
+//     loader found a thread without a large value in one of its rows (hardly any of
+//     ordinary data);
 //   * warp 12, one thread, issues S = Q K^T (Q pairs stay in TMEM) and, once a
 //     lane's weights are in TMEM over its scores, O = P V into the shared O
 //     columns, so one lane's softmax runs under the other's products;
@@ -53,14 +54,15 @@
 namespace gncx {
 
 constexpr int kTtThreads = 512;
-constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12, kTtSizeWarp = 13;
+constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12, kTtSizeWarp = 13;  // and 14
 // Registers per thread: softmax, loaders, products (whose warpgroup is filled
-// up by idle warps); together at most the 512 x 128 that the block is launched
-// with.  With 184 for head size 256 the softmax spills in its loop: 346 us instead
-// of 193 (16 heads, 4 KV heads, 64 nodes, 32768 rows).
+// up by the warps of the rows' scales); together at most the 512 x 128 that the block
+// is launched with.  Head size 256 (16 heads, 4 KV heads, 64 nodes, 32768 rows): 156.9
+// us, with 192, 96 and 32 164.5, with 192, 104 and 24 165.9.  32 heads, 8 KV heads of
+// 128, 16 nodes, 32768 rows: 75.7 us, with 176, 120 and 40 78.0.
 template <int HD>
 struct TtRegs {
-    static constexpr int kSoftmax = HD > 128 ? 192 : 176, kLoad = HD > 128 ? 96 : 112, kMma = HD > 128 ? 32 : 48;
+    static constexpr int kSoftmax = HD > 128 ? 184 : 176, kLoad = HD > 128 ? 104 : 112, kMma = HD > 128 ? 40 : 48;
     static_assert(2 * kSoftmax + kLoad + kMma <= 4 * 128, "a split that can be had");
 };
 constexpr int kTtStages = 2;              // K and V operand tiles
@@ -72,7 +74,7 @@ constexpr int kTtScales = 4;              // tiles whose scales are kept
 // nothing of the rows that make up the tile's output, whatever the weights and
 // sizes of V's other rows are: what is below 2^-30 of the largest weight times V is cut.
 constexpr int kTtHead = 4, kTtTop = 14;
-// A V row whose largest value is below kTtSmall in its chunk's scale has a scale of
+// A row whose largest value is below kTtSmall in its chunk's scale has a scale of
 // its own.  It is looked for where a value of a lane is 2^-kTtSpan of the chunk's largest.
 constexpr float kTtSmall = 8.0f;
 constexpr int kTtSpan = 8;
@@ -100,9 +102,11 @@ struct TtLayout {
     static constexpr int kChunk = kRows * HD * 4;
     static constexpr int oStaging = kTtStages * kStage;
     static constexpr int oScale = oStaging + 16 * kChunk;     // int [kTtScales][2][8]
-    static constexpr int oRows = oScale + kTtScales * 2 * 8 * 4;  // of V's rows, in flagged tiles: int [kTtScales][kKeys], and whether they differ [kTtScales]
-    static constexpr int oBar = oRows + kTtScales * (kKeys + 1) * 4;
-    static constexpr int kBars = 5 * kTtStages + 2 + 6 + 2;
+    // of the rows, in flagged tiles: int [kTtScales][2][kKeys]; whether any differs from its chunk's: [kTtScales][2]
+    static constexpr int oRows = oScale + kTtScales * 2 * 8 * 4;
+    static constexpr int oDiffer = oRows + kTtScales * 2 * kKeys * 4;
+    static constexpr int oBar = oDiffer + kTtScales * 2 * 4;
+    static constexpr int kBars = 6 * kTtStages + 2 + 6 + 2;
     static constexpr int oState = oBar + kBars * 8;    // what the lanes tell each other of each row: float [2][128]
     static constexpr int oTurn = oState + 2 * 128 * 4;  // per softmax warp: 16 columns of its 32 rows of Q
     static constexpr int kTurn = 32 * 20 * 4;
@@ -186,13 +190,15 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     constexpr int HO = WIDE ? 128 : HD;  // columns of a lane's output
     constexpr bool kShared = ALT || WIDE;  // both lanes on the same rows, S of tile t in block t & 1
     extern __shared__ __align__(128) uint8_t sm[];
-    int* scales = reinterpret_cast<int*>(sm + L::oScale);  // of the chunks; | 1: V's rows may differ
+    int* scales = reinterpret_cast<int*>(sm + L::oScale);  // of the chunks; | 1: the rows may differ
     int* row_scales = reinterpret_cast<int*>(sm + L::oRows);
+    int* rows_differ = reinterpret_cast<int*>(sm + L::oDiffer);
     uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + L::oBar);
     uint64_t* kempty = kfull + kTtStages;
     uint64_t* vfull = kempty + kTtStages;
     uint64_t* vempty = vfull + kTtStages;
-    uint64_t* vsized = vempty + kTtStages;  // V's small rows have scales of their own
+    uint64_t* ksized = vempty + kTtStages;  // small rows have scales of their own
+    uint64_t* vsized = ksized + kTtStages;
     uint64_t* sfull = vsized + kTtStages;  // [lane]
     uint64_t* pfull = sfull + 2;
     uint64_t* ofull = pfull + 2;
@@ -222,6 +228,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             mbar_init(&kempty[i], 1);
             mbar_init(&vfull[i], 4);
             mbar_init(&vempty[i], 1);
+            mbar_init(&ksized[i], 1);
             mbar_init(&vsized[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -311,7 +318,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             constexpr int kAhead = ALT ? 2 : 1;  // the next tile into the same S
             bool ok = wait_warp(qfull, 0);
             for (int t = 0; ok && t < min(kAhead, n_tiles); ++t) {
-                ok = wait_warp(&kfull[t], 0);
+                ok = wait_warp(&ksized[t], 0);
                 if (!ok) break;
                 tc_fence_after();
                 for (int x = 0; x < (kShared ? 1 : nl); ++x) scores(kShared ? t : x, t);
@@ -330,7 +337,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     if (i == nl - 1) commit(&vempty[t & 1]);
                     const int t2 = t + kAhead;
                     if (t2 < n_tiles && !(WIDE && i == 1)) {  // WIDE: lane 1 was through with tile t2 - 2 before oempty
-                        if (i == 0) ok = wait_warp(&kfull[t2 & 1], (t2 >> 1) & 1);
+                        if (i == 0) ok = wait_warp(&ksized[t2 & 1], (t2 >> 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
                         scores(WIDE ? t2 & 1 : x, t2);
@@ -339,16 +346,18 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 }
             commit(done);  // nothing of this CTA's is in flight when TMEM is freed
             if (!mbar_wait(done, 0)) record_error(a.err, kErrTimeout);
-        } else if (warp == kTtSizeWarp) {
-            // ---------------- small rows of V get scales of their own, in the chunks that are flagged ----------------
-            for (int t = 0; t < n_tiles && wait_warp(&vfull[t & 1], (t >> 1) & 1); ++t) {
-                const int* sv = scales + (t & (kTtScales - 1)) * 16 + 8;
-                const unsigned flags = __ballot_sync(0xffffffffu, lane < 8 && (sv[lane & 7] & 1));
+        } else if (warp <= kTtSizeWarp + 1) {
+            // ---------------- small rows of K, of V get scales of their own, in the chunks that are flagged ----------------
+            const int kind = warp - kTtSizeWarp;  // 0: K, 1: V
+            for (int t = 0; t < n_tiles && wait_warp(kind ? &vfull[t & 1] : &kfull[t & 1], (t >> 1) & 1); ++t) {
+                const int slot = 2 * (t & (kTtScales - 1)) + kind;
+                const int* words = scales + 8 * slot;
+                const unsigned flags = __ballot_sync(0xffffffffu, lane < 8 && (words[lane & 7] & 1));
                 if (flags) {
-                    int* row_v = row_scales + (t & (kTtScales - 1)) * KEYS;
-                    for (int j = lane; j < KEYS; j += 32) row_v[j] = sv[j / CR] & ~1;
+                    int* of_row = row_scales + slot * KEYS;
+                    for (int j = lane; j < KEYS; j += 32) of_row[j] = words[j / CR] & ~1;
                     __syncwarp();
-                    uint8_t* tile = sm + (t & 1) * L::kStage + 2 * L::kPart;
+                    uint8_t* tile = sm + (t & 1) * L::kStage + 2 * kind * L::kPart;
                     const int valid = j1 - j0 - KEYS * t;
                     bool apart = false;
 #pragma unroll 1
@@ -367,7 +376,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
 #pragma unroll 1
                         for (int r = 0; r < CR; ++r) {
                             if (larges >> r * G & ((1u << G) - 1)) continue;
-                            const float* g = a.vc + ((size_t)(j0 + KEYS * t + CR * c + r) * a.n_kv + kvh) * a.hd;
+                            const float* g = (kind ? a.vc : a.kc) + ((size_t)(j0 + KEYS * t + CR * c + r) * a.n_kv + kvh) * a.hd;
                             auto value = [&](int d) {
                                 const float y = d < a.hd ? g[d] : 0.0f;
                                 return fabsf(y) == INFINITY ? 0.0f : y;
@@ -384,15 +393,15 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                                 to[0] = h;
                                 to[L::kPart / 2] = __float2half_rn(y - __half2float(h));
                             }
-                            if (lane == 0) row_v[CR * c + r] = s;
+                            if (lane == 0) of_row[CR * c + r] = s;
                             apart = true;
                         }
                     }
-                    if (lane == 0) row_scales[kTtScales * KEYS + (t & (kTtScales - 1))] = apart;
+                    if (lane == 0) rows_differ[slot] = apart;
                     fence_async_smem();
                     __syncwarp();
                 }
-                if (lane == 0) mbar_arrive(&vsized[t & 1]);
+                if (lane == 0) mbar_arrive(kind ? &vsized[t & 1] : &ksized[t & 1]);
             }
         }
     } else if (warp >= kTtLoadWarp) {
@@ -466,7 +475,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 }
                 // rows that may be much smaller than the largest one (or not there): in most chunks each lane sees
                 // in each of its rows a value that is not small, and one vote tells
-                const bool apart = i >= 2 && __any_sync(0xffffffffu, __float_as_uint(least) + (kTtSpan << 23) < top);
+                const bool apart = __any_sync(0xffffffffu, __float_as_uint(least) + (kTtSpan << 23) < top);
                 if (lane == 0) sc[8 * (i >> 1) + chunk] = s | (int)apart;
                 if (i & 1) {
                     fence_async_smem();
@@ -575,31 +584,35 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 tc_fence_after();
                 const int4* sc = reinterpret_cast<const int4*>(scales + (t & (kTtScales - 1)) * 16);
                 const int valid = j1 - j0 - KEYS * t;
-                const int4 k0 = sc[0], k1 = sc[1];
                 // 2^(-sq - sk) may need two factors
                 auto factor = [&](int sk) {
                     const int n = -sq - sk, h = n >> 1;
                     return a.scale2 * pow2i(h) * pow2i(n - h);
                 };
+                // The words are not written again before this warp is through with the tile, so that its
+                // threads agree; the rows' own scales are there with the scores (K), with vsized (V).
+                const int* sk = reinterpret_cast<const int*>(sc);
                 auto differ = [](const int4& p, const int4& q) {
                     const int c = p.x;
                     return ((p.y ^ c) | (p.z ^ c)) | ((p.w ^ c) | (q.x ^ c)) | ((q.y ^ c) | (q.z ^ c)) | (q.w ^ c);
                 };
-                const bool even_k = differ(k0, k1) == 0;
-                int V = 0, flagged = 0;
-                bool even_v = false;
-                // The words are not written again before this warp is through with the tile, so that its
-                // threads agree.
+                auto flagged = [&](int kind) {
+                    const int4 p = sc[2 * kind], q = sc[2 * kind + 1];
+                    return (((p.x | p.y) | (p.z | p.w) | (q.x | q.y) | (q.z | q.w)) & 1) != 0;
+                };
+                auto apart = [&](int kind) { return flagged(kind) && rows_differ[2 * (t & (kTtScales - 1)) + kind]; };
+                const int4 k0 = sc[0], k1 = sc[1];
+                const bool even_k = (differ(k0, k1) | (k0.x & 1)) == 0;
+                constexpr int kUneven = 1 << 20;
+                int V = kUneven;  // the scale of all of V's rows
                 auto look = [&] {
                     const int4 v0 = sc[2], v1 = sc[3];
-                    V = v0.x & ~1;
-                    flagged = ((v0.x | v0.y) | (v0.z | v0.w) | (v1.x | v1.y) | (v1.z | v1.w)) & 1;
-                    even_v = (differ(v0, v1) & ~1) == 0;
+                    if ((differ(v0, v1) | (v0.x & 1)) == 0) V = v0.x;
                 };
                 if (v_in) look();
-                const float f0 = factor(k0.x);
+                const float f0 = factor(k0.x & ~1);
                 float tm = -INFINITY;
-                if (even_k && valid >= KEYS && f0 >= 0.0f) {
+                if (even_k && f0 >= 0.0f) {  // behind the last row it is there again
 #pragma unroll 1
                     for (int h = 0; h < KEYS / 32; ++h) {
                         float s[32];
@@ -608,15 +621,23 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                         for (int j = 0; j < 32; j += 2) tm = fmaxf(tm, fmaxf(s[j], s[j + 1]));
                     }
                     tm *= f0;
+                } else if (apart(0)) {
+                    const int* of_row = row_scales + 2 * (t & (kTtScales - 1)) * KEYS;
+#pragma unroll 1
+                    for (int b = 0; b < min(KEYS, valid); b += 4) {
+                        float s[4];
+                        tmem_ld4f(ts + b, s);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) tm = fmaxf(tm, s[j] * factor(of_row[b + j]));
+                    }
                 } else {
 #pragma unroll 1
                     for (int b = 0; b < KEYS / 16; ++b) {
                         float s[16];
                         tmem_ld16f(ts + 16 * b, s);
-                        const int* sk = reinterpret_cast<const int*>(sc) + 16 / CR * b;
                         float f[16 / CR];
 #pragma unroll
-                        for (int i = 0; i < 16 / CR; ++i) f[i] = factor(sk[i]);
+                        for (int i = 0; i < 16 / CR; ++i) f[i] = factor(sk[16 / CR * b + i] & ~1);
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
                             if (16 * b + j < valid) tm = fmaxf(tm, s[j] * f[j / CR]);
@@ -635,16 +656,16 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     if (!ok) break;
                     look();
                 }
-                if (flagged) {
+                if (V == kUneven && flagged(1)) {
                     ok = wait_warp(&vsized[t & 1], (t >> 1) & 1);
                     if (!ok) break;
-                    even_v = even_v && !row_scales[kTtScales * KEYS + (t & (kTtScales - 1))];
+                    if ((differ(sc[2], sc[3]) & ~1) == 0 && !apart(1)) V = sc[2].x & ~1;
                 }
-                // The unit 2^-n.  With one scale 2^V for all of V's rows the weights are taken
+                // The unit 2^-n.  With one scale 2^V for all of V's rows (and K's by chunks) the weights are taken
                 // times 2^m, m = n - V; else each times 2^(n - its row's scale).
                 float back = 1.0f;  // 2^-m
                 f32x2 sum = 0;
-                if (even_v) {
+                if (V != kUneven && (even_k || !apart(0))) {
                     // a whole number by rounding in the last place of 1.5 * 2^23; at most what 2^-m and 2^-n can be
                     const float magic = 12582912.0f;
                     const int zero = __float_as_int(magic), r = min(__float_as_int(fmaxf((float)kTtTop + ref - tm, 0.0f) + magic), zero + 126 - max(V, 0));
@@ -674,33 +695,35 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                             float s[16];
                             uint32_t p[16];
                             tmem_ld16f(ts + 16 * b, s);
-                            const int* sk = reinterpret_cast<const int*>(sc) + 16 / CR * b;
                             float f[16 / CR];
 #pragma unroll
-                            for (int i = 0; i < 16 / CR; ++i) f[i] = factor(sk[i]);
+                            for (int i = 0; i < 16 / CR; ++i) f[i] = factor(sk[16 / CR * b + i] & ~1);
 #pragma unroll
                             for (int j = 0; j < 16; j += 2) {
-                                const float c = f[j / CR];
-                                const float e0 = 16 * b + j < valid ? ex2(fmaf(s[j], c, shift)) : 0.0f;
-                                const float e1 = 16 * b + j + 1 < valid ? ex2(fmaf(s[j + 1], c, shift)) : 0.0f;
-                                sum = add2(sum, pack2(e0, e1));
-                                split2(pack2(e0, e1), p[j / 2], p[8 + j / 2]);
+                                float e[2] = {0.0f, 0.0f};
+#pragma unroll
+                                for (int y = j; y < j + 2; ++y)
+                                    if (16 * b + y < valid)
+                                        e[y - j] = ex2(fmaf(s[y], f[j / CR], shift));
+                                const f32x2 e2 = pack2(e[0], e[1]);
+                                sum = add2(sum, e2);
+                                split2(e2, p[j / 2], p[8 + j / 2]);
                             }
                             tmem_st16(tp + 16 * b, p);
                         }
                     }
                 } else {
-                    const int* sk = reinterpret_cast<const int*>(sc);
-                    const int* row_v = row_scales + (t & (kTtScales - 1)) * KEYS;
-                    auto scale_v = [&](int j) { return (float)(flagged ? row_v[j] : sk[8 + j / CR]); };
+                    const int* of_row = row_scales + 2 * (t & (kTtScales - 1)) * KEYS;
+                    const bool own_k = flagged(0), own_v = flagged(1);
+                    auto scale_k = [&](int j) { return own_k ? of_row[j] : sk[j / CR]; };
+                    auto scale_v = [&](int j) { return (float)(own_v ? of_row[KEYS + j] : sk[8 + j / CR]); };
                     float most = -INFINITY;  // exponent of the largest weight times V, in V's units
 #pragma unroll 1
-                    for (int b = 0; b < KEYS; b += 16) {
-                        float s[16];
-                        tmem_ld16f(ts + b, s);
+                    for (int b = 0; b < min(KEYS, valid); b += 4) {  // behind the last row it is there again
+                        float s[4];
+                        tmem_ld4f(ts + b, s);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (b + j < valid) most = fmaxf(most, s[j] * factor(sk[(b + j) / CR]) - scale_v(b + j));
+                        for (int j = 0; j < 4; ++j) most = fmaxf(most, s[j] * factor(scale_k(b + j)) - scale_v(b + j));
                     }
                     const float n = floorf(fminf(fmaxf((float)kTtTop + ref - most, -126.0f), 126.0f));
                     beta = pow2i(-(int)n);
@@ -716,7 +739,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
 #pragma unroll
                                 for (int y = j; y < j + 2; ++y)
                                     if (b + y < valid) {
-                                        const float z = fmaf(s[y], factor(sk[(b + y) / CR]), -ref);
+                                        const float z = fmaf(s[y], factor(scale_k(b + y)), -ref);
                                         e[y - j] = ex2(z);
                                         w[y - j] = ex2(z + (n - scale_v(b + y)));
                                     }

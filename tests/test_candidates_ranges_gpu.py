@@ -230,3 +230,49 @@ def test_tree_sparse_v(gpu, form, share):
     check_rows(out, q, k, v, up, pos0, 1.0, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
     for _ in range(20):
         assert torch.equal(out, run_tree(gpu, q, k, v, up, pos0, 1.0, 0))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("r", [6, 13, 18, 22, 26, 30, 40])
+def test_tree_large_rows_do_not_blur_k(gpu, form, r):
+    """Rows of K 2^r larger than their neighbours, which get no weight: the others' scores keep their bits."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = uneven(90, n, nh, nkv, hd, pos0)
+    large = torch.arange(pos0 + n, device="cuda") % 8 == 3
+    large[96:104] = True
+    k[large] = 0
+    k[large, :, 0] = -(2.0**r) * 0.4  # q's first column is 1: a score of -2^r and lower
+    k[large, :, 1] = 2.0**r * 0.2
+    q[..., 1] = 0.25
+    up = make_tree("random", n, 91)
+    for row in (11, 99):
+        k[row, :, 0] = -(2.0**5)
+        k[row, :, 1] = 0
+    out = run_tree(gpu, q, k, v, up, pos0, 1.0, 0)
+    check_rows(out, q, k, v, up, pos0, 1.0, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("lowest,highest", [(-60, 0), (-20, 2), (-6, 3)])
+def test_tree_k_and_v_rows_of_any_size(gpu, form, lowest, highest):
+    """Rows of K and V of any size next to each other; each row's own sum |q k| bounds its score's error."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = randn(95, n, nh, hd), randn(96, pos0 + n, nkv, hd), randn(97, pos0 + n, nkv, hd)
+    k *= 2.0 ** torch.randint(lowest, highest + 1, (pos0 + n, nkv, 1), device="cuda", generator=gen(98))
+    v *= 2.0 ** torch.randint(3 * lowest // 2, highest + 1, (pos0 + n, nkv, 1), device="cuda", generator=gen(99))
+    up = make_tree("random", n, 93)
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0)
+    check_rows(out, q, k, v, up, pos0, hd**-0.5, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("share", [0.3, 0.9, 0.99])
+def test_tree_sparse_k(gpu, form, share):
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = randn(100, n, nh, hd), randn(101, pos0 + n, nkv, hd), randn(102, pos0 + n, nkv, hd)
+    k[torch.rand(k.shape, device="cuda", generator=gen(103)) < share] = 0
+    up = make_tree("random", n, 94)
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0)
+    check_rows(out, q, k, v, up, pos0, hd**-0.5, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+    for _ in range(20):
+        assert torch.equal(out, run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0))

@@ -34,7 +34,7 @@ def roles(form, n_tiles, sized, own_weights=True, both_arrive=True):
     of_scores = (lambda t: (t >> 1) & 1) if shared else (lambda t: t & 1)
     products = []
     for t in range(min(ahead, n_tiles)):
-        products.append(("wait", f"k{t}", 0))
+        products.append(("wait", f"k{t} sized", 0))
         products += [("commit", f"s{t if shared else x}") for x in range(1 if shared else halves)]
         products.append(("commit", f"k{t} free"))
     outputs = 0
@@ -49,17 +49,17 @@ def roles(form, n_tiles, sized, own_weights=True, both_arrive=True):
             then = t + ahead
             if then < n_tiles and not (wide and i == 1):
                 if i == 0:
-                    products.append(("wait", f"k{then & 1}", (then >> 1) & 1))
+                    products.append(("wait", f"k{then & 1} sized", (then >> 1) & 1))
                 products.append(("commit", f"s{then & 1 if wide else x}"))
                 if wide or i == halves - 1:
                     products.append(("commit", f"k{then & 1} free"))
-    loads, sizes = [], []
+    loads, sizes = [], {"k": [], "v": []}
     for t in range(n_tiles):
         for kind in "kv":
             if t >= 2:
                 loads.append(("wait", f"{kind}{t & 1} free", ((t >> 1) - 1) & 1))
             loads.append(("arrive", f"{kind}{t & 1}"))
-        sizes += [("wait", f"v{t & 1}", (t >> 1) & 1), ("arrive", f"v{t & 1} sized")]
+            sizes[kind] += [("wait", f"{kind}{t & 1}", (t >> 1) & 1), ("arrive", f"{kind}{t & 1} sized")]
     lanes = []
     for x in range(2 if shared or halves == 2 else 1):
         for has_rows in (True, False):
@@ -74,7 +74,7 @@ def roles(form, n_tiles, sized, own_weights=True, both_arrive=True):
                     lane.append(("arrive", f"p{x}"))
                 lane += [("wait", f"o{x}", of_lane(t)), ("arrive", "o free")]
             lanes.append(lane)
-    return [products, loads, sizes, *lanes], {"p0": 2, "p1": 2, "o free": 2}
+    return [products, loads, *sizes.values(), *lanes], {"p0": 2, "p1": 2, "o free": 2}
 
 
 def held(model):
@@ -113,10 +113,10 @@ def held(model):
 
 
 @pytest.mark.parametrize("form", ["one lane", "two lanes", "alternating lanes", "columns above 128"])
-@pytest.mark.parametrize("n_tiles,sized", [(1, ()), (2, (1,)), (4, ()), (4, (0, 1, 2, 3)), (5, (1, 4))])
+@pytest.mark.parametrize("n_tiles,sized", [(1, ()), (2, (1,)), (4, (0, 1, 2, 3)), (4, (1, 2))])
 def test_no_order_of_the_roles_holds_one(form, n_tiles, sized):
     assert held(roles(form, n_tiles, sized, *kernel_order())) == []
 
 
 def test_the_model_sees_an_overtaken_wait():
-    assert held(roles("columns above 128", 5, (), False, False)) != []
+    assert held(roles("columns above 128", 4, (), False, False)) != []
