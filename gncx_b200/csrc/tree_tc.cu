@@ -57,14 +57,11 @@ constexpr int kTtThreads = 512;
 constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12, kTtSizeWarp = 13;  // and 14
 // Registers per thread: softmax, loaders, products (whose warpgroup is filled
 // up by the warps of the rows' scales); together at most the 512 x 128 that the block
-// is launched with.  Head size 256 (16 heads, 4 KV heads, 64 nodes, 32768 rows): 156.9
-// us, with 192, 96 and 32 164.5, with 192, 104 and 24 165.9.  32 heads, 8 KV heads of
-// 128, 16 nodes, 32768 rows: 75.7 us, with 176, 120 and 40 78.0.
-template <int HD>
-struct TtRegs {
-    static constexpr int kSoftmax = HD > 128 ? 184 : 176, kLoad = HD > 128 ? 104 : 112, kMma = HD > 128 ? 40 : 48;
-    static_assert(2 * kSoftmax + kLoad + kMma <= 4 * 128, "a split that can be had");
-};
+// is launched with.  32 heads, 8 KV heads of 128, 16 nodes, 32768 rows: 75.7 us, with
+// 176, 120 and 40 78.0.  16 heads, 4 KV heads of 256, 64 nodes, 32768 rows: 163.9 us,
+// with 184, 104 and 40 167.6, with 192, 96 and 32 178.3.
+constexpr int kTtSoftmaxRegs = 176, kTtLoadRegs = 112, kTtMmaRegs = 48;
+static_assert(2 * kTtSoftmaxRegs + kTtLoadRegs + kTtMmaRegs <= 4 * 128, "a split that can be had");
 constexpr int kTtStages = 2;              // K and V operand tiles
 constexpr int kTtScales = 4;              // tiles whose scales are kept
 // Weights are 2^(score - reference), with the score at most kTtHead above the
@@ -271,7 +268,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     };
 
     if (warp >= kTtMmaWarp) {
-        regs_dec<TtRegs<HD>::kMma>();
+        regs_dec<kTtMmaRegs>();
         if (warp == kTtMmaWarp) {
             // ---------------- products: the warp waits, one thread issues ----------------
             constexpr uint32_t idesc_s = umma_idesc_f16(128, KEYS), idesc_o = umma_idesc_f16(128, HO) | kUmmaTransB;
@@ -406,7 +403,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         }
     } else if (warp >= kTtLoadWarp) {
         // ---------------- loaders: warp w takes two of the eight chunks of rows of each tile ----------------
-        regs_dec<TtRegs<HD>::kLoad>();
+        regs_dec<kTtLoadRegs>();
         const int lw = warp - kTtLoadWarp;
         const size_t pstride = (size_t)a.n_kv * a.hd;
         const float* src[2] = {a.kc + (size_t)kvh * a.hd, a.vc + (size_t)kvh * a.hd};
@@ -487,7 +484,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if ((warp >> 2) < nl || kShared) {
         // ---------------- softmax and output: a thread per query row (and lane) ----------------
-        regs_inc<TtRegs<HD>::kSoftmax>();
+        regs_inc<kTtSoftmaxRegs>();
         const int x = warp >> 2;
         const int first = r0 + (kShared ? 0 : 128 * x) + 32 * (warp & 3), row = first + lane;
         const bool active = first < rows;  // of the warp
@@ -564,6 +561,9 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         tc_fence_before();
         if (x == 0 || !ALT) mbar_arrive(qfull);
 
+        // The least scale of K with scores of up to 2^22 (the products' sum is 2^38 at most): beyond, the rounding
+        // of one takes its distance from the reference out of fp16's range where that is not taken last.
+        const int tame = 16 + (int)(__float_as_uint(fabsf(a.scale2)) >> 23) - 126 - __reduce_min_sync(0xffffffffu, sq);
         float T = -INFINITY, l = 0.0f;
         f32x2 o[HO / 2];
 #pragma unroll
@@ -602,7 +602,6 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 };
                 auto apart = [&](int kind) { return flagged(kind) && rows_differ[2 * (t & (kTtScales - 1)) + kind]; };
                 const int4 k0 = sc[0], k1 = sc[1];
-                const bool even_k = (differ(k0, k1) | (k0.x & 1)) == 0;
                 constexpr int kUneven = 1 << 20;
                 int V = kUneven;  // the scale of all of V's rows
                 auto look = [&] {
@@ -611,6 +610,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 };
                 if (v_in) look();
                 const float f0 = factor(k0.x & ~1);
+                const bool even_k = (differ(k0, k1) | (k0.x & 1)) == 0 && k0.x >= tame;
                 float tm = -INFINITY;
                 if (even_k && f0 >= 0.0f) {  // behind the last row it is there again
 #pragma unroll 1
@@ -665,10 +665,16 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                 // times 2^m, m = n - V; else each times 2^(n - its row's scale).
                 float back = 1.0f;  // 2^-m
                 f32x2 sum = 0;
-                if (V != kUneven && (even_k || !apart(0))) {
+                auto all_tame = [&] {
+                    int least = sk[0];
+#pragma unroll 1
+                    for (int c = 1; c < 8; ++c) least = min(least, sk[c]);
+                    return least >= tame;
+                };
+                if (V != kUneven && (even_k || (!apart(0) && all_tame()))) {
                     // a whole number by rounding in the last place of 1.5 * 2^23; at most what 2^-m and 2^-n can be
                     const float magic = 12582912.0f;
-                    const int zero = __float_as_int(magic), r = min(__float_as_int(fmaxf((float)kTtTop + ref - tm, 0.0f) + magic), zero + 126 - max(V, 0));
+                    const int zero = __float_as_int(magic), r = min(__float_as_int(fmaxf((float)kTtTop + (ref - tm), 0.0f) + magic), zero + 126 - max(V, 0));
                     const int m = r - zero;
                     const float shift = (__int_as_float(r) - magic) - ref;
                     back = pow2i(-m);
@@ -717,15 +723,15 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     const bool own_k = flagged(0), own_v = flagged(1);
                     auto scale_k = [&](int j) { return own_k ? of_row[j] : sk[j / CR]; };
                     auto scale_v = [&](int j) { return (float)(own_v ? of_row[KEYS + j] : sk[8 + j / CR]); };
-                    float most = -INFINITY;  // exponent of the largest weight times V, in V's units
+                    float most = -INFINITY;  // exponent of the largest weight times V
 #pragma unroll 1
                     for (int b = 0; b < min(KEYS, valid); b += 4) {  // behind the last row it is there again
                         float s[4];
                         tmem_ld4f(ts + b, s);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) most = fmaxf(most, s[j] * factor(scale_k(b + j)) - scale_v(b + j));
+                        for (int j = 0; j < 4; ++j) most = fmaxf(most, (__fmul_rn(s[j], factor(scale_k(b + j))) - ref) - scale_v(b + j));
                     }
-                    const float n = floorf(fminf(fmaxf((float)kTtTop + ref - most, -126.0f), 126.0f));
+                    const float n = floorf(fminf(fmaxf((float)kTtTop - most, -126.0f), 126.0f));
                     beta = pow2i(-(int)n);
                     if (writes)
 #pragma unroll 1
@@ -739,7 +745,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
 #pragma unroll
                                 for (int y = j; y < j + 2; ++y)
                                     if (b + y < valid) {
-                                        const float z = fmaf(s[y], factor(scale_k(b + y)), -ref);
+                                        const float z = __fmul_rn(s[y], factor(scale_k(b + y))) - ref;
                                         e[y - j] = ex2(z);
                                         w[y - j] = ex2(z + (n - scale_v(b + y)));
                                     }

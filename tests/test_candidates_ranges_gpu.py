@@ -276,3 +276,26 @@ def test_tree_sparse_k(gpu, form, share):
     check_rows(out, q, k, v, up, pos0, hd**-0.5, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
     for _ in range(20):
         assert torch.equal(out, run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 1e12, 1e20, -1e9])
+def test_tree_scores_of_any_size(gpu, form, size):
+    """One row's score is far above the others', all of them beyond what fp32 resolves to one: its V comes out.
+
+    With one weight of 1, off by 2^-22 as a pair and a few roundings, the output is off by 8 u; and by what the pairs cut
+    of V: a row's largest value is at least 2^3 in its scale (else it has a scale of its own), half a step of the lo part
+    is 2^-25, so 2^-28 of the row's largest value."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = uneven(110, n, nh, nkv, hd, pos0)
+    row = 137
+    k[row, :, 0] = 8.0
+    out = run_tree(gpu, q * size, k * (1 if size > 0 else -1), v, make_tree("random", n, 111), pos0, 1.0, 0)
+    want = v[row].repeat_interleave(nh // nkv, 0).expand_as(out)
+    assert bool(((out - want).abs() <= 8 * U * want.abs() + 2.0**-28 * want.abs().amax(-1, keepdim=True)).all())
+    # and small ones with a large scale, or V of any size
+    k *= 1e-3
+    v *= 2.0 ** torch.randint(-30, 30, (pos0 + n, nkv, 1), device="cuda", generator=gen(112))
+    out = run_tree(gpu, q, k, v, make_tree("random", n, 111), pos0, float(abs(size)) * 1e3, 0)
+    want = v[row].repeat_interleave(nh // nkv, 0).expand_as(out)
+    assert bool(((out - want).abs() <= 8 * U * want.abs() + 2.0**-28 * want.abs().amax(-1, keepdim=True)).all())
