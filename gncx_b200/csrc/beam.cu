@@ -916,6 +916,10 @@ static cudaError_t reorder_launch_v(ReorderArgs a, size_t n_bytes, cudaStream_t 
 int reorder_launch(void* state, int n_states, size_t state_stride, int n_slots, size_t slot_stride, size_t n_bytes,
                    const int32_t* index, int32_t* err, cudaStream_t st) {
     ReorderArgs a{static_cast<uint8_t*>(state), state_stride, slot_stride, 0, n_states, n_slots, index, err};
+    if (n_slots == 1) {  // nothing can move: one column of one state looks at the index
+        a.n_states = 1;
+        n_bytes = 4;
+    }
     const bool wide = (((uintptr_t)state | state_stride | slot_stride | n_bytes) & 15) == 0;
     const cudaError_t e = wide ? reorder_launch_v<uint4>(a, n_bytes, st) : reorder_launch_v<uint32_t>(a, n_bytes, st);
     return e == cudaSuccess ? kOk : kErrCuda;

@@ -1077,8 +1077,8 @@ int32_t gncx_state_reorder(void* state, int32_t n_states, size_t state_stride, i
     const bool by_slot = (n_states <= 1 || state_stride >= n_bytes) && slot_stride >= (size_t)(n_states - 1) * state_stride + n_bytes;
     bool capturing;
     GNCX_TRY(begin_call(fn, &capturing));
-    if (n_states == 0 || n_slots < 2 || n_bytes == 0) return finish(kOk);
-    if (!by_state && !by_slot) return refuse(kErrInvalidArg, fn, "the slots overlap");
+    if (n_states == 0 || n_slots == 0 || n_bytes == 0) return finish(kOk);
+    if (n_slots > 1 && !by_state && !by_slot) return refuse(kErrInvalidArg, fn, "the slots overlap");
     GNCX_TRY(check_buf(fn, state, "state", 4));
     GNCX_TRY(check_buf(fn, index, "index", 4));
     return finish(reorder_launch(state, n_states, state_stride, n_slots, slot_stride, n_bytes, index, g_rt.d_err, stream()));

@@ -5,8 +5,8 @@ test_candidates_gpu.py."""
 import numpy as np
 import pytest
 
-from test_candidates_gpu import (EVICTS, _clean, attend, check_tree, evict_weights, gen, make_tree, randn, run_evict, run_tree,  # noqa: F401
-                                 tree_seen)
+from test_candidates_gpu import (EVICTS, INVALID, P, _clean, attend, check_tree, evict_weights, gen, make_tree, ok, randn,  # noqa: F401
+                                 run_evict, run_tree, tree_path, tree_seen)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -299,3 +299,22 @@ def test_tree_scores_of_any_size(gpu, form, size):
     out = run_tree(gpu, q, k, v, make_tree("random", n, 111), pos0, float(abs(size)) * 1e3, 0)
     want = v[row].repeat_interleave(nh // nkv, 0).expand_as(out)
     assert bool(((out - want).abs() <= 8 * U * want.abs() + 2.0**-28 * want.abs().amax(-1, keepdim=True)).all())
+
+
+# ---------------------------------------------------------------- reordering
+def test_reorder_one_slot_looks_at_its_index(gpu):
+    x = randn(120, 3, 1, 64)
+    y = x.clone()
+    for i in (1, 5, -2, 2**31 - 1, -(2**31)):
+        index = torch.tensor([i], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        assert gpu.gncx_state_reorder(P(y), 3, 256, 1, 256, 256, P(index)) == INVALID, i
+        gpu.gncx_clear_error()
+    for i in (0, -1):
+        index = torch.tensor([i], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        ok(gpu, gpu.gncx_state_reorder(P(y), 3, 256, 1, 256, 256, P(index)))
+        ok(gpu, gpu.gncx_state_reorder(P(y), 3, 0, 1, 0, 256, P(index)))  # strides that no second slot or state uses
+    torch.cuda.synchronize()
+    assert torch.equal(x, y)
+    assert gpu.gncx_state_reorder(P(y), 3, 256, 1, 256, 256, None) == INVALID
