@@ -318,3 +318,88 @@ def test_reorder_one_slot_looks_at_its_index(gpu):
     torch.cuda.synchronize()
     assert torch.equal(x, y)
     assert gpu.gncx_state_reorder(P(y), 3, 256, 1, 256, 256, None) == INVALID
+
+
+# ---------------------------------------------------------------- forms that smaller shapes pass by
+def one_launch(nh, nkv, pos0, n, hd, window):
+    """Whether few query rows over a short cache go to the form of one launch (148 SMs)."""
+    rows, fit = n * nh // nkv, 15 // nkv
+    seen = pos0 + n - (max(0, pos0 - window + 1) if window else 0)
+    if n > 64:
+        return False
+    return seen <= (256 if hd > 128 else 768) if rows <= 8 * fit else rows <= 16 * fit and hd <= 128 and seen <= 384
+
+
+# Head sizes that are no multiple of 16: on the CUDA cores, with splits and records of their own.
+OTHER = [(2, 1, 4, 1000, 3, 0), (5, 5, 20, 900, 30, 0), (4, 2, 36, 300, 70, 50), (3, 3, 60, 64, 100, 0), (8, 4, 100, 1000, 9, 0), (6, 3, 132, 2000, 40, 0),
+         (12, 4, 136, 8192, 16, 0), (4, 1, 252, 1500, 70, 300), (148, 148, 20, 33, 65, 0), (8, 1, 100, 31, 200, 0), (2, 2, 132, 5001, 2, 4096),
+         (16, 2, 252, 32, 65, 7), (1, 1, 12, 70001, 1, 0)]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,pos0,n,window", OTHER)
+@pytest.mark.parametrize("kind", ["random", "chain", "star"])
+def test_tree_other_head_sizes(gpu, nh, nkv, hd, pos0, n, window, kind):
+    assert hd % 16 and not one_launch(nh, nkv, pos0, n, hd, window)
+    rows = pos0 + n
+    q, k, v = randn(130, n, nh, hd) * 2, randn(131, rows + 3, nkv, hd), randn(132, rows + 3, nkv, hd)
+    k[rows:], v[rows:] = float("nan"), float("nan")
+    lo = max(0, pos0 - window + 1) if window else 0
+    k[:min(lo, pos0)], v[:min(lo, pos0)] = float("nan"), float("inf")
+    up = make_tree(kind, n, pos0 + n + 2)
+    keep = k.clone(), v.clone()
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, window)
+    group = nh // nkv
+    for i in sorted({0, n // 2, n - 1}):
+        seen = torch.tensor(tree_seen(up, i, pos0, window), device="cuda")
+        for h in sorted({0, nh // 2, nh - 1}):
+            ref, tol, _, _ = attend(q[i, h], k[seen][:, h // group], v[seen][:, h // group], hd**-0.5)
+            assert bool(((out[i, h].double() - ref).abs() <= tol).all()), (i, h)
+    assert bool(out.isfinite().all())
+    assert torch.equal(out, run_tree(gpu, q, k, v, up, pos0, hd**-0.5, window))
+    assert torch.equal(k.view(torch.int32), keep[0].view(torch.int32)) and torch.equal(v.view(torch.int32), keep[1].view(torch.int32))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_tree_infinite_and_nan_rows_show_in_each_form(gpu, form):
+    """A NaN in a seen row reaches the outputs of its KV head, an infinity of V its column, and no other head's."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    group, up = nh // nkv, make_tree("random", n, 141)
+    for row in (0, 70, pos0 - 1):
+        q, k, v = randn(140, n, nh, hd), randn(141, pos0 + n, nkv, hd), randn(142, pos0 + n, nkv, hd)
+        k[row, 0, 5], v[row, 1, 7], v[row, 1, hd - 1] = float("nan"), float("inf"), float("-inf")
+        out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0).view(n, nkv, group, hd)
+        assert bool(out[:, 0].isnan().all())
+        assert bool((out[:, 1, :, 7] == float("inf")).all()) and bool((out[:, 1, :, hd - 1] == float("-inf")).all())
+        out[:, 0], out[:, 1, :, 7], out[:, 1, :, hd - 1] = 0, 0, 0
+        assert bool(out.isfinite().all())
+        v[row, 1] = float("nan")  # all of a row of V
+        out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0).view(n, nkv, group, hd)
+        assert bool(out[:, 1].isnan().all()) and bool(out[:, 2:].isfinite().all())
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if f != "one launch"])
+def test_tree_bad_parents_are_an_error_in_each_form(gpu, form):
+    nh, nkv, hd, pos0, n = FORMS[form]
+    pos0, n = max(pos0, 2000 // nkv), 4
+    assert not one_launch(nh, nkv, pos0, n, hd, 0)
+    q, k, v = randn(150, n, nh, hd), randn(151, pos0 + n, nkv, hd), randn(152, pos0 + n, nkv, hd)
+    out = torch.zeros_like(q)
+    for up in ([-1, 1, 0, 0], [-1, 0, 3, 0], [-1, 0, -2, 0], [5, 0, 0, 0], [-1, 0, 0, 2**31 - 1]):
+        parents = torch.tensor(up, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        st = gpu.gncx_attention_tree(P(q), P(k), P(v), P(parents), pos0, n, nh, nkv, hd, 0.1, 0, P(out), None, 0)
+        assert st == INVALID and gpu.gncx_last_error() == INVALID, up
+        gpu.gncx_clear_error()
+    ok(gpu, gpu.gncx_sync())
+    up = make_tree("random", n, 153)
+    check_tree(run_tree(gpu, q, k, v, up, pos0, 0.1, 0), q, k, v, up, pos0, 0.1, 0, [0, 3])
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_tree_other_branches_do_not_leak_in_each_form(gpu, form):
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = randn(160, n, nh, hd), randn(161, pos0 + n, nkv, hd), randn(162, pos0 + n, nkv, hd)
+    up = make_tree("random", n, 163)
+    k[pos0 + n - 1], v[pos0 + n - 1] = float("nan"), float("inf")  # no other node's ancestor
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0)
+    check_tree(out, q, k, v, up, pos0, hd**-0.5, 0, sorted({0, (n - 1) // 2, max(0, n - 2)}))
