@@ -2,16 +2,15 @@
 // tensor cores, with fp32 accuracy.
 //
 // Every fp32 operand x is used as a pair of fp16 values: with a power of two s
-// that brings the largest |x| of its group into [2^11, 2^15),
+// that brings the largest |x| of its row into [2^3, 2^15),
 //   hi = fp16(x s),  lo = fp16(x s - hi),
-// so that hi + lo keeps 22 bits of x (or 2^-36 of the group's largest value,
-// where that is more), and a b is the sum of the products hi hi, lo hi and
+// so that hi + lo keeps 22 bits of x (or 2^-25 / s, where that is more: at least 2^-28
+// of the row's largest value), and a b is the sum of the products hi hi, lo hi and
 // hi lo, each exact in the fp32 accumulator; lo lo (2^-22 of the product) is
 // left out.  bf16 pairs would keep 16 bits, a tf32 pair costs twice the tensor
-// time.  Groups: a query row; 8 cache rows of K or V (4 for head sizes above 128), of
-// which a row below 2^-8 of the largest is a group of its own (so 2^-28 of a row's
-// largest value are kept at least).  The weights are split in a unit that goes by the
-// largest weight times V of the tile.
+// time.  A query row has a scale of its own; K's rows share one in a CTA, and V's, and
+// the rows that it does not suit have scales of their own.  The weights are split in a
+// unit that goes by the largest weight times V of the tile.
 //
 // One CTA takes up to 256 query rows of one KV head as two lanes A and B of
 // 128 and walks its split of the cache in tiles of 64 rows, each K and V row
@@ -20,9 +19,9 @@
 // their sums at the end:
 //   * loader warps 8-11 bring chunks of 8 rows in with cp.async (four in flight per
 //     warp, 64 KB per SM), split them and write the K-major operand tiles;
-//   * warps 13 and 14 give K's and V's small rows their scales, in the chunks whose
-//     loader found a thread without a large value in one of its rows (hardly any of
-//     ordinary data);
+//   * warps 13 and 14 give rows of K and V that are small or large by the CTA's scale
+//     their own, in the chunks whose loader found a thread without a large value in one
+//     of its rows, or with too large a one (hardly any of ordinary data);
 //   * warp 12, one thread, issues S = Q K^T (Q pairs stay in TMEM) and, once a
 //     lane's weights are in TMEM over its scores, O = P V into the shared O
 //     columns, so one lane's softmax runs under the other's products;
@@ -63,18 +62,19 @@ constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12, kTtSizeWarp = 13;  // and 14
 constexpr int kTtSoftmaxRegs = 176, kTtLoadRegs = 112, kTtMmaRegs = 48;
 static_assert(2 * kTtSoftmaxRegs + kTtLoadRegs + kTtMmaRegs <= 4 * 128, "a split that can be had");
 constexpr int kTtStages = 2;              // K and V operand tiles
-constexpr int kTtScales = 4;              // tiles whose scales are kept
+constexpr int kTtScales = 4;              // tiles whose rows' scales are kept
 // Weights are 2^(score - reference), with the score at most kTtHead above the
-// reference.  A tile's product with V
-// has a unit of its own for each query row: 2^-n with the weights times 2^(n - V's
-// scale), the largest of them about 2^kTtTop.  So fp16 pairs lose
-// nothing of the rows that make up the tile's output, whatever the weights and
-// sizes of V's other rows are: what is below 2^-30 of the largest weight times V is cut.
+// reference.  A tile's product with V has a unit of its own for each query row: 2^-n
+// with the weights times 2^(n - V's scale), the largest of them about 2^kTtTop.  So fp16
+// pairs lose nothing of the rows that make up the tile's output, whatever the weights
+// and sizes of V's other rows are: what is cut is below 2^-26 of the largest weight
+// times V.
 constexpr int kTtHead = 4, kTtTop = 14;
-// A row whose largest value is below kTtSmall in its chunk's scale has a scale of
-// its own.  It is looked for where a value of a lane is 2^-kTtSpan of the chunk's largest.
-constexpr float kTtSmall = 8.0f;
-constexpr int kTtSpan = 8;
+// K's rows share one scale in a CTA, and V's, by the largest value of the first chunks;
+// a row whose largest value is not in [kTtSmall, kTtLarge) in it has a scale of its
+// own.  (Scales by chunks, in steps of 2^4, make the tiles uneven where ordinary values
+// lie around a step: 64 nodes over 32768 rows, 32 heads, 8 KV heads of 128, 147 us.)
+constexpr float kTtSmall = 8.0f, kTtLarge = 32768.0f;
 // ALT from so many tiles per CTA.  16 heads, 8 KV heads of 128, 16 nodes: 8192
 // rows (7 tiles) 27.4 us with both lanes, 29.8 with one; 32 heads, 32 nodes, 32768
 // rows (28 tiles) 79.8 and 88.3; with 4 tiles the joining costs more than it saves
@@ -92,15 +92,15 @@ constexpr int kTtQ = 0, kTtS = 256, kTtP = 320, kTtO = 384, kTtCols = 512;
 template <int HD>
 struct TtLayout {
     static constexpr int kKeys = tree_tc_keys(HD);
-    static constexpr int kRows = kKeys / 8;             // of a chunk: the rows that share a scale
+    static constexpr int kRows = kKeys / 8;             // of a chunk: the rows that a loader warp takes at a time
     static constexpr int kStride = kKeys * 16 + 16;     // bytes between 8-column chunks of a tile: shifted by a bank group
     static constexpr int kPart = HD / 8 * kStride;      // one of K hi, K lo, V hi, V lo
     static constexpr int kStage = 4 * kPart;
     static constexpr int kChunk = kRows * HD * 4;
     static constexpr int oStaging = kTtStages * kStage;
-    static constexpr int oScale = oStaging + 16 * kChunk;     // int [kTtScales][2][8]
-    // of the rows, in flagged tiles: int [kTtScales][2][kKeys]; whether any differs from its chunk's: [kTtScales][2]
-    static constexpr int oRows = oScale + kTtScales * 2 * 8 * 4;
+    static constexpr int oFlags = oStaging + 16 * kChunk;  // of the chunks: uint8_t [kTtScales][2][8]
+    // of the rows, in flagged tiles: int [kTtScales][2][kKeys]; whether any differs from the CTA's: [kTtScales][2]
+    static constexpr int oRows = oFlags + kTtScales * 2 * 8;
     static constexpr int oDiffer = oRows + kTtScales * 2 * kKeys * 4;
     static constexpr int oBar = oDiffer + kTtScales * 2 * 4;
     static constexpr int kBars = 6 * kTtStages + 2 + 6 + 2;
@@ -124,12 +124,9 @@ __device__ __forceinline__ void cp_async16_row(void* smem, const void* gmem, int
 
 __device__ __forceinline__ float pow2i(int n) { return __int_as_float((n + 127) << 23); }  // -126 <= n <= 127
 
-// Exponent s with max * 2^s in [2^11, 2^15) for the largest magnitude `max`
-// (its bits), a multiple of 4 up to 124.
-__device__ __forceinline__ int scale_exp(uint32_t bits) {
-    const int s = 14 - ((int)(bits >> 23) - 127);
-    return min(s & ~3, 124);
-}
+// Exponent s with max * 2^s in [2^11, 2^12) for the largest magnitude `max` (its
+// bits), up to 124.
+__device__ __forceinline__ int scale_exp(uint32_t bits) { return min(11 + 127 - (int)(bits >> 23), 124); }
 
 // hi = fp16(x), lo = fp16(x - hi) of two values
 __device__ __forceinline__ void split2(f32x2 x, uint32_t& hi, uint32_t& lo) {
@@ -142,37 +139,19 @@ __device__ __forceinline__ void split2(f32x2 x, uint32_t& hi, uint32_t& lo) {
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-__device__ __forceinline__ float abs_max4(const float* x) {
-    return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-}
-// The largest magnitude of this lane's values; `least`: the least of its fours' largest.
+// The largest magnitude of this lane's values; `even` and `odd`: the least of its even
+// and odd fours' largest.
 template <int N>
-__device__ __forceinline__ float lane_max(const float (&x)[N], float& least) {
-    float m = abs_max4(x);
-    least = m;
+__device__ __forceinline__ float lane_max(const float (&x)[N], float& even, float& odd) {
+    float m = 0.0f;
+    even = odd = INFINITY;
 #pragma unroll
-    for (int i = 4; i < N; i += 4) {
-        const float y = abs_max4(x + i);
+    for (int i = 0; i < N; i += 4) {
+        const float y = fmaxf(fmaxf(fabsf(x[i]), fabsf(x[i + 1])), fmaxf(fabsf(x[i + 2]), fabsf(x[i + 3])));
         m = fmaxf(m, y);
-        least = fminf(least, y);
+        (i & 4 ? odd : even) = fminf(i & 4 ? odd : even, y);
     }
     return m;
-}
-// Bits of the largest finite magnitude of the warp's values, from the lanes'; inf(i)
-// is called for an infinite x[i].
-template <int N, class Inf>
-__device__ __forceinline__ uint32_t warp_max_bits(float m, float (&x)[N], Inf inf) {
-    uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-    if (b == 0x7F800000u) {
-        m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (fabsf(x[i]) == INFINITY) inf(i);
-            else m = fmaxf(m, fabsf(x[i]));
-        }
-        b = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-    }
-    return b;
 }
 
 // ALT: at most 128 query rows, both lanes on them, tile t on lane t & 1.
@@ -187,14 +166,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     constexpr int HO = WIDE ? 128 : HD;  // columns of a lane's output
     constexpr bool kShared = ALT || WIDE;  // both lanes on the same rows, S of tile t in block t & 1
     extern __shared__ __align__(128) uint8_t sm[];
-    int* scales = reinterpret_cast<int*>(sm + L::oScale);  // of the chunks; | 1: the rows may differ
+    uint8_t* flags = sm + L::oFlags;  // chunks with rows that may need scales of their own
     int* row_scales = reinterpret_cast<int*>(sm + L::oRows);
     int* rows_differ = reinterpret_cast<int*>(sm + L::oDiffer);
     uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + L::oBar);
     uint64_t* kempty = kfull + kTtStages;
     uint64_t* vfull = kempty + kTtStages;
     uint64_t* vempty = vfull + kTtStages;
-    uint64_t* ksized = vempty + kTtStages;  // small rows have scales of their own
+    uint64_t* ksized = vempty + kTtStages;  // rows have the scales they need
     uint64_t* vsized = ksized + kTtStages;
     uint64_t* sfull = vsized + kTtStages;  // [lane]
     uint64_t* pfull = sfull + 2;
@@ -209,6 +188,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
     // in the records
     __shared__ unsigned infinite[2][HD / 32];
     __shared__ int any_infinite;
+    __shared__ unsigned first_top[2];  // bits of the largest value of K's and V's first chunks
+    __shared__ int cta_scale[2];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, kvh = blockIdx.y, r0 = blockIdx.z * tree_tc_rows(HD);
@@ -238,6 +219,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         mbar_init(joined, 128);
         mbar_init(done, 1);
         any_infinite = 0;
+        first_top[0] = first_top[1] = 0;
         fence_barrier_init();
     }
     if (tid < HD / 16) infinite[0][tid] = 0;
@@ -344,54 +326,89 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             commit(done);  // nothing of this CTA's is in flight when TMEM is freed
             if (!mbar_wait(done, 0)) record_error(a.err, kErrTimeout);
         } else if (warp <= kTtSizeWarp + 1) {
-            // ---------------- small rows of K, of V get scales of their own, in the chunks that are flagged ----------------
+            // ---------------- small and large rows of K, of V get scales of their own, in the chunks that are flagged ----------------
             const int kind = warp - kTtSizeWarp;  // 0: K, 1: V
             for (int t = 0; t < n_tiles && wait_warp(kind ? &vfull[t & 1] : &kfull[t & 1], (t >> 1) & 1); ++t) {
                 const int slot = 2 * (t & (kTtScales - 1)) + kind;
-                const int* words = scales + 8 * slot;
-                const unsigned flags = __ballot_sync(0xffffffffu, lane < 8 && (words[lane & 7] & 1));
-                if (flags) {
+                const unsigned flagged = __ballot_sync(0xffffffffu, lane < 8 && flags[8 * slot + (lane & 7)]);
+                if (flagged) {
                     int* of_row = row_scales + slot * KEYS;
-                    for (int j = lane; j < KEYS; j += 32) of_row[j] = words[j / CR] & ~1;
+                    for (int j = lane; j < KEYS; j += 32) of_row[j] = cta_scale[kind];
                     __syncwarp();
                     uint8_t* tile = sm + (t & 1) * L::kStage + 2 * kind * L::kPart;
-                    const int valid = j1 - j0 - KEYS * t;
                     bool apart = false;
 #pragma unroll 1
-                    for (unsigned left = flags; left; left &= left - 1) {
+                    for (unsigned left = flagged; left; left &= left - 1) {
                         const int c = __ffs(left) - 1;
                         constexpr int G = 32 / CR;  // lanes per row
-                        bool large = CR * c + lane / G >= valid;
+                        float most = 0.0f;
 #pragma unroll 1
                         for (int p = lane % G; p < HD / 8; p += G) {
                             const uint4 h = *reinterpret_cast<const uint4*>(tile + p * L::kStride + (CR * c + lane / G) * 16);
                             auto abs2 = [](uint32_t u) { u &= 0x7FFF7FFFu; return *reinterpret_cast<const __half2*>(&u); };
                             const float2 m = __half22float2(__hmax2(__hmax2(abs2(h.x), abs2(h.y)), __hmax2(abs2(h.z), abs2(h.w))));
-                            large |= fmaxf(m.x, m.y) >= kTtSmall;
+                            most = fmaxf(most, fmaxf(m.x, m.y));
                         }
-                        const unsigned larges = __ballot_sync(0xffffffffu, large);
-#pragma unroll 1
+                        const unsigned larges = __ballot_sync(0xffffffffu, most >= kTtSmall);
+                        const unsigned too_large = __ballot_sync(0xffffffffu, most >= kTtLarge);
+                        unsigned todo = 0;  // the rows to do again
+#pragma unroll
                         for (int r = 0; r < CR; ++r) {
-                            if (larges >> r * G & ((1u << G) - 1)) continue;
-                            const float* g = (kind ? a.vc : a.kc) + ((size_t)(j0 + KEYS * t + CR * c + r) * a.n_kv + kvh) * a.hd;
-                            auto value = [&](int d) {
-                                const float y = d < a.hd ? g[d] : 0.0f;
-                                return fabsf(y) == INFINITY ? 0.0f : y;
-                            };
-                            float m = 0.0f;
+                            const unsigned group = ((1u << G) - 1) << r * G;
+                            todo |= (unsigned)(!(larges & group) || (too_large & group)) << r;
+                        }
+                        apart |= todo != 0;
+                        constexpr int B = HD > 128 ? 2 : 4, NC = (HD + 127) / 128;  // rows at a time, float4s of a lane
 #pragma unroll 1
-                            for (int d = lane; d < HD; d += 32) m = fmaxf(m, fabsf(value(d)));
-                            const int s = scale_exp(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
-#pragma unroll 1
-                            for (int d = lane; d < HD; d += 32) {
-                                const float y = value(d) * pow2i(s);
-                                const __half h = __float2half_rn(y);
-                                __half* to = reinterpret_cast<__half*>(tile + (d >> 3) * L::kStride + (CR * c + r) * 16) + (d & 7);
-                                to[0] = h;
-                                to[L::kPart / 2] = __float2half_rn(y - __half2float(h));
+                        while (todo) {
+                            int r[B];
+                            float4 y[B][NC];
+#pragma unroll
+                            for (int b = 0; b < B; ++b) {
+                                r[b] = CR * c + __ffs(todo) - 1;
+                                const bool some = todo != 0;
+                                todo &= todo - 1;
+#pragma unroll
+                                for (int i = 0; i < NC; ++i) {
+                                    const int d = 4 * (lane + 32 * i);
+                                    const float* g = (kind ? a.vc : a.kc) + ((size_t)min(j0 + KEYS * t + r[b], j1 - 1) * a.n_kv + kvh) * a.hd + d;
+                                    y[b][i] = some && d < a.hd ? *reinterpret_cast<const float4*>(g) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                }
+                                if (!some) r[b] = -1;
                             }
-                            if (lane == 0) of_row[CR * c + r] = s;
-                            apart = true;
+#pragma unroll
+                            for (int b = 0; b < B; ++b) {
+                                if (r[b] < 0) break;
+                                float m = 0.0f;
+                                auto finite = [&](float& z, int col) {
+                                    if (fabsf(z) < INFINITY) m = fmaxf(m, fabsf(z));
+                                    if (fabsf(z) == INFINITY && kind) {
+                                        atomicOr(&infinite[z < 0.0f][col >> 5], 1u << (col & 31));
+                                        any_infinite = 1;
+                                        z = 0.0f;
+                                    }
+                                };
+#pragma unroll
+                                for (int i = 0; i < NC; ++i) {
+                                    const int col = 4 * (lane + 32 * i);
+                                    finite(y[b][i].x, col), finite(y[b][i].y, col + 1), finite(y[b][i].z, col + 2), finite(y[b][i].w, col + 3);
+                                }
+                                const int s = scale_exp(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+                                const f32x2 f = pack2(pow2i(s), pow2i(s));
+#pragma unroll
+                                for (int i = 0; i < NC; ++i) {
+                                    const int d4 = lane + 32 * i;
+                                    uint8_t* to = tile + (d4 >> 1) * L::kStride + r[b] * 16 + (d4 & 1) * 8;
+                                    uint2 hi, lo;
+                                    split2(mul2(pack2(y[b][i].x, y[b][i].y), f), hi.x, lo.x);
+                                    split2(mul2(pack2(y[b][i].z, y[b][i].w), f), hi.y, lo.y);
+                                    if (4 * d4 < HD) {
+                                        *reinterpret_cast<uint2*>(to) = hi;
+                                        *reinterpret_cast<uint2*>(to + L::kPart) = lo;
+                                    }
+                                }
+                                if (lane == 0) of_row[r[b]] = s;
+                            }
                         }
                     }
                     if (lane == 0) rows_differ[slot] = apart;
@@ -408,6 +425,8 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         const size_t pstride = (size_t)a.n_kv * a.hd;
         const float* src[2] = {a.kc + (size_t)kvh * a.hd, a.vc + (size_t)kvh * a.hd};
         uint8_t* staging = sm + L::oStaging + lw * 4 * L::kChunk;
+        float scale_k = 0.0f, scale_v = 0.0f;  // the CTA's
+        const bool in1 = 4 * (WIDE ? lane + 32 : lane % (HD / 4)) < a.hd;  // the lane's columns (WIDE: of its odd fours) are there
         // chunk i of tile t: the warp's first and second rows of K, of V; a lane's
         // k-th float4 of a chunk is float4 col(k) of its row at(k)
         constexpr int LPR = HD / 4, NK = CR * HD / 128;
@@ -421,7 +440,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             if (t < n_tiles && row + CR <= j1 && 4 * col(NK - 1) < a.hd) {
 #pragma unroll
                 for (int k = 0; k < NK; ++k) cp_async16_row(d + at(k) * HD + 4 * col(k), g + (size_t)at(k) * pstride + 4 * col(k));
-            } else if (t < n_tiles) {  // zeros past the last column; past the last row that row again, which keeps the scales even
+            } else if (t < n_tiles) {  // zeros past the last column; past the last row that row again, so that none is small there
 #pragma unroll 1
                 for (int k = 0; k < NK; ++k) {
                     const bool some = 4 * col(k) < a.hd;
@@ -434,7 +453,6 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         bool ok = true;
         for (int t = 0; t < n_tiles && ok; ++t) {
             uint8_t* tile = sm + (t & 1) * L::kStage;
-            int* sc = scales + (t & (kTtScales - 1)) * 16;
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
                 asm volatile("cp.async.wait_group 3;" ::: "memory");
@@ -447,17 +465,19 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     const float4 v = *reinterpret_cast<const float4*>(st + at(k) * HD + 4 * col(k));
                     x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
                 }
-                float least;
-                const uint32_t top = warp_max_bits(lane_max(x, least), x, [&](int e) {
-                    if (i < 2) return;
-                    const int c = 4 * col(e >> 2) + (e & 3);
-                    atomicOr(&infinite[x[e] < 0.0f][c >> 5], 1u << (c & 31));
-                    any_infinite = 1;
-                    x[e] = 0.0f;
-                });
-                const int s = scale_exp(top);
+                float even, odd;
+                const float most = lane_max(x, even, odd);
+                if (t == 0 && (i & 1) == 0) {
+                    const unsigned top = __reduce_max_sync(0xffffffffu, most < INFINITY ? __float_as_uint(most) : 0u);
+                    if (lane == 0) atomicMax(&first_top[i >> 1], top);
+                    asm volatile("bar.sync 2, 128;" ::: "memory");
+                    const int s = scale_exp(first_top[i >> 1]);
+                    (i ? scale_v : scale_k) = pow2i(s);
+                    if (lane == 0) cta_scale[i >> 1] = s;  // all four warps the same
+                }
                 issue(t + 1, i);  // the chunk is in registers
-                const f32x2 f = pack2(pow2i(s), pow2i(s));
+                const float fs = i < 2 ? scale_k : scale_v;
+                const f32x2 f = pack2(fs, fs);
                 if ((i & 1) == 0 && t >= kTtStages) ok = wait_warp(i ? &vempty[t & 1] : &kempty[t & 1], ((t >> 1) - 1) & 1);
                 if (!ok) break;
                 uint8_t* d = tile + (i >> 1) * 2 * L::kPart + CR * chunk * 16;
@@ -470,10 +490,11 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     *reinterpret_cast<uint2*>(dk) = hi;
                     *reinterpret_cast<uint2*>(dk + L::kPart) = lo;
                 }
-                // rows that may be much smaller than the largest one (or not there): in most chunks each lane sees
-                // in each of its rows a value that is not small, and one vote tells
-                const bool apart = __any_sync(0xffffffffu, __float_as_uint(least) + (kTtSpan << 23) < top);
-                if (lane == 0) sc[8 * (i >> 1) + chunk] = s | (int)apart;
+                // rows that may be small, or large: in most chunks each lane sees in each of its rows a value
+                // that is not small, and one vote tells
+                const float least = WIDE ? fminf(even, in1 ? odd : INFINITY) : in1 ? fminf(even, odd) : INFINITY;
+                const bool apart = __any_sync(0xffffffffu, least * fs < kTtSmall || most * fs >= kTtLarge);
+                if (lane == 0) flags[(2 * (t & (kTtScales - 1)) + (i >> 1)) * 8 + chunk] = apart;
                 if (i & 1) {
                     fence_async_smem();
                     __syncwarp();
@@ -582,35 +603,29 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
             const bool writes = !WIDE || x == 0;
             if (active) {
                 tc_fence_after();
-                const int4* sc = reinterpret_cast<const int4*>(scales + (t & (kTtScales - 1)) * 16);
                 const int valid = j1 - j0 - KEYS * t;
                 // 2^(-sq - sk) may need two factors
                 auto factor = [&](int sk) {
                     const int n = -sq - sk, h = n >> 1;
                     return a.scale2 * pow2i(h) * pow2i(n - h);
                 };
-                // The words are not written again before this warp is through with the tile, so that its
+                // The flags are not written again before this warp is through with the tile, so that its
                 // threads agree; the rows' own scales are there with the scores (K), with vsized (V).
-                const int* sk = reinterpret_cast<const int*>(sc);
-                auto differ = [](const int4& p, const int4& q) {
-                    const int c = p.x;
-                    return ((p.y ^ c) | (p.z ^ c)) | ((p.w ^ c) | (q.x ^ c)) | ((q.y ^ c) | (q.z ^ c)) | (q.w ^ c);
-                };
+                const int slot = 2 * (t & (kTtScales - 1));
                 auto flagged = [&](int kind) {
-                    const int4 p = sc[2 * kind], q = sc[2 * kind + 1];
-                    return (((p.x | p.y) | (p.z | p.w) | (q.x | q.y) | (q.z | q.w)) & 1) != 0;
+                    const uint2 c = *reinterpret_cast<const uint2*>(flags + 8 * (slot + kind));
+                    return (c.x | c.y) != 0;
                 };
-                auto apart = [&](int kind) { return flagged(kind) && rows_differ[2 * (t & (kTtScales - 1)) + kind]; };
-                const int4 k0 = sc[0], k1 = sc[1];
-                constexpr int kUneven = 1 << 20;
-                int V = kUneven;  // the scale of all of V's rows
+                auto apart = [&](int kind) { return flagged(kind) && rows_differ[slot + kind]; };
+                const float f0 = factor(cta_scale[0]);
+                const bool even_k = !flagged(0) && cta_scale[0] >= tame;
+                int V = 0;
+                bool even_v = false;
                 auto look = [&] {
-                    const int4 v0 = sc[2], v1 = sc[3];
-                    if ((differ(v0, v1) | (v0.x & 1)) == 0) V = v0.x;
+                    V = cta_scale[1];
+                    even_v = !flagged(1);
                 };
                 if (v_in) look();
-                const float f0 = factor(k0.x & ~1);
-                const bool even_k = (differ(k0, k1) | (k0.x & 1)) == 0 && k0.x >= tame;
                 float tm = -INFINITY;
                 if (even_k && f0 >= 0.0f) {  // behind the last row it is there again
 #pragma unroll 1
@@ -621,26 +636,14 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                         for (int j = 0; j < 32; j += 2) tm = fmaxf(tm, fmaxf(s[j], s[j + 1]));
                     }
                     tm *= f0;
-                } else if (apart(0)) {
-                    const int* of_row = row_scales + 2 * (t & (kTtScales - 1)) * KEYS;
+                } else {
+                    const bool own_k = apart(0);
 #pragma unroll 1
                     for (int b = 0; b < min(KEYS, valid); b += 4) {
                         float s[4];
                         tmem_ld4f(ts + b, s);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) tm = fmaxf(tm, s[j] * factor(of_row[b + j]));
-                    }
-                } else {
-#pragma unroll 1
-                    for (int b = 0; b < KEYS / 16; ++b) {
-                        float s[16];
-                        tmem_ld16f(ts + 16 * b, s);
-                        float f[16 / CR];
-#pragma unroll
-                        for (int i = 0; i < 16 / CR; ++i) f[i] = factor(sk[16 / CR * b + i] & ~1);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (16 * b + j < valid) tm = fmaxf(tm, s[j] * f[j / CR]);
+                        for (int j = 0; j < 4; ++j) tm = fmaxf(tm, s[j] * (own_k ? factor(row_scales[slot * KEYS + b + j]) : f0));
                     }
                 }
                 // the reference follows the maximum only when that has grown by more
@@ -656,22 +659,16 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     if (!ok) break;
                     look();
                 }
-                if (V == kUneven && flagged(1)) {
+                if (!even_v) {
                     ok = wait_warp(&vsized[t & 1], (t >> 1) & 1);
                     if (!ok) break;
-                    if ((differ(sc[2], sc[3]) & ~1) == 0 && !apart(1)) V = sc[2].x & ~1;
+                    even_v = !rows_differ[slot + 1];
                 }
-                // The unit 2^-n.  With one scale 2^V for all of V's rows (and K's by chunks) the weights are taken
+                // The unit 2^-n.  With the CTA's scales, 2^V for V's rows, the weights are taken
                 // times 2^m, m = n - V; else each times 2^(n - its row's scale).
                 float back = 1.0f;  // 2^-m
                 f32x2 sum = 0;
-                auto all_tame = [&] {
-                    int least = sk[0];
-#pragma unroll 1
-                    for (int c = 1; c < 8; ++c) least = min(least, sk[c]);
-                    return least >= tame;
-                };
-                if (V != kUneven && (even_k || (!apart(0) && all_tame()))) {
+                if (even_v && (even_k || (!apart(0) && cta_scale[0] >= tame))) {
                     // a whole number by rounding in the last place of 1.5 * 2^23; at most what 2^-m and 2^-n can be
                     const float magic = 12582912.0f;
                     const int zero = __float_as_int(magic), r = min(__float_as_int(fmaxf((float)kTtTop + (ref - tm), 0.0f) + magic), zero + 126 - max(V, 0));
@@ -679,7 +676,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                     const float shift = (__int_as_float(r) - magic) - ref;
                     back = pow2i(-m);
                     beta = pow2i(-m - V);
-                    if (writes && even_k && valid >= KEYS) {
+                    if (writes && valid >= KEYS) {
                         const f32x2 f02 = pack2(f0, f0), shift2 = pack2(shift, shift);
 #pragma unroll 1
                         for (int b = 0; b < KEYS / 16; ++b) {
@@ -701,16 +698,13 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                             float s[16];
                             uint32_t p[16];
                             tmem_ld16f(ts + 16 * b, s);
-                            float f[16 / CR];
-#pragma unroll
-                            for (int i = 0; i < 16 / CR; ++i) f[i] = factor(sk[16 / CR * b + i] & ~1);
 #pragma unroll
                             for (int j = 0; j < 16; j += 2) {
                                 float e[2] = {0.0f, 0.0f};
 #pragma unroll
                                 for (int y = j; y < j + 2; ++y)
                                     if (16 * b + y < valid)
-                                        e[y - j] = ex2(fmaf(s[y], f[j / CR], shift));
+                                        e[y - j] = ex2(fmaf(s[y], f0, shift));
                                 const f32x2 e2 = pack2(e[0], e[1]);
                                 sum = add2(sum, e2);
                                 split2(e2, p[j / 2], p[8 + j / 2]);
@@ -719,17 +713,17 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
                         }
                     }
                 } else {
-                    const int* of_row = row_scales + 2 * (t & (kTtScales - 1)) * KEYS;
+                    const int* of_row = row_scales + slot * KEYS;
                     const bool own_k = flagged(0), own_v = flagged(1);
-                    auto scale_k = [&](int j) { return own_k ? of_row[j] : sk[j / CR]; };
-                    auto scale_v = [&](int j) { return (float)(own_v ? of_row[KEYS + j] : sk[8 + j / CR]); };
+                    auto factor_k = [&](int j) { return own_k ? factor(of_row[j]) : f0; };
+                    auto scale_v = [&](int j) { return (float)(own_v ? of_row[KEYS + j] : V); };
                     float most = -INFINITY;  // exponent of the largest weight times V
 #pragma unroll 1
                     for (int b = 0; b < min(KEYS, valid); b += 4) {  // behind the last row it is there again
                         float s[4];
                         tmem_ld4f(ts + b, s);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) most = fmaxf(most, (__fmul_rn(s[j], factor(scale_k(b + j))) - ref) - scale_v(b + j));
+                        for (int j = 0; j < 4; ++j) most = fmaxf(most, (__fmul_rn(s[j], factor_k(b + j)) - ref) - scale_v(b + j));
                     }
                     const float n = floorf(fminf(fmaxf((float)kTtTop - most, -126.0f), 126.0f));
                     beta = pow2i(-(int)n);
@@ -745,7 +739,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
 #pragma unroll
                                 for (int y = j; y < j + 2; ++y)
                                     if (b + y < valid) {
-                                        const float z = __fmul_rn(s[y], factor(scale_k(b + y))) - ref;
+                                        const float z = __fmul_rn(s[y], factor_k(b + y)) - ref;
                                         e[y - j] = ex2(z);
                                         w[y - j] = ex2(z + (n - scale_v(b + y)));
                                     }

@@ -117,17 +117,20 @@ def attend_rows(q, k, v, scale):
     A score is off by ds_j = (LAM sqrt(hd) + 14 + 2 C) u scale sum |q k_j| (the terms of test_candidates_gpu.py), its
     weight by that and the exponential's (2 + |x_j|) u, x_j its distance from the maximum in powers of two, and the sum
     of the weights by the weights' errors and its own rounding: D.  Each term p_j v_j of an output is off by its weight's
-    error, D, the pairs' 12 u and the output's sum, (LAM sqrt(n) + 24) u.  What the pairs cut: less than 2^-30 of the
-    largest p_j max |v_j| a row; in K less than 2^-32 of max |k_j| an element."""
+    error, D, the pairs' 12 u and the output's sum, (LAM sqrt(n) + 24) u.  What the pairs cut, half a step of the lo
+    part, 2^-25: as rows are scaled to a largest value in [2^3, 2^15), 2^-28 of max |k_j| or max |v_j| an element; and as
+    the largest weight times V in a row's scale is scaled to at least 2^13, 2^-25 2^15 / (2^13 2^3) = 2^-26 of the
+    largest p_j max |v_j| for a row's weight (for hardly more than half of the rows, at random: LAM sqrt(n / 4))."""
     q, k, v = q.double(), k.double(), v.double()
     n, hd = k.shape
     s = (k @ q) * scale
     c = LAM * hd**0.5 + 14 + 2 * max(24, 3 * ((hd + 15) // 16))
     p = torch.softmax(s, 0)
-    ds = abs(scale) * (c * U * (k.abs() @ q.abs()) + 2.0**-32 * q.abs().sum() * k.abs().amax(1))
+    ds = abs(scale) * (c * U * (k.abs() @ q.abs()) + 2.0**-28 * q.abs().sum() * k.abs().amax(1))
     r = ds + (2 + (s.max() - s) / np.log(2.0)) * U
     off = r + (p * r).sum() + (2 * LAM * n**0.5 + 36) * U
-    cut = 2.0**-30 * (LAM * n**0.5 + 8) * (p * v.abs().amax(1)).max()
+    pv = p * v.abs().amax(1)
+    cut = 2.0**-28 * pv.sum() + 2.0**-27 * (LAM * n**0.5 + 8) * pv.max()
     return p @ v, (p * off) @ v.abs() + cut + 1e-36
 
 
@@ -403,3 +406,37 @@ def test_tree_other_branches_do_not_leak_in_each_form(gpu, form):
     k[pos0 + n - 1], v[pos0 + n - 1] = float("nan"), float("inf")  # no other node's ancestor
     out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0)
     check_tree(out, q, k, v, up, pos0, hd**-0.5, 0, sorted({0, (n - 1) // 2, max(0, n - 2)}))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("kind", ["growing", "shrinking", "zeros first", "zeros last", "all zeros"])
+def test_tree_sizes_that_change_along_the_cache(gpu, form, kind):
+    """K and V whose size at the start of a CTA's rows says little about the others'."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = randn(170, n, nh, hd), randn(171, pos0 + n, nkv, hd), randn(172, pos0 + n, nkv, hd)
+    at = torch.linspace(-14, 14, pos0 + n, device="cuda")[:, None, None]
+    if kind in ("growing", "shrinking"):
+        size = 2.0 ** (at if kind == "growing" else -at)
+        k, v = k * size * 2.0**-12, v * size
+    rows = torch.arange(pos0 + n, device="cuda")
+    none = {"zeros first": rows % 100 < 70, "zeros last": rows % 100 >= 30, "all zeros": rows >= 0}.get(kind, rows < 0)
+    k[none], v[none] = 0, 0
+    up = make_tree("random", n, 173)
+    out = run_tree(gpu, q, k, v, up, pos0, hd**-0.5, 0)
+    check_rows(out, q, k, v, up, pos0, hd**-0.5, 0, sorted({0, n // 2, n - 1}), sorted({0, nh // 2, nh - 1}))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_tree_infinite_v_among_rows_of_other_sizes(gpu, form):
+    """Infinities in small, large and ordinary rows of V, one of each sign in a row and both in a column."""
+    nh, nkv, hd, pos0, n = FORMS[form]
+    q, k, v = randn(180, n, nh, hd), randn(181, pos0 + n, nkv, hd), randn(182, pos0 + n, nkv, hd)
+    v[7], v[90], v[201] = v[7] * 1e-9, v[90] * 1e9, v[201] * 0
+    inf = float("inf")
+    v[7, 0, 3], v[7, 0, 4], v[90, 0, 5], v[90, 0, hd - 1], v[201, 0, 0], v[150, 0, 6], v[151, 0, 6] = inf, -inf, -inf, inf, inf, inf, -inf
+    out = run_tree(gpu, q, k, v, make_tree("random", n, 183), pos0, hd**-0.5, 0).view(n, nkv, nh // nkv, hd)[:, 0]
+    for col, want in ((3, inf), (4, -inf), (5, -inf), (hd - 1, inf), (0, inf)):
+        assert bool((out[..., col] == want).all()), col
+    assert bool(out[..., 6].isnan().all())
+    cols = [c for c in range(hd) if c not in (0, 3, 4, 5, 6, hd - 1)]
+    assert bool(out[..., cols].isfinite().all())
