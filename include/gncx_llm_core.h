@@ -257,8 +257,14 @@ int32_t gncx_mqa_attention_step_noalloc(const float* q_vec, const float* k_vec, 
  * only rows whose position is above its own minus W.  q and out are
  * [n_tok][n_heads * head_dim].  Rows that a node does not see are not read for
  * it.  A node with an invalid parent is an error; its output is unspecified.
- * Split softmax, fp32 accuracy (as gncx_mqa_attention_step_ext's default
- * mode); gncx_set_exact_attention has no effect.  The accepted path's rows are
+ * Split softmax (as gncx_mqa_attention_step_ext's default mode);
+ * gncx_set_exact_attention has no effect.  Products and sums are fp32, or, on
+ * the tensor cores (head sizes that are multiples of 16, but for few query rows
+ * over a short cache), of pairs of fp16 values that keep 22 bits of each value
+ * within 2^-6 of the largest of its row (of q, K or V), and of smaller ones what
+ * is above 2^-28 of it: as good as fp32 in sums over ordinary rows, while a value
+ * far below its row's largest loses relative accuracy.  Rows of any size may lie
+ * next to each other.  The accepted path's rows are
  * brought together with gncx_state_reorder. */
 int32_t gncx_attention_tree(const float* q, const float* k_cache, const float* v_cache, const int32_t* parents,
                             int32_t pos0, int32_t n_tok, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
@@ -300,8 +306,9 @@ size_t gncx_kv_evict_workspace(int32_t n_rows, int32_t n_keep, int32_t n_kv_head
 /* One step of beam search: the n_out (1..256) best continuations of n_beam
  * (1..256) beams.  Candidate (b, t) scores
  * scores[b] + logits[b][t] - log sum_t exp(logits[b][t]), in double precision;
- * a beam with finished[b] != 0 has the one candidate (b, eos) with scores[b]
- * (finished may be NULL).  Ranked by score, then beam, then logit, then token.
+ * a beam with finished[b] != 0 has the one candidate (b, eos) with scores[b].
+ * finished may be NULL; where it is given, eos must be a token of the
+ * vocabulary, whether or not a beam has ended.  Ranked by score, then beam, then logit, then token.
  * A score of -inf or NaN is no candidate (a beam whose logits hold a NaN or
  * +inf has none); where candidates run out, score -inf, parent -1, token -1.
  * logits are [n_beam][vocab].  out_finished (may be NULL): the beam had ended
