@@ -21,7 +21,8 @@
 // The first kernel is bound by instruction issue (about 60 % busy, 45 instructions a
 // logit, a third of them the exponential): 25.8 us for 64 beams of 151936 logits, 9
 // of them ended, 1.3 TB/s.  The merge is one CTA's chain of dependent reads and
-// barriers, 8 to 11 us alone and cold.  Both: 30.7 us; 4 beams 12.8 us.  Slower:
+// barriers, alone and cold, under ncu, 10 us for 4 beams and 13 for 64.  Both: 30.7 us;
+// 4 beams 12.8 us.  Slower:
 // appending by a ballot per logit (48.7 us against 34.7 then), two CTAs per SM
 // (31.3 us), more than fit it (4: 9 % slower).
 #include <cuda_runtime.h>

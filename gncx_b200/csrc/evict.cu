@@ -28,10 +28,14 @@
 //     selection of the n_keep-th key over keys in registers, then the lists of
 //     free and of moving rows by prefix sums;
 //   * evict_move_kernel copies the rows (few rows: the selecting kernel does).
-// The selection is a chain of dependent steps (14 us of 8 KV heads' 32768 rows: a
-// read, then per digit a histogram, a cluster barrier, the other CTAs' counts and
-// a scan), the moves are bound by HBM (21 us for 52 MB read and as much written):
-// 32768 -> 8192 rows 29.9 us.  One row of 4097: 3.6 us, two dependent reads.
+// The selection is a chain of dependent steps (under ncu 17 us of 8 KV heads' 32768
+// rows: a read, then per digit a histogram, a cluster barrier, the other CTAs' counts
+// and a scan), the moves are bound by HBM (23 us there for 54 MB read and as much
+// written): 32768 -> 8192 rows 34 us in a graph, 42 where more rows are protected than
+// stay and the first digit is looked at again.  One row of 4097: 3.6 us, two dependent
+// reads.  Above 131072 rows one CTA per KV head selects, reading the weights four times:
+// 262144 -> 65536 rows 681 us, of which the selection takes 529 (131072 -> 32768 rows
+// with a cluster 107 us); one row of 262144 441 us.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include "common.cuh"

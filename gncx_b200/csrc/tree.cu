@@ -22,11 +22,13 @@
 // tree_tc.cu has the dense range's kernel on the tensor cores, for head sizes that
 // are multiples of 16; tree_dense_kernel serves the others.  It is bound by
 // shared memory: a 16-byte read per 4 (values) to 13 (scores) multiply-adds; 12
-// heads, 4 KV heads of 136, 16 nodes over 8192 rows: 98 us, 0.37 TB/s.  The merge
-// is bound by the latency of its dependent reads (parents, rows, records: 8 us
-// alone and cold for 33 nodes and 8 KV heads), so all that comes before the
+// heads, 4 KV heads of 136, 16 nodes over 8192 rows: 112 us with the merge, 0.32 TB/s.
+// (The tensor-core kernel loads, pads and stores in steps of four columns, so that it
+// could take these sizes too; it has not been measured on them.)  The merge
+// is bound by the latency of its dependent reads (parents, rows, records: 10 us
+// alone and cold, under ncu, for 33 nodes and 8 KV heads), so all that comes before the
 // records runs before it waits for the dense kernel, and a thread has eight
-// records in flight: 5 nodes over 511 rows, both kernels 10.4 us.
+// records in flight: 5 nodes over 511 rows, both kernels 10.2 us.
 //
 // Few query rows over a short cache take one launch, tree_one_kernel, a cluster
 // of CTAs on the CUDA cores: bound by its chain of reads, sums over lanes and
@@ -579,10 +581,11 @@ static void tree_geometry(TreeArgs& a, int sm_count) {
 // Query rows per cluster where one launch does everything, 0 where not: the clusters
 // run side by side (15 of 8 CTAs do, 16 took twice the time) and the cache is short.
 // One launch against the two kernels: 16 heads, 8 KV heads of 128, 4 nodes (8 query
-// rows): 10 cache rows 6.0 us and 11.3, 511 rows 8.4 and 11.6, 700 rows 8.8 and
-// 12.2; on 2 KV heads of 64, 700 rows 7.9 and 8.7, 1000 rows 9.1 and 8.2.  5 nodes
-// (16 rows per cluster): 256 rows 8.8 and 10.8, 511 rows 10.8 and 10.8.  Head size
-// 256: 128 rows 9.2 and 10.8, 384 rows 11.7 and 11.0.
+// rows): 10 cache rows 5.8 us and 10.6, 511 rows 8.1 and 10.1, 700 rows 8.7 and
+// 10.5; on 2 KV heads of 64, 700 rows 7.9 and 8.4, 1000 rows 8.9 and 8.7.  5 nodes
+// (16 rows per cluster): 256 rows 9.0 and 10.0, 384 rows 9.9 and 10.2, 511 rows 10.9
+// and 10.4.  Head size 256: 128 rows 8.3 and 11.0, 256 rows 10.1 and 11.1, 384 rows 10.9
+// and 11.2.
 static int tree_one_rows(const TreeArgs& a, int sm_count) {
     const int64_t len = (int64_t)a.pos0 + a.n_tok - (a.window > 0 ? max(0, a.pos0 - a.window + 1) : 0);
     const int64_t fit = sm_count * 13 / 16 / kToCluster / a.n_kv;  // clusters per KV head

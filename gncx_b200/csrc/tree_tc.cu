@@ -36,12 +36,14 @@
 // What bounds it: latency, with the tensor pipe, shared memory and the issue slots
 // each about half busy.  64 nodes, 32 heads, 8 KV heads of 128, 32768 rows: 114 us
 // with the merge (2.4 TB/s; three fp16 products at 910 TFLOP/s, of which the
-// pipe alone would need 60 us), tensor pipe 45 % busy, issue 46 %.  1 node:
-// 70 us, 3.8 TB/s.  16 heads, 4 KV heads of 256, 64 nodes, 32768 rows: 157 us (tree.cu's
-// CUDA-core kernel: 3799 us).  Slower: two threads per row with 16 softmax warps
-// (128 us for the first case), lanes of different tiles in CTAs of 128 rows with 8
-// loader warps (147 us), Q's lo parts in shared memory for a second S buffer
-// (121 us), a weight reference without the pass for the maximum (118 us).
+// pipe alone would need 60 us), tensor pipe 50 % of its cycles, issue 46 %.  1 node:
+// 72 to 76 us, 3.6 TB/s.  16 heads, 4 KV heads of 256, 64 nodes, 32768 rows: 152 us
+// (tree.cu's CUDA-core kernel: 3799 us).  Where rows need scales of their own the tile
+// takes 3 to 4 times as long (all rows of random sizes over 2^12, the first case: 408 to
+// 460 us).  Slower, each against the kernel of its day (114 to 118 us): two threads per
+// row with 16 softmax warps (128 us for the first case), lanes of different tiles in CTAs
+// of 128 rows with 8 loader warps (147 us), Q's lo parts in shared memory for a second S
+// buffer (121 us), a weight reference without the pass for the maximum (118 us).
 #include <cuda_fp16.h>
 #include "common.cuh"
 #include "kernels.h"
@@ -56,9 +58,9 @@ constexpr int kTtThreads = 512;
 constexpr int kTtLoadWarp = 8, kTtMmaWarp = 12, kTtSizeWarp = 13;  // and 14
 // Registers per thread: softmax, loaders, products (whose warpgroup is filled
 // up by the warps of the rows' scales); together at most the 512 x 128 that the block
-// is launched with.  32 heads, 8 KV heads of 128, 16 nodes, 32768 rows: 75.7 us, with
-// 176, 120 and 40 78.0.  16 heads, 4 KV heads of 256, 64 nodes, 32768 rows: 163.9 us,
-// with 184, 104 and 40 167.6, with 192, 96 and 32 178.3.
+// is launched with.  64 nodes, 32 heads, 8 KV heads of 128, 32768 rows: 115.0 us; with
+// 176, 120 and 40 124.0, with 184, 104 and 40 122.8.  Head size 256 (16 heads, 4 KV heads,
+// 64 nodes, 32768 rows): 151.8 us, 148.3 and 157.1.
 constexpr int kTtSoftmaxRegs = 176, kTtLoadRegs = 112, kTtMmaRegs = 48;
 static_assert(2 * kTtSoftmaxRegs + kTtLoadRegs + kTtMmaRegs <= 4 * 128, "a split that can be had");
 constexpr int kTtStages = 2;              // K and V operand tiles
@@ -76,15 +78,15 @@ constexpr int kTtHead = 4, kTtTop = 14;
 // lie around a step: 64 nodes over 32768 rows, 32 heads, 8 KV heads of 128, 147 us.)
 constexpr float kTtSmall = 8.0f, kTtLarge = 32768.0f;
 // ALT from so many tiles per CTA.  16 heads, 8 KV heads of 128, 16 nodes: 8192
-// rows (7 tiles) 27.4 us with both lanes, 29.8 with one; 32 heads, 32 nodes, 32768
-// rows (28 tiles) 79.8 and 88.3; with 4 tiles the joining costs more than it saves
-// (32 heads, 24 nodes, 4096 rows: 24.0 and 23.3).
+// rows (7 tiles) 29.5 us with both lanes, 31.7 with one; 32 heads, 32 nodes, 32768
+// rows (28 tiles) 79.2 and 87.5; with 4 tiles the joining costs as much as it saves
+// (32 heads, 24 nodes, 4096 rows: 23.3 and 23.2).
 constexpr int kTtAltTiles = 6;
 // Rows of a warp above which Q and the records go through shared memory, so that a
 // load or store touches 8 rows or fewer: 33 nodes, 32 heads, 8 KV heads of 128, 4097
-// rows 25.9 us against 26.8 without, 58 nodes, 3 heads, one KV head of 256, 102 rows
-// 16.4 against 22.5; with few rows it costs more than it saves (5 nodes, 16 heads, 8
-// KV heads, 511 rows: 11.6 against 10.8).
+// rows 27.1 us against 28.4 without, 58 nodes, 3 heads, one KV head of 256, 102 rows
+// 16.5 against 22.0; with few rows it costs more than it saves (5 nodes, 16 heads, 8
+// KV heads, 511 rows: 11.6 against 10.3).
 constexpr int kTtTurn = 16;
 // TMEM columns: Q pairs, scores, (head sizes above 128: weights), outputs
 constexpr int kTtQ = 0, kTtS = 256, kTtP = 320, kTtO = 384, kTtCols = 512;
