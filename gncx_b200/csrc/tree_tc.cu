@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(kTtThreads, 1) tree_tc_kernel(const TreeArgs a
         bool ok = true;
 #pragma unroll 1
         for (int t = ALT ? x : 0; t < n_tiles; t += ALT ? 2 : 1) {
-            // V is mostly there when the scores are: its scales are then looked at under the first pass
+            // V is mostly there when the scores are: its flags are then looked at before the first pass
             bool v_in = __all_sync(0xffffffffu, mbar_test(&vfull[t & 1], (t >> 1) & 1));
             ok = wait_warp(&sfull[WIDE ? t & 1 : x], phase_s(t));
             if (!ok) break;
